@@ -100,6 +100,17 @@ SIGNATURES = {
     "hk_moe_fp8blk_forward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_float, c_void_p,
                                       c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                       c_void_p, c_size_t, c_void_p]),
+    "hk_moe_permute": (c_int, [c_void_p] * 2 + [c_int] * 3 + [c_void_p] * 2),
+    "hk_moe_permute_backward": (c_int, [c_void_p] * 2 + [c_int] * 3 + [c_void_p] * 3),
+    "hk_moe_unpermute_backward": (c_int, [c_void_p] * 4 + [c_int] * 3 + [c_void_p] * 3),
+    "hk_moe_grouped_gemm": (c_int, [c_void_p] * 4 + [c_int] * 4 + [c_void_p]),
+    "hk_moe_grouped_gemm_dgrad": (c_int, [c_void_p] * 4 + [c_int] * 4 + [c_void_p]),
+    "hk_moe_grouped_gemm_wgrad": (c_int, [c_void_p] * 4 + [c_int] * 5 + [c_void_p]),
+    "hk_linear_cross_entropy_workspace_bytes": (c_size_t, [c_int] * 4),
+    "hk_linear_cross_entropy": (c_int, [c_void_p] * 3 + [c_int] + [c_void_p] * 2 + [c_int] * 3 +
+                                [c_void_p, c_size_t, c_void_p]),
+    "hk_linear_cross_entropy_backward": (c_int, [c_void_p] * 3 + [c_int] + [c_void_p] * 4 + [c_int] * 4 +
+                                         [c_void_p, c_size_t, c_void_p]),
 }
 
 

@@ -56,4 +56,8 @@ int moe_topk_grouped_sigmoid_check(int T, int E, int k, int n_group, int topk_gr
 void moe_launch_build_items(const int32_t* expert_offsets, int E, int bm, int n_tiles_n1, MoeItem* items1,
                             int n_tiles_n2, MoeItem* items2, int32_t* num_items, hipStream_t s);
 
+// y[t] = add[t] + sum_j w[t, j] o[slot_to_pos[t k + j]] (hk_moe_unpermute_add without its checks; w null: weights of 1).
+int moe_launch_unpermute(const void* o, const float* w, const int32_t* slot_to_pos, int T, int k, int H, const void* add, void* y,
+                         hipStream_t s);
+
 }  // namespace hk

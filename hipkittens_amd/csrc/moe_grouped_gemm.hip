@@ -1,0 +1,154 @@
+// The experts' products of a mixture-of-experts layer in bf16, for training: rows in the order of their experts
+// (expert_offsets [E+1], on the device) times the experts' weights W [E, N, K], and both gradients.
+//
+//   forward  y[r]  = x[r] W[e]^T             contraction along the rows of both operands
+//   dgrad    dx[r] = dy[r] W[e]              across W's rows
+//   wgrad    dW[e] = sum_{r of e} dy[r]^T x[r]   across the rows of both; an expert without rows gets zeros
+//
+// fp32 accumulation, one rounding. No workspace and one launch: how many tiles of rows an expert has is known on the
+// device only, so the grid holds the most there can be, and every workgroup finds its tile by a scan over the offsets.
+#include "gemm_layouts.h"
+#include "moe_common.h"
+#include "../../include/hk355.h"
+
+namespace hk {
+
+constexpr int kGroupedMaxE = 512;
+
+struct GroupedTile { int expert, row0, rows, tile_n; };   // expert < 0: no such tile
+
+// Tile `id` of the list: expert by expert, columns by columns, the tiles of rows of one (expert, columns) side by side. Offsets
+// are held inside [0, R] and in order whatever they hold. Each wave scans by itself: lane l holds experts 8 l .. 8 l + 7.
+__device__ __forceinline__ GroupedTile grouped_tile(const int32_t* __restrict__ offsets, int E, int R, int tile_m, int tiles_n, int id) {
+    const int lane = lane_id();
+    int lo[8], hi[8], tiles[8], mine = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int e = 8 * lane + j;
+        lo[j] = e < E ? min(max(offsets[e], 0), R) : 0;
+        hi[j] = e < E ? min(max(offsets[e + 1], lo[j]), R) : 0;
+        tiles[j] = e < E ? (hi[j] - lo[j] + tile_m - 1) / tile_m * tiles_n : 0;
+        mine += tiles[j];
+    }
+    int upto = mine;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int u = __shfl_up(upto, d, 64);
+        if (lane >= d) upto += u;
+    }
+    int at = upto - mine;
+    GroupedTile t{-1, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        if (id >= at && id < at + tiles[j]) {
+            const int tiles_m = tiles[j] / tiles_n, in = id - at;
+            t = GroupedTile{8 * lane + j, lo[j] + in % tiles_m * tile_m, 0, in / tiles_m};
+            t.rows = min(hi[j] - t.row0, tile_m);
+        }
+        at += tiles[j];
+    }
+    const uint64_t holder = __ballot(t.expert >= 0);
+    if (!holder) return GroupedTile{-1, 0, 0, 0};
+    const int src = __ffsll((unsigned long long)holder) - 1;
+    return GroupedTile{__builtin_amdgcn_readlane(t.expert, src), __builtin_amdgcn_readlane(t.row0, src),
+                       __builtin_amdgcn_readlane(t.rows, src), __builtin_amdgcn_readlane(t.tile_n, src)};
+}
+
+// x [R, K] W [E, N, K] -> y [R, N]; DGRAD: x [R, N] W [E, N, K] -> y [R, K]
+template <bool DGRAD>
+__global__ __launch_bounds__(256) void grouped_gemm_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ W,
+                                                           const int32_t* __restrict__ offsets, uint16_t* __restrict__ y,
+                                                           int R, int E, int N, int K, int tiles_n) {
+    extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
+    const GroupedTile t = grouped_tile(offsets, E, R, kLayoutTile, tiles_n, xcd_chunk_order(blockIdx.x, gridDim.x, kCuPerXcd));
+    if (t.expert < 0) return;
+    const int in = DGRAD ? N : K, out = DGRAD ? K : N, col0 = t.tile_n * kLayoutTile;
+    const uint16_t* We = W + (size_t)t.expert * N * K;
+    v4f acc[4][4];
+    tile_product<false, DGRAD>(smem, operand_along(x, 2ull * in, t.row0, t.row0 + t.rows, in),
+                               DGRAD ? operand_across(We, 2ull * K, col0, N) : operand_along(We, 2ull * K, col0, N, K), in, acc);
+    const int w = wave_id(), row = (w >> 1) * 64, col = col0 + (w & 1) * 64;
+    store_tile(acc, y + (size_t)(t.row0 + row) * out + col, out, t.rows - row, out - col);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void grouped_wgrad_kernel(const uint16_t* __restrict__ dy, const uint16_t* __restrict__ x,
+                                                            const int32_t* __restrict__ offsets, T* __restrict__ dW, int R,
+                                                            int E, int N, int K, int tiles_m, int tiles_n) {
+    extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
+    const int id = xcd_chunk_order(blockIdx.x, gridDim.x, kCuPerXcd);
+    const int e = id / (tiles_m * tiles_n);
+    int pm, pn;
+    grouped_raster(id - e * tiles_m * tiles_n, tiles_m, tiles_n, 8, pm, pn);
+    const int lo = to_sgpr(min(max(offsets[e], 0), R)), rows = to_sgpr(min(max(offsets[e + 1], lo), R)) - lo;
+    const int row0 = pm * kLayoutTile, col0 = pn * kLayoutTile;
+    v4f acc[4][4];
+    tile_product<true, true>(smem, operand_across(dy + (size_t)lo * N, 2ull * N, row0, rows),
+                             operand_across(x + (size_t)lo * K, 2ull * K, col0, rows), rows, acc);
+    const int w = wave_id(), row = row0 + (w >> 1) * 64, col = col0 + (w & 1) * 64;
+    store_tile(acc, dW + (size_t)e * N * K + (size_t)row * K + col, K, N - row, K - col);
+}
+
+static int grouped_check(const void* a, const void* b, const void* c, const void* offsets, int R, int E, int N, int K) {
+    if (!a || !b || !c || !offsets) return HK_ERR_NULL_POINTER;
+    // (a row of 2^24 elements: 32-bit offsets inside a K-step's rows)
+    if (R <= 0 || R >= (1 << 30) || E <= 0 || E > kGroupedMaxE || N <= 0 || K <= 0 || (N % 8) != 0 || (K % 8) != 0 ||
+        N > (1 << 21) || K > (1 << 21))
+        return HK_ERR_BAD_SHAPE;
+    if (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c) & 15u) return HK_ERR_BAD_ALIGNMENT;
+    return HK_OK;
+}
+
+// most tiles of rows there can be: every expert with rows may leave one tile short of `tile` rows by all but one
+static long long grouped_tiles_m(int R, int E, int tile) {
+    const long long used = R < E ? R : E;
+    return (R + used * (tile - 1)) / tile;
+}
+
+template <bool DGRAD>
+static int launch_grouped(const void* x, const void* W, const int32_t* offsets, void* y, int R, int E, int N, int K, hipStream_t s) {
+    const int tiles_n = ((DGRAD ? K : N) + kLayoutTile - 1) / kLayoutTile;
+    const long long grid = grouped_tiles_m(R, E, kLayoutTile) * tiles_n;
+    if (grid >= (1ll << 31)) return HK_ERR_BAD_SHAPE;
+    auto kern = grouped_gemm_kernel<DGRAD>;
+    static DeviceOnce configured;
+    if (!set_lds_limit_once((const void*)kern, kLayoutLdsBytes, configured)) return HK_ERR_LAUNCH;
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), kLayoutLdsBytes, s, (const uint16_t*)x, (const uint16_t*)W, offsets,
+                       (uint16_t*)y, R, E, N, K, tiles_n);
+    return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
+}
+
+template <typename T>
+static int launch_wgrad(const void* dy, const void* x, const int32_t* offsets, void* dW, int R, int E, int N, int K, hipStream_t s) {
+    const int tiles_m = (N + kLayoutTile - 1) / kLayoutTile, tiles_n = (K + kLayoutTile - 1) / kLayoutTile;
+    const long long grid = (long long)E * tiles_m * tiles_n;
+    if (grid >= (1ll << 31)) return HK_ERR_BAD_SHAPE;
+    auto kern = grouped_wgrad_kernel<T>;
+    static DeviceOnce configured;
+    if (!set_lds_limit_once((const void*)kern, kLayoutLdsBytes, configured)) return HK_ERR_LAUNCH;
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), kLayoutLdsBytes, s, (const uint16_t*)dy, (const uint16_t*)x, offsets,
+                       (T*)dW, R, E, N, K, tiles_m, tiles_n);
+    return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
+}
+
+}  // namespace hk
+
+extern "C" int hk_moe_grouped_gemm(const void* x_bf16, const void* w_bf16, const int32_t* expert_offsets, void* y_bf16, int R,
+                                   int E, int N, int K, void* stream) {
+    if (const int st = hk::grouped_check(x_bf16, w_bf16, y_bf16, expert_offsets, R, E, N, K)) return st;
+    return hk::launch_grouped<false>(x_bf16, w_bf16, expert_offsets, y_bf16, R, E, N, K, (hipStream_t)stream);
+}
+
+extern "C" int hk_moe_grouped_gemm_dgrad(const void* dy_bf16, const void* w_bf16, const int32_t* expert_offsets, void* dx_bf16,
+                                         int R, int E, int N, int K, void* stream) {
+    if (const int st = hk::grouped_check(dy_bf16, w_bf16, dx_bf16, expert_offsets, R, E, N, K)) return st;
+    return hk::launch_grouped<true>(dy_bf16, w_bf16, expert_offsets, dx_bf16, R, E, N, K, (hipStream_t)stream);
+}
+
+extern "C" int hk_moe_grouped_gemm_wgrad(const void* dy_bf16, const void* x_bf16, const int32_t* expert_offsets, void* dw,
+                                         int dw_type, int R, int E, int N, int K, void* stream) {
+    if (const int st = hk::grouped_check(dy_bf16, x_bf16, dw, expert_offsets, R, E, N, K)) return st;
+    if (dw_type != 0 && dw_type != 1) return HK_ERR_UNSUPPORTED;
+    return dw_type == 0 ? hk::launch_wgrad<uint16_t>(dy_bf16, x_bf16, expert_offsets, dw, R, E, N, K, (hipStream_t)stream)
+                        : hk::launch_wgrad<float>(dy_bf16, x_bf16, expert_offsets, dw, R, E, N, K, (hipStream_t)stream);
+}

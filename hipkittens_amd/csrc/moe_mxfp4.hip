@@ -1470,7 +1470,7 @@ namespace hk {
 // H = 2880, k = 4 2.4 / 2.1; H = 7168, k = 8: 16 tokens 4.7 / 2.5, 128 6.0 / 3.4, 255 7.0 / 5.1 (whole layers gain
 // less than their timings differ by). From 256 on there is a workgroup for every CU either way (not measured split).
 // o has T * k rows; a position outside [0, T * k) (a caller's broken slot_to_pos) is not read and adds
-// nothing, like an expert id out of range in the sort.
+// nothing, like an expert id out of range in the sort. Without weights (w null) they all count as 1.
 template <int KU>
 __global__ __launch_bounds__(256) void moe_unpermute_kernel(const uint16_t* __restrict__ o,
                                                             const float* __restrict__ w,
@@ -1483,7 +1483,7 @@ __global__ __launch_bounds__(256) void moe_unpermute_kernel(const uint16_t* __re
 #pragma unroll
     for (int j = 0; j < KU; ++j) {
         pos[j] = j < k ? slot_to_pos[(size_t)t * k + j] : -1;
-        wt[j] = j < k ? w[(size_t)t * k + j] : 0.f;
+        wt[j] = j < k ? (w ? w[(size_t)t * k + j] : 1.f) : 0.f;
     }
     const uint32_t n_rows = (uint32_t)T * (uint32_t)k;
     for (int c = blockIdx.y * blockDim.x + threadIdx.x; c < H / 8; c += gridDim.y * blockDim.x) {
@@ -1516,7 +1516,7 @@ __global__ __launch_bounds__(256) void moe_unpermute_kernel(const uint16_t* __re
             for (int j = 0; j < k; ++j) {
                 const int pj = slot_to_pos[(size_t)t * k + j];
                 if ((uint32_t)pj >= n_rows) continue;
-                const float wj = w[(size_t)t * k + j];
+                const float wj = w ? w[(size_t)t * k + j] : 1.f;
                 const v4i raw = *(const v4i*)(o + (size_t)pj * H + c * 8);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -1626,17 +1626,24 @@ extern "C" int hk_mxfp8_quantize_rows(const void* x_bf16, int rows, int cols, vo
     return launch_mx_quantize_rows<true>(x_bf16, rows, cols, codes, scales, scale_pitch, (hipStream_t)stream);
 }
 
+namespace hk {
+int moe_launch_unpermute(const void* o, const float* w, const int32_t* slot_to_pos, int T, int k, int H, const void* add, void* y,
+                         hipStream_t s) {
+    auto kern = k <= 4 ? moe_unpermute_kernel<4> : k <= 8 ? moe_unpermute_kernel<8> : moe_unpermute_kernel<0>;
+    const bool split = T < moe_num_compute_units();
+    const dim3 grid(T, split ? min((H / 8 + 63) / 64, 65535) : 1);
+    hipLaunchKernelGGL(kern, grid, dim3(split ? 64 : 256), 0, s, (const uint16_t*)o, w, slot_to_pos, T, k, H, (const uint16_t*)add,
+                       (uint16_t*)y);
+    return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
+}
+}  // namespace hk
+
 extern "C" int hk_moe_unpermute_add(const void* o_bf16, const float* w, const int32_t* slot_to_pos, int T,
                                     int k, int H, const void* add_bf16_or_null, void* y_bf16, void* stream) {
     if (!o_bf16 || !w || !slot_to_pos || !y_bf16) return HK_ERR_NULL_POINTER;
     if (T <= 0 || k <= 0 || H <= 0 || (H % 8) != 0) return HK_ERR_BAD_SHAPE;
     if (((uintptr_t)o_bf16 | (uintptr_t)y_bf16 | (uintptr_t)add_bf16_or_null) & 15u) return HK_ERR_BAD_ALIGNMENT;
-    auto kern = k <= 4 ? moe_unpermute_kernel<4> : k <= 8 ? moe_unpermute_kernel<8> : moe_unpermute_kernel<0>;
-    const bool split = T < moe_num_compute_units();
-    const dim3 grid(T, split ? min((H / 8 + 63) / 64, 65535) : 1);
-    hipLaunchKernelGGL(kern, grid, dim3(split ? 64 : 256), 0, (hipStream_t)stream, (const uint16_t*)o_bf16,
-                       w, slot_to_pos, T, k, H, (const uint16_t*)add_bf16_or_null, (uint16_t*)y_bf16);
-    return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
+    return hk::moe_launch_unpermute(o_bf16, w, slot_to_pos, T, k, H, add_bf16_or_null, y_bf16, (hipStream_t)stream);
 }
 
 extern "C" int hk_moe_unpermute(const void* o_bf16, const float* w, const int32_t* slot_to_pos, int T, int k,

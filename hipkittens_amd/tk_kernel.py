@@ -686,3 +686,173 @@ def dispatch_moe_fp8blk(x, x_scales, router_logits, router_bias, w13, w13_scales
             float(routed_scale), w13.data_ptr(), w13_scales.data_ptr(), w2.data_ptr(), w2_scales.data_ptr(),
             y.data_ptr(), T, H, I, E, int(topk), layout, p_add, workspace.data_ptr(), workspace.numel(), _stream(x))
     _lib.check(st, "dispatch_moe_fp8blk")
+
+
+# ------------------------------------------------------------ training: MoE rows and products, output head
+def _same_device(*tensors):
+    if len({t.device for t in tensors if t is not None}) != 1:
+        raise RuntimeError("all tensors must be on the same device")
+
+
+def _check_positions(rows, name, slot_to_pos, T: int, H: int) -> int:
+    """-> k of `rows` [T*k, H] and slot_to_pos [T*k]"""
+    _check_tensor(rows, name, _BF16, 2)
+    _check_tensor(slot_to_pos, "slot_to_pos", _I32, 1)
+    S = rows.shape[0]
+    if T <= 0 or S % T or S == 0 or rows.shape[1] != H or slot_to_pos.shape[0] != S:
+        raise RuntimeError(f"shape mismatch: {T} tokens of {H} elements, {name} {tuple(rows.shape)}, "
+                           f"slot_to_pos {tuple(slot_to_pos.shape)}")
+    return S // T
+
+
+def dispatch_moe_permute(x, slot_to_pos, xp) -> None:
+    """Rows to the order of their experts: xp[slot_to_pos[t*k+j]] = x[t] with x [T,H], xp [T*k,H] bf16 and slot_to_pos [T*k]
+    from dispatch_moe_sort. A position outside [0, T*k) has no row; rows of xp that no slot names stay as they were."""
+    _check_tensor(x, "x", _BF16, 2)
+    T, H = x.shape
+    k = _check_positions(xp, "xp", slot_to_pos, T, H)
+    _same_device(x, slot_to_pos, xp)
+    with torch.cuda.device(x.device):
+        st = _lib.load_library().hk_moe_permute(x.data_ptr(), slot_to_pos.data_ptr(), T, k, H, xp.data_ptr(), _stream(x))
+    _lib.check(st, "dispatch_moe_permute")
+
+
+def dispatch_moe_permute_backward(dxp, slot_to_pos, dx, add=None) -> None:
+    """Gradient of dispatch_moe_permute: dx [T,H] = (add [T,H] if given) + sum_j dxp[slot_to_pos[t*k+j]], summed in fp32."""
+    _check_tensor(dx, "dx", _BF16, 2)
+    T, H = dx.shape
+    k = _check_positions(dxp, "dxp", slot_to_pos, T, H)
+    if add is not None:
+        _check_tensor(add, "add", _BF16, 2)
+        if tuple(add.shape) != (T, H):
+            raise RuntimeError("add must be [T, H]")
+    _same_device(dxp, slot_to_pos, dx, add)
+    with torch.cuda.device(dx.device):
+        st = _lib.load_library().hk_moe_permute_backward(dxp.data_ptr(), slot_to_pos.data_ptr(), T, k, H,
+                                                         add.data_ptr() if add is not None else None, dx.data_ptr(), _stream(dx))
+    _lib.check(st, "dispatch_moe_permute_backward")
+
+
+def dispatch_moe_unpermute_backward(dy, o, weights, slot_to_pos, do, dweights) -> None:
+    """Gradients of dispatch_moe_unpermute: do[pos] = weights[t,j] * dy[t] and dweights[t,j] = <dy[t], o[pos]> with
+    pos = slot_to_pos[t*k+j]; dy [T,H], o and do [T*k,H] bf16, weights and dweights [T,k] fp32. A slot without a row has a
+    dweights of 0; rows of do that no slot names stay as they were."""
+    _check_tensor(dy, "dy", _BF16, 2)
+    T, H = dy.shape
+    k = _check_positions(o, "o", slot_to_pos, T, H)
+    _check_tensor(do, "do", _BF16, 2)
+    _check_tensor(weights, "weights", _F32, 2)
+    _check_tensor(dweights, "dweights", _F32, 2)
+    if tuple(do.shape) != tuple(o.shape) or tuple(weights.shape) != (T, k) or tuple(dweights.shape) != (T, k):
+        raise RuntimeError("shape mismatch between dy, o, weights, do and dweights")
+    _same_device(dy, o, weights, slot_to_pos, do, dweights)
+    with torch.cuda.device(dy.device):
+        st = _lib.load_library().hk_moe_unpermute_backward(dy.data_ptr(), o.data_ptr(), weights.data_ptr(),
+                                                           slot_to_pos.data_ptr(), T, k, H, do.data_ptr(),
+                                                           dweights.data_ptr(), _stream(dy))
+    _lib.check(st, "dispatch_moe_unpermute_backward")
+
+
+def _check_grouped(rows_n, name_n, rows_k, name_k, w, name_w, w_types, expert_offsets):
+    """-> (R, E, N, K) of rows_n [R,N], rows_k [R,K], w [E,N,K] and expert_offsets [E+1]"""
+    _check_tensor(rows_n, name_n, _BF16, 2)
+    _check_tensor(rows_k, name_k, _BF16, 2)
+    _check_tensor(w, name_w, w_types, 3)
+    _check_tensor(expert_offsets, "expert_offsets", _I32, 1)
+    E, N, K = w.shape
+    R = rows_n.shape[0]
+    if rows_n.shape[1] != N or tuple(rows_k.shape) != (R, K) or expert_offsets.shape[0] != E + 1:
+        raise RuntimeError(f"shape mismatch: {name_n} {tuple(rows_n.shape)}, {name_k} {tuple(rows_k.shape)}, "
+                           f"{name_w} {tuple(w.shape)}, expert_offsets {tuple(expert_offsets.shape)}")
+    _same_device(rows_n, rows_k, w, expert_offsets)
+    return R, E, N, K
+
+
+def dispatch_moe_grouped_gemm(x, w, expert_offsets, y) -> None:
+    """The experts' products: y[r] = x[r] @ w[e].T for the rows expert_offsets[e] <= r < expert_offsets[e+1]; x [R,K],
+    w [E,N,K], y [R,N] bf16, expert_offsets [E+1] int32 (dispatch_moe_sort). Rows behind the last offset are left alone."""
+    R, E, N, K = _check_grouped(y, "y", x, "x", w, "w", _BF16, expert_offsets)
+    with torch.cuda.device(x.device):
+        st = _lib.load_library().hk_moe_grouped_gemm(x.data_ptr(), w.data_ptr(), expert_offsets.data_ptr(), y.data_ptr(),
+                                                     R, E, N, K, _stream(x))
+    _lib.check(st, "dispatch_moe_grouped_gemm")
+
+
+def dispatch_moe_grouped_gemm_dgrad(dy, w, expert_offsets, dx) -> None:
+    """Gradient of dispatch_moe_grouped_gemm in x: dx[r] = dy[r] @ w[e]; dy [R,N], w [E,N,K], dx [R,K]."""
+    R, E, N, K = _check_grouped(dy, "dy", dx, "dx", w, "w", _BF16, expert_offsets)
+    with torch.cuda.device(dy.device):
+        st = _lib.load_library().hk_moe_grouped_gemm_dgrad(dy.data_ptr(), w.data_ptr(), expert_offsets.data_ptr(),
+                                                           dx.data_ptr(), R, E, N, K, _stream(dy))
+    _lib.check(st, "dispatch_moe_grouped_gemm_dgrad")
+
+
+def dispatch_moe_grouped_gemm_wgrad(dy, x, expert_offsets, dw) -> None:
+    """Gradient of dispatch_moe_grouped_gemm in w: dw[e] = dy[rows of e].T @ x[rows of e]; dy [R,N], x [R,K], dw [E,N,K] in
+    bf16 or fp32. Every expert's is written, zeros for one without rows."""
+    R, E, N, K = _check_grouped(dy, "dy", x, "x", dw, "dw", _BF16 + _F32, expert_offsets)
+    with torch.cuda.device(dy.device):
+        st = _lib.load_library().hk_moe_grouped_gemm_wgrad(dy.data_ptr(), x.data_ptr(), expert_offsets.data_ptr(),
+                                                           dw.data_ptr(), int(dw.dtype == torch.float32), R, E, N, K, _stream(dy))
+    _lib.check(st, "dispatch_moe_grouped_gemm_wgrad")
+
+
+_LABELS = (torch.int32, torch.int64)
+
+
+def linear_cross_entropy_workspace_bytes(M: int, V: int, K: int, backward: bool = True) -> int:
+    """Bytes of workspace of dispatch_linear_cross_entropy; with `backward` enough for both directions."""
+    return int(_lib.load_library().hk_linear_cross_entropy_workspace_bytes(int(M), int(V), int(K), int(bool(backward))))
+
+
+def _check_head(x, w, labels, rows, workspace):
+    """-> (M, V, K); `rows`: (tensor, name) pairs of [M] fp32"""
+    _check_tensor(x, "x", _BF16, 2)
+    _check_tensor(w, "w", _BF16, 2)
+    _check_tensor(labels, "labels", _LABELS, 1)
+    _check_tensor(workspace, "workspace", _U8, 1)
+    M, K = x.shape
+    if w.shape[1] != K or labels.shape[0] != M:
+        raise RuntimeError(f"shape mismatch: x {tuple(x.shape)}, w {tuple(w.shape)}, labels {tuple(labels.shape)}")
+    for t, name in rows:
+        _check_tensor(t, name, _F32, 1)
+        if t.shape[0] != M:
+            raise RuntimeError(f"{name} must be [{M}], got {tuple(t.shape)}")
+    _same_device(x, w, labels, workspace, *(t for t, _ in rows))
+    return M, w.shape[0], K
+
+
+def dispatch_linear_cross_entropy(x, w, labels, loss, lse, workspace) -> None:
+    """Softmax cross entropy of the logits x @ w.T, which are never in memory: lse[m] = log sum exp of row m's logits,
+    loss[m] = lse[m] - the label's logit; 0 for a label outside [0, V) (torch's -100, say). x [M,K], w [V,K] bf16, labels [M]
+    int32 or int64, loss and lse [M] fp32. workspace: linear_cross_entropy_workspace_bytes(M, V, K, backward=False) bytes."""
+    M, V, K = _check_head(x, w, labels, ((loss, "loss"), (lse, "lse")), workspace)
+    with torch.cuda.device(x.device):
+        st = _lib.load_library().hk_linear_cross_entropy(
+            x.data_ptr(), w.data_ptr(), labels.data_ptr(), int(labels.dtype == torch.int64), loss.data_ptr(), lse.data_ptr(),
+            M, V, K, workspace.data_ptr(), workspace.numel(), _stream(x))
+    _lib.check(st, "dispatch_linear_cross_entropy")
+
+
+def dispatch_linear_cross_entropy_backward(x, w, labels, lse, dloss, dx, dw, workspace) -> None:
+    """Gradients of dispatch_linear_cross_entropy for dloss [M] fp32 (the gradient of each row's loss) and the forward's lse:
+    dx [M,K] bf16 and dw [V,K] bf16 or fp32; either may be None. A row whose label lies outside [0, V) has no gradient.
+    workspace: linear_cross_entropy_workspace_bytes(M, V, K) bytes."""
+    M, V, K = _check_head(x, w, labels, ((lse, "lse"), (dloss, "dloss")), workspace)
+    if dx is None and dw is None:
+        raise RuntimeError("one of dx and dw must be given")
+    if dx is not None:
+        _check_tensor(dx, "dx", _BF16, 2)
+        if tuple(dx.shape) != (M, K):
+            raise RuntimeError("dx must have the shape of x")
+    if dw is not None:
+        _check_tensor(dw, "dw", _BF16 + _F32, 2)
+        if tuple(dw.shape) != (V, K):
+            raise RuntimeError("dw must have the shape of w")
+    _same_device(x, dx, dw)
+    with torch.cuda.device(x.device):
+        st = _lib.load_library().hk_linear_cross_entropy_backward(
+            x.data_ptr(), w.data_ptr(), labels.data_ptr(), int(labels.dtype == torch.int64), lse.data_ptr(), dloss.data_ptr(),
+            dx.data_ptr() if dx is not None else None, dw.data_ptr() if dw is not None else None,
+            int(dw is not None and dw.dtype == torch.float32), M, V, K, workspace.data_ptr(), workspace.numel(), _stream(x))
+    _lib.check(st, "dispatch_linear_cross_entropy_backward")
