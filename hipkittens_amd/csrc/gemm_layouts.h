@@ -164,23 +164,4 @@ __device__ __forceinline__ TileOperand operand_across(const void* p, uint64_t pi
     return o;
 }
 
-// C rows of `ldc` elements from tile row `row` on (rows, cols: what is left of C there): bf16, or fp32 as it is.
-template <typename T, int MT, int NT>
-__device__ __forceinline__ void store_tile(const v4f (&acc)[MT][NT], T* __restrict__ C, int64_t ldc, int64_t rows, int64_t cols) {
-    const int r = lane_id() & 15, g = lane_id() >> 4;
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        const int row = 16 * m + r;
-        if (row >= rows) continue;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int col = 16 * n + 4 * g;
-            if (col >= cols) continue;   // (cols is a multiple of 4)
-            T* p = C + row * ldc + col;
-            if constexpr (sizeof(T) == 4) *(v4f*)p = acc[m][n];
-            else *(v2i*)p = v2i{(int)pack_bf16(acc[m][n].x, acc[m][n].y), (int)pack_bf16(acc[m][n].z, acc[m][n].w)};
-        }
-    }
-}
-
 }  // namespace hk

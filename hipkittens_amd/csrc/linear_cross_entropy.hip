@@ -12,10 +12,13 @@
 // is bf16; it adds 2^-9 relative to each term of sums whose result is rounded to bf16), then dx += dl W in fp32 and dW = dl^T x.
 #include <algorithm>
 
-#include "gemm_layouts.h"
+#include "gemm_layouts_ring.h"
+#include "moe_common.h"
 #include "../../include/hk355.h"
 
 namespace hk {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct HeadLabels {
     const void* p;
@@ -27,47 +30,61 @@ struct HeadLabels {
     }
 };
 
-constexpr int kHeadCols = kLayoutTile / 2;   // columns of one partial result: a wave's
-
+template <typename Tile>
 __global__ __launch_bounds__(256) void head_logits_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ W,
                                                           HeadLabels labels, int M, int V, int K, int tiles_m, int tiles_n,
                                                           float2* __restrict__ partial, float* __restrict__ label_logit) {
     extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
     int pm, pn;
     grouped_raster(xcd_chunk_order(blockIdx.x, tiles_m * tiles_n, kCuPerXcd), tiles_m, tiles_n, 8, pm, pn);
-    const int w = wave_id(), row0 = pm * kLayoutTile, col0 = pn * kLayoutTile;
-    v4f acc[4][4];
-    tile_product<false, false>(smem, operand_along(x, 2ull * K, row0, min(M, row0 + kLayoutTile), K),
-                               operand_along(W, 2ull * K, col0, min(V, col0 + kLayoutTile), K), K, acc);
+    const int w = wave_id(), row0 = pm * Tile::kTile, col0 = pn * Tile::kTile;
+    v4f acc[Tile::F][Tile::F];
+    Tile::template product<false, false>(smem, operand_along(x, 2ull * K, row0, min(M, row0 + Tile::kTile), K),
+                               operand_along(W, 2ull * K, col0, min(V, col0 + Tile::kTile), K), K, acc);
     const int r = lane_id() & 15, g = lane_id() >> 4;
-    const int row = row0 + (w >> 1) * 64 + r, col = col0 + (w & 1) * 64 + 4 * g;
+    const int row = row0 + (w >> 1) * Tile::kPatch + r, first = col0 + (w & 1) * Tile::kPatch, left = V - first;
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
+    for (int m = 0; m < Tile::F; ++m) {
         const int at = row + 16 * m;
+        v4f l[Tile::F];
+#pragma unroll
+        for (int n = 0; n < Tile::F; ++n) l[n] = acc[m][n];
+        if (left < Tile::kPatch) {   // columns behind V
+#pragma unroll
+            for (int n = 0; n < Tile::F; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) l[n][j] = 16 * n + 4 * g + j < left ? l[n][j] : -INFINITY;
+        }
+        const int label = (at < M ? labels.at(at, V) : -1) - first;   // its column of the patch
+        const bool here = label >= 0 && label < Tile::kPatch && ((label >> 2) & 3) == g;   // ... among this lane's
+        if (__any(here)) {
+            float mine = 0.f;
+#pragma unroll
+            for (int n = 0; n < Tile::F; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) mine = label == 16 * n + 4 * g + j ? l[n][j] : mine;
+            if (here) label_logit[at] = mine;
+        }
         float top = -INFINITY;
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (col + 16 * n + j < V) top = fmaxf(top, acc[m][n][j]);
+        for (int n = 0; n < Tile::F; ++n) top = fmaxf(fmaxf(top, fmaxf(l[n].x, l[n].y)), fmaxf(l[n].z, l[n].w));
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
+        // exponents of 2 from here on: the sum is exactly relative to 2^top2, whatever the rounding of top2
+        const float top2 = top * kLog2e, off = top == -INFINITY ? 0.f : -top2;
         float sum = 0.f;
-        const int label = at < M ? labels.at(at, V) : -1;
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (int n = 0; n < Tile::F; ++n)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (col + 16 * n + j < V) sum += __expf(acc[m][n][j] - top);
-                if (col + 16 * n + j == label) label_logit[at] = acc[m][n][j];
-            }
+            for (int j = 0; j < 4; ++j) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(l[n][j], kLog2e, off));
         sum += __shfl_xor(sum, 16, 64);
         sum += __shfl_xor(sum, 32, 64);
-        if (g == 0 && at < M) partial[(size_t)(col / kHeadCols) * M + at] = make_float2(top, sum);
+        if (g == 0 && at < M) partial[(size_t)(first / Tile::kPatch) * M + at] = make_float2(top2, sum);
+        slot_fence();   // (one row block's values in registers at a time)
     }
 }
 
-// Joins the partial results of a row: 16 rows a workgroup, 16 threads each, thread i every 16th block from i on; then thread by thread.
+// Joins the partial results (exponents of 2) of a row: 16 rows a workgroup, 16 threads each, thread i every 16th block from i on; then thread by thread.
 __global__ __launch_bounds__(256) void head_loss_kernel(const float2* __restrict__ partial, const float* __restrict__ label_logit,
                                                         HeadLabels labels, int M, int V, int blocks, float* __restrict__ loss,
                                                         float* __restrict__ lse) {
@@ -77,7 +94,7 @@ __global__ __launch_bounds__(256) void head_loss_kernel(const float2* __restrict
     auto join = [](float2 a, float2 b) {
         const float top = fmaxf(a.x, b.x);
         // (a block of columns behind V, or of logits of -inf, has a sum of 0 and adds nothing)
-        return top == -INFINITY ? make_float2(top, a.y + b.y) : make_float2(top, a.y * __expf(a.x - top) + b.y * __expf(b.x - top));
+        return top == -INFINITY ? make_float2(top, a.y + b.y) : make_float2(top, a.y * __builtin_amdgcn_exp2f(a.x - top) + b.y * __builtin_amdgcn_exp2f(b.x - top));
     };
     float2 all = make_float2(-INFINITY, 0.f);
     if (m < M)
@@ -86,13 +103,14 @@ __global__ __launch_bounds__(256) void head_loss_kernel(const float2* __restrict
     __syncthreads();
     if (seg == 0 && m < M) {
         for (int s = 1; s < 16; ++s) all = join(all, part[s][r]);
-        const float l = all.x + logf(all.y);
+        const float l = (all.x + log2f(all.y)) * kLn2;
         lse[m] = l;
         loss[m] = labels.at(m, V) >= 0 ? l - label_logit[m] : 0.f;
     }
 }
 
 // dl of the columns [v0, v0 + cols) of the vocabulary; `width` columns of it are written, those behind V as zeros.
+template <typename Tile>
 __global__ __launch_bounds__(256) void head_dlogits_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ W,
                                                            HeadLabels labels, const float* __restrict__ lse,
                                                            const float* __restrict__ dloss, int M, int V, int K, int v0, int width,
@@ -100,107 +118,195 @@ __global__ __launch_bounds__(256) void head_dlogits_kernel(const uint16_t* __res
     extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
     int pm, pn;
     grouped_raster(xcd_chunk_order(blockIdx.x, tiles_m * tiles_n, kCuPerXcd), tiles_m, tiles_n, 8, pm, pn);
-    const int w = wave_id(), row0 = pm * kLayoutTile, col0 = v0 + pn * kLayoutTile;
-    v4f acc[4][4];
-    tile_product<false, false>(smem, operand_along(x, 2ull * K, row0, min(M, row0 + kLayoutTile), K),
-                               operand_along(W, 2ull * K, col0, min(V, col0 + kLayoutTile), K), K, acc);
+    const int w = wave_id(), row0 = pm * Tile::kTile, col0 = v0 + pn * Tile::kTile;
+    v4f acc[Tile::F][Tile::F];
+    Tile::template product<false, false>(smem, operand_along(x, 2ull * K, row0, min(M, row0 + Tile::kTile), K),
+                               operand_along(W, 2ull * K, col0, min(V, col0 + Tile::kTile), K), K, acc);
     const int r = lane_id() & 15, g = lane_id() >> 4;
-    const int row = row0 + (w >> 1) * 64, col = col0 + (w & 1) * 64;
+    const int row = row0 + (w >> 1) * Tile::kPatch, col = col0 + (w & 1) * Tile::kPatch, left = V - col;
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
+    for (int m = 0; m < Tile::F; ++m) {
         const int at = row + 16 * m + r;
         const int label = at < M ? labels.at(at, V) : -1;
-        const float scale = label >= 0 ? dloss[at] : 0.f, l = at < M ? lse[at] : 0.f;
+        const float scale = label >= 0 ? dloss[at] : 0.f, lse2 = label >= 0 ? lse[at] * kLog2e : 0.f;
+        v4f d[Tile::F];
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (int n = 0; n < Tile::F; ++n)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int v = col + 16 * n + 4 * g + j;
-                const float p = __expf(acc[m][n][j] - l) - (v == label ? 1.f : 0.f);
-                acc[m][n][j] = label >= 0 && v < V ? scale * p : 0.f;
-            }
+            for (int j = 0; j < 4; ++j) d[n][j] = scale * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[m][n][j], kLog2e, -lse2));
+        if (__any(label >= col && label < col + Tile::kPatch)) {
+#pragma unroll
+            for (int n = 0; n < Tile::F; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) d[n][j] -= label == col + 16 * n + 4 * g + j ? scale : 0.f;
+        }
+        if (left < Tile::kPatch || __any(label < 0)) {   // zeros, not products with zero
+#pragma unroll
+            for (int n = 0; n < Tile::F; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) d[n][j] = label >= 0 && 16 * n + 4 * g + j < left ? d[n][j] : 0.f;
+        }
+        store_block_row(d, m, dl + (size_t)row * pitch + (col - v0), pitch, M - row, v0 + width - col);
+        slot_fence();
     }
-    store_tile(acc, dl + (size_t)row * pitch + (col - v0), pitch, M - row, v0 + width - col);
 }
 
-// dx of one piece, dl [M, cols] W [cols rows from v0 on]: `first` writes the fp32 sums, others add to them, `last` rounds.
-__global__ __launch_bounds__(256) void head_dx_kernel(const uint16_t* __restrict__ dl, const uint16_t* __restrict__ W, int M, int V,
-                                                      int K, int v0, int width, int pitch, int tiles_m, int tiles_n, bool first,
-                                                      bool last, float* __restrict__ sums, uint16_t* __restrict__ dx) {
-    extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
+// Both gradients of one piece in one launch: first the items of dx, dl [M, cols] W [cols rows from v0 on], then those of dW,
+// dl^T x. The contraction of dx runs over the piece, a few hundred K-steps for few tiles: with dW's tiles behind it in the same
+// grid CUs that hold no item of dx work on dW from the start, and `splits` cuts it where its items would still outlast the rest.
+struct HeadPiece {
+    const uint16_t *dl, *W, *x;
+    float* sums;      // [splits][M][K]: dx so far, when there are several pieces or splits
+    uint16_t* dx;
+    int M, V, K, v0, cols, pitch;
+    int tiles_m, tiles_k, tiles_v, splits, split_cols;   // splits 0: no dx; tiles_v 0: no dW
+    bool first, last, reduce;   // reduce: a launch of its own adds the splits and rounds
+};
+
+template <typename Tile>
+__device__ __forceinline__ void head_dx_item(uint8_t* smem, const HeadPiece& p, int id) {
+    const int tiles = p.tiles_m * p.tiles_k, split = id / tiles;
     int pm, pn;
-    grouped_raster(xcd_chunk_order(blockIdx.x, tiles_m * tiles_n, kCuPerXcd), tiles_m, tiles_n, 8, pm, pn);
-    const int w = wave_id(), row0 = pm * kLayoutTile, col0 = pn * kLayoutTile;
-    v4f acc[4][4];
-    tile_product<false, true>(smem, operand_along(dl, 2ull * pitch, row0, min(M, row0 + kLayoutTile), width),
-                              operand_across(W + (size_t)v0 * K, 2ull * K, col0, min(width, V - v0)), width, acc);
+    grouped_raster(id - split * tiles, p.tiles_m, p.tiles_k, 8, pm, pn);
+    const int w = wave_id(), row0 = pm * Tile::kTile, col0 = pn * Tile::kTile;
+    const int c0 = split * p.split_cols, n = min(p.split_cols, (p.cols + 7) / 8 * 8 - c0);   // (columns of dl behind `cols`: zeros)
+    v4f acc[Tile::F][Tile::F];
+    Tile::template product<false, true>(smem, operand_along(p.dl + c0, 2ull * p.pitch, row0, min(p.M, row0 + Tile::kTile), n),
+                                        operand_across(p.W + (size_t)(p.v0 + c0) * p.K, 2ull * p.K, col0, min(n, p.V - p.v0 - c0)), n, acc);
     const int r = lane_id() & 15, g = lane_id() >> 4;
-    const int row = row0 + (w >> 1) * 64, col = col0 + (w & 1) * 64;
-    if (!first) {
+    const int row = row0 + (w >> 1) * Tile::kPatch, col = col0 + (w & 1) * Tile::kPatch;
+    float* sums = p.sums + (size_t)split * p.M * p.K;
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
+    for (int m = 0; m < Tile::F; ++m) {
+        const int at = row + 16 * m + r;
+        v4f v[Tile::F];
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
-                if (row + 16 * m + r < M && col + 16 * n + 4 * g < K)
-                    acc[m][n] += *(const v4f*)(sums + (size_t)(row + 16 * m + r) * K + col + 16 * n + 4 * g);
+        for (int c = 0; c < Tile::F; ++c) {
+            v[c] = acc[m][c];
+            if (!p.first && at < p.M && col + 16 * c + 4 * g < p.K) v[c] += *(const v4f*)(sums + (size_t)at * p.K + col + 16 * c + 4 * g);
+        }
+        if (p.last && !p.reduce) store_block_row(v, m, p.dx + (size_t)row * p.K + col, p.K, p.M - row, p.K - col);
+        else store_block_row(v, m, sums + (size_t)row * p.K + col, p.K, p.M - row, p.K - col);
+        slot_fence();
     }
-    if (last) store_tile(acc, dx + (size_t)row * K + col, K, M - row, K - col);
-    else store_tile(acc, sums + (size_t)row * K + col, K, M - row, K - col);
 }
 
-// dW of one piece: dl^T x over the M rows.
-template <typename T>
-__global__ __launch_bounds__(256) void head_dw_kernel(const uint16_t* __restrict__ dl, const uint16_t* __restrict__ x, int M, int cols,
-                                                      int K, int pitch, int tiles_m, int tiles_n, T* __restrict__ dw) {
+template <typename Tile, typename T>
+__global__ __launch_bounds__(256) void head_gradients_kernel(HeadPiece p, T* __restrict__ dw) {
     extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
+    const int dx_items = p.splits * p.tiles_m * p.tiles_k;
+    if ((int)blockIdx.x < dx_items) {
+        head_dx_item<Tile>(smem, p, xcd_chunk_order(blockIdx.x, dx_items, kCuPerXcd));
+        return;
+    }
     int pm, pn;
-    grouped_raster(xcd_chunk_order(blockIdx.x, tiles_m * tiles_n, kCuPerXcd), tiles_m, tiles_n, 8, pm, pn);
-    const int w = wave_id(), row0 = pm * kLayoutTile, col0 = pn * kLayoutTile;
-    v4f acc[4][4];
-    tile_product<true, true>(smem, operand_across(dl, 2ull * pitch, row0, M), operand_across(x, 2ull * K, col0, M), M, acc);
-    const int row = row0 + (w >> 1) * 64, col = col0 + (w & 1) * 64;
-    store_tile(acc, dw + (size_t)row * K + col, K, cols - row, K - col);
+    grouped_raster(xcd_chunk_order(blockIdx.x - dx_items, p.tiles_v * p.tiles_k, kCuPerXcd), p.tiles_v, p.tiles_k, 8, pm, pn);
+    const int w = wave_id(), row0 = pm * Tile::kTile, col0 = pn * Tile::kTile;
+    v4f acc[Tile::F][Tile::F];
+    Tile::template product<true, true>(smem, operand_across(p.dl, 2ull * p.pitch, row0, p.M), operand_across(p.x, 2ull * p.K, col0, p.M), p.M, acc);
+    const int row = row0 + (w >> 1) * Tile::kPatch, col = col0 + (w & 1) * Tile::kPatch;
+    store_patch(acc, dw + (size_t)row * p.K + col, p.K, p.cols - row, p.K - col);
 }
 
-static int head_tiles(int n) { return (n + kLayoutTile - 1) / kLayoutTile; }
-static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+// dx = the splits' sums, added in order (n = M K, a multiple of 8).
+__global__ __launch_bounds__(256) void head_dx_reduce_kernel(const float* __restrict__ sums, int splits, size_t n, uint16_t* __restrict__ dx) {
+    const size_t at = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (at >= n) return;
+    v4f v = *(const v4f*)(sums + at);
+    for (int s = 1; s < splits; ++s) v += *(const v4f*)(sums + (size_t)s * n + at);
+    *(v2i*)(dx + at) = v2i{(int)pack_bf16(v.x, v.y), (int)pack_bf16(v.z, v.w)};
+}
 
-// forward: label logits, then the partial results; backward: dl of a piece, then the fp32 sums of dx
-struct HeadForwardLayout {
+static int tiles_of(int n, int tile) { return (n + tile - 1) / tile; }
+static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+static bool head_use_256(int rows, int cols, int k) {   // a product of rows x cols over k
+    return prefer_tile256((double)tiles_of(rows, 256) * tiles_of(cols, 256), (double)tiles_of(rows, 128) * tiles_of(cols, 128),
+                          tiles_of(k, kLayoutStep), moe_num_compute_units());
+}
+
+// forward: label logits, then the partial results
+struct HeadForwardPlan {
+    bool tile256;
+    int blocks;   // columns of a partial result: a wave's patch
     size_t label_logit, partial, bytes;
-    HeadForwardLayout(int M, int V) {
+    HeadForwardPlan(int M, int V, int K) {
+        tile256 = head_use_256(M, V, K);
+        blocks = 2 * tiles_of(V, tile256 ? 256 : 128);
         label_logit = 0;
         partial = up256((size_t)M * 4);
-        bytes = partial + up256((size_t)M * 2 * head_tiles(V) * sizeof(float2));
+        bytes = partial + up256((size_t)M * blocks * sizeof(float2));
     }
 };
-struct HeadBackwardLayout {
-    int piece;   // columns of a piece, a multiple of the tile
+// backward: dl of a piece, then the fp32 sums of dx
+struct HeadBackwardPlan {
+    int piece;   // columns of a piece, a multiple of 256
+    bool logits256, grads256;
+    int splits, split_cols;
     size_t dl, sums, bytes;
-    HeadBackwardLayout(int M, int V, int K) {
+    HeadBackwardPlan(int M, int V, int K) {
         // pieces of 256 MB, and rows of at most 4 MB (32-bit offsets inside a K-step's rows)
-        const long long most = std::min((256ll << 20) / (2ll * M), 1ll << 21) / kLayoutTile * kLayoutTile;
-        const long long all = (long long)head_tiles(V) * kLayoutTile;
-        piece = (int)(most < kLayoutTile ? kLayoutTile : most < all ? most : all);
+        const long long most = std::min((256ll << 20) / (2ll * M), 1ll << 21) / 256 * 256, all = (long long)tiles_of(V, 256) * 256;
+        piece = (int)std::max(256ll, std::min(most, all));
+        const int cols = std::min(piece, V);
+        logits256 = head_use_256(M, cols, K);
+        // dx and dW together: K-steps of all tiles over the workgroups that run at once
+        const int slots = moe_num_compute_units(), steps_v = tiles_of(cols, kLayoutStep), steps_m = tiles_of(M, kLayoutStep);
+        const double dx256 = (double)tiles_of(M, 256) * tiles_of(K, 256), dw256 = (double)tiles_of(cols, 256) * tiles_of(K, 256);
+        const double dx128 = (double)tiles_of(M, 128) * tiles_of(K, 128), dw128 = (double)tiles_of(cols, 128) * tiles_of(K, 128);
+        const double large = (dx256 * (7.0 + 1.43 * steps_v) + dw256 * (7.0 + 1.43 * steps_m)) / slots;
+        const double small = (dx128 * (2.7 + kSmallStepAlong * steps_v) + dw128 * (2.7 + kSmallStepAcross * steps_m)) / (2.0 * slots);
+        grads256 = large < small;
+        const double total = grads256 ? dx256 * steps_v + dw256 * steps_m : dx128 * steps_v + dw128 * steps_m;
+        const double share = total / (grads256 ? slots : 2 * slots);   // K-steps of one workgroup's place
+        const int per_split = std::max(8, std::min(steps_v, (int)share));
+        splits = tiles_of(steps_v, per_split);
+        split_cols = tiles_of(steps_v, splits) * kLayoutStep;
+        splits = tiles_of(cols, split_cols);
         dl = 0;
         sums = up256((size_t)M * piece * 2);
-        bytes = sums + (piece < V ? up256((size_t)M * K * 4) : 0);
+        bytes = sums + (piece < V || splits > 1 ? up256((size_t)splits * M * K * 4) : 0);
     }
 };
 
 static int head_check(int M, int V, int K) {
     if (M <= 0 || V <= 0 || K <= 0 || (K % 8) != 0 || M >= (1 << 30) || V >= (1 << 30) || K > (1 << 21)) return HK_ERR_BAD_SHAPE;
-    if ((long long)head_tiles(M) * (head_tiles(V) > head_tiles(K) ? head_tiles(V) : head_tiles(K)) >= (1ll << 31) ||
-        (long long)head_tiles(V) * head_tiles(K) >= (1ll << 31))
+    if ((long long)tiles_of(M, 128) * tiles_of(V, 128) >= (1ll << 30) || (long long)tiles_of(M, 128) * tiles_of(K, 128) >= (1ll << 30) ||
+        (long long)tiles_of(V, 128) * tiles_of(K, 128) >= (1ll << 30))
         return HK_ERR_BAD_SHAPE;
     return HK_OK;
 }
 
-template <typename... P, typename... A>
+template <typename Tile, typename... P, typename... A>
 static int launch_head(void (*kern)(P...), DeviceOnce& once, long long tiles, hipStream_t s, A... args) {
-    if (!set_lds_limit_once((const void*)kern, kLayoutLdsBytes, once)) return HK_ERR_LAUNCH;
-    hipLaunchKernelGGL(kern, dim3((unsigned)tiles), dim3(256), kLayoutLdsBytes, s, args...);
+    if (!set_lds_limit_once((const void*)kern, Tile::kLds, once)) return HK_ERR_LAUNCH;
+    hipLaunchKernelGGL(kern, dim3((unsigned)tiles), dim3(256), Tile::kLds, s, args...);
     return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
+}
+
+template <typename Tile>
+static int launch_logits(const uint16_t* x, const uint16_t* W, HeadLabels labels, int M, int V, int K, float2* partial, float* label_logit,
+                         hipStream_t s) {
+    static DeviceOnce once;
+    const int tm = tiles_of(M, Tile::kTile), tv = tiles_of(V, Tile::kTile);
+    return launch_head<Tile>(head_logits_kernel<Tile>, once, (long long)tm * tv, s, x, W, labels, M, V, K, tm, tv, partial, label_logit);
+}
+template <typename Tile>
+static int launch_dlogits(const uint16_t* x, const uint16_t* W, HeadLabels labels, const float* lse, const float* dloss, int M, int V, int K,
+                          int v0, int cols, int pitch, uint16_t* dl, hipStream_t s) {
+    static DeviceOnce once;
+    const int tm = tiles_of(M, Tile::kTile), tv = tiles_of(cols, Tile::kTile);
+    return launch_head<Tile>(head_dlogits_kernel<Tile>, once, (long long)tm * tv, s, x, W, labels, lse, dloss, M, V, K, v0, (cols + 7) / 8 * 8,
+                             pitch, tm, tv, dl);
+}
+template <typename Tile, typename T>
+static int launch_gradients(HeadPiece p, bool dx, T* dw, hipStream_t s) {
+    static DeviceOnce once;
+    p.tiles_m = tiles_of(p.M, Tile::kTile);
+    p.tiles_k = tiles_of(p.K, Tile::kTile);
+    p.tiles_v = dw ? tiles_of(p.cols, Tile::kTile) : 0;
+    p.splits = dx ? tiles_of(p.cols, p.split_cols) : 0;
+    const long long items = (long long)p.splits * p.tiles_m * p.tiles_k + (long long)p.tiles_v * p.tiles_k;
+    return launch_head<Tile>(head_gradients_kernel<Tile, T>, once, items, s, p, dw ? dw + (size_t)p.v0 * p.K : nullptr);
 }
 
 }  // namespace hk
@@ -208,7 +314,7 @@ static int launch_head(void (*kern)(P...), DeviceOnce& once, long long tiles, hi
 extern "C" size_t hk_linear_cross_entropy_workspace_bytes(int M, int V, int K, int backward) {
     using namespace hk;
     if (head_check(M, V, K) != HK_OK) return 0;
-    const size_t f = HeadForwardLayout(M, V).bytes, b = backward ? HeadBackwardLayout(M, V, K).bytes : 0;
+    const size_t f = HeadForwardPlan(M, V, K).bytes, b = backward ? HeadBackwardPlan(M, V, K).bytes : 0;
     return f > b ? f : b;
 }
 
@@ -219,18 +325,18 @@ extern "C" int hk_linear_cross_entropy(const void* x_bf16, const void* w_bf16, c
     if (const int st = head_check(M, V, K)) return st;
     if (label_type != 0 && label_type != 1) return HK_ERR_UNSUPPORTED;
     if (((uintptr_t)x_bf16 | (uintptr_t)w_bf16 | (uintptr_t)workspace) & 15u) return HK_ERR_BAD_ALIGNMENT;
-    const HeadForwardLayout L(M, V);
+    const HeadForwardPlan L(M, V, K);
     if (!workspace || workspace_bytes < L.bytes) return HK_ERR_WORKSPACE;
     const hipStream_t s = (hipStream_t)stream;
-    uint8_t* ws = (uint8_t*)workspace;
+    float2* partial = (float2*)((uint8_t*)workspace + L.partial);
+    float* label_logit = (float*)((uint8_t*)workspace + L.label_logit);
     const HeadLabels lab{labels, label_type};
-    const int tm = head_tiles(M), tn = head_tiles(V);
-    static DeviceOnce once;
-    const int st = launch_head(head_logits_kernel, once, (long long)tm * tn, s, (const uint16_t*)x_bf16, (const uint16_t*)w_bf16, lab, M, V,
-                               K, tm, tn, (float2*)(ws + L.partial), (float*)(ws + L.label_logit));
+    const uint16_t *x = (const uint16_t*)x_bf16, *w = (const uint16_t*)w_bf16;
+    const int st = L.tile256 ? launch_logits<LayoutTile256>(x, w, lab, M, V, K, partial, label_logit, s)
+                             : launch_logits<LayoutTile128>(x, w, lab, M, V, K, partial, label_logit, s);
     if (st != HK_OK) return st;
-    hipLaunchKernelGGL(head_loss_kernel, dim3((M + 15) / 16), dim3(256), 0, s, (const float2*)(ws + L.partial),
-                       (const float*)(ws + L.label_logit), lab, M, V, 2 * tn, loss, lse);
+    hipLaunchKernelGGL(head_loss_kernel, dim3((M + 15) / 16), dim3(256), 0, s, (const float2*)partial, (const float*)label_logit, lab, M, V,
+                       L.blocks, loss, lse);
     return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
 }
 
@@ -244,32 +350,38 @@ extern "C" int hk_linear_cross_entropy_backward(const void* x_bf16, const void* 
     if ((label_type != 0 && label_type != 1) || (dw_type != 0 && dw_type != 1)) return HK_ERR_UNSUPPORTED;
     if (((uintptr_t)x_bf16 | (uintptr_t)w_bf16 | (uintptr_t)dx_bf16_or_null | (uintptr_t)dw_or_null | (uintptr_t)workspace) & 15u)
         return HK_ERR_BAD_ALIGNMENT;
-    const HeadBackwardLayout L(M, V, K);
+    const HeadBackwardPlan L(M, V, K);
     if (!workspace || workspace_bytes < L.bytes) return HK_ERR_WORKSPACE;
     const hipStream_t s = (hipStream_t)stream;
     uint8_t* ws = (uint8_t*)workspace;
     const HeadLabels lab{labels, label_type};
-    uint16_t* dl = (uint16_t*)(ws + L.dl);
     const uint16_t *x = (const uint16_t*)x_bf16, *w = (const uint16_t*)w_bf16;
-    const int tm = head_tiles(M), tk = head_tiles(K);
-    static DeviceOnce once_dl, once_dx, once_dw, once_dw32;
+    uint16_t* dl = (uint16_t*)(ws + L.dl);
+    const bool want_dx = dx_bf16_or_null != nullptr;
+    HeadPiece p{dl, w, x, (float*)(ws + L.sums), (uint16_t*)dx_bf16_or_null, M, V, K, 0, 0, L.piece, 0, 0, 0, 0, L.split_cols,
+                false, false, L.splits > 1};
     for (int v0 = 0; v0 < V; v0 += L.piece) {
-        const int cols = V - v0 < L.piece ? V - v0 : L.piece, width = (cols + 7) / 8 * 8, tv = head_tiles(cols);
-        int st = launch_head(head_dlogits_kernel, once_dl, (long long)tm * tv, s, x, w, lab, lse, dloss, M, V, K, v0, width, L.piece, tm, tv, dl);
+        p.v0 = v0;
+        p.cols = V - v0 < L.piece ? V - v0 : L.piece;
+        p.first = v0 == 0;
+        p.last = v0 + p.cols == V;
+        int st = L.logits256 ? launch_dlogits<LayoutTile256>(x, w, lab, lse, dloss, M, V, K, v0, p.cols, L.piece, dl, s)
+                             : launch_dlogits<LayoutTile128>(x, w, lab, lse, dloss, M, V, K, v0, p.cols, L.piece, dl, s);
         if (st != HK_OK) return st;
-        if (dx_bf16_or_null) {
-            st = launch_head(head_dx_kernel, once_dx, (long long)tm * tk, s, (const uint16_t*)dl, w, M, V, K, v0, width, L.piece, tm, tk,
-                             v0 == 0, v0 + L.piece >= V, (float*)(ws + L.sums), (uint16_t*)dx_bf16_or_null);
-            if (st != HK_OK) return st;
-        }
-        if (dw_or_null) {
-            const size_t at = (size_t)v0 * K;
-            st = dw_type == 0 ? launch_head(head_dw_kernel<uint16_t>, once_dw, (long long)tv * tk, s, (const uint16_t*)dl, x, M, cols, K, L.piece,
-                                            tv, tk, (uint16_t*)dw_or_null + at)
-                              : launch_head(head_dw_kernel<float>, once_dw32, (long long)tv * tk, s, (const uint16_t*)dl, x, M, cols, K, L.piece,
-                                            tv, tk, (float*)dw_or_null + at);
-            if (st != HK_OK) return st;
-        }
+        if (dw_type == 0)
+            st = L.grads256 ? launch_gradients<LayoutTile256>(p, want_dx, (uint16_t*)dw_or_null, s)
+                            : launch_gradients<LayoutTile128>(p, want_dx, (uint16_t*)dw_or_null, s);
+        else
+            st = L.grads256 ? launch_gradients<LayoutTile256>(p, want_dx, (float*)dw_or_null, s)
+                            : launch_gradients<LayoutTile128>(p, want_dx, (float*)dw_or_null, s);
+        if (st != HK_OK) return st;
+        if (V - v0 <= L.piece) break;
+    }
+    if (want_dx && L.splits > 1) {
+        const size_t n = (size_t)M * K;
+        hipLaunchKernelGGL(head_dx_reduce_kernel, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, s, (const float*)(ws + L.sums),
+                           L.splits, n, (uint16_t*)dx_bf16_or_null);
+        if (hipGetLastError() != hipSuccess) return HK_ERR_LAUNCH;
     }
     return HK_OK;
 }

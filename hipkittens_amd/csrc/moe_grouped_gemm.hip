@@ -7,7 +7,7 @@
 //
 // fp32 accumulation, one rounding. No workspace and one launch: how many tiles of rows an expert has is known on the
 // device only, so the grid holds the most there can be, and every workgroup finds its tile by a scan over the offsets.
-#include "gemm_layouts.h"
+#include "gemm_layouts_ring.h"
 #include "moe_common.h"
 #include "../../include/hk355.h"
 
@@ -17,7 +17,8 @@ constexpr int kGroupedMaxE = 512;
 
 struct GroupedTile { int expert, row0, rows, tile_n; };   // expert < 0: no such tile
 
-// Tile `id` of the list: expert by expert, columns by columns, the tiles of rows of one (expert, columns) side by side. Offsets
+// Tile `id` of the list: expert by expert, inside an expert in groups of eight tiles of rows that go over the columns side by
+// side, so that an XCD's run of 32 tiles shares its operands (8192 x 8192 x 8192 731 us; with all 32 tiles of rows side by side 1078). Offsets
 // are held inside [0, R] and in order whatever they hold. Each wave scans by itself: lane l holds experts 8 l .. 8 l + 7.
 __device__ __forceinline__ GroupedTile grouped_tile(const int32_t* __restrict__ offsets, int E, int R, int tile_m, int tiles_n, int id) {
     const int lane = lane_id();
@@ -41,8 +42,9 @@ __device__ __forceinline__ GroupedTile grouped_tile(const int32_t* __restrict__ 
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         if (id >= at && id < at + tiles[j]) {
-            const int tiles_m = tiles[j] / tiles_n, in = id - at;
-            t = GroupedTile{8 * lane + j, lo[j] + in % tiles_m * tile_m, 0, in / tiles_m};
+            int pm, pn;
+            grouped_raster(id - at, tiles[j] / tiles_n, tiles_n, 8, pm, pn);
+            t = GroupedTile{8 * lane + j, lo[j] + pm * tile_m, 0, pn};
             t.rows = min(hi[j] - t.row0, tile_m);
         }
         at += tiles[j];
@@ -55,23 +57,23 @@ __device__ __forceinline__ GroupedTile grouped_tile(const int32_t* __restrict__ 
 }
 
 // x [R, K] W [E, N, K] -> y [R, N]; DGRAD: x [R, N] W [E, N, K] -> y [R, K]
-template <bool DGRAD>
+template <typename Tile, bool DGRAD>
 __global__ __launch_bounds__(256) void grouped_gemm_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ W,
                                                            const int32_t* __restrict__ offsets, uint16_t* __restrict__ y,
                                                            int R, int E, int N, int K, int tiles_n) {
     extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
-    const GroupedTile t = grouped_tile(offsets, E, R, kLayoutTile, tiles_n, xcd_chunk_order(blockIdx.x, gridDim.x, kCuPerXcd));
+    const GroupedTile t = grouped_tile(offsets, E, R, Tile::kTile, tiles_n, xcd_chunk_order(blockIdx.x, gridDim.x, kCuPerXcd));
     if (t.expert < 0) return;
-    const int in = DGRAD ? N : K, out = DGRAD ? K : N, col0 = t.tile_n * kLayoutTile;
+    const int in = DGRAD ? N : K, out = DGRAD ? K : N, col0 = t.tile_n * Tile::kTile;
     const uint16_t* We = W + (size_t)t.expert * N * K;
-    v4f acc[4][4];
-    tile_product<false, DGRAD>(smem, operand_along(x, 2ull * in, t.row0, t.row0 + t.rows, in),
-                               DGRAD ? operand_across(We, 2ull * K, col0, N) : operand_along(We, 2ull * K, col0, N, K), in, acc);
-    const int w = wave_id(), row = (w >> 1) * 64, col = col0 + (w & 1) * 64;
-    store_tile(acc, y + (size_t)(t.row0 + row) * out + col, out, t.rows - row, out - col);
+    v4f acc[Tile::F][Tile::F];
+    Tile::template product<false, DGRAD>(smem, operand_along(x, 2ull * in, t.row0, t.row0 + t.rows, in),
+                                         DGRAD ? operand_across(We, 2ull * K, col0, N) : operand_along(We, 2ull * K, col0, N, K), in, acc);
+    const int w = wave_id(), row = (w >> 1) * Tile::kPatch, col = col0 + (w & 1) * Tile::kPatch;
+    store_patch(acc, y + (size_t)(t.row0 + row) * out + col, out, t.rows - row, out - col);
 }
 
-template <typename T>
+template <typename Tile, typename T>
 __global__ __launch_bounds__(256) void grouped_wgrad_kernel(const uint16_t* __restrict__ dy, const uint16_t* __restrict__ x,
                                                             const int32_t* __restrict__ offsets, T* __restrict__ dW, int R,
                                                             int E, int N, int K, int tiles_m, int tiles_n) {
@@ -81,17 +83,24 @@ __global__ __launch_bounds__(256) void grouped_wgrad_kernel(const uint16_t* __re
     int pm, pn;
     grouped_raster(id - e * tiles_m * tiles_n, tiles_m, tiles_n, 8, pm, pn);
     const int lo = to_sgpr(min(max(offsets[e], 0), R)), rows = to_sgpr(min(max(offsets[e + 1], lo), R)) - lo;
-    const int row0 = pm * kLayoutTile, col0 = pn * kLayoutTile;
-    v4f acc[4][4];
-    tile_product<true, true>(smem, operand_across(dy + (size_t)lo * N, 2ull * N, row0, rows),
-                             operand_across(x + (size_t)lo * K, 2ull * K, col0, rows), rows, acc);
-    const int w = wave_id(), row = row0 + (w >> 1) * 64, col = col0 + (w & 1) * 64;
-    store_tile(acc, dW + (size_t)e * N * K + (size_t)row * K + col, K, N - row, K - col);
+    const int row0 = pm * Tile::kTile, col0 = pn * Tile::kTile;
+    v4f acc[Tile::F][Tile::F];
+    if (rows > 0) {
+        Tile::template product<true, true>(smem, operand_across(dy + (size_t)lo * N, 2ull * N, row0, rows),
+                                           operand_across(x + (size_t)lo * K, 2ull * K, col0, rows), rows, acc);
+    } else {
+#pragma unroll
+        for (int m = 0; m < Tile::F; ++m)
+#pragma unroll
+            for (int n = 0; n < Tile::F; ++n) acc[m][n] = v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    const int w = wave_id(), row = row0 + (w >> 1) * Tile::kPatch, col = col0 + (w & 1) * Tile::kPatch;
+    store_patch(acc, dW + (size_t)e * N * K + (size_t)row * K + col, K, N - row, K - col);
 }
 
 static int grouped_check(const void* a, const void* b, const void* c, const void* offsets, int R, int E, int N, int K) {
     if (!a || !b || !c || !offsets) return HK_ERR_NULL_POINTER;
-    // (a row of 2^24 elements: 32-bit offsets inside a K-step's rows)
+    // (rows of at most 4 MB: 32-bit offsets inside a K-step's or a tile's rows)
     if (R <= 0 || R >= (1 << 30) || E <= 0 || E > kGroupedMaxE || N <= 0 || K <= 0 || (N % 8) != 0 || (K % 8) != 0 ||
         N > (1 << 21) || K > (1 << 21))
         return HK_ERR_BAD_SHAPE;
@@ -105,30 +114,54 @@ static long long grouped_tiles_m(int R, int E, int tile) {
     return (R + used * (tile - 1)) / tile;
 }
 
-template <bool DGRAD>
-static int launch_grouped(const void* x, const void* W, const int32_t* offsets, void* y, int R, int E, int N, int K, hipStream_t s) {
-    const int tiles_n = ((DGRAD ? K : N) + kLayoutTile - 1) / kLayoutTile;
-    const long long grid = grouped_tiles_m(R, E, kLayoutTile) * tiles_n;
+template <typename Tile, bool DGRAD>
+static int launch_grouped_tile(const void* x, const void* W, const int32_t* offsets, void* y, int R, int E, int N, int K, hipStream_t s) {
+    const int tiles_n = ((DGRAD ? K : N) + Tile::kTile - 1) / Tile::kTile;
+    const long long grid = grouped_tiles_m(R, E, Tile::kTile) * tiles_n;
     if (grid >= (1ll << 31)) return HK_ERR_BAD_SHAPE;
-    auto kern = grouped_gemm_kernel<DGRAD>;
+    auto kern = grouped_gemm_kernel<Tile, DGRAD>;
     static DeviceOnce configured;
-    if (!set_lds_limit_once((const void*)kern, kLayoutLdsBytes, configured)) return HK_ERR_LAUNCH;
-    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), kLayoutLdsBytes, s, (const uint16_t*)x, (const uint16_t*)W, offsets,
+    if (!set_lds_limit_once((const void*)kern, Tile::kLds, configured)) return HK_ERR_LAUNCH;
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), Tile::kLds, s, (const uint16_t*)x, (const uint16_t*)W, offsets,
                        (uint16_t*)y, R, E, N, K, tiles_n);
     return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
 }
 
-template <typename T>
-static int launch_wgrad(const void* dy, const void* x, const int32_t* offsets, void* dW, int R, int E, int N, int K, hipStream_t s) {
-    const int tiles_m = (N + kLayoutTile - 1) / kLayoutTile, tiles_n = (K + kLayoutTile - 1) / kLayoutTile;
+// The tile by prefer_tile256 with the tiles of rows that an expert has on average when the rows spread over the experts
+// unevenly: one at least, else rows / tile + 0.6. (Forward, us, small / large: N = 4096, K = 7168, 32 experts: 1024 rows 320 / 341,
+// 4096 457 / 482, 8192 764 / 539, 65536 4130 / 2873; 128 experts of 5760 x 2880, 16384 rows 1057 / 947; 8 of 1024 x 1024, 4096 rows
+// 20 / 27. The rule's one miss there: 32 experts of 64 rows, small 428, large 359.)
+static bool grouped_use_256(int R, int E, int in, int out) {
+    const double used = R < E ? R : E, mean = R / used;
+    const double m256 = mean / 256 + 0.6, m128 = mean / 128 + 0.6;
+    return prefer_tile256(used * (m256 > 1 ? m256 : 1) * ((out + 255) / 256), used * (m128 > 1 ? m128 : 1) * ((out + 127) / 128),
+                          (in + kLayoutStep - 1) / kLayoutStep, moe_num_compute_units());
+}
+template <bool DGRAD>
+static int launch_grouped(const void* x, const void* W, const int32_t* offsets, void* y, int R, int E, int N, int K, hipStream_t s) {
+    const int in = DGRAD ? N : K, out = DGRAD ? K : N;
+    return grouped_use_256(R, E, in, out) ? launch_grouped_tile<LayoutTile256, DGRAD>(x, W, offsets, y, R, E, N, K, s)
+                                          : launch_grouped_tile<LayoutTile128, DGRAD>(x, W, offsets, y, R, E, N, K, s);
+}
+
+template <typename Tile, typename T>
+static int launch_wgrad_tile(const void* dy, const void* x, const int32_t* offsets, void* dW, int R, int E, int N, int K, hipStream_t s) {
+    const int tiles_m = (N + Tile::kTile - 1) / Tile::kTile, tiles_n = (K + Tile::kTile - 1) / Tile::kTile;
     const long long grid = (long long)E * tiles_m * tiles_n;
     if (grid >= (1ll << 31)) return HK_ERR_BAD_SHAPE;
-    auto kern = grouped_wgrad_kernel<T>;
+    auto kern = grouped_wgrad_kernel<Tile, T>;
     static DeviceOnce configured;
-    if (!set_lds_limit_once((const void*)kern, kLayoutLdsBytes, configured)) return HK_ERR_LAUNCH;
-    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), kLayoutLdsBytes, s, (const uint16_t*)dy, (const uint16_t*)x, offsets,
+    if (!set_lds_limit_once((const void*)kern, Tile::kLds, configured)) return HK_ERR_LAUNCH;
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), Tile::kLds, s, (const uint16_t*)dy, (const uint16_t*)x, offsets,
                        (T*)dW, R, E, N, K, tiles_m, tiles_n);
     return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
+}
+template <typename T>
+static int launch_wgrad(const void* dy, const void* x, const int32_t* offsets, void* dW, int R, int E, int N, int K, hipStream_t s) {
+    const double e = E, n256 = (N + 255) / 256, k256 = (K + 255) / 256, n128 = (N + 127) / 128, k128 = (K + 127) / 128;
+    return prefer_tile256(e * n256 * k256, e * n128 * k128, (R / E + kLayoutStep - 1) / kLayoutStep, moe_num_compute_units(), kSmallStepAcross)
+               ? launch_wgrad_tile<LayoutTile256, T>(dy, x, offsets, dW, R, E, N, K, s)
+               : launch_wgrad_tile<LayoutTile128, T>(dy, x, offsets, dW, R, E, N, K, s);
 }
 
 }  // namespace hk

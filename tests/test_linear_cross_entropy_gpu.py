@@ -7,6 +7,8 @@ pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 SHAPES = [(1, 1, 8), (1, 1000, 64), (7, 129, 72), (64, 128, 64), (100, 777, 264), (129, 257, 136), (256, 512, 512),
           (300, 2049, 72), (1025, 1300, 200)]
+# rows, classes and widths at which 256x256 tiles take over in one product or another, dx cut into several pieces of its sum
+LARGE = [(2, 20011, 264), (513, 33000, 520), (2000, 9001, 1032), (3000, 17000, 776)]
 
 
 def _case(M, V, K, seed, label_dtype=torch.int64, spread=2.0, ignored=0.2):
@@ -77,7 +79,7 @@ def _run(hk, x, w, labels, dloss, dw_dtype=torch.bfloat16, workspace=None, want_
     return loss[:M], lse[:M], dx[:M] if want_dx else None, dw[:V] if want_dw else None
 
 
-@pytest.mark.parametrize("M,V,K", SHAPES)
+@pytest.mark.parametrize("M,V,K", SHAPES + LARGE)
 @pytest.mark.parametrize("label_dtype", [torch.int32, torch.int64])
 def test_loss_and_gradients(hk, M, V, K, label_dtype):
     print(f"linear cross entropy M={M} V={V} K={K} {label_dtype}", flush=True)

@@ -38,11 +38,24 @@ def _close(got, want, size, terms, half_step):
     assert torch.isfinite(got).all()
 
 
+# enough tiles for the 256x256 kernels in every product: rows on both sides of a tile, K-steps on both sides of one and two
+LARGE = [([2049, 0, 255, 257, 1, 3000, 63, 65, 129], 3, 2312, 2056), ([4000, 1000, 4500], 0, 1544, 1800), ([9000], 9, 1800, 72)]
+
+
+@pytest.mark.parametrize("case", range(len(LARGE)))
+def test_large_products_and_gradients(hk, case):
+    rows, unused, N, K = LARGE[case]
+    _products_and_gradients(hk, rows, unused, N, K, 1000 + case)
+
+
 @pytest.mark.parametrize("N,K", WIDTHS)
 @pytest.mark.parametrize("case", range(len(ROWS)))
 def test_products_and_gradients(hk, case, N, K):
-    rows, unused = ROWS[case]
-    off, offsets, x, dy, w = _case(rows, unused, N, K, 17 * case + N + K)
+    _products_and_gradients(hk, *ROWS[case], N, K, 17 * case + N + K)
+
+
+def _products_and_gradients(hk, rows, unused, N, K, seed):
+    off, offsets, x, dy, w = _case(rows, unused, N, K, seed)
     R, E = x.shape[0], len(rows)
     print(f"grouped rows={rows[:8]} unused={unused} N={N} K={K}", flush=True)
     y = torch.full((R + 1, N), 777.0, dtype=torch.bfloat16, device=DEV)
