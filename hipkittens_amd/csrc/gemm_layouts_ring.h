@@ -271,12 +271,16 @@ __device__ __forceinline__ void store_patch(const v4f (&acc)[F][F], T* __restric
 }
 
 // The two tiles as the kernels take them: product() leaves acc[F][F] of 16x16 blocks of the wave's patch, rows
-// kPatch (w / 2) and columns kPatch (w % 2) of the tile.
+// kPatch (w / 2) and columns kPatch (w % 2) of the tile; read_row() gives an epilogue one row of blocks.
 struct LayoutTile128 {
     static constexpr int kTile = kLayoutTile, kPatch = kTile / 2, F = 4, kLds = kLayoutLdsBytes;
     template <bool A_ACROSS, bool B_ACROSS>
     static __device__ __forceinline__ void product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K, v4f (&acc)[F][F]) {
         tile_product<A_ACROSS, B_ACROSS>(smem, A, B, K, acc);
+    }
+    static __device__ __forceinline__ void read_row(const v4f (&acc)[F], v4f (&v)[F]) {
+#pragma unroll
+        for (int n = 0; n < F; ++n) v[n] = acc[n];
     }
 };
 struct LayoutTile256 {
@@ -284,6 +288,18 @@ struct LayoutTile256 {
     template <bool A_ACROSS, bool B_ACROSS>
     static __device__ __forceinline__ void product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K, v4f (&acc)[F][F]) {
         ring_product<A_ACROSS, B_ACROSS>(smem, A, B, K, acc);
+    }
+    // One row of blocks out of the accumulation registers, here and no sooner: an epilogue with branches otherwise has the
+    // compiler move all 256 into vector registers at once, and spill.
+    static __device__ __forceinline__ void read_row(const v4f (&acc)[F], v4f (&v)[F]) {
+#pragma unroll
+        for (int n = 0; n < F; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float x;
+                asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(x) : "a"(acc[n][j]));
+                v[n][j] = x;
+            }
     }
 };
 

@@ -9,7 +9,10 @@
 // Forward: one tile product; its epilogue leaves each row's maximum and sum of exponentials over the tile's columns (fp32) and
 // the label's logit, a second launch joins them column block by column block, in order. Backward, for pieces of the vocabulary:
 // the logits again, with dl rounded to bf16 as the epilogue (an operand of the two products that follow, whose other operand
-// is bf16; it adds 2^-9 relative to each term of sums whose result is rounded to bf16), then dx += dl W in fp32 and dW = dl^T x.
+// is bf16), then dx += dl W in fp32 and dW = dl^T x. The rounding is at most 2^-8 of each term, and a row's largest term is most
+// often its label's, scale (p - 1): that one's remainder, r[m], is kept in fp32 and its products r[m] W[label] and r[m] x[m] are
+// added in the epilogues of dx and dW. (Error of dx and dW against 64 bits, relative, with its own rounding of 0.0017: 1111 rows
+// RESID.)
 #include <algorithm>
 
 #include "gemm_layouts_ring.h"
@@ -47,8 +50,7 @@ __global__ __launch_bounds__(256) void head_logits_kernel(const uint16_t* __rest
     for (int m = 0; m < Tile::F; ++m) {
         const int at = row + 16 * m;
         v4f l[Tile::F];
-#pragma unroll
-        for (int n = 0; n < Tile::F; ++n) l[n] = acc[m][n];
+        Tile::read_row(acc[m], l);
         if (left < Tile::kPatch) {   // columns behind V
 #pragma unroll
             for (int n = 0; n < Tile::F; ++n)
@@ -109,15 +111,69 @@ __global__ __launch_bounds__(256) void head_loss_kernel(const float2* __restrict
     }
 }
 
-// dl of the columns [v0, v0 + cols) of the vocabulary; `width` columns of it are written, those behind V as zeros.
+__device__ __forceinline__ float bf16_value(float v) { return __uint_as_float(pack_bf16(0.f, v) & 0xffff0000u); }
+__device__ __forceinline__ v4f bf16_quad(const uint16_t* p) {
+    const v2i q = *(const v2i*)p;
+    return v4f{__uint_as_float((uint32_t)q.x << 16), __uint_as_float((uint32_t)q.x & 0xffff0000u),
+               __uint_as_float((uint32_t)q.y << 16), __uint_as_float((uint32_t)q.y & 0xffff0000u)};
+}
+
+// Rows by the block of 16 classes that holds their label: list = the rows of block 0, of block 1, .. in ascending order,
+// starts[b] = where block b's begin (blocks + 1 entries). One workgroup per 256 classes: the labels below its first class tell
+// where its rows begin, wave w places those of blocks 4 w .. 4 w + 3, by ballots, in order.
+struct HeadRows {
+    int32_t *starts, *list;
+    int groups;   // of 256 classes; 0: not wanted
+};
+__device__ __forceinline__ void head_label_rows(int* counts, const HeadLabels& labels, int M, int V, const HeadRows& rows, int group) {
+    const int lane = lane_id(), w = wave_id(), first = group * 256 + 64 * w;
+    int below = 0, in[4] = {0, 0, 0, 0};
+    for (int m0 = 0; m0 < M; m0 += 64) {
+        const int label = m0 + lane < M ? labels.at(m0 + lane, V) : -1;
+        below += __popcll(__ballot(label >= 0 && label < group * 256));
+#pragma unroll
+        for (int b = 0; b < 4; ++b) in[b] += __popcll(__ballot(label >= first + 16 * b && label < first + 16 * b + 16));
+    }
+    if (lane == 0) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) counts[4 * w + b] = in[b];
+    }
+    __syncthreads();
+    int at[4], run = below;
+#pragma unroll
+    for (int b = 0; b < 16; ++b) {
+        if (b >> 2 == w) at[b & 3] = run;
+        run += counts[b];
+    }
+    if (lane == 0) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) rows.starts[group * 16 + 4 * w + b] = at[b];
+        if (w == 3 && group == rows.groups - 1) rows.starts[rows.groups * 16] = run;
+    }
+    for (int m0 = 0; m0 < M; m0 += 64) {
+        const int label = m0 + lane < M ? labels.at(m0 + lane, V) : -1;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const bool mine = label >= first + 16 * b && label < first + 16 * b + 16;
+            const uint64_t all = __ballot(mine);
+            if (mine) rows.list[at[b] + __popcll(all & ((1ull << lane) - 1ull))] = m0 + lane;
+            at[b] += __popcll(all);
+        }
+    }
+}
+
+// dl of the columns [v0, v0 + cols) of the vocabulary; `width` columns of it are written, those behind V as zeros. The first
+// `rows.groups` workgroups sort the rows by label for the launch behind this one.
 template <typename Tile>
 __global__ __launch_bounds__(256) void head_dlogits_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ W,
                                                            HeadLabels labels, const float* __restrict__ lse,
                                                            const float* __restrict__ dloss, int M, int V, int K, int v0, int width,
-                                                           int pitch, int tiles_m, int tiles_n, uint16_t* __restrict__ dl) {
+                                                           int pitch, int tiles_m, int tiles_n, uint16_t* __restrict__ dl,
+                                                           float* __restrict__ resid, HeadRows rows) {
     extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
+    if ((int)blockIdx.x < rows.groups) return head_label_rows((int*)smem, labels, M, V, rows, blockIdx.x);
     int pm, pn;
-    grouped_raster(xcd_chunk_order(blockIdx.x, tiles_m * tiles_n, kCuPerXcd), tiles_m, tiles_n, 8, pm, pn);
+    grouped_raster(xcd_chunk_order(blockIdx.x - rows.groups, tiles_m * tiles_n, kCuPerXcd), tiles_m, tiles_n, 8, pm, pn);
     const int w = wave_id(), row0 = pm * Tile::kTile, col0 = v0 + pn * Tile::kTile;
     v4f acc[Tile::F][Tile::F];
     Tile::template product<false, false>(smem, operand_along(x, 2ull * K, row0, min(M, row0 + Tile::kTile), K),
@@ -130,15 +186,23 @@ __global__ __launch_bounds__(256) void head_dlogits_kernel(const uint16_t* __res
         const int label = at < M ? labels.at(at, V) : -1;
         const float scale = label >= 0 ? dloss[at] : 0.f, lse2 = label >= 0 ? lse[at] * kLog2e : 0.f;
         v4f d[Tile::F];
+        Tile::read_row(acc[m], d);
 #pragma unroll
         for (int n = 0; n < Tile::F; ++n)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) d[n][j] = scale * __builtin_amdgcn_exp2f(__builtin_fmaf(acc[m][n][j], kLog2e, -lse2));
-        if (__any(label >= col && label < col + Tile::kPatch)) {
+            for (int j = 0; j < 4; ++j) d[n][j] = scale * __builtin_amdgcn_exp2f(__builtin_fmaf(d[n][j], kLog2e, -lse2));
+        const bool here = label >= col && label < col + Tile::kPatch && ((label >> 2) & 3) == g;   // among this lane's
+        if (__any(here)) {
+            float rest = 0.f;
 #pragma unroll
             for (int n = 0; n < Tile::F; ++n)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) d[n][j] -= label == col + 16 * n + 4 * g + j ? scale : 0.f;
+                for (int j = 0; j < 4; ++j) {
+                    const bool hot = label == col + 16 * n + 4 * g + j;
+                    d[n][j] -= hot ? scale : 0.f;
+                    rest = hot ? d[n][j] - bf16_value(d[n][j]) : rest;
+                }
+            if (here) resid[at] = rest;
         }
         if (left < Tile::kPatch || __any(label < 0)) {   // zeros, not products with zero
 #pragma unroll
@@ -157,6 +221,9 @@ __global__ __launch_bounds__(256) void head_dlogits_kernel(const uint16_t* __res
 struct HeadPiece {
     const uint16_t *dl, *W, *x;
     float* sums;      // [splits][M][K]: dx so far, when there are several pieces or splits
+    HeadLabels labels;
+    const float* resid;              // r[m], of the rows whose label lies in this piece or an earlier one
+    const int32_t *starts, *list;    // rows by their label's block of 16 classes
     uint16_t* dx;
     int M, V, K, v0, cols, pitch;
     int tiles_m, tiles_k, tiles_v, splits, split_cols;   // splits 0: no dx; tiles_v 0: no dW
@@ -180,13 +247,23 @@ __device__ __forceinline__ void head_dx_item(uint8_t* smem, const HeadPiece& p, 
     for (int m = 0; m < Tile::F; ++m) {
         const int at = row + 16 * m + r;
         v4f v[Tile::F];
+        Tile::read_row(acc[m], v);
 #pragma unroll
         for (int c = 0; c < Tile::F; ++c) {
-            v[c] = acc[m][c];
             if (!p.first && at < p.M && col + 16 * c + 4 * g < p.K) v[c] += *(const v4f*)(sums + (size_t)at * p.K + col + 16 * c + 4 * g);
         }
-        if (p.last && !p.reduce) store_block_row(v, m, p.dx + (size_t)row * p.K + col, p.K, p.M - row, p.K - col);
-        else store_block_row(v, m, sums + (size_t)row * p.K + col, p.K, p.M - row, p.K - col);
+        if (p.last && !p.reduce) {
+            const int label = at < p.M ? p.labels.at(at, p.V) : -1;
+            if (label >= 0) {
+                const float rest = p.resid[at];
+#pragma unroll
+                for (int c = 0; c < Tile::F; ++c)
+                    if (col + 16 * c + 4 * g < p.K) v[c] += rest * bf16_quad(p.W + (size_t)label * p.K + col + 16 * c + 4 * g);
+            }
+            store_block_row(v, m, p.dx + (size_t)row * p.K + col, p.K, p.M - row, p.K - col);
+        } else {
+            store_block_row(v, m, sums + (size_t)row * p.K + col, p.K, p.M - row, p.K - col);
+        }
         slot_fence();
     }
 }
@@ -201,19 +278,76 @@ __global__ __launch_bounds__(256) void head_gradients_kernel(HeadPiece p, T* __r
     }
     int pm, pn;
     grouped_raster(xcd_chunk_order(blockIdx.x - dx_items, p.tiles_v * p.tiles_k, kCuPerXcd), p.tiles_v, p.tiles_k, 8, pm, pn);
+    const int lane = lane_id(), r = lane & 15, g = lane >> 4;
     const int w = wave_id(), row0 = pm * Tile::kTile, col0 = pn * Tile::kTile;
+    const int row = row0 + (w >> 1) * Tile::kPatch, col = col0 + (w & 1) * Tile::kPatch;
+    // The rows with a label among this wave's classes, in the order of their blocks: the first 64 of them, one per lane, with label
+    // and remainder, before the product.
+    const int block0 = (p.v0 + row) / 16, blocks = min(Tile::F, max(0, (p.cols - row + 15) / 16));
+    const int begin = blocks ? to_sgpr(p.starts[block0]) : 0, count = blocks ? to_sgpr(p.starts[block0 + blocks]) - begin : 0;
+    int my_row = 0, my_label = -1;
+    float my_rest = 0.f;
+    auto entries = [&](int first) {
+        if (first + lane < count) {
+            my_row = p.list[begin + first + lane];
+            my_label = p.labels.at(my_row, p.V);
+            my_rest = p.resid[my_row];
+        }
+    };
+    entries(0);
     v4f acc[Tile::F][Tile::F];
     Tile::template product<true, true>(smem, operand_across(p.dl, 2ull * p.pitch, row0, p.M), operand_across(p.x, 2ull * p.K, col0, p.M), p.M, acc);
-    const int row = row0 + (w >> 1) * Tile::kPatch, col = col0 + (w & 1) * Tile::kPatch;
-    store_patch(acc, dw + (size_t)row * p.K + col, p.K, p.cols - row, p.K - col);
+    // Their columns of x, 64 rows at a time, in this wave's part of the LDS that the product is done with, several rows
+    // under way at once. (One row after another, a latency each: 8192 rows and 129280 classes, 8 entries a wave, 30 us a tile.)
+    constexpr int kRowBytes = 2 * Tile::kPatch, kLanes = kRowBytes / 16, kAtOnce = 64 / kLanes;   // lanes of a row, rows of a load
+    block_barrier();
+    uint8_t* mine = smem + w * 64 * kRowBytes;
+    auto stage = [&](int first) {
+        const int n = min(64, count - first), piece = lane % kLanes * 8;
+        for (int e0 = 0; e0 < n; e0 += 4 * kAtOnce) {
+            v4i q[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int e = e0 + i * kAtOnce + lane / kLanes, at = __shfl(my_row, e & 63, 64);
+                q[i] = v4i{0, 0, 0, 0};
+                if (e < n && col + piece < p.K) q[i] = *(const v4i*)(p.x + (size_t)at * p.K + col + piece);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) *(v4i*)(mine + (e0 / kAtOnce + i) * 1024 + lane * 16) = q[i];
+        }
+    };
+    if (count > 0) stage(0);
+    int next = 0;
+#pragma unroll
+    for (int m = 0; m < Tile::F; ++m) {
+        v4f v[Tile::F];
+        Tile::read_row(acc[m], v);
+        while (next < count) {
+            const int label = __builtin_amdgcn_readlane(my_label, next & 63);
+            if (label / 16 != block0 + m) break;
+            const float rest = (label & 15) == r ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(my_rest), next & 63)) : 0.f;
+#pragma unroll
+            for (int c = 0; c < Tile::F; ++c) v[c] += rest * bf16_quad((const uint16_t*)(mine + (next & 63) * kRowBytes) + 16 * c + 4 * g);
+            if ((++next & 63) == 0 && next < count) {
+                entries(next);
+                stage(next);
+            }
+        }
+        store_block_row(v, m, dw + (size_t)row * p.K + col, p.K, p.cols - row, p.K - col);
+        slot_fence();
+    }
 }
 
-// dx = the splits' sums, added in order (n = M K, a multiple of 8).
-__global__ __launch_bounds__(256) void head_dx_reduce_kernel(const float* __restrict__ sums, int splits, size_t n, uint16_t* __restrict__ dx) {
-    const size_t at = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
+// dx = the splits' sums, added in order, and the label's remainder (a thread: four columns of a row; K a multiple of 8).
+__global__ __launch_bounds__(256) void head_dx_reduce_kernel(const float* __restrict__ sums, int splits, int M, int V, int K, HeadLabels labels,
+                                                             const float* __restrict__ resid, const uint16_t* __restrict__ W,
+                                                             uint16_t* __restrict__ dx) {
+    const size_t n = (size_t)M * K, at = ((size_t)blockIdx.x * 256 + threadIdx.x) * 4;
     if (at >= n) return;
+    const int m = (int)(at / K), label = labels.at(m, V);
     v4f v = *(const v4f*)(sums + at);
     for (int s = 1; s < splits; ++s) v += *(const v4f*)(sums + (size_t)s * n + at);
+    if (label >= 0) v += resid[m] * bf16_quad(W + (size_t)label * K + (at - (size_t)m * K));
     *(v2i*)(dx + at) = v2i{(int)pack_bf16(v.x, v.y), (int)pack_bf16(v.z, v.w)};
 }
 
@@ -242,7 +376,7 @@ struct HeadBackwardPlan {
     int piece;   // columns of a piece, a multiple of 256
     bool logits256, grads256;
     int splits, split_cols;
-    size_t dl, sums, bytes;
+    size_t resid, starts, list, dl, sums, bytes;
     HeadBackwardPlan(int M, int V, int K) {
         // pieces of 256 MB, and rows of at most 4 MB (32-bit offsets inside a K-step's rows)
         const long long most = std::min((256ll << 20) / (2ll * M), 1ll << 21) / 256 * 256, all = (long long)tiles_of(V, 256) * 256;
@@ -262,8 +396,11 @@ struct HeadBackwardPlan {
         splits = tiles_of(steps_v, per_split);
         split_cols = tiles_of(steps_v, splits) * kLayoutStep;
         splits = tiles_of(cols, split_cols);
-        dl = 0;
-        sums = up256((size_t)M * piece * 2);
+        resid = 0;
+        list = up256((size_t)M * 4);
+        starts = list + up256((size_t)M * 4);
+        dl = starts + up256(((size_t)tiles_of(V, 256) * 16 + 1) * 4);
+        sums = dl + up256((size_t)M * piece * 2);
         bytes = sums + (piece < V || splits > 1 ? up256((size_t)splits * M * K * 4) : 0);
     }
 };
@@ -292,11 +429,11 @@ static int launch_logits(const uint16_t* x, const uint16_t* W, HeadLabels labels
 }
 template <typename Tile>
 static int launch_dlogits(const uint16_t* x, const uint16_t* W, HeadLabels labels, const float* lse, const float* dloss, int M, int V, int K,
-                          int v0, int cols, int pitch, uint16_t* dl, hipStream_t s) {
+                          int v0, int cols, int pitch, uint16_t* dl, float* resid, HeadRows rows, hipStream_t s) {
     static DeviceOnce once;
     const int tm = tiles_of(M, Tile::kTile), tv = tiles_of(cols, Tile::kTile);
-    return launch_head<Tile>(head_dlogits_kernel<Tile>, once, (long long)tm * tv, s, x, W, labels, lse, dloss, M, V, K, v0, (cols + 7) / 8 * 8,
-                             pitch, tm, tv, dl);
+    return launch_head<Tile>(head_dlogits_kernel<Tile>, once, (long long)tm * tv + rows.groups, s, x, W, labels, lse, dloss, M, V, K, v0,
+                             (cols + 7) / 8 * 8, pitch, tm, tv, dl, resid, rows);
 }
 template <typename Tile, typename T>
 static int launch_gradients(HeadPiece p, bool dx, T* dw, hipStream_t s) {
@@ -358,15 +495,18 @@ extern "C" int hk_linear_cross_entropy_backward(const void* x_bf16, const void* 
     const uint16_t *x = (const uint16_t*)x_bf16, *w = (const uint16_t*)w_bf16;
     uint16_t* dl = (uint16_t*)(ws + L.dl);
     const bool want_dx = dx_bf16_or_null != nullptr;
-    HeadPiece p{dl, w, x, (float*)(ws + L.sums), (uint16_t*)dx_bf16_or_null, M, V, K, 0, 0, L.piece, 0, 0, 0, 0, L.split_cols,
+    float* resid = (float*)(ws + L.resid);
+    int32_t *starts = (int32_t*)(ws + L.starts), *list = (int32_t*)(ws + L.list);
+    HeadPiece p{dl, w, x, (float*)(ws + L.sums), lab, resid, starts, list, (uint16_t*)dx_bf16_or_null, M, V, K, 0, 0, L.piece, 0, 0, 0, 0, L.split_cols,
                 false, false, L.splits > 1};
     for (int v0 = 0; v0 < V; v0 += L.piece) {
         p.v0 = v0;
         p.cols = V - v0 < L.piece ? V - v0 : L.piece;
         p.first = v0 == 0;
         p.last = v0 + p.cols == V;
-        int st = L.logits256 ? launch_dlogits<LayoutTile256>(x, w, lab, lse, dloss, M, V, K, v0, p.cols, L.piece, dl, s)
-                             : launch_dlogits<LayoutTile128>(x, w, lab, lse, dloss, M, V, K, v0, p.cols, L.piece, dl, s);
+        const HeadRows rows{starts, list, dw_or_null && v0 == 0 ? tiles_of(V, 256) : 0};
+        int st = L.logits256 ? launch_dlogits<LayoutTile256>(x, w, lab, lse, dloss, M, V, K, v0, p.cols, L.piece, dl, resid, rows, s)
+                             : launch_dlogits<LayoutTile128>(x, w, lab, lse, dloss, M, V, K, v0, p.cols, L.piece, dl, resid, rows, s);
         if (st != HK_OK) return st;
         if (dw_type == 0)
             st = L.grads256 ? launch_gradients<LayoutTile256>(p, want_dx, (uint16_t*)dw_or_null, s)
@@ -380,7 +520,7 @@ extern "C" int hk_linear_cross_entropy_backward(const void* x_bf16, const void* 
     if (want_dx && L.splits > 1) {
         const size_t n = (size_t)M * K;
         hipLaunchKernelGGL(head_dx_reduce_kernel, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, s, (const float*)(ws + L.sums),
-                           L.splits, n, (uint16_t*)dx_bf16_or_null);
+                           L.splits, M, V, K, lab, (const float*)resid, w, (uint16_t*)dx_bf16_or_null);
         if (hipGetLastError() != hipSuccess) return HK_ERR_LAUNCH;
     }
     return HK_OK;

@@ -45,12 +45,12 @@ def _reference(x, w, labels, dloss):
     hot[counts, at[counts]] = 1.0
     scale = torch.where(counts, dloss.double(), 0.0)[:, None]
     dl = scale * (p - hot)
-    # p is off by its exponent's error, the difference by a step of fp32 of its larger side, dl by half a step of bf16
+    # p is off by its exponent's error, the difference by a step of fp32 of its larger side, dl by half a step of bf16 but for the label's
     d = scale.abs() * (p * (dl_err + lse_err[:, None] + 2**-19) + (p + hot) * 2**-22)
     # fp32 and bf16 hold no normal number below 2^-126: an exponential, a dl, a product or a sum below it may come out as 0
     # (a logit 88 below lse: p < 2^-126), once each
     tiny = 2.0**-126
-    d = d + (dl.abs() + d) * 2**-8 + (scale.abs() + 1) * tiny
+    d = d + (dl.abs() + d) * 2**-8 * (1 - hot) + (scale.abs() + 1) * tiny   # the label's remainder is kept: no half step there
     dx, dw = dl @ wd, dl.t().contiguous() @ xd
     dx_err = d @ wd.abs() + (dl.abs() @ wd.abs()) * 2 * (V + 8) * 2**-24 + 2 * (V + 1) * tiny
     dw_err = d.t().contiguous() @ xd.abs() + (dl.abs().t().contiguous() @ xd.abs()) * 2 * (M + 8) * 2**-24 + 2 * (M + 1) * tiny
@@ -131,6 +131,26 @@ def test_every_row_ignored_and_rows_that_do_not_count(hk):
     rest[20:22] = False
     assert torch.isnan(loss[20]) and torch.isnan(lse[20]) and torch.isnan(dx[20]).all() and not torch.isfinite(loss[21])
     assert torch.equal(loss[rest], clean[0][rest]) and torch.equal(dx[rest], clean[2][rest])
+
+
+@pytest.mark.parametrize("M,V,K", [(700, 300, 72), (2100, 17000, 776)])
+def test_labels_that_crowd_a_few_classes(hk, M, V, K):
+    """Hundreds of rows with one label, and more than 64 among the classes of one wave: none in the blocks around them."""
+    print(f"linear cross entropy, crowded labels M={M} V={V} K={K}", flush=True)
+    x, w, labels, dloss = _case(M, V, K, 12)
+    kind = torch.arange(M, device=DEV) % 3
+    labels = torch.where(kind == 0, 37, torch.where(kind == 1, V - 1 - torch.arange(M, device=DEV) % 130, labels))
+    lse_r, loss_r, dx_r, dw_r, _ = _reference(x, w, labels, dloss)
+    loss, lse, dx, dw = _run(hk, x, w, labels, dloss, torch.float32)
+    _within(loss, *loss_r)
+    _within(dx, *dx_r, 2**-8)
+    _within(dw, *dw_r, 2**-24)
+    # every label the same
+    same = torch.full_like(labels, V // 2)
+    _, _, dx_r, dw_r, _ = _reference(x, w, same, dloss)
+    _, _, dx, dw = _run(hk, x, w, same, dloss, torch.float32)
+    _within(dx, *dx_r, 2**-8)
+    _within(dw, *dw_r, 2**-24)
 
 
 def test_one_gradient_alone_has_the_same_bits(hk):
