@@ -1,4 +1,4 @@
-// The GEMM dispatchers' argument checks and launches for ordinary arguments, as a CPython module (`_dispatch`).
+// The dispatchers' argument checks and launches (GEMMs, the MoE layers' rows and products in training) for ordinary arguments, as a CPython module (`_dispatch`).
 //
 // A launch takes the runtime about 3 us; the same checks in Python, a call through ctypes and the attribute reads for it
 // took 3 (FP8, BF16) to 6 us (MXFP4 with a workspace: six tensors) on top, which is what a GEMM of a few microseconds
@@ -16,6 +16,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cstring>
 #include <limits>
 
 #include "../../include/hk355.h"
@@ -32,19 +33,25 @@ struct Entries {
     decltype(&hk_mxfp4_gemm_ws) mxfp4_ws;
     decltype(&hk_mxfp4_gemm_pitched) mxfp4_pitched;
     decltype(&hk_mxfp4_quantize_rows) mxfp4_quantize;
+    decltype(&hk_moe_permute) permute;
+    decltype(&hk_moe_permute_backward) permute_backward;
+    decltype(&hk_moe_unpermute_backward) unpermute_backward;
+    decltype(&hk_moe_grouped_gemm) grouped;
+    decltype(&hk_moe_grouped_gemm_dgrad) grouped_dgrad;
+    decltype(&hk_moe_grouped_gemm_wgrad) grouped_wgrad;
 };
 Entries entries{};
 PyTypeObject* parameter_type = nullptr;
 
 struct Operand {
     void* data;
-    int64_t rows, cols;   // cols of a vector: its length
+    int64_t outer, rows, cols;   // cols of a vector: its length; outer: matrices of a stack
     int device;
 };
 
 using Types = std::initializer_list<at::ScalarType>;
 
-// A plain contiguous GPU tensor of `ndim` dimensions (1 or 2) and one of `types`, nothing around its memory.
+// A plain contiguous GPU tensor of `ndim` dimensions (1 to 3) and one of `types`, nothing around its memory.
 bool operand(PyObject* o, Types types, int ndim, Operand& out) {
     if (Py_TYPE(o) != reinterpret_cast<PyTypeObject*>(THPVariableClass) && Py_TYPE(o) != parameter_type) return false;
     const at::Tensor& t = THPVariable_Unpack(o);
@@ -59,11 +66,12 @@ bool operand(PyObject* o, Types types, int ndim, Operand& out) {
     for (const at::ScalarType s : types) known = known || s == type;
     if (!known) return false;
     const auto sizes = t.sizes();
-    out.rows = ndim == 2 ? sizes[0] : 1;
+    out.outer = ndim == 3 ? sizes[0] : 1;
+    out.rows = ndim >= 2 ? sizes[ndim - 2] : 1;
     out.cols = sizes[ndim - 1];
     out.device = t.device().index();
     constexpr int64_t kMax = std::numeric_limits<int>::max();
-    if (out.rows > kMax || (ndim == 2 && out.cols > kMax / 2)) return false;
+    if (out.outer > kMax || out.rows > kMax || (ndim >= 2 && out.cols > kMax / 2)) return false;
     out.data = t.data_ptr();
     return true;
 }
@@ -168,25 +176,119 @@ PyObject* mxfp4_quantize_rows(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
+constexpr Types kF32{at::kFloat}, kI32{at::kInt};
+// The training entry points ask the runtime about the current device (compute units, LDS limits): calls for another one are
+// left to Python, which makes it the current one.
+bool current(int device) { return device == static_cast<int>(c10::hip::current_device()); }
+// rows [T k, H] and slot_to_pos [T k] of tokens [T, H]
+bool routed_rows(const Operand& tokens, const Operand& rows, const Operand& pos) {
+    return tokens.rows > 0 && rows.rows > 0 && rows.rows % tokens.rows == 0 && rows.cols == tokens.cols && pos.cols == rows.rows &&
+           rows.device == tokens.device && pos.device == tokens.device && current(tokens.device);
+}
+
+// (x, slot_to_pos, xp)
+PyObject* moe_permute(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Operand x, pos, xp;
+        if (n != 3 || !operand(args[0], kBf16, 2, x) || !operand(args[1], kI32, 1, pos) || !operand(args[2], kBf16, 2, xp) ||
+            !routed_rows(x, xp, pos))
+            Py_RETURN_NONE;
+        void* s = stream_of(x.device);
+        return launch([&] {
+            return entries.permute(x.data, (const int32_t*)pos.data, (int)x.rows, (int)(xp.rows / x.rows), (int)x.cols, xp.data, s);
+        });
+    });
+}
+
+// (dxp, slot_to_pos, dx, add or None)
+PyObject* moe_permute_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Operand dxp, pos, dx, add{};
+        if (n != 4 || !operand(args[0], kBf16, 2, dxp) || !operand(args[1], kI32, 1, pos) || !operand(args[2], kBf16, 2, dx) ||
+            !routed_rows(dx, dxp, pos) ||
+            (args[3] != Py_None && (!operand(args[3], kBf16, 2, add) || add.rows != dx.rows || add.cols != dx.cols || add.device != dx.device)))
+            Py_RETURN_NONE;
+        void* s = stream_of(dx.device);
+        return launch([&] {
+            return entries.permute_backward(dxp.data, (const int32_t*)pos.data, (int)dx.rows, (int)(dxp.rows / dx.rows), (int)dx.cols,
+                                            args[3] != Py_None ? add.data : nullptr, dx.data, s);
+        });
+    });
+}
+
+// (dy, o, weights, slot_to_pos, do, dweights)
+PyObject* moe_unpermute_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Operand dy, o, w, pos, d_o, dw;
+        if (n != 6 || !operand(args[0], kBf16, 2, dy) || !operand(args[1], kBf16, 2, o) || !operand(args[2], kF32, 2, w) ||
+            !operand(args[3], kI32, 1, pos) || !operand(args[4], kBf16, 2, d_o) || !operand(args[5], kF32, 2, dw) ||
+            !routed_rows(dy, o, pos) || d_o.rows != o.rows || d_o.cols != o.cols || w.rows != dy.rows || w.rows * w.cols != o.rows ||
+            dw.rows != w.rows || dw.cols != w.cols || w.device != dy.device || d_o.device != dy.device || dw.device != dy.device)
+            Py_RETURN_NONE;
+        void* s = stream_of(dy.device);
+        return launch([&] {
+            return entries.unpermute_backward(dy.data, o.data, (const float*)w.data, (const int32_t*)pos.data, (int)dy.rows, (int)w.cols,
+                                              (int)dy.cols, d_o.data, (float*)dw.data, s);
+        });
+    });
+}
+
+// rows_n [R, N], rows_k [R, K], w [E, N, K], offsets [E + 1]
+bool grouped_shapes(const Operand& rows_n, const Operand& rows_k, const Operand& w, const Operand& offsets) {
+    return rows_n.rows == rows_k.rows && rows_n.cols == w.rows && rows_k.cols == w.cols && offsets.cols == w.outer + 1 &&
+           rows_k.device == rows_n.device && w.device == rows_n.device && offsets.device == rows_n.device && current(rows_n.device);
+}
+// (x, w, expert_offsets, y) and (dy, w, expert_offsets, dx)
+template <bool DGRAD>
+PyObject* grouped(PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Operand in, w, offsets, out;
+        if (n != 4 || !operand(args[0], kBf16, 2, in) || !operand(args[1], kBf16, 3, w) || !operand(args[2], kI32, 1, offsets) ||
+            !operand(args[3], kBf16, 2, out) || !grouped_shapes(DGRAD ? in : out, DGRAD ? out : in, w, offsets))
+            Py_RETURN_NONE;
+        void* s = stream_of(in.device);
+        return launch([&] {
+            return (DGRAD ? entries.grouped_dgrad : entries.grouped)(in.data, w.data, (const int32_t*)offsets.data, out.data, (int)in.rows,
+                                                                     (int)w.outer, (int)w.rows, (int)w.cols, s);
+        });
+    });
+}
+PyObject* moe_grouped_gemm(PyObject*, PyObject* const* args, Py_ssize_t n) { return grouped<false>(args, n); }
+PyObject* moe_grouped_gemm_dgrad(PyObject*, PyObject* const* args, Py_ssize_t n) { return grouped<true>(args, n); }
+// (dy, x, expert_offsets, dw)
+PyObject* moe_grouped_gemm_wgrad(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Operand dy, x, offsets, dw;
+        if (n != 4 || !operand(args[0], kBf16, 2, dy) || !operand(args[1], kBf16, 2, x) || !operand(args[2], kI32, 1, offsets)) Py_RETURN_NONE;
+        const bool fp32 = operand(args[3], kF32, 3, dw);
+        if ((!fp32 && !operand(args[3], kBf16, 3, dw)) || !grouped_shapes(dy, x, dw, offsets)) Py_RETURN_NONE;
+        void* s = stream_of(dy.device);
+        return launch([&] {
+            return entries.grouped_wgrad(dy.data, x.data, (const int32_t*)offsets.data, dw.data, fp32 ? 1 : 0, (int)dy.rows, (int)dw.outer,
+                                         (int)dw.rows, (int)dw.cols, s);
+        });
+    });
+}
+
 // The library's functions by address, in the order of Entries.
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
-    void* p[8];
-    if (n != 8) return PyErr_Format(PyExc_TypeError, "bind: 8 addresses");
-    for (int i = 0; i < 8; ++i) {
+    constexpr int kCount = sizeof(Entries) / sizeof(void*);
+    void* p[kCount];
+    if (n != kCount) return PyErr_Format(PyExc_TypeError, "bind: %d addresses", kCount);
+    for (int i = 0; i < kCount; ++i) {
         p[i] = PyLong_AsVoidPtr(args[i]);
         if (!p[i]) return PyErr_Occurred() ? nullptr : PyErr_Format(PyExc_ValueError, "bind: null address");
     }
-    entries = {reinterpret_cast<decltype(Entries::fp8)>(p[0]), reinterpret_cast<decltype(Entries::fp8_ws)>(p[1]),
-               reinterpret_cast<decltype(Entries::bf16)>(p[2]), reinterpret_cast<decltype(Entries::bf16_ws)>(p[3]),
-               reinterpret_cast<decltype(Entries::mxfp4)>(p[4]), reinterpret_cast<decltype(Entries::mxfp4_ws)>(p[5]),
-               reinterpret_cast<decltype(Entries::mxfp4_pitched)>(p[6]),
-               reinterpret_cast<decltype(Entries::mxfp4_quantize)>(p[7])};
+    static_assert(sizeof(Entries) == sizeof(p));
+    std::memcpy(&entries, p, sizeof(p));
     Py_RETURN_NONE;
 }
 
 #define HK_METHOD(NAME) {#NAME, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(NAME)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {HK_METHOD(bind), HK_METHOD(fp8_gemm), HK_METHOD(bf16_gemm), HK_METHOD(mxfp4_gemm),
-                         HK_METHOD(mxfp4_quantize_rows), {nullptr, nullptr, 0, nullptr}};
+                         HK_METHOD(mxfp4_quantize_rows), HK_METHOD(moe_permute), HK_METHOD(moe_permute_backward),
+                         HK_METHOD(moe_unpermute_backward), HK_METHOD(moe_grouped_gemm), HK_METHOD(moe_grouped_gemm_dgrad),
+                         HK_METHOD(moe_grouped_gemm_wgrad), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_dispatch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -37,11 +37,11 @@ __device__ __forceinline__ v2i lds_read_tr(uint32_t addr) {
     return __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t*)(uintptr_t)addr));
 }
 
-// Tile product of four waves, each a quarter (TILE / 2 square) of TILE x TILE, two LDS stages: the next K-step is loaded
-// while this one is multiplied. acc[m][n] holds, for tile row 16 m + lane % 16 of the wave's quarter, its columns
+// Tile product of four waves, each a quarter (TILE / 2 square) of TILE x TILE. Two LDS stages: the next K-step is loaded while this
+// one is multiplied, two workgroups on a CU. One: each K-step in turn, four workgroups on a CU, for contractions of a few K-steps. acc[m][n] holds, for tile row 16 m + lane % 16 of the wave's quarter, its columns
 // 16 n + 4 (lane / 16) .. +4.
 constexpr int kLayoutTile = 128;
-constexpr int kLayoutLdsBytes = 2 * 2 * kLayoutTile * 128;
+constexpr int kLayoutStageBytes = 2 * kLayoutTile * 128;
 
 template <bool ACROSS>
 struct TileLoader {
@@ -101,7 +101,7 @@ __device__ __forceinline__ Frag4 tile_fragment(uint32_t tile, int first, int f) 
     return out;
 }
 
-template <bool A_ACROSS, bool B_ACROSS>
+template <bool A_ACROSS, bool B_ACROSS, int STAGES>
 __device__ __forceinline__ void tile_product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K,
                                              v4f (&acc)[4][4]) {
     constexpr uint32_t kOperand = kLayoutTile * 128, kStage = 2 * kOperand;
@@ -119,15 +119,21 @@ __device__ __forceinline__ void tile_product(uint8_t* smem, const TileOperand& A
         lb.load(0, mine + kOperand);
     }
     for (int kt = 0; kt < nk; ++kt) {
+        if (STAGES == 1 && kt > 0) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            block_barrier();   // everyone has read the one stage
+            la.load(kt, mine);
+            lb.load(kt, mine + kOperand);
+        }
         wait_vmcnt<0>();   // this wave's part of K-step kt has landed ...
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         block_barrier();   // ... everyone's, and everyone has read the other stage
-        if (kt + 1 < nk) {
+        if (STAGES == 2 && kt + 1 < nk) {
             const uint32_t next = mine + (uint32_t)((kt + 1) & 1) * kStage;
             la.load(kt + 1, next);
             lb.load(kt + 1, next + kOperand);
         }
-        const uint32_t at = lds0 + (uint32_t)(kt & 1) * kStage;
+        const uint32_t at = lds0 + (STAGES == 2 ? (uint32_t)(kt & 1) * kStage : 0u);
         Frag4 b[4];
 #pragma unroll
         for (int n = 0; n < 4; ++n) b[n] = tile_fragment<B_ACROSS>(at + kOperand, wn * 64, n);

@@ -272,17 +272,19 @@ __device__ __forceinline__ void store_patch(const v4f (&acc)[F][F], T* __restric
 
 // The two tiles as the kernels take them: product() leaves acc[F][F] of 16x16 blocks of the wave's patch, rows
 // kPatch (w / 2) and columns kPatch (w % 2) of the tile; read_row() gives an epilogue one row of blocks.
-struct LayoutTile128 {
-    static constexpr int kTile = kLayoutTile, kPatch = kTile / 2, F = 4, kLds = kLayoutLdsBytes;
+template <int STAGES>
+struct LayoutTile128Stages {
+    static constexpr int kTile = kLayoutTile, kPatch = kTile / 2, F = 4, kLds = STAGES * kLayoutStageBytes;
     template <bool A_ACROSS, bool B_ACROSS>
     static __device__ __forceinline__ void product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K, v4f (&acc)[F][F]) {
-        tile_product<A_ACROSS, B_ACROSS>(smem, A, B, K, acc);
+        tile_product<A_ACROSS, B_ACROSS, STAGES>(smem, A, B, K, acc);
     }
     static __device__ __forceinline__ void read_row(const v4f (&acc)[F], v4f (&v)[F]) {
 #pragma unroll
         for (int n = 0; n < F; ++n) v[n] = acc[n];
     }
 };
+typedef LayoutTile128Stages<2> LayoutTile128;
 struct LayoutTile256 {
     static constexpr int kTile = kRingTile, kPatch = kTile / 2, F = 8, kLds = kRingLdsBytes;
     template <bool A_ACROSS, bool B_ACROSS>
@@ -309,7 +311,7 @@ struct LayoutTile256 {
 // weights with 3, 9 and 33 K-steps 660, 1167, 3013 / 628, 1290, 3738; small_step: the small kernel's K-step, which the gradient of
 // the weights (both operands in runs of 256 bytes) takes faster than the others.
 constexpr double kSmallStepAlong = 1.1, kSmallStepAcross = 0.945;
-inline bool prefer_tile256(double tiles256, double tiles128, int k_steps, int cus, double small_step = kSmallStepAlong) {
+inline bool prefer_tile256(double tiles256, double tiles128, double k_steps, int cus, double small_step = kSmallStepAlong) {
     auto rounds = [](double tiles, double at_once) { return tiles <= at_once ? 1.0 : tiles / at_once + 0.2; };
     return rounds(tiles256, cus) * (7.0 + 1.43 * k_steps) < rounds(tiles128, 2.0 * cus) * (2.7 + small_step * k_steps);
 }

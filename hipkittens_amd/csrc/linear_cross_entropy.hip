@@ -23,6 +23,10 @@ namespace hk {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
+// Tile rows of a raster group, as the BF16 GEMM takes them: bands where the operands do not fit the memory-side cache (us, without /
+// with: forward 8192 x 129280 x 7168 10957 / 10600, 4096 x 201088 x 2880 3555 / 3522, backward of the first 33689 / 32919).
+__device__ __forceinline__ int head_group(int band_n, int tiles_n) { return band_n < tiles_n ? 4 : 8; }
+
 struct HeadLabels {
     const void* p;
     int is64;
@@ -35,11 +39,11 @@ struct HeadLabels {
 
 template <typename Tile>
 __global__ __launch_bounds__(256) void head_logits_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ W,
-                                                          HeadLabels labels, int M, int V, int K, int tiles_m, int tiles_n,
+                                                          HeadLabels labels, int M, int V, int K, int tiles_m, int tiles_n, int band_n,
                                                           float2* __restrict__ partial, float* __restrict__ label_logit) {
     extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
     int pm, pn;
-    grouped_raster(xcd_chunk_order(blockIdx.x, tiles_m * tiles_n, kCuPerXcd), tiles_m, tiles_n, 8, pm, pn);
+    banded_raster(xcd_chunk_order(blockIdx.x, tiles_m * tiles_n, kCuPerXcd), tiles_m, tiles_n, head_group(band_n, tiles_n), band_n, pm, pn);
     const int w = wave_id(), row0 = pm * Tile::kTile, col0 = pn * Tile::kTile;
     v4f acc[Tile::F][Tile::F];
     Tile::template product<false, false>(smem, operand_along(x, 2ull * K, row0, min(M, row0 + Tile::kTile), K),
@@ -168,12 +172,13 @@ template <typename Tile>
 __global__ __launch_bounds__(256) void head_dlogits_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ W,
                                                            HeadLabels labels, const float* __restrict__ lse,
                                                            const float* __restrict__ dloss, int M, int V, int K, int v0, int width,
-                                                           int pitch, int tiles_m, int tiles_n, uint16_t* __restrict__ dl,
+                                                           int pitch, int tiles_m, int tiles_n, int band_n,
+                                                           uint16_t* __restrict__ dl,
                                                            float* __restrict__ resid, HeadRows rows) {
     extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
     if ((int)blockIdx.x < rows.groups) return head_label_rows((int*)smem, labels, M, V, rows, blockIdx.x);
     int pm, pn;
-    grouped_raster(xcd_chunk_order(blockIdx.x - rows.groups, tiles_m * tiles_n, kCuPerXcd), tiles_m, tiles_n, 8, pm, pn);
+    banded_raster(xcd_chunk_order(blockIdx.x - rows.groups, tiles_m * tiles_n, kCuPerXcd), tiles_m, tiles_n, head_group(band_n, tiles_n), band_n, pm, pn);
     const int w = wave_id(), row0 = pm * Tile::kTile, col0 = v0 + pn * Tile::kTile;
     v4f acc[Tile::F][Tile::F];
     Tile::template product<false, false>(smem, operand_along(x, 2ull * K, row0, min(M, row0 + Tile::kTile), K),
@@ -226,7 +231,7 @@ struct HeadPiece {
     const int32_t *starts, *list;    // rows by their label's block of 16 classes
     uint16_t* dx;
     int M, V, K, v0, cols, pitch;
-    int tiles_m, tiles_k, tiles_v, splits, split_cols;   // splits 0: no dx; tiles_v 0: no dW
+    int tiles_m, tiles_k, tiles_v, band_dx, band_dw, splits, split_cols;   // splits 0: no dx; tiles_v 0: no dW
     bool first, last, reduce;   // reduce: a launch of its own adds the splits and rounds
 };
 
@@ -234,7 +239,7 @@ template <typename Tile>
 __device__ __forceinline__ void head_dx_item(uint8_t* smem, const HeadPiece& p, int id) {
     const int tiles = p.tiles_m * p.tiles_k, split = id / tiles;
     int pm, pn;
-    grouped_raster(id - split * tiles, p.tiles_m, p.tiles_k, 8, pm, pn);
+    banded_raster(id - split * tiles, p.tiles_m, p.tiles_k, head_group(p.band_dx, p.tiles_k), p.band_dx, pm, pn);
     const int w = wave_id(), row0 = pm * Tile::kTile, col0 = pn * Tile::kTile;
     const int c0 = split * p.split_cols, n = min(p.split_cols, (p.cols + 7) / 8 * 8 - c0);   // (columns of dl behind `cols`: zeros)
     v4f acc[Tile::F][Tile::F];
@@ -277,7 +282,7 @@ __global__ __launch_bounds__(256) void head_gradients_kernel(HeadPiece p, T* __r
         return;
     }
     int pm, pn;
-    grouped_raster(xcd_chunk_order(blockIdx.x - dx_items, p.tiles_v * p.tiles_k, kCuPerXcd), p.tiles_v, p.tiles_k, 8, pm, pn);
+    banded_raster(xcd_chunk_order(blockIdx.x - dx_items, p.tiles_v * p.tiles_k, kCuPerXcd), p.tiles_v, p.tiles_k, head_group(p.band_dw, p.tiles_k), p.band_dw, pm, pn);
     const int lane = lane_id(), r = lane & 15, g = lane >> 4;
     const int w = wave_id(), row0 = pm * Tile::kTile, col0 = pn * Tile::kTile;
     const int row = row0 + (w >> 1) * Tile::kPatch, col = col0 + (w & 1) * Tile::kPatch;
@@ -425,7 +430,8 @@ static int launch_logits(const uint16_t* x, const uint16_t* W, HeadLabels labels
                          hipStream_t s) {
     static DeviceOnce once;
     const int tm = tiles_of(M, Tile::kTile), tv = tiles_of(V, Tile::kTile);
-    return launch_head<Tile>(head_logits_kernel<Tile>, once, (long long)tm * tv, s, x, W, labels, M, V, K, tm, tv, partial, label_logit);
+    return launch_head<Tile>(head_logits_kernel<Tile>, once, (long long)tm * tv, s, x, W, labels, M, V, K, tm, tv,
+                             raster_band(2ll * K * ((long long)M + V), tv), partial, label_logit);
 }
 template <typename Tile>
 static int launch_dlogits(const uint16_t* x, const uint16_t* W, HeadLabels labels, const float* lse, const float* dloss, int M, int V, int K,
@@ -433,7 +439,7 @@ static int launch_dlogits(const uint16_t* x, const uint16_t* W, HeadLabels label
     static DeviceOnce once;
     const int tm = tiles_of(M, Tile::kTile), tv = tiles_of(cols, Tile::kTile);
     return launch_head<Tile>(head_dlogits_kernel<Tile>, once, (long long)tm * tv + rows.groups, s, x, W, labels, lse, dloss, M, V, K, v0,
-                             (cols + 7) / 8 * 8, pitch, tm, tv, dl, resid, rows);
+                             (cols + 7) / 8 * 8, pitch, tm, tv, raster_band(2ll * K * ((long long)M + cols), tv), dl, resid, rows);
 }
 template <typename Tile, typename T>
 static int launch_gradients(HeadPiece p, bool dx, T* dw, hipStream_t s) {
@@ -441,6 +447,8 @@ static int launch_gradients(HeadPiece p, bool dx, T* dw, hipStream_t s) {
     p.tiles_m = tiles_of(p.M, Tile::kTile);
     p.tiles_k = tiles_of(p.K, Tile::kTile);
     p.tiles_v = dw ? tiles_of(p.cols, Tile::kTile) : 0;
+    p.band_dx = raster_band(2ll * p.cols * ((long long)p.M + p.K), p.tiles_k);
+    p.band_dw = raster_band(2ll * p.M * ((long long)p.cols + p.K), p.tiles_k);
     p.splits = dx ? tiles_of(p.cols, p.split_cols) : 0;
     const long long items = (long long)p.splits * p.tiles_m * p.tiles_k + (long long)p.tiles_v * p.tiles_k;
     return launch_head<Tile>(head_gradients_kernel<Tile, T>, once, items, s, p, dw ? dw + (size_t)p.v0 * p.K : nullptr);
@@ -497,7 +505,7 @@ extern "C" int hk_linear_cross_entropy_backward(const void* x_bf16, const void* 
     const bool want_dx = dx_bf16_or_null != nullptr;
     float* resid = (float*)(ws + L.resid);
     int32_t *starts = (int32_t*)(ws + L.starts), *list = (int32_t*)(ws + L.list);
-    HeadPiece p{dl, w, x, (float*)(ws + L.sums), lab, resid, starts, list, (uint16_t*)dx_bf16_or_null, M, V, K, 0, 0, L.piece, 0, 0, 0, 0, L.split_cols,
+    HeadPiece p{dl, w, x, (float*)(ws + L.sums), lab, resid, starts, list, (uint16_t*)dx_bf16_or_null, M, V, K, 0, 0, L.piece, 0, 0, 0, 0, 0, 0, L.split_cols,
                 false, false, L.splits > 1};
     for (int v0 = 0; v0 < V; v0 += L.piece) {
         p.v0 = v0;

@@ -20,7 +20,8 @@ struct GroupedTile { int expert, row0, rows, tile_n; };   // expert < 0: no such
 // Tile `id` of the list: expert by expert, inside an expert in groups of eight tiles of rows that go over the columns side by
 // side, so that an XCD's run of 32 tiles shares its operands (8192 x 8192 x 8192 731 us; with all 32 tiles of rows side by side 1078). Offsets
 // are held inside [0, R] and in order whatever they hold. Each wave scans by itself: lane l holds experts 8 l .. 8 l + 7.
-__device__ __forceinline__ GroupedTile grouped_tile(const int32_t* __restrict__ offsets, int E, int R, int tile_m, int tiles_n, int id) {
+__device__ __forceinline__ GroupedTile grouped_tile(const int32_t* __restrict__ offsets, int E, int R, int tile_m, int tiles_n,
+                                                    int in, int out, int id) {
     const int lane = lane_id();
     int lo[8], hi[8], tiles[8], mine = 0;
 #pragma unroll
@@ -43,7 +44,10 @@ __device__ __forceinline__ GroupedTile grouped_tile(const int32_t* __restrict__ 
     for (int j = 0; j < 8; ++j) {
         if (id >= at && id < at + tiles[j]) {
             int pm, pn;
-            grouped_raster(id - at, tiles[j] / tiles_n, tiles_n, 8, pm, pn);
+            // bands where the expert's operands do not fit the memory-side cache (raster_band's rule; 8192 rows of 65536 x 4096:
+            // 3425 us, with them 3002)
+            const bool banded = 2ll * ((long long)(hi[j] - lo[j]) + out) * in > (320ll << 20);
+            banded_raster(id - at, tiles[j] / tiles_n, tiles_n, banded ? 4 : 8, banded ? 16 : tiles_n, pm, pn);
             t = GroupedTile{8 * lane + j, lo[j] + pm * tile_m, 0, pn};
             t.rows = min(hi[j] - t.row0, tile_m);
         }
@@ -62,9 +66,10 @@ __global__ __launch_bounds__(256) void grouped_gemm_kernel(const uint16_t* __res
                                                            const int32_t* __restrict__ offsets, uint16_t* __restrict__ y,
                                                            int R, int E, int N, int K, int tiles_n) {
     extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
-    const GroupedTile t = grouped_tile(offsets, E, R, Tile::kTile, tiles_n, xcd_chunk_order(blockIdx.x, gridDim.x, kCuPerXcd));
+    const int in = DGRAD ? N : K, out = DGRAD ? K : N;
+    const GroupedTile t = grouped_tile(offsets, E, R, Tile::kTile, tiles_n, in, out, xcd_chunk_order(blockIdx.x, gridDim.x, kCuPerXcd));
     if (t.expert < 0) return;
-    const int in = DGRAD ? N : K, out = DGRAD ? K : N, col0 = t.tile_n * Tile::kTile;
+    const int col0 = t.tile_n * Tile::kTile;
     const uint16_t* We = W + (size_t)t.expert * N * K;
     v4f acc[Tile::F][Tile::F];
     Tile::template product<false, DGRAD>(smem, operand_along(x, 2ull * in, t.row0, t.row0 + t.rows, in),
@@ -159,7 +164,18 @@ static int launch_wgrad_tile(const void* dy, const void* x, const int32_t* offse
 template <typename T>
 static int launch_wgrad(const void* dy, const void* x, const int32_t* offsets, void* dW, int R, int E, int N, int K, hipStream_t s) {
     const double e = E, n256 = (N + 255) / 256, k256 = (K + 255) / 256, n128 = (N + 127) / 128, k128 = (K + 127) / 128;
-    return prefer_tile256(e * n256 * k256, e * n128 * k128, (R / E + kLayoutStep - 1) / kLayoutStep, moe_num_compute_units(), kSmallStepAcross)
+    const int cus = moe_num_compute_units();
+    const double steps = (double)R / E / kLayoutStep + 0.5;
+    // Enough small tiles for four of the single-stage kernel on every CU, whose loads, products and stores then overlap one
+    // another's: up to about 300 rows an expert. (us, large / two stages / one: 32 experts of 4096 x 7168, 32 rows each 461 / 447 / 367,
+    // 128 634 / 635 / 565, 256 800 / 874 / 784, 384 936 / 1092 / 962; 128 experts of 2880 x 2880, 128 rows, fp32 1090 / 1117 / 1017;
+    // fewer tiles, 8 experts of 1024 x 1024: 24 / 14 / 18.)
+    if (e * n128 * k128 >= 4.0 * cus) {
+        const double large = e * n256 * k256 / cus * (7.0 + 1.43 * steps), single = e * n128 * k128 / (4.0 * cus) * (3.8 + 2.08 * steps);
+        return large < single ? launch_wgrad_tile<LayoutTile256, T>(dy, x, offsets, dW, R, E, N, K, s)
+                              : launch_wgrad_tile<LayoutTile128Stages<1>, T>(dy, x, offsets, dW, R, E, N, K, s);
+    }
+    return prefer_tile256(e * n256 * k256, e * n128 * k128, steps, cus, kSmallStepAcross)
                ? launch_wgrad_tile<LayoutTile256, T>(dy, x, offsets, dW, R, E, N, K, s)
                : launch_wgrad_tile<LayoutTile128, T>(dy, x, offsets, dW, R, E, N, K, s);
 }

@@ -55,6 +55,8 @@ class _NoNative:
         return None
 
     bf16_gemm = mxfp4_gemm = mxfp4_quantize_rows = fp8_gemm
+    moe_permute = moe_permute_backward = moe_unpermute_backward = fp8_gemm
+    moe_grouped_gemm = moe_grouped_gemm_dgrad = moe_grouped_gemm_wgrad = fp8_gemm
 
 
 def _load_native():
@@ -708,6 +710,9 @@ def _check_positions(rows, name, slot_to_pos, T: int, H: int) -> int:
 def dispatch_moe_permute(x, slot_to_pos, xp) -> None:
     """Rows to the order of their experts: xp[slot_to_pos[t*k+j]] = x[t] with x [T,H], xp [T*k,H] bf16 and slot_to_pos [T*k]
     from dispatch_moe_sort. A position outside [0, T*k) has no row; rows of xp that no slot names stay as they were."""
+    st = (_native or _load_native()).moe_permute(x, slot_to_pos, xp)
+    if st is not None:
+        return _lib.check(st, "dispatch_moe_permute")
     _check_tensor(x, "x", _BF16, 2)
     T, H = x.shape
     k = _check_positions(xp, "xp", slot_to_pos, T, H)
@@ -719,6 +724,9 @@ def dispatch_moe_permute(x, slot_to_pos, xp) -> None:
 
 def dispatch_moe_permute_backward(dxp, slot_to_pos, dx, add=None) -> None:
     """Gradient of dispatch_moe_permute: dx [T,H] = (add [T,H] if given) + sum_j dxp[slot_to_pos[t*k+j]], summed in fp32."""
+    st = (_native or _load_native()).moe_permute_backward(dxp, slot_to_pos, dx, add)
+    if st is not None:
+        return _lib.check(st, "dispatch_moe_permute_backward")
     _check_tensor(dx, "dx", _BF16, 2)
     T, H = dx.shape
     k = _check_positions(dxp, "dxp", slot_to_pos, T, H)
@@ -737,6 +745,9 @@ def dispatch_moe_unpermute_backward(dy, o, weights, slot_to_pos, do, dweights) -
     """Gradients of dispatch_moe_unpermute: do[pos] = weights[t,j] * dy[t] and dweights[t,j] = <dy[t], o[pos]> with
     pos = slot_to_pos[t*k+j]; dy [T,H], o and do [T*k,H] bf16, weights and dweights [T,k] fp32. A slot without a row has a
     dweights of 0; rows of do that no slot names stay as they were."""
+    st = (_native or _load_native()).moe_unpermute_backward(dy, o, weights, slot_to_pos, do, dweights)
+    if st is not None:
+        return _lib.check(st, "dispatch_moe_unpermute_backward")
     _check_tensor(dy, "dy", _BF16, 2)
     T, H = dy.shape
     k = _check_positions(o, "o", slot_to_pos, T, H)
@@ -771,6 +782,9 @@ def _check_grouped(rows_n, name_n, rows_k, name_k, w, name_w, w_types, expert_of
 def dispatch_moe_grouped_gemm(x, w, expert_offsets, y) -> None:
     """The experts' products: y[r] = x[r] @ w[e].T for the rows expert_offsets[e] <= r < expert_offsets[e+1]; x [R,K],
     w [E,N,K], y [R,N] bf16, expert_offsets [E+1] int32 (dispatch_moe_sort). Rows behind the last offset are left alone."""
+    st = (_native or _load_native()).moe_grouped_gemm(x, w, expert_offsets, y)
+    if st is not None:
+        return _lib.check(st, "dispatch_moe_grouped_gemm")
     R, E, N, K = _check_grouped(y, "y", x, "x", w, "w", _BF16, expert_offsets)
     with torch.cuda.device(x.device):
         st = _lib.load_library().hk_moe_grouped_gemm(x.data_ptr(), w.data_ptr(), expert_offsets.data_ptr(), y.data_ptr(),
@@ -780,6 +794,9 @@ def dispatch_moe_grouped_gemm(x, w, expert_offsets, y) -> None:
 
 def dispatch_moe_grouped_gemm_dgrad(dy, w, expert_offsets, dx) -> None:
     """Gradient of dispatch_moe_grouped_gemm in x: dx[r] = dy[r] @ w[e]; dy [R,N], w [E,N,K], dx [R,K]."""
+    st = (_native or _load_native()).moe_grouped_gemm_dgrad(dy, w, expert_offsets, dx)
+    if st is not None:
+        return _lib.check(st, "dispatch_moe_grouped_gemm_dgrad")
     R, E, N, K = _check_grouped(dy, "dy", dx, "dx", w, "w", _BF16, expert_offsets)
     with torch.cuda.device(dy.device):
         st = _lib.load_library().hk_moe_grouped_gemm_dgrad(dy.data_ptr(), w.data_ptr(), expert_offsets.data_ptr(),
@@ -790,6 +807,9 @@ def dispatch_moe_grouped_gemm_dgrad(dy, w, expert_offsets, dx) -> None:
 def dispatch_moe_grouped_gemm_wgrad(dy, x, expert_offsets, dw) -> None:
     """Gradient of dispatch_moe_grouped_gemm in w: dw[e] = dy[rows of e].T @ x[rows of e]; dy [R,N], x [R,K], dw [E,N,K] in
     bf16 or fp32. Every expert's is written, zeros for one without rows."""
+    st = (_native or _load_native()).moe_grouped_gemm_wgrad(dy, x, expert_offsets, dw)
+    if st is not None:
+        return _lib.check(st, "dispatch_moe_grouped_gemm_wgrad")
     R, E, N, K = _check_grouped(dy, "dy", x, "x", dw, "dw", _BF16 + _F32, expert_offsets)
     with torch.cuda.device(dy.device):
         st = _lib.load_library().hk_moe_grouped_gemm_wgrad(dy.data_ptr(), x.data_ptr(), expert_offsets.data_ptr(),

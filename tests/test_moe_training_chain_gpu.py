@@ -1,0 +1,210 @@
+"""The training entry points together, as a step through one mixture-of-experts layer and the output head uses them: router,
+sort, permute, two products of the experts with SiLU between them, weighted sum, head and loss, and everything back, against
+the same step by torch's autograd in 64 bits; on another stream than the default, and captured into a graph."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+class Step:
+    """One layer and a head; `forward` and `backward` write into buffers made once."""
+
+    def __init__(self, hk, T, E, k, H, I, V, seed, masked):
+        self.tk = tk = hk.tk_kernel
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        bf = lambda *s, std=1.0: (torch.randn(*s, device=DEV, generator=g) * std).to(torch.bfloat16)
+        self.T, self.E, self.k, self.H, self.I, self.V = T, E, k, H, I, V
+        self.x, self.w1, self.w2 = bf(T, H), bf(E, 2 * I, H, std=H**-0.5), bf(E, H, I, std=I**-0.5)
+        self.head = bf(V, H, std=2 * H**-0.5)
+        self.logits = torch.randn(T, E, device=DEV, generator=g)
+        self.labels = torch.randint(0, V, (T,), device=DEV, generator=g)
+        self.mask = torch.rand(T, device=DEV, generator=g) < masked
+        self.labels[self.mask] = -100
+        self.dloss = torch.full((T,), 1.0 / max(1, int((~self.mask).sum())), device=DEV)
+        e = lambda *s, dtype=torch.bfloat16: torch.full(s, 77, dtype=dtype, device=DEV)
+        S = T * k
+        self.ids, self.weights = e(T, k, dtype=torch.int32), e(T, k, dtype=torch.float32)
+        self.sorted, self.offsets = e(S, dtype=torch.int32), e(E + 1, dtype=torch.int32)
+        self.pos = e(S, dtype=torch.int32)
+        self.sort_ws = e(tk.moe_sort_workspace_bytes(T, k, E), dtype=torch.uint8)
+        self.xp, self.h1, self.act, self.o, self.y = e(S, H), e(S, 2 * I), e(S, I), e(S, H), e(T, H)
+        self.loss, self.lse = e(T, dtype=torch.float32), e(T, dtype=torch.float32)
+        self.head_ws = e(tk.linear_cross_entropy_workspace_bytes(T, V, H), dtype=torch.uint8)
+        self.dy, self.dhead = e(T, H), e(V, H, dtype=torch.float32)
+        self.do, self.dweights = e(S, H), e(T, k, dtype=torch.float32)
+        self.dact, self.dh1, self.dxp, self.dx = e(S, I), e(S, 2 * I), e(S, H), e(T, H)
+        self.dw1, self.dw2 = e(E, 2 * I, H, dtype=torch.float32), e(E, H, I, dtype=torch.float32)
+        self.outs = [self.loss, self.lse, self.dhead, self.dweights, self.dx, self.dw1, self.dw2]
+
+    def run(self):
+        tk = self.tk
+        tk.dispatch_moe_topk_softmax(self.logits, self.ids, self.weights)
+        self.ids.masked_fill_(self.mask[:, None], -1)   # padding takes no part
+        self.pos.fill_(-1)
+        tk.dispatch_moe_sort(self.ids, self.sorted, self.offsets, self.pos, self.sort_ws)
+        tk.dispatch_moe_permute(self.x, self.pos, self.xp)
+        tk.dispatch_moe_grouped_gemm(self.xp, self.w1, self.offsets, self.h1)
+        gate, up = self.h1.float().chunk(2, dim=1)
+        self.act.copy_(torch.nn.functional.silu(gate) * up)
+        tk.dispatch_moe_grouped_gemm(self.act, self.w2, self.offsets, self.o)
+        tk.dispatch_moe_unpermute(self.o, self.weights, self.pos, self.y)
+        tk.dispatch_linear_cross_entropy(self.y, self.head, self.labels, self.loss, self.lse, self.head_ws)
+        tk.dispatch_linear_cross_entropy_backward(self.y, self.head, self.labels, self.lse, self.dloss, self.dy, self.dhead,
+                                                  self.head_ws)
+        tk.dispatch_moe_unpermute_backward(self.dy, self.o, self.weights, self.pos, self.do, self.dweights)
+        tk.dispatch_moe_grouped_gemm_wgrad(self.do, self.act, self.offsets, self.dw2)
+        tk.dispatch_moe_grouped_gemm_dgrad(self.do, self.w2, self.offsets, self.dact)
+        d, s = self.dact.float(), torch.sigmoid(gate)
+        self.dh1[:, :self.I].copy_(d * up * s * (1 + gate * (1 - s)))
+        self.dh1[:, self.I:].copy_(d * gate * s)
+        tk.dispatch_moe_grouped_gemm_wgrad(self.dh1, self.xp, self.offsets, self.dw1)
+        tk.dispatch_moe_grouped_gemm_dgrad(self.dh1, self.w1, self.offsets, self.dxp)
+        tk.dispatch_moe_permute_backward(self.dxp, self.pos, self.dx)
+
+    def reference(self):
+        """The same step in 64 bits on the CPU with autograd: loss and the gradients of x, w1, w2, head and the choices' weights."""
+        c = lambda t: t.detach().double().cpu().requires_grad_(True)
+        x, w1, w2, head = c(self.x), c(self.w1), c(self.w2), c(self.head)
+        top, ids = self.logits.double().cpu().topk(self.k, dim=1)
+        weights = torch.softmax(top, dim=1).requires_grad_(True)
+        live = ~self.mask.cpu()
+        ys = []
+        for t in range(self.T):
+            y = torch.zeros(self.H, dtype=torch.float64)
+            if live[t]:
+                for j in range(self.k):
+                    e = int(ids[t, j])
+                    gate, up = (w1[e] @ x[t]).chunk(2)
+                    y = y + weights[t, j] * (w2[e] @ (torch.nn.functional.silu(gate) * up))
+            ys.append(y)
+        logits = torch.stack(ys) @ head.t()
+        loss = torch.nn.functional.cross_entropy(logits, self.labels.cpu(), reduction="none", ignore_index=-100)
+        (loss * self.dloss.double().cpu()).sum().backward()
+        return loss.detach(), torch.logsumexp(logits.detach(), dim=1), head.grad, weights.grad, x.grad, w1.grad, w2.grad
+
+
+def _check(step):
+    """Each result against the 64-bit step, relative in the Frobenius norm. Between input and result lie at most eight
+    roundings to bf16 (xp is exact; h1, act, o, y, dl, dy, do, dact, dh1, dxp, dx: eleven on the longest way), each off by at
+    most 2^-8 of its value, independent of one another, and products that leave the norm of such an error about where it was:
+    sqrt(11) 2^-8 = 0.013 for uncorrelated errors; twice that is asked for. The loss passes h1, act, o and y: sqrt(4) 2^-8
+    of the logits' size."""
+    names = ("loss", "lse", "dhead", "dweights", "dx", "dw1", "dw2")
+    for name, got, want in zip(names, step.outs, step.reference()):
+        got = got.double().cpu()
+        assert torch.isfinite(got).all(), name
+        err = float((got - want).norm() / want.norm())
+        assert err <= 0.026, (name, err)
+
+
+@pytest.mark.parametrize("T,E,k,H,I,V,masked", [(37, 5, 2, 72, 40, 333, 0.2), (160, 8, 4, 136, 64, 1000, 0.0), (1, 3, 1, 64, 32, 50, 0.0)])
+def test_a_training_step_against_autograd(hk, T, E, k, H, I, V, masked):
+    print(f"training step T={T} E={E} k={k} H={H} I={I} V={V}", flush=True)
+    step = Step(hk, T, E, k, H, I, V, T, masked)
+    step.run()
+    torch.cuda.synchronize()
+    _check(step)
+
+
+def test_a_step_on_another_stream(hk):
+    """Everything goes to the current stream: the inputs are only there once that stream has made them."""
+    print("training step on a side stream", flush=True)
+    step = Step(hk, 300, 8, 2, 136, 64, 2000, 5, 0.1)
+    step.run()
+    torch.cuda.synchronize()
+    want = [o.clone() for o in step.outs]
+    side = torch.cuda.Stream()
+    x, head = step.x.clone(), step.head.clone()
+    step.x.zero_(), step.head.zero_()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        big = torch.empty(1 << 26, device=DEV)
+        for _ in range(20):
+            big.add_(1.0)            # holds the stream back
+        step.x.copy_(x)
+        step.head.copy_(head)
+        step.run()
+    side.synchronize()
+    for got, w in zip(step.outs, want):
+        assert torch.equal(got.view(torch.uint8), w.view(torch.uint8))
+
+
+def test_a_step_in_a_graph(hk):
+    print("training step in a graph", flush=True)
+    step = Step(hk, 256, 8, 4, 264, 128, 3000, 6, 0.1)
+    step.run()
+    torch.cuda.synchronize()
+    want = [o.clone() for o in step.outs]
+    other = [(step.xp, 5.0), (step.o, 5.0), (step.do, 5.0)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step.run()
+    for rep in range(3):
+        for o in step.outs:
+            o.zero_()
+        for buf, value in other:
+            buf.fill_(value)
+        step.head_ws.fill_(0xFF)     # nothing in the workspaces is kept from one call to the next
+        step.sort_ws.fill_(0xFF)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, w in zip(step.outs, want):
+            assert torch.equal(got.view(torch.uint8), w.view(torch.uint8)), rep
+
+
+def test_two_graphs_with_one_workspace(hk):
+    """Two captured heads of different sizes that share a workspace, replayed one after the other in either order."""
+    print("two head graphs with one workspace", flush=True)
+    tk = hk.tk_kernel
+    g = torch.Generator(device=DEV).manual_seed(8)
+    sizes = [(300, 5000, 136), (70, 900, 264)]
+    ws = torch.empty(max(tk.linear_cross_entropy_workspace_bytes(*s) for s in sizes), dtype=torch.uint8, device=DEV)
+    graphs, outs, wants, kept = [], [], [], []
+    for M, V, K in sizes:
+        x = torch.randn(M, K, device=DEV, generator=g).to(torch.bfloat16)
+        w = (torch.randn(V, K, device=DEV, generator=g) * K**-0.5).to(torch.bfloat16)
+        labels = torch.randint(0, V, (M,), device=DEV, generator=g)
+        out = [torch.empty(M, device=DEV), torch.empty(M, device=DEV), torch.empty_like(x), torch.empty_like(w)]
+        dloss = torch.ones(M, device=DEV)
+
+        def run(x=x, w=w, labels=labels, out=out, dloss=dloss):
+            tk.dispatch_linear_cross_entropy(x, w, labels, out[0], out[1], ws)
+            tk.dispatch_linear_cross_entropy_backward(x, w, labels, out[1], dloss, out[2], out[3], ws)
+
+        kept.append(run)   # a graph reads the tensors it was captured with: they live as long as it does
+        run()
+        torch.cuda.synchronize()
+        wants.append([o.clone() for o in out])
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run()
+        graphs.append(graph)
+        outs.append(out)
+    for order in ((0, 1), (1, 0), (0, 0, 1)):
+        for out in outs:
+            for o in out:
+                o.zero_()
+        for i in order:
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        for out, want in zip(outs, wants):
+            for o, w in zip(out, want):
+                assert torch.equal(o, w)
+
+
+def test_native_and_python_dispatchers_agree(hk, monkeypatch):
+    """The same step with the calls checked in Python."""
+    print("training step without the native dispatchers", flush=True)
+    tk = hk.tk_kernel
+    step = Step(hk, 100, 6, 2, 136, 64, 500, 9, 0.1)
+    step.run()
+    want = [o.clone() for o in step.outs]
+    monkeypatch.setattr(tk, "_native", tk._NoNative)
+    for o in step.outs:
+        o.zero_()
+    step.run()
+    for got, w in zip(step.outs, want):
+        assert torch.equal(got.view(torch.uint8), w.view(torch.uint8))
