@@ -22,9 +22,11 @@ __device__ __forceinline__ void mfma_bf16_acc(v4f& acc, const v4i& x, const v4i&
     asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(x), "v"(y));
 }
 
-// Loads and reads of one operand. Load i (0..7) of a wave: along, rows 32 i + 8 w .. +8; across, K rows 8 i + 2 w and the next.
-template <bool ACROSS>
+// Loads and reads of one operand of a tile of TILE rows (columns): TILE / 32 loads a wave. Load i: along, rows 32 i + 8 w .. +8; across,
+// TILE 256, K rows 8 i + 2 w and the next, TILE 128, 16 i + 4 w .. +4.
+template <bool ACROSS, int TILE = kRingTile>
 struct RingOperand {
+    static constexpr uint32_t kRow = 2 * TILE;   // across: bytes of a K row in LDS
     uint64_t base;        // descriptor of the K-step that is loaded next
     int64_t left;
     uint32_t voff[2];     // even / odd loads (across: the swizzle takes bit 3 of the K row)
@@ -32,7 +34,7 @@ struct RingOperand {
     uint32_t rd[2];       // along: the lane's two chunks of its row; across: rd[0] = the lane's address in fragment 0
     static __device__ __forceinline__ int64_t step(uint32_t pitch) { return (int64_t)kLayoutStep * pitch; }
 
-    // `patch`: which 128 rows (columns) of the tile this wave reads
+    // `patch`: which half of the tile's rows (columns) this wave reads
     __device__ __forceinline__ void init(const TileOperand& op, int K, int patch, uint32_t lds0) {
         const uint32_t lane = lane_id(), w = wave_id(), r = lane & 15, g = lane >> 4;
         base = ((uint64_t)to_sgpr((uint32_t)((uint64_t)op.base >> 32)) << 32) | to_sgpr((uint32_t)(uint64_t)op.base);
@@ -42,12 +44,13 @@ struct RingOperand {
         if constexpr (ACROSS) {
 #pragma unroll
             for (int odd = 0; odd < 2; ++odd) {
-                const uint32_t k = 2 * w + (lane >> 5);
-                voff[odd] = k * pitch + (((lane & 31u) ^ across_swz(k + 8 * odd)) * 16u);
+                constexpr uint32_t kChunks = kRow / 16, kLoadRows = 64 / kChunks;   // chunks of a row, rows of a load
+                const uint32_t k = kLoadRows * w + lane / kChunks;
+                voff[odd] = k * pitch + (((lane % kChunks) ^ across_swz(k + 4 * kLoadRows * odd)) * 16u);
+                round = 4u * kLoadRows * pitch;
             }
-            round = 8u * pitch;
             const uint32_t k = 8 * g + (r >> 2);
-            rd[0] = lds0 + k * (2 * kRingTile) + (((16u * patch + ((r >> 1) & 1u)) ^ across_swz(k)) * 16u) + (r & 1u) * 8u;
+            rd[0] = lds0 + k * kRow + (((TILE / 16u * patch + ((r >> 1) & 1u)) ^ across_swz(k)) * 16u) + (r & 1u) * 8u;
             rd[1] = 0;
         } else {
             const uint32_t R = 8 * w + (lane >> 3), c = swz_chunk(R, lane & 7) * 16u;
@@ -55,8 +58,8 @@ struct RingOperand {
             round = 32u * pitch;
             const int nk = (K + kLayoutStep - 1) / kLayoutStep;
             tail_or = (int)c >= 2 * (K - (nk - 1) * kLayoutStep) ? 0x80000000u : 0u;
-            rd[0] = lds0 + (128u * patch + r) * 128u + swz_chunk(r, g) * 16u;
-            rd[1] = lds0 + (128u * patch + r) * 128u + swz_chunk(r, g + 4) * 16u;
+            rd[0] = lds0 + (TILE / 2u * patch + r) * 128u + swz_chunk(r, g) * 16u;
+            rd[1] = lds0 + (TILE / 2u * patch + r) * 128u + swz_chunk(r, g + 4) * 16u;
         }
     }
     // the descriptor's next K-step
@@ -83,7 +86,6 @@ struct RingOperand {
     __device__ __forceinline__ v4i half(int f, uint32_t slot) const {
         if constexpr (ACROSS) {
             const uint32_t at = (rd[0] ^ (32u * f)) + slot;
-            constexpr int kRow = 2 * kRingTile;
             const v2i a = lds_read_tr(at + (32 * H) * kRow), b = lds_read_tr(at + (32 * H + 4) * kRow);
             return v4i{a.x, a.y, b.x, b.y};
         } else {
@@ -146,7 +148,7 @@ __device__ __forceinline__ void ring_product(uint8_t* smem, const TileOperand& A
         const bool more = kt + 2 < nk;
         const v4i da = oa.srd(more), db = ob.srd(more);
         const uint32_t vor_a = kt + 2 == nk - 1 ? oa.tail_or : 0u, vor_b = kt + 2 == nk - 1 ? ob.tail_or : 0u;
-        const uint32_t rows_a = RingOperand<A_ACROSS>::opaque(oa.round), rows_b = RingOperand<B_ACROSS>::opaque(ob.round);
+        const uint32_t rows_a = oa.opaque(oa.round), rows_b = ob.opaque(ob.round);
         auto load_b = [&](int i) __attribute__((always_inline)) {
             switch (i) {
                 case 0: ob.template load<0>(mine_b + off2, db, vor_b, rows_b); break;
@@ -219,6 +221,108 @@ __device__ __forceinline__ void ring_product(uint8_t* smem, const TileOperand& A
         }
         off1 = off2;
         off2 = off2 == 2 * kRingSlot ? 0u : off2 + kRingSlot;
+    };
+    int kt = 0;
+    for (; kt + 1 < nk; kt += 2) {
+        step.template operator()<0>(kt);
+        step.template operator()<1>(kt + 1);
+    }
+    if (kt < nk) step.template operator()<0>(kt);
+    wait_vmcnt<0>();   // nothing may still be writing LDS when the workgroup retires or uses it otherwise
+    mfma_drain_agpr(acc);
+}
+
+// 128x128 tiles in the same manner, for problems with no more tiles than CUs, where one workgroup has a CU to itself: four LDS
+// stages, three K-steps ahead, the next K-step's fragments read behind the MFMAs of this one (a quarter of the tile and 32
+// MFMAs a wave and K-step). (Weight gradient of 16384 rows, 64 tiles of 256 K-steps:
+// 155 us with two stages, 117 here, now bound by the loads' latency; loss of 100 x 10000 x 4096 52 / 39; 16 rows of 4 experts of 4096 x 4096
+// 45 / 33.)
+constexpr int kDeepStages = 4, kDeepStage = 2 * kLayoutTile * 128;
+template <bool A_ACROSS, bool B_ACROSS>
+__device__ __forceinline__ void deep_product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K, v4f (&acc)[4][4]) {
+    constexpr int S = kDeepStages, kLoads = 4;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)smem, w = wave_id();
+    const uint32_t mine = to_sgpr(lds0 + w * 1024u);
+    RingOperand<A_ACROSS, kLayoutTile> oa;
+    RingOperand<B_ACROSS, kLayoutTile> ob;
+    oa.init(A, K, w >> 1, lds0);
+    ob.init(B, K, w & 1, lds0 + kDeepStage / 2);
+    const int nk = (K + kLayoutStep - 1) / kLayoutStep;
+    const uint32_t step_a = A_ACROSS ? to_sgpr(kLayoutStep * A.pitch) : 128u, step_b = B_ACROSS ? to_sgpr(kLayoutStep * B.pitch) : 128u;
+#pragma unroll
+    for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[m][n] = v4f{0.f, 0.f, 0.f, 0.f};
+    struct Frag { v4i lo, hi; };
+    Frag af[2][4], bf[2][4];
+    v4i da, db;
+    uint32_t vor_a = 0, vor_b = 0, rows_a = 0, rows_b = 0;
+    auto next_step = [&](int kt) __attribute__((always_inline)) {   // the descriptors' K-step
+        da = oa.srd(kt < nk);
+        db = ob.srd(kt < nk);
+        vor_a = kt == nk - 1 ? oa.tail_or : 0u;
+        vor_b = kt == nk - 1 ? ob.tail_or : 0u;
+        rows_a = oa.opaque(oa.round);
+        rows_b = ob.opaque(ob.round);
+        oa.advance(step_a);
+        ob.advance(step_b);
+    };
+    auto load = [&](int i, uint32_t stage) __attribute__((always_inline)) {   // 0 .. 3: A, 4 .. 7: B
+        switch (i) {
+            case 0: oa.template load<0>(mine + stage, da, vor_a, rows_a); break;
+            case 1: oa.template load<1>(mine + stage, da, vor_a, rows_a); break;
+            case 2: oa.template load<2>(mine + stage, da, vor_a, rows_a); break;
+            case 3: oa.template load<3>(mine + stage, da, vor_a, rows_a); break;
+            case 4: ob.template load<0, kDeepStage / 2>(mine + stage, db, vor_b, rows_b); break;
+            case 5: ob.template load<1, kDeepStage / 2>(mine + stage, db, vor_b, rows_b); break;
+            case 6: ob.template load<2, kDeepStage / 2>(mine + stage, db, vor_b, rows_b); break;
+            default: ob.template load<3, kDeepStage / 2>(mine + stage, db, vor_b, rows_b); break;
+        }
+    };
+    // half u (0 .. 15) of a K-step's fragments into register set Q
+    auto read = [&]<int Q>(int u, uint32_t stage) __attribute__((always_inline)) {
+        const int f = u / 4, h = u & 1;
+        if ((u & 2) == 0) {
+            if (h) bf[Q][f].hi = ob.template half<1>(f, stage);
+            else bf[Q][f].lo = ob.template half<0>(f, stage);
+        } else {
+            if (h) af[Q][f].hi = oa.template half<1>(f, stage);
+            else af[Q][f].lo = oa.template half<0>(f, stage);
+        }
+    };
+#pragma unroll
+    for (int p = 0; p < S; ++p) {
+        next_step(p);
+#pragma unroll
+        for (int i = 0; i < 2 * kLoads; ++i) load(i, p * kDeepStage);
+    }
+    wait_vmcnt<(S - 1) * 2 * kLoads>();
+    block_barrier();
+#pragma unroll
+    for (int u = 0; u < 16; ++u) read.template operator()<0>(u, 0u);
+    uint32_t at = 0, at1 = kDeepStage;   // stages of K-steps kt and kt + 1
+    auto step = [&]<int P>(int kt) __attribute__((always_inline)) {
+        // this K-step's fragments are here, so its stage is free once everyone says so; the next K-step has landed
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        wait_vmcnt<(S - 2) * 2 * kLoads>();
+        block_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        next_step(kt + S);
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+            for (int pass = 0; pass < 2; ++pass)
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    if (pass == 0) mfma_bf16_acc(acc[m][n], bf[P][n].lo, af[P][m].lo);
+                    else mfma_bf16_acc(acc[m][n], bf[P][n].hi, af[P][m].hi);
+                    const int q = 8 * m + 4 * pass + n;
+                    if (q < 16) read.template operator()<P ^ 1>(q, at1);
+                    else if (q & 1) load((q - 16) / 2, at);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+        at = at1;
+        at1 = at1 == (S - 1) * kDeepStage ? 0u : at1 + kDeepStage;
     };
     int kt = 0;
     for (; kt + 1 < nk; kt += 2) {
@@ -305,6 +409,18 @@ struct LayoutTile256 {
     }
 };
 
+struct LayoutTile128Deep {
+    static constexpr int kTile = kLayoutTile, kPatch = kTile / 2, F = 4, kLds = kDeepStages * kDeepStage;
+    template <bool A_ACROSS, bool B_ACROSS>
+    static __device__ __forceinline__ void product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K, v4f (&acc)[F][F]) {
+        deep_product<A_ACROSS, B_ACROSS>(smem, A, B, K, acc);
+    }
+    static __device__ __forceinline__ void read_row(const v4f (&acc)[F], v4f (&v)[F]) {
+#pragma unroll
+        for (int n = 0; n < F; ++n) v[n] = acc[n];
+    }
+};
+
 // Whether 256x256 tiles take less time than 128x128 ones: rounds of workgroups over the CUs (one of the large kernel or two of
 // the small one on a CU; a round that is not full is a round, later ones run into each other) times a fixed part and a part per
 // K-step, us. The constants are fits to 32 experts of 4096 x 7168: 65536 rows forward 2873 large / 4130 small, gradient of the
@@ -314,6 +430,12 @@ constexpr double kSmallStepAlong = 1.1, kSmallStepAcross = 0.945;
 inline bool prefer_tile256(double tiles256, double tiles128, double k_steps, int cus, double small_step = kSmallStepAlong) {
     auto rounds = [](double tiles, double at_once) { return tiles <= at_once ? 1.0 : tiles / at_once + 0.2; };
     return rounds(tiles256, cus) * (7.0 + 1.43 * k_steps) < rounds(tiles128, 2.0 * cus) * (2.7 + small_step * k_steps);
+}
+// The tile and the number of LDS stages of the small one: four where no CU gets a second workgroup anyway.
+enum LayoutChoice { kLayout256, kLayout128, kLayout128Deep };
+inline LayoutChoice choose_layout(double tiles256, double tiles128, double k_steps, int cus, double small_step = kSmallStepAlong) {
+    if (prefer_tile256(tiles256, tiles128, k_steps, cus, small_step)) return kLayout256;
+    return tiles128 <= cus ? kLayout128Deep : kLayout128;
 }
 
 }  // namespace hk

@@ -358,19 +358,19 @@ __global__ __launch_bounds__(256) void head_dx_reduce_kernel(const float* __rest
 
 static int tiles_of(int n, int tile) { return (n + tile - 1) / tile; }
 static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
-static bool head_use_256(int rows, int cols, int k) {   // a product of rows x cols over k
-    return prefer_tile256((double)tiles_of(rows, 256) * tiles_of(cols, 256), (double)tiles_of(rows, 128) * tiles_of(cols, 128),
-                          tiles_of(k, kLayoutStep), moe_num_compute_units());
+static LayoutChoice head_choice(int rows, int cols, int k) {   // a product of rows x cols over k
+    return choose_layout((double)tiles_of(rows, 256) * tiles_of(cols, 256), (double)tiles_of(rows, 128) * tiles_of(cols, 128),
+                         tiles_of(k, kLayoutStep), moe_num_compute_units());
 }
 
 // forward: label logits, then the partial results
 struct HeadForwardPlan {
-    bool tile256;
+    LayoutChoice tile;
     int blocks;   // columns of a partial result: a wave's patch
     size_t label_logit, partial, bytes;
     HeadForwardPlan(int M, int V, int K) {
-        tile256 = head_use_256(M, V, K);
-        blocks = 2 * tiles_of(V, tile256 ? 256 : 128);
+        tile = head_choice(M, V, K);
+        blocks = 2 * tiles_of(V, tile == kLayout256 ? 256 : 128);
         label_logit = 0;
         partial = up256((size_t)M * 4);
         bytes = partial + up256((size_t)M * blocks * sizeof(float2));
@@ -379,7 +379,8 @@ struct HeadForwardPlan {
 // backward: dl of a piece, then the fp32 sums of dx
 struct HeadBackwardPlan {
     int piece;   // columns of a piece, a multiple of 256
-    bool logits256, grads256;
+    LayoutChoice logits;
+    bool grads256;
     int splits, split_cols;
     size_t resid, starts, list, dl, sums, bytes;
     HeadBackwardPlan(int M, int V, int K) {
@@ -387,7 +388,7 @@ struct HeadBackwardPlan {
         const long long most = std::min((256ll << 20) / (2ll * M), 1ll << 21) / 256 * 256, all = (long long)tiles_of(V, 256) * 256;
         piece = (int)std::max(256ll, std::min(most, all));
         const int cols = std::min(piece, V);
-        logits256 = head_use_256(M, cols, K);
+        logits = head_choice(M, cols, K);
         // dx and dW together: K-steps of all tiles over the workgroups that run at once
         const int slots = moe_num_compute_units(), steps_v = tiles_of(cols, kLayoutStep), steps_m = tiles_of(M, kLayoutStep);
         const double dx256 = (double)tiles_of(M, 256) * tiles_of(K, 256), dw256 = (double)tiles_of(cols, 256) * tiles_of(K, 256);
@@ -477,8 +478,9 @@ extern "C" int hk_linear_cross_entropy(const void* x_bf16, const void* w_bf16, c
     float* label_logit = (float*)((uint8_t*)workspace + L.label_logit);
     const HeadLabels lab{labels, label_type};
     const uint16_t *x = (const uint16_t*)x_bf16, *w = (const uint16_t*)w_bf16;
-    const int st = L.tile256 ? launch_logits<LayoutTile256>(x, w, lab, M, V, K, partial, label_logit, s)
-                             : launch_logits<LayoutTile128>(x, w, lab, M, V, K, partial, label_logit, s);
+    const int st = L.tile == kLayout256   ? launch_logits<LayoutTile256>(x, w, lab, M, V, K, partial, label_logit, s)
+                   : L.tile == kLayout128 ? launch_logits<LayoutTile128>(x, w, lab, M, V, K, partial, label_logit, s)
+                                          : launch_logits<LayoutTile128Deep>(x, w, lab, M, V, K, partial, label_logit, s);
     if (st != HK_OK) return st;
     hipLaunchKernelGGL(head_loss_kernel, dim3((M + 15) / 16), dim3(256), 0, s, (const float2*)partial, (const float*)label_logit, lab, M, V,
                        L.blocks, loss, lse);
@@ -513,8 +515,9 @@ extern "C" int hk_linear_cross_entropy_backward(const void* x_bf16, const void* 
         p.first = v0 == 0;
         p.last = v0 + p.cols == V;
         const HeadRows rows{starts, list, dw_or_null && v0 == 0 ? tiles_of(V, 256) : 0};
-        int st = L.logits256 ? launch_dlogits<LayoutTile256>(x, w, lab, lse, dloss, M, V, K, v0, p.cols, L.piece, dl, resid, rows, s)
-                             : launch_dlogits<LayoutTile128>(x, w, lab, lse, dloss, M, V, K, v0, p.cols, L.piece, dl, resid, rows, s);
+        int st = L.logits == kLayout256   ? launch_dlogits<LayoutTile256>(x, w, lab, lse, dloss, M, V, K, v0, p.cols, L.piece, dl, resid, rows, s)
+                 : L.logits == kLayout128 ? launch_dlogits<LayoutTile128>(x, w, lab, lse, dloss, M, V, K, v0, p.cols, L.piece, dl, resid, rows, s)
+                                          : launch_dlogits<LayoutTile128Deep>(x, w, lab, lse, dloss, M, V, K, v0, p.cols, L.piece, dl, resid, rows, s);
         if (st != HK_OK) return st;
         if (dw_type == 0)
             st = L.grads256 ? launch_gradients<LayoutTile256>(p, want_dx, (uint16_t*)dw_or_null, s)

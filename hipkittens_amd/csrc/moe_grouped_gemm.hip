@@ -132,21 +132,23 @@ static int launch_grouped_tile(const void* x, const void* W, const int32_t* offs
     return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
 }
 
-// The tile by prefer_tile256 with the tiles of rows that an expert has on average when the rows spread over the experts
+// The tile by choose_layout with the tiles of rows that an expert has on average when the rows spread over the experts
 // unevenly: one at least, else rows / tile + 0.6. (Forward, us, small / large: N = 4096, K = 7168, 32 experts: 1024 rows 320 / 341,
 // 4096 457 / 482, 8192 764 / 539, 65536 4130 / 2873; 128 experts of 5760 x 2880, 16384 rows 1057 / 947; 8 of 1024 x 1024, 4096 rows
 // 20 / 27. The rule's one miss there: 32 experts of 64 rows, small 428, large 359.)
-static bool grouped_use_256(int R, int E, int in, int out) {
+static LayoutChoice grouped_choice(int R, int E, int in, int out) {
     const double used = R < E ? R : E, mean = R / used;
     const double m256 = mean / 256 + 0.6, m128 = mean / 128 + 0.6;
-    return prefer_tile256(used * (m256 > 1 ? m256 : 1) * ((out + 255) / 256), used * (m128 > 1 ? m128 : 1) * ((out + 127) / 128),
-                          (in + kLayoutStep - 1) / kLayoutStep, moe_num_compute_units());
+    return choose_layout(used * (m256 > 1 ? m256 : 1) * ((out + 255) / 256), used * (m128 > 1 ? m128 : 1) * ((out + 127) / 128),
+                         (in + kLayoutStep - 1) / kLayoutStep, moe_num_compute_units());
 }
 template <bool DGRAD>
 static int launch_grouped(const void* x, const void* W, const int32_t* offsets, void* y, int R, int E, int N, int K, hipStream_t s) {
-    const int in = DGRAD ? N : K, out = DGRAD ? K : N;
-    return grouped_use_256(R, E, in, out) ? launch_grouped_tile<LayoutTile256, DGRAD>(x, W, offsets, y, R, E, N, K, s)
-                                          : launch_grouped_tile<LayoutTile128, DGRAD>(x, W, offsets, y, R, E, N, K, s);
+    switch (grouped_choice(R, E, DGRAD ? N : K, DGRAD ? K : N)) {
+        case kLayout256: return launch_grouped_tile<LayoutTile256, DGRAD>(x, W, offsets, y, R, E, N, K, s);
+        case kLayout128: return launch_grouped_tile<LayoutTile128, DGRAD>(x, W, offsets, y, R, E, N, K, s);
+        default: return launch_grouped_tile<LayoutTile128Deep, DGRAD>(x, W, offsets, y, R, E, N, K, s);
+    }
 }
 
 template <typename Tile, typename T>
@@ -175,9 +177,11 @@ static int launch_wgrad(const void* dy, const void* x, const int32_t* offsets, v
         return large < single ? launch_wgrad_tile<LayoutTile256, T>(dy, x, offsets, dW, R, E, N, K, s)
                               : launch_wgrad_tile<LayoutTile128Stages<1>, T>(dy, x, offsets, dW, R, E, N, K, s);
     }
-    return prefer_tile256(e * n256 * k256, e * n128 * k128, steps, cus, kSmallStepAcross)
-               ? launch_wgrad_tile<LayoutTile256, T>(dy, x, offsets, dW, R, E, N, K, s)
-               : launch_wgrad_tile<LayoutTile128, T>(dy, x, offsets, dW, R, E, N, K, s);
+    switch (choose_layout(e * n256 * k256, e * n128 * k128, steps, cus, kSmallStepAcross)) {
+        case kLayout256: return launch_wgrad_tile<LayoutTile256, T>(dy, x, offsets, dW, R, E, N, K, s);
+        case kLayout128: return launch_wgrad_tile<LayoutTile128, T>(dy, x, offsets, dW, R, E, N, K, s);
+        default: return launch_wgrad_tile<LayoutTile128Deep, T>(dy, x, offsets, dW, R, E, N, K, s);
+    }
 }
 
 }  // namespace hk

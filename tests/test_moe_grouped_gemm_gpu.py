@@ -39,7 +39,8 @@ def _close(got, want, size, terms, half_step):
 
 
 # enough tiles for the 256x256 kernels in every product: rows on both sides of a tile, K-steps on both sides of one and two
-LARGE = [([2049, 0, 255, 257, 1, 3000, 63, 65, 129], 3, 2312, 2056), ([4000, 1000, 4500], 0, 1544, 1800), ([9000], 9, 1800, 72)]
+LARGE = [([2049, 0, 255, 257, 1, 3000, 63, 65, 129], 3, 2312, 2056), ([4000, 1000, 4500], 0, 1544, 1800), ([9000], 9, 1800, 72),
+         ([100, 0, 64, 65, 127, 128, 129, 191, 257, 1] * 4, 0, 776, 840)]   # (tiles enough for the single-stage kernel, several K-steps)
 
 
 @pytest.mark.parametrize("case", range(len(LARGE)))
