@@ -143,8 +143,8 @@ __device__ __forceinline__ void ring_product(uint8_t* smem, const TileOperand& A
     uint32_t off1 = kRingSlot, off2 = 2 * kRingSlot;
 
     auto step = [&]<int P>(int kt) __attribute__((always_inline)) {
-        oa.advance(step_a);
-        ob.advance(step_b);
+        oa.advance(oa.opaque(step_a));   // (else multiples of it are held for the unrolled K-steps)
+        ob.advance(ob.opaque(step_b));
         const bool more = kt + 2 < nk;
         const v4i da = oa.srd(more), db = ob.srd(more);
         const uint32_t vor_a = kt + 2 == nk - 1 ? oa.tail_or : 0u, vor_b = kt + 2 == nk - 1 ? ob.tail_or : 0u;

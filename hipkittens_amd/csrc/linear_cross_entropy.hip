@@ -289,7 +289,7 @@ __global__ __launch_bounds__(256) void head_gradients_kernel(HeadPiece p, T* __r
     // The rows with a label among this wave's classes, in the order of their blocks: the first 64 of them, one per lane, with label
     // and remainder, before the product.
     const int block0 = (p.v0 + row) / 16, blocks = min(Tile::F, max(0, (p.cols - row + 15) / 16));
-    const int begin = blocks ? to_sgpr(p.starts[block0]) : 0, count = blocks ? to_sgpr(p.starts[block0 + blocks]) - begin : 0;
+    int begin = blocks ? to_sgpr(p.starts[block0]) : 0, count = blocks ? to_sgpr(p.starts[block0 + blocks]) - begin : 0;
     int my_row = 0, my_label = -1;
     float my_rest = 0.f;
     auto entries = [&](int first) {
@@ -300,8 +300,11 @@ __global__ __launch_bounds__(256) void head_gradients_kernel(HeadPiece p, T* __r
         }
     };
     entries(0);
+    asm volatile("" : "+v"(begin), "+v"(count));   // (in vector registers over the product, which needs the scalar ones)
     v4f acc[Tile::F][Tile::F];
     Tile::template product<true, true>(smem, operand_across(p.dl, 2ull * p.pitch, row0, p.M), operand_across(p.x, 2ull * p.K, col0, p.M), p.M, acc);
+    begin = to_sgpr(begin);
+    count = to_sgpr(count);
     // Their columns of x, 64 rows at a time, in this wave's part of the LDS that the product is done with, several rows
     // under way at once. (One row after another, a latency each: 8192 rows and 129280 classes, 8 entries a wave, 30 us a tile.)
     constexpr int kRowBytes = 2 * Tile::kPatch, kLanes = kRowBytes / 16, kAtOnce = 64 / kLanes;   // lanes of a row, rows of a load
@@ -384,8 +387,10 @@ struct HeadBackwardPlan {
     int splits, split_cols;
     size_t resid, starts, list, dl, sums, bytes;
     HeadBackwardPlan(int M, int V, int K) {
-        // pieces of 256 MB, and rows of at most 4 MB (32-bit offsets inside a K-step's rows)
-        const long long most = std::min((256ll << 20) / (2ll * M), 1ll << 21) / 256 * 256, all = (long long)tiles_of(V, 256) * 256;
+        // Pieces of 512 MB: a piece's items of dx are the longer and its tiles the more, the fewer pieces there are (backward, us, pieces of
+        // 128 / 256 / 512 / 2048 MB: 4096 x 201088 x 2880 11492 / 11737 / 11571 / 11331, 8192 x 129280 x 7168 34150 / 33106 / 32755 /
+        // 33109, 16384 x 50257 x 1024 7282 / 5552 / 4747 / 4644). Rows of at most 4 MB: 32-bit offsets inside a K-step's rows.
+        const long long most = std::min((512ll << 20) / (2ll * M), 1ll << 21) / 256 * 256, all = (long long)tiles_of(V, 256) * 256;
         piece = (int)std::max(256ll, std::min(most, all));
         const int cols = std::min(piece, V);
         logits = head_choice(M, cols, K);
@@ -398,7 +403,7 @@ struct HeadBackwardPlan {
         grads256 = large < small;
         const double total = grads256 ? dx256 * steps_v + dw256 * steps_m : dx128 * steps_v + dw128 * steps_m;
         const double share = total / (grads256 ? slots : 2 * slots);   // K-steps of one workgroup's place
-        const int per_split = std::max(8, std::min(steps_v, (int)share));
+        const int per_split = std::max(8, (int)std::min((double)steps_v, share));
         splits = tiles_of(steps_v, per_split);
         split_cols = tiles_of(steps_v, splits) * kLayoutStep;
         splits = tiles_of(cols, split_cols);
