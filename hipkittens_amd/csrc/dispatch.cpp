@@ -1,4 +1,4 @@
-// The dispatchers' argument checks and launches (GEMMs, the MoE layers' rows and products in training) for ordinary arguments, as a CPython module (`_dispatch`).
+// The dispatchers' argument checks and launches (GEMMs; the MoE layers' rows and products and the output head in training) for ordinary arguments, as a CPython module (`_dispatch`).
 //
 // A launch takes the runtime about 3 us; the same checks in Python, a call through ctypes and the attribute reads for it
 // took 3 (FP8, BF16) to 6 us (MXFP4 with a workspace: six tensors) on top, which is what a GEMM of a few microseconds
@@ -39,6 +39,8 @@ struct Entries {
     decltype(&hk_moe_grouped_gemm) grouped;
     decltype(&hk_moe_grouped_gemm_dgrad) grouped_dgrad;
     decltype(&hk_moe_grouped_gemm_wgrad) grouped_wgrad;
+    decltype(&hk_linear_cross_entropy) head_loss;
+    decltype(&hk_linear_cross_entropy_backward) head_gradients;
 };
 Entries entries{};
 PyTypeObject* parameter_type = nullptr;
@@ -270,6 +272,59 @@ PyObject* moe_grouped_gemm_wgrad(PyObject*, PyObject* const* args, Py_ssize_t n)
     });
 }
 
+struct Head {
+    Operand x, w, labels, ws;
+    int label_type;
+};
+// x [M, K], w [V, K], labels [M], workspace
+bool head(PyObject* x, PyObject* w, PyObject* labels, PyObject* ws, Head& h) {
+    if (!operand(x, kBf16, 2, h.x) || !operand(w, kBf16, 2, h.w) || !operand(ws, kByte, 1, h.ws)) return false;
+    h.label_type = operand(labels, {at::kLong}, 1, h.labels) ? 1 : 0;
+    if (!h.label_type && !operand(labels, kI32, 1, h.labels)) return false;
+    return h.w.cols == h.x.cols && h.labels.cols == h.x.rows && h.w.device == h.x.device && h.labels.device == h.x.device &&
+           h.ws.device == h.x.device && current(h.x.device);
+}
+bool head_rows(PyObject* o, const Head& h, Operand& out) {
+    return operand(o, kF32, 1, out) && out.cols == h.x.rows && out.device == h.x.device;
+}
+
+// (x, w, labels, loss, lse, workspace)
+PyObject* linear_cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Head h;
+        Operand loss, lse;
+        if (n != 6 || !head(args[0], args[1], args[2], args[5], h) || !head_rows(args[3], h, loss) || !head_rows(args[4], h, lse)) Py_RETURN_NONE;
+        void* s = stream_of(h.x.device);
+        return launch([&] {
+            return entries.head_loss(h.x.data, h.w.data, h.labels.data, h.label_type, (float*)loss.data, (float*)lse.data, (int)h.x.rows,
+                                     (int)h.w.rows, (int)h.x.cols, h.ws.data, (size_t)h.ws.cols, s);
+        });
+    });
+}
+
+// (x, w, labels, lse, dloss, dx or None, dw or None, workspace)
+PyObject* linear_cross_entropy_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Head h;
+        Operand lse, dloss, dx{}, dw{};
+        if (n != 8 || !head(args[0], args[1], args[2], args[7], h) || !head_rows(args[3], h, lse) || !head_rows(args[4], h, dloss) ||
+            (args[5] == Py_None && args[6] == Py_None) ||
+            (args[5] != Py_None && (!operand(args[5], kBf16, 2, dx) || dx.rows != h.x.rows || dx.cols != h.x.cols || dx.device != h.x.device)))
+            Py_RETURN_NONE;
+        bool fp32 = false;
+        if (args[6] != Py_None) {
+            fp32 = operand(args[6], kF32, 2, dw);
+            if ((!fp32 && !operand(args[6], kBf16, 2, dw)) || dw.rows != h.w.rows || dw.cols != h.w.cols || dw.device != h.x.device) Py_RETURN_NONE;
+        }
+        void* s = stream_of(h.x.device);
+        return launch([&] {
+            return entries.head_gradients(h.x.data, h.w.data, h.labels.data, h.label_type, (const float*)lse.data, (const float*)dloss.data,
+                                          args[5] != Py_None ? dx.data : nullptr, args[6] != Py_None ? dw.data : nullptr, fp32 ? 1 : 0,
+                                          (int)h.x.rows, (int)h.w.rows, (int)h.x.cols, h.ws.data, (size_t)h.ws.cols, s);
+        });
+    });
+}
+
 // The library's functions by address, in the order of Entries.
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
     constexpr int kCount = sizeof(Entries) / sizeof(void*);
@@ -288,7 +343,8 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyMethodDef methods[] = {HK_METHOD(bind), HK_METHOD(fp8_gemm), HK_METHOD(bf16_gemm), HK_METHOD(mxfp4_gemm),
                          HK_METHOD(mxfp4_quantize_rows), HK_METHOD(moe_permute), HK_METHOD(moe_permute_backward),
                          HK_METHOD(moe_unpermute_backward), HK_METHOD(moe_grouped_gemm), HK_METHOD(moe_grouped_gemm_dgrad),
-                         HK_METHOD(moe_grouped_gemm_wgrad), {nullptr, nullptr, 0, nullptr}};
+                         HK_METHOD(moe_grouped_gemm_wgrad), HK_METHOD(linear_cross_entropy),
+                         HK_METHOD(linear_cross_entropy_backward), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_dispatch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

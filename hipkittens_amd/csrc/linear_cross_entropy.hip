@@ -4,7 +4,8 @@
 //   forward   lse[m] = log sum_v exp l[m, v],  loss[m] = lse[m] - l[m, label[m]]
 //   backward  dl[m, v] = dloss[m] (exp(l[m, v] - lse[m]) - [v = label[m]]),  dx = dl W,  dW = dl^T x
 //
-// A row whose label lies outside [0, V) has no loss: loss 0, dl 0 (lse is written all the same).
+// A row whose label lies outside [0, V) has no loss: loss 0, dl 0 (lse is written all the same), and takes no part in dx and dW
+// whatever its x holds.
 //
 // Forward: one tile product; its epilogue leaves each row's maximum and sum of exponentials over the tile's columns (fp32) and
 // the label's logit, a second launch joins them column block by column block, in order. Backward, for pieces of the vocabulary:
@@ -127,8 +128,28 @@ __device__ __forceinline__ v4f bf16_quad(const uint16_t* p) {
 // where its rows begin, wave w places those of blocks 4 w .. 4 w + 3, by ballots, in order.
 struct HeadRows {
     int32_t *starts, *list;
-    int groups;   // of 256 classes; 0: not wanted
+    uint16_t* x;          // x with zeros for the rows that count for nothing
+    int groups, copies;   // workgroups of 256 classes, of kHeadCopyRows rows of x; 0: not wanted
 };
+constexpr int kHeadCopyRows = 4;
+// Rows of x for dW, whose products with dl's zeros must be zeros whatever a row without a label (padding) holds.
+__device__ __forceinline__ void head_copy_rows(const uint16_t* __restrict__ x, const HeadLabels& labels, int M, int V, int K,
+                                               uint16_t* __restrict__ out, int group) {
+    const int64_t m0 = (int64_t)group * kHeadCopyRows;
+    const int chunks = K / 8, n = (int)min((int64_t)kHeadCopyRows, M - m0) * chunks;
+    for (int c0 = threadIdx.x; c0 < n; c0 += 4 * 256) {
+        v4i row[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int c = c0 + i * 256;
+            row[i] = v4i{0, 0, 0, 0};
+            if (c < n && labels.at(m0 + c / chunks, V) >= 0) row[i] = *(const v4i*)(x + m0 * K + (int64_t)c * 8);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (c0 + i * 256 < n) *(v4i*)(out + m0 * K + (int64_t)(c0 + i * 256) * 8) = row[i];
+    }
+}
 __device__ __forceinline__ void head_label_rows(int* counts, const HeadLabels& labels, int M, int V, const HeadRows& rows, int group) {
     const int lane = lane_id(), w = wave_id(), first = group * 256 + 64 * w;
     int below = 0, in[4] = {0, 0, 0, 0};
@@ -167,7 +188,7 @@ __device__ __forceinline__ void head_label_rows(int* counts, const HeadLabels& l
 }
 
 // dl of the columns [v0, v0 + cols) of the vocabulary; `width` columns of it are written, those behind V as zeros. The first
-// `rows.groups` workgroups sort the rows by label for the launch behind this one.
+// workgroups sort the rows by label and copy x for the launch behind this one.
 template <typename Tile>
 __global__ __launch_bounds__(256) void head_dlogits_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ W,
                                                            HeadLabels labels, const float* __restrict__ lse,
@@ -176,9 +197,11 @@ __global__ __launch_bounds__(256) void head_dlogits_kernel(const uint16_t* __res
                                                            uint16_t* __restrict__ dl,
                                                            float* __restrict__ resid, HeadRows rows) {
     extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
+    const int extra = rows.groups + rows.copies;
     if ((int)blockIdx.x < rows.groups) return head_label_rows((int*)smem, labels, M, V, rows, blockIdx.x);
+    if ((int)blockIdx.x < extra) return head_copy_rows(x, labels, M, V, K, rows.x, blockIdx.x - rows.groups);
     int pm, pn;
-    banded_raster(xcd_chunk_order(blockIdx.x - rows.groups, tiles_m * tiles_n, kCuPerXcd), tiles_m, tiles_n, head_group(band_n, tiles_n), band_n, pm, pn);
+    banded_raster(xcd_chunk_order(blockIdx.x - extra, tiles_m * tiles_n, kCuPerXcd), tiles_m, tiles_n, head_group(band_n, tiles_n), band_n, pm, pn);
     const int w = wave_id(), row0 = pm * Tile::kTile, col0 = v0 + pn * Tile::kTile;
     v4f acc[Tile::F][Tile::F];
     Tile::template product<false, false>(smem, operand_along(x, 2ull * K, row0, min(M, row0 + Tile::kTile), K),
@@ -224,7 +247,7 @@ __global__ __launch_bounds__(256) void head_dlogits_kernel(const uint16_t* __res
 // dl^T x. The contraction of dx runs over the piece, a few hundred K-steps for few tiles: with dW's tiles behind it in the same
 // grid CUs that hold no item of dx work on dW from the start, and `splits` cuts it where its items would still outlast the rest.
 struct HeadPiece {
-    const uint16_t *dl, *W, *x;
+    const uint16_t *dl, *W, *x;   // x: with zeros for the rows that count for nothing
     float* sums;      // [splits][M][K]: dx so far, when there are several pieces or splits
     HeadLabels labels;
     const float* resid;              // r[m], of the rows whose label lies in this piece or an earlier one
@@ -385,7 +408,7 @@ struct HeadBackwardPlan {
     LayoutChoice logits;
     bool grads256;
     int splits, split_cols;
-    size_t resid, starts, list, dl, sums, bytes;
+    size_t resid, starts, list, x, dl, sums, bytes;
     HeadBackwardPlan(int M, int V, int K) {
         // Pieces of 512 MB: a piece's items of dx are the longer and its tiles the more, the fewer pieces there are (backward, us, pieces of
         // 128 / 256 / 512 / 2048 MB: 4096 x 201088 x 2880 11492 / 11737 / 11571 / 11331, 8192 x 129280 x 7168 34150 / 33106 / 32755 /
@@ -410,7 +433,8 @@ struct HeadBackwardPlan {
         resid = 0;
         list = up256((size_t)M * 4);
         starts = list + up256((size_t)M * 4);
-        dl = starts + up256(((size_t)tiles_of(V, 256) * 16 + 1) * 4);
+        x = starts + up256(((size_t)tiles_of(V, 256) * 16 + 1) * 4);
+        dl = x + up256((size_t)M * K * 2);
         sums = dl + up256((size_t)M * piece * 2);
         bytes = sums + (piece < V || splits > 1 ? up256((size_t)splits * M * K * 4) : 0);
     }
@@ -418,9 +442,9 @@ struct HeadBackwardPlan {
 
 static int head_check(int M, int V, int K) {
     if (M <= 0 || V <= 0 || K <= 0 || (K % 8) != 0 || M >= (1 << 30) || V >= (1 << 30) || K > (1 << 21)) return HK_ERR_BAD_SHAPE;
-    if ((long long)tiles_of(M, 128) * tiles_of(V, 128) >= (1ll << 30) || (long long)tiles_of(M, 128) * tiles_of(K, 128) >= (1ll << 30) ||
-        (long long)tiles_of(V, 128) * tiles_of(K, 128) >= (1ll << 30))
-        return HK_ERR_BAD_SHAPE;
+    // (a launch has fewer than 2^32 threads, so fewer than 2^24 workgroups; half of it for each part of the gradients' launch)
+    const long long tm = tiles_of(M, 128), tv = tiles_of(V, 128), tk = tiles_of(K, 128), most = 1ll << 23;
+    if (tm * tv >= most || tm * tk >= most || tv * tk >= most) return HK_ERR_BAD_SHAPE;
     return HK_OK;
 }
 
@@ -444,7 +468,7 @@ static int launch_dlogits(const uint16_t* x, const uint16_t* W, HeadLabels label
                           int v0, int cols, int pitch, uint16_t* dl, float* resid, HeadRows rows, hipStream_t s) {
     static DeviceOnce once;
     const int tm = tiles_of(M, Tile::kTile), tv = tiles_of(cols, Tile::kTile);
-    return launch_head<Tile>(head_dlogits_kernel<Tile>, once, (long long)tm * tv + rows.groups, s, x, W, labels, lse, dloss, M, V, K, v0,
+    return launch_head<Tile>(head_dlogits_kernel<Tile>, once, (long long)tm * tv + rows.groups + rows.copies, s, x, W, labels, lse, dloss, M, V, K, v0,
                              (cols + 7) / 8 * 8, pitch, tm, tv, raster_band(2ll * K * ((long long)M + cols), tv), dl, resid, rows);
 }
 template <typename Tile, typename T>
@@ -512,14 +536,16 @@ extern "C" int hk_linear_cross_entropy_backward(const void* x_bf16, const void* 
     const bool want_dx = dx_bf16_or_null != nullptr;
     float* resid = (float*)(ws + L.resid);
     int32_t *starts = (int32_t*)(ws + L.starts), *list = (int32_t*)(ws + L.list);
-    HeadPiece p{dl, w, x, (float*)(ws + L.sums), lab, resid, starts, list, (uint16_t*)dx_bf16_or_null, M, V, K, 0, 0, L.piece, 0, 0, 0, 0, 0, 0, L.split_cols,
+    uint16_t* x0 = (uint16_t*)(ws + L.x);
+    HeadPiece p{dl, w, x0, (float*)(ws + L.sums), lab, resid, starts, list, (uint16_t*)dx_bf16_or_null, M, V, K, 0, 0, L.piece, 0, 0, 0, 0, 0, 0, L.split_cols,
                 false, false, L.splits > 1};
     for (int v0 = 0; v0 < V; v0 += L.piece) {
         p.v0 = v0;
         p.cols = V - v0 < L.piece ? V - v0 : L.piece;
         p.first = v0 == 0;
         p.last = v0 + p.cols == V;
-        const HeadRows rows{starts, list, dw_or_null && v0 == 0 ? tiles_of(V, 256) : 0};
+        const bool first_dw = dw_or_null && v0 == 0;
+        const HeadRows rows{starts, list, x0, first_dw ? tiles_of(V, 256) : 0, first_dw ? tiles_of(M, kHeadCopyRows) : 0};
         int st = L.logits == kLayout256   ? launch_dlogits<LayoutTile256>(x, w, lab, lse, dloss, M, V, K, v0, p.cols, L.piece, dl, resid, rows, s)
                  : L.logits == kLayout128 ? launch_dlogits<LayoutTile128>(x, w, lab, lse, dloss, M, V, K, v0, p.cols, L.piece, dl, resid, rows, s)
                                           : launch_dlogits<LayoutTile128Deep>(x, w, lab, lse, dloss, M, V, K, v0, p.cols, L.piece, dl, resid, rows, s);

@@ -14,6 +14,7 @@
 namespace hk {
 
 constexpr int kGroupedMaxE = 512;
+constexpr long long kMaxWorkgroups = 1ll << 24;   // of 256 threads: a launch has fewer than 2^32
 
 struct GroupedTile { int expert, row0, rows, tile_n; };   // expert < 0: no such tile
 
@@ -123,7 +124,7 @@ template <typename Tile, bool DGRAD>
 static int launch_grouped_tile(const void* x, const void* W, const int32_t* offsets, void* y, int R, int E, int N, int K, hipStream_t s) {
     const int tiles_n = ((DGRAD ? K : N) + Tile::kTile - 1) / Tile::kTile;
     const long long grid = grouped_tiles_m(R, E, Tile::kTile) * tiles_n;
-    if (grid >= (1ll << 31)) return HK_ERR_BAD_SHAPE;
+    if (grid >= kMaxWorkgroups) return HK_ERR_BAD_SHAPE;
     auto kern = grouped_gemm_kernel<Tile, DGRAD>;
     static DeviceOnce configured;
     if (!set_lds_limit_once((const void*)kern, Tile::kLds, configured)) return HK_ERR_LAUNCH;
@@ -155,7 +156,7 @@ template <typename Tile, typename T>
 static int launch_wgrad_tile(const void* dy, const void* x, const int32_t* offsets, void* dW, int R, int E, int N, int K, hipStream_t s) {
     const int tiles_m = (N + Tile::kTile - 1) / Tile::kTile, tiles_n = (K + Tile::kTile - 1) / Tile::kTile;
     const long long grid = (long long)E * tiles_m * tiles_n;
-    if (grid >= (1ll << 31)) return HK_ERR_BAD_SHAPE;
+    if (grid >= kMaxWorkgroups) return HK_ERR_BAD_SHAPE;
     auto kern = grouped_wgrad_kernel<Tile, T>;
     static DeviceOnce configured;
     if (!set_lds_limit_once((const void*)kern, Tile::kLds, configured)) return HK_ERR_LAUNCH;

@@ -91,7 +91,8 @@ __global__ __launch_bounds__(256) void moe_unpermute_backward_kernel(const uint1
 }
 
 static int permute_check(int T, int k, int H, uintptr_t pointers) {
-    if (T <= 0 || k <= 0 || H <= 0 || (H % 8) != 0 || (long long)T * k > (1ll << 30)) return HK_ERR_BAD_SHAPE;
+    // (a workgroup of 256 threads per token, and a launch has fewer than 2^32)
+    if (T <= 0 || T >= (1 << 24) || k <= 0 || H <= 0 || (H % 8) != 0 || (long long)T * k > (1ll << 30)) return HK_ERR_BAD_SHAPE;
     return (pointers & 15u) ? HK_ERR_BAD_ALIGNMENT : HK_OK;
 }
 

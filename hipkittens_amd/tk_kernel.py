@@ -57,6 +57,7 @@ class _NoNative:
     bf16_gemm = mxfp4_gemm = mxfp4_quantize_rows = fp8_gemm
     moe_permute = moe_permute_backward = moe_unpermute_backward = fp8_gemm
     moe_grouped_gemm = moe_grouped_gemm_dgrad = moe_grouped_gemm_wgrad = fp8_gemm
+    linear_cross_entropy = linear_cross_entropy_backward = fp8_gemm
 
 
 def _load_native():
@@ -846,6 +847,9 @@ def dispatch_linear_cross_entropy(x, w, labels, loss, lse, workspace) -> None:
     """Softmax cross entropy of the logits x @ w.T, which are never in memory: lse[m] = log sum exp of row m's logits,
     loss[m] = lse[m] - the label's logit; 0 for a label outside [0, V) (torch's -100, say). x [M,K], w [V,K] bf16, labels [M]
     int32 or int64, loss and lse [M] fp32. workspace: linear_cross_entropy_workspace_bytes(M, V, K, backward=False) bytes."""
+    st = (_native or _load_native()).linear_cross_entropy(x, w, labels, loss, lse, workspace)
+    if st is not None:
+        return _lib.check(st, "dispatch_linear_cross_entropy")
     M, V, K = _check_head(x, w, labels, ((loss, "loss"), (lse, "lse")), workspace)
     with torch.cuda.device(x.device):
         st = _lib.load_library().hk_linear_cross_entropy(
@@ -856,8 +860,11 @@ def dispatch_linear_cross_entropy(x, w, labels, loss, lse, workspace) -> None:
 
 def dispatch_linear_cross_entropy_backward(x, w, labels, lse, dloss, dx, dw, workspace) -> None:
     """Gradients of dispatch_linear_cross_entropy for dloss [M] fp32 (the gradient of each row's loss) and the forward's lse:
-    dx [M,K] bf16 and dw [V,K] bf16 or fp32; either may be None. A row whose label lies outside [0, V) has no gradient.
-    workspace: linear_cross_entropy_workspace_bytes(M, V, K) bytes."""
+    dx [M,K] bf16 and dw [V,K] bf16 or fp32; either may be None. A row whose label lies outside [0, V) has no gradient,
+    whatever its x holds. workspace: linear_cross_entropy_workspace_bytes(M, V, K) bytes."""
+    st = (_native or _load_native()).linear_cross_entropy_backward(x, w, labels, lse, dloss, dx, dw, workspace)
+    if st is not None:
+        return _lib.check(st, "dispatch_linear_cross_entropy_backward")
     M, V, K = _check_head(x, w, labels, ((lse, "lse"), (dloss, "dloss")), workspace)
     if dx is None and dw is None:
         raise RuntimeError("one of dx and dw must be given")

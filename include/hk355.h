@@ -474,7 +474,7 @@ int hk_moe_fp8blk_forward_bf16(const void* x_bf16, const float* router_logits,
 
 /* Rows to the order of their experts: xp[slot_to_pos[t*k+j], :] = x[t, :]. x [T, H], xp [T*k, H] bf16. A position outside
  * [0, T*k) has no row; rows of xp that no slot names stay as they were. Positions inside must differ from one another (two
- * slots with one position: one of the two rows stands there). H % 8 == 0, T*k <= 2^30; x and xp must not overlap. */
+ * slots with one position: one of the two rows stands there). H % 8 == 0, T < 2^24, T*k <= 2^30; x and xp must not overlap. */
 int hk_moe_permute(const void* x_bf16, const int32_t* slot_to_pos, int T, int k, int H, void* xp_bf16, void* stream);
 /* Its gradient: dx[t, :] = bf16(add[t, :] + sum_j dxp[slot_to_pos[t*k+j], :]), add [T, H] bf16 or NULL (it may be dx itself).
  * A token without a row gets add, or zeros. */
@@ -489,8 +489,8 @@ int hk_moe_unpermute_backward(const void* dy_bf16, const void* o_bf16, const flo
 /* The experts' products in bf16: y[r, :] = bf16(x[r, :] W[e]^T) for the rows r of [expert_offsets[e], expert_offsets[e+1]).
  * x [R, K], w [E, N, K], y [R, N]; expert_offsets [E+1] int32 on the device, ascending, the last at most R. Rows behind it
  * are neither read nor written, and an expert's result depends on its own rows only. (Offsets are held inside [0, R] and in
- * order whatever they hold.) Requirements: N % 8 == 0, K % 8 == 0, both at most 2^21, E <= 512, R < 2^30, all of x, w, y
- * 16-byte aligned; no workspace. */
+ * order whatever they hold.) Requirements: N % 8 == 0, K % 8 == 0, both at most 2^21, E <= 512, R < 2^30, fewer than 2^24
+ * tiles of 128 x 128 in all; x, w and y 16-byte aligned; no workspace. */
 int hk_moe_grouped_gemm(const void* x_bf16, const void* w_bf16, const int32_t* expert_offsets, void* y_bf16, int R, int E,
                         int N, int K, void* stream);
 /* Its gradients: dx[r, :] = bf16(dy[r, :] W[e]), and dw[e] = sum over the expert's rows of dy[r, :]^T x[r, :] (dw [E, N, K], bf16 with
@@ -502,17 +502,18 @@ int hk_moe_grouped_gemm_wgrad(const void* dy_bf16, const void* x_bf16, const int
 
 /* Softmax cross entropy of the logits x W^T without the logits in memory: lse[m] = log sum_v exp(x[m] . w[v]) and
  * loss[m] = lse[m] - x[m] . w[label[m]]. x [M, K], w [V, K] bf16; labels [M] int32 (label_type 0) or int64 (1); loss, lse [M]
- * fp32. A label outside [0, V) counts for nothing: loss 0 (lse is written). Requirements: K % 8 == 0, K <= 2^21,
- * M, V < 2^30, x and w 16-byte aligned; workspace: hk_linear_cross_entropy_workspace_bytes(M, V, K, 0) bytes, 16-byte
- * aligned, nothing in it is kept from one call to the next. */
+ * fp32. A label outside [0, V) counts for nothing: loss 0 (lse is written). Requirements: K % 8 == 0, K <= 2^21, M, V < 2^30,
+ * fewer than 2^23 tiles of 128 x 128 in M x V, M x K and V x K; x and w 16-byte aligned; workspace 16-byte aligned, of
+ * hk_linear_cross_entropy_workspace_bytes(M, V, K, 0) bytes (0 for a shape that is refused), nothing in it is kept from one
+ * call to the next. */
 size_t hk_linear_cross_entropy_workspace_bytes(int M, int V, int K, int backward);
 int hk_linear_cross_entropy(const void* x_bf16, const void* w_bf16, const void* labels, int label_type, float* loss, float* lse,
                             int M, int V, int K, void* workspace, size_t workspace_bytes, void* stream);
 /* Its gradients for dloss [M] fp32 (the gradient of each row's loss; for a mean 1 / rows that count) and the forward's lse:
  * dl[m,v] = dloss[m] * (exp(x[m] . w[v] - lse[m]) - [v = label[m]]), 0 for a row whose label counts for nothing (whatever its
  * dloss and lse are); dx [M, K] = bf16(dl w), dw [V, K] = dl^T x in bf16 (dw_type 0) or fp32 (1). Either of dx and dw may be
- * NULL. Goes over the vocabulary in pieces; dl of a piece is held in bf16. A row that counts for nothing is still multiplied by
- * its zeros in dw: its x has to be finite. workspace: hk_linear_cross_entropy_workspace_bytes(M, V, K, 1) bytes (enough for
+ * NULL. Goes over the vocabulary in pieces; dl of a piece is held in bf16 (its label's term with an fp32 remainder). A row that counts for
+ * nothing takes no part, whatever its x holds. workspace: hk_linear_cross_entropy_workspace_bytes(M, V, K, 1) bytes (enough for
  * the forward too). */
 int hk_linear_cross_entropy_backward(const void* x_bf16, const void* w_bf16, const void* labels, int label_type,
                                      const float* lse, const float* dloss, void* dx_bf16_or_null, void* dw_or_null, int dw_type,

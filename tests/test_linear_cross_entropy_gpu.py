@@ -120,6 +120,15 @@ def test_every_row_ignored_and_rows_that_do_not_count(hk):
     none = torch.full_like(labels, -100)
     loss, lse, dx, dw = _run(hk, x, w, none, torch.full_like(dloss, float("nan")))
     assert torch.all(loss == 0) and torch.all(dx == 0) and torch.all(dw == 0)
+    # rows without a label take no part, whatever they hold
+    pad = torch.arange(M, device=DEV) % 7 == 3
+    some = torch.where(pad, -100, labels)
+    clean = _run(hk, x, w, some, dloss)
+    x2 = x.clone()
+    x2[pad] = float("nan")
+    x2[3] = float("inf")
+    got = _run(hk, x2, w, some, torch.where(pad, float("nan"), dloss))
+    assert torch.equal(got[0], clean[0]) and torch.equal(got[2], clean[2]) and torch.equal(got[3], clean[3])
     # a row's NaN or infinity stays in its row of loss, lse and dx
     labels[10] = -100
     x2 = x.clone()

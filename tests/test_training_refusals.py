@@ -23,7 +23,7 @@ def test_permute_family(p):
         args = [p, p, 4, 2, 64, p, None]
         args[at] = None
         assert lib.hk_moe_permute(*args) == NULL
-    for T, k, H in ((0, 2, 64), (4, 0, 64), (4, 2, 0), (4, 2, 60), (-1, 2, 64), (1 << 29, 3, 64), (IMAX, IMAX, 8)):
+    for T, k, H in ((1 << 24, 1, 64), (0, 2, 64), (4, 0, 64), (4, 2, 0), (4, 2, 60), (-1, 2, 64), (1 << 29, 3, 64), (IMAX, IMAX, 8)):
         assert lib.hk_moe_permute(p, p, T, k, H, p, None) == SHAPE
         assert lib.hk_moe_permute_backward(p, p, T, k, H, None, p, None) == SHAPE
         assert lib.hk_moe_unpermute_backward(p, p, p, p, T, k, H, p, p, None) == SHAPE
@@ -48,6 +48,9 @@ def test_grouped_products(p):
         assert lib.hk_moe_grouped_gemm(p, p, p, p, R, E, N, K, None) == SHAPE
         assert lib.hk_moe_grouped_gemm_dgrad(p, p, p, p, R, E, N, K, None) == SHAPE
         assert lib.hk_moe_grouped_gemm_wgrad(p, p, p, p, 0, R, E, N, K, None) == SHAPE
+    # more tiles than a launch has workgroups
+    assert lib.hk_moe_grouped_gemm(p, p, p, p, 1 << 29, 1, 1 << 20, 64, None) == SHAPE
+    assert lib.hk_moe_grouped_gemm_wgrad(p, p, p, p, 0, 64, 512, 1 << 16, 1 << 16, None) == SHAPE
     assert lib.hk_moe_grouped_gemm(p + 8, p, p, p, 4, 2, 64, 64, None) == ALIGN
     assert lib.hk_moe_grouped_gemm_dgrad(p, p + 2, p, p, 4, 2, 64, 64, None) == ALIGN
     assert lib.hk_moe_grouped_gemm_wgrad(p, p, p, p + 4, 1, 4, 2, 64, 64, None) == ALIGN
@@ -67,7 +70,7 @@ def test_linear_cross_entropy(p):
         assert lib.hk_linear_cross_entropy_backward(*args) == NULL
     assert lib.hk_linear_cross_entropy_backward(p, p, p, 1, p, p, None, None, 0, 4, 100, 64, p, big, None) == NULL
     for M, V, K in ((0, 100, 64), (4, 0, 64), (4, 100, 0), (4, 100, 60), (1 << 30, 100, 64), (4, 1 << 30, 64),
-                    (1 << 25, 1 << 25, 64), (4, 100, (1 << 21) + 8)):
+                    (1 << 25, 1 << 25, 64), (1 << 20, 1 << 20, 64), (4, 100, (1 << 21) + 8)):
         assert lib.hk_linear_cross_entropy(p, p, p, 1, p, p, M, V, K, p, big, None) == SHAPE
         assert lib.hk_linear_cross_entropy_backward(p, p, p, 1, p, p, p, p, 0, M, V, K, p, big, None) == SHAPE
         assert lib.hk_linear_cross_entropy_workspace_bytes(M, V, K, 0) == 0
@@ -86,7 +89,7 @@ def test_linear_cross_entropy(p):
     assert lib.hk_linear_cross_entropy_backward(p, p, p, 1, p, p, p, p, 0, 4, 100, 64, None, both, None) == WORKSPACE
     # the logits are not kept: far less than M x V bytes for many rows and classes, and no overflow in the sizes
     assert 0 < lib.hk_linear_cross_entropy_workspace_bytes(16384, 201088, 2880, 1) < 16384 * 201088 // 4
-    assert lib.hk_linear_cross_entropy_workspace_bytes(1 << 22, 201088, 64, 0) >= (1 << 22) * 4
+    assert lib.hk_linear_cross_entropy_workspace_bytes(1 << 19, 201088, 64, 0) >= (1 << 19) * 201088 // 128 * 8
 
 
 def test_python_boundary():
