@@ -89,17 +89,18 @@ __global__ __launch_bounds__(256) void grouped_wgrad_kernel(const uint16_t* __re
     int pm, pn;
     grouped_raster(id - e * tiles_m * tiles_n, tiles_m, tiles_n, 8, pm, pn);
     const int lo = to_sgpr(min(max(offsets[e], 0), R)), rows = to_sgpr(min(max(offsets[e + 1], lo), R)) - lo;
+    if (rows == 0) {   // zeros, in one run per workgroup
+        constexpr int kVec = 16 / sizeof(T);
+        const size_t n = (size_t)N * K / kVec, run = (n + tiles_m * tiles_n - 1) / (tiles_m * tiles_n);
+        const size_t from = (size_t)(id - e * tiles_m * tiles_n) * run, to = min(n, from + run);
+        v4i* out = (v4i*)(dW + (size_t)e * N * K);
+        for (size_t i = from + threadIdx.x; i < to; i += 256) out[i] = v4i{0, 0, 0, 0};
+        return;
+    }
     const int row0 = pm * Tile::kTile, col0 = pn * Tile::kTile;
     v4f acc[Tile::F][Tile::F];
-    if (rows > 0) {
-        Tile::template product<true, true>(smem, operand_across(dy + (size_t)lo * N, 2ull * N, row0, rows),
-                                           operand_across(x + (size_t)lo * K, 2ull * K, col0, rows), rows, acc);
-    } else {
-#pragma unroll
-        for (int m = 0; m < Tile::F; ++m)
-#pragma unroll
-            for (int n = 0; n < Tile::F; ++n) acc[m][n] = v4f{0.f, 0.f, 0.f, 0.f};
-    }
+    Tile::template product<true, true>(smem, operand_across(dy + (size_t)lo * N, 2ull * N, row0, rows),
+                                       operand_across(x + (size_t)lo * K, 2ull * K, col0, rows), rows, acc);
     const int w = wave_id(), row = row0 + (w >> 1) * Tile::kPatch, col = col0 + (w & 1) * Tile::kPatch;
     store_patch(acc, dW + (size_t)e * N * K + (size_t)row * K + col, K, N - row, K - col);
 }
