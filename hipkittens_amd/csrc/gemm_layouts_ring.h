@@ -234,9 +234,9 @@ __device__ __forceinline__ void ring_product(uint8_t* smem, const TileOperand& A
 
 // 128x128 tiles in the same manner, for problems with no more tiles than CUs, where one workgroup has a CU to itself: four LDS
 // stages, three K-steps ahead, the next K-step's fragments read behind the MFMAs of this one (a quarter of the tile and 32
-// MFMAs a wave and K-step). (Weight gradient of 16384 rows, 64 tiles of 256 K-steps:
-// 155 us with two stages, 117 here, now bound by the loads' latency; loss of 100 x 10000 x 4096 52 / 39; 16 rows of 4 experts of 4096 x 4096
-// 45 / 33.)
+// MFMAs a wave and K-step). Weight gradient of 16384 rows, 64 tiles of 256 K-steps: 155 us with two stages, 117 here, 31 bytes
+// a clock into each CU, which bounds it (five stages: 116); loss of 100 x 10000 x 4096 52 / 39; 16 rows of 4 experts of 4096 x 4096
+// 45 / 33.
 constexpr int kDeepStages = 4, kDeepStage = 2 * kLayoutTile * 128;
 template <bool A_ACROSS, bool B_ACROSS>
 __device__ __forceinline__ void deep_product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K, v4f (&acc)[4][4]) {

@@ -136,66 +136,74 @@ __device__ __forceinline__ v4f bf16_quad(const uint16_t* p) {
 
 // Rows by the block of 16 classes that holds their label: list = the rows of block 0, of block 1, .. in ascending order,
 // starts[b] = where block b's begin (blocks + 1 entries). One workgroup per 256 classes: the labels below its first class tell
-// where its rows begin, wave w places those of blocks 4 w .. 4 w + 3, by ballots, in order.
+// where its rows begin. Each wave takes a quarter of the rows, in order, twice: to count (lane b < 16: rows of block b) and to place.
+// Eight times 64 labels are read at a time; rows among the 256 classes are few, and taken one by one.
 struct HeadRows {
     int32_t *starts, *list;
     uint16_t* x;          // x with zeros for the rows that count for nothing
     int groups, copies;   // workgroups of 256 classes, of kHeadCopyRows rows of x; 0: not wanted
 };
-constexpr int kHeadCopyRows = 4;
+constexpr int kHeadCopyRows = 8;
 // Rows of x for dW, whose products with dl's zeros must be zeros whatever a row without a label (padding) holds.
 __device__ __forceinline__ void head_copy_rows(const uint16_t* __restrict__ x, const HeadLabels& labels, int M, int V, int K,
                                                uint16_t* __restrict__ out, int group) {
     const int64_t m0 = (int64_t)group * kHeadCopyRows;
     const int chunks = K / 8, n = (int)min((int64_t)kHeadCopyRows, M - m0) * chunks;
-    for (int c0 = threadIdx.x; c0 < n; c0 += 4 * 256) {
-        v4i row[4];
+    for (int c0 = threadIdx.x; c0 < n; c0 += 8 * 256) {
+        v4i row[8];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 8; ++i) {
             const int c = c0 + i * 256;
             row[i] = v4i{0, 0, 0, 0};
             if (c < n && labels.at(m0 + c / chunks, V) >= 0) row[i] = *(const v4i*)(x + m0 * K + (int64_t)c * 8);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 8; ++i)
             if (c0 + i * 256 < n) *(v4i*)(out + m0 * K + (int64_t)(c0 + i * 256) * 8) = row[i];
     }
 }
 __device__ __forceinline__ void head_label_rows(int* counts, const HeadLabels& labels, int M, int V, const HeadRows& rows, int group) {
-    const int lane = lane_id(), w = wave_id(), first = group * 256 + 64 * w;
-    int below = 0, in[4] = {0, 0, 0, 0};
-    for (int m0 = 0; m0 < M; m0 += 64) {
-        const int label = m0 + lane < M ? labels.at(m0 + lane, V) : -1;
-        below += __popcll(__ballot(label >= 0 && label < group * 256));
+    const int lane = lane_id(), w = wave_id(), first = group * 256;
+    const int quarter = (M + 3) / 4, from = min(w * quarter, M), to = min(from + quarter, M);
+    int below = 0;
+    // found(row, block), wave by wave in the order of the rows
+    auto scan = [&](auto found) __attribute__((always_inline)) {
+        for (int m0 = from; m0 < to; m0 += 8 * 64) {
+            int label[8];
 #pragma unroll
-        for (int b = 0; b < 4; ++b) in[b] += __popcll(__ballot(label >= first + 16 * b && label < first + 16 * b + 16));
-    }
-    if (lane == 0) {
+            for (int i = 0; i < 8; ++i) label[i] = m0 + 64 * i + lane < to ? labels.at(m0 + 64 * i + lane, V) : -1;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) counts[4 * w + b] = in[b];
-    }
-    __syncthreads();
-    int at[4], run = below;
-#pragma unroll
-    for (int b = 0; b < 16; ++b) {
-        if (b >> 2 == w) at[b & 3] = run;
-        run += counts[b];
-    }
-    if (lane == 0) {
-#pragma unroll
-        for (int b = 0; b < 4; ++b) rows.starts[group * 16 + 4 * w + b] = at[b];
-        if (w == 3 && group == rows.groups - 1) rows.starts[rows.groups * 16] = run;
-    }
-    for (int m0 = 0; m0 < M; m0 += 64) {
-        const int label = m0 + lane < M ? labels.at(m0 + lane, V) : -1;
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const bool mine = label >= first + 16 * b && label < first + 16 * b + 16;
-            const uint64_t all = __ballot(mine);
-            if (mine) rows.list[at[b] + __popcll(all & ((1ull << lane) - 1ull))] = m0 + lane;
-            at[b] += __popcll(all);
+            for (int i = 0; i < 8; ++i) {
+                below += __popcll(__ballot(label[i] >= 0 && label[i] < first));
+                uint64_t in = __ballot(label[i] >= first && label[i] < first + 256);
+                while (in) {
+                    const int l = __ffsll((unsigned long long)in) - 1;
+                    in &= in - 1;
+                    found(m0 + 64 * i + l, (__builtin_amdgcn_readlane(label[i], l) - first) / 16);
+                }
+            }
         }
+    };
+    int mine = 0;
+    scan([&](int, int block) __attribute__((always_inline)) { mine += lane == block ? 1 : 0; });
+    if (lane < 16) counts[w * 17 + lane] = mine;
+    if (lane == 16) counts[w * 17 + 16] = below;
+    __syncthreads();
+    int at = 0;   // lane b: where this wave's first row of block b goes
+    if (lane <= 16) {
+        for (int v = 0; v < 4; ++v) {
+            at += counts[v * 17 + 16];
+            for (int b = 0; b < lane; ++b) at += counts[v * 17 + b];
+        }
+        if (w == 0 && (lane < 16 || group == rows.groups - 1)) rows.starts[group * 16 + lane] = at;
+        if (lane < 16)
+            for (int v = 0; v < w; ++v) at += counts[v * 17 + lane];
     }
+    scan([&](int row, int block) __attribute__((always_inline)) {
+        const int pos = __builtin_amdgcn_readlane(at, block);
+        if (lane == 0) rows.list[pos] = row;
+        at += lane == block ? 1 : 0;
+    });
 }
 
 // dl of the columns [v0, v0 + cols) of the vocabulary; `width` columns of it are written, those behind V as zeros. The last
