@@ -1,4 +1,5 @@
-// The dispatchers' argument checks and launches (GEMMs; the MoE layers' rows and products and the output head in training) for ordinary arguments, as a CPython module (`_dispatch`).
+// The dispatchers' argument checks and launches (GEMMs; the MoE layers' rows and products and the output head in training)
+// for ordinary arguments, as a CPython module (`_dispatch`).
 //
 // A launch takes the runtime about 3 us; the same checks in Python, a call through ctypes and the attribute reads for it
 // took 3 (FP8, BF16) to 6 us (MXFP4 with a workspace: six tensors) on top, which is what a GEMM of a few microseconds

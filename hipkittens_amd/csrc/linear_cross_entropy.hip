@@ -461,8 +461,9 @@ struct HeadBackwardPlan {
 };
 
 static int head_check(int M, int V, int K) {
-    if (M <= 0 || V <= 0 || K <= 0 || (K % 8) != 0 || M >= (1 << 30) || V >= (1 << 30) || K > (1 << 21)) return HK_ERR_BAD_SHAPE;
-    // (a launch has fewer than 2^32 threads, so fewer than 2^24 workgroups; half of it for each part of the gradients' launch)
+    // (a launch has fewer than 2^32 threads: the join takes 64 a row. So fewer than 2^24 workgroups of 256: half of it for the tiles, or for each
+    // part of the gradients' launch, a quarter each for the copies of kHeadCopyRows rows and for the sort by label)
+    if (M <= 0 || V <= 0 || K <= 0 || (K % 8) != 0 || M >= (1 << 25) || V >= (1 << 30) || K > (1 << 21)) return HK_ERR_BAD_SHAPE;
     const long long tm = tiles_of(M, 128), tv = tiles_of(V, 128), tk = tiles_of(K, 128), most = 1ll << 23;
     if (tm * tv >= most || tm * tk >= most || tv * tk >= most) return HK_ERR_BAD_SHAPE;
     return HK_OK;

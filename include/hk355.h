@@ -470,6 +470,7 @@ int hk_moe_fp8blk_forward_bf16(const void* x_bf16, const float* router_logits,
  * No counterpart in the reference. bf16 activations, gradients and weights, fp32 accumulation and statistics, every result
  * rounded once. Nothing here uses atomics: results are the same on every call. Tables of positions and offsets are those of
  * hk_moe_sort; prefill slot_to_pos with -1 where ids outside [0, E) may occur (the sort leaves such slots' entries alone).
+ * Outputs and workspaces overlap neither the inputs nor one another, where nothing else is said.
  */
 
 /* Rows to the order of their experts: xp[slot_to_pos[t*k+j], :] = x[t, :]. x [T, H], xp [T*k, H] bf16. A position outside
@@ -502,7 +503,7 @@ int hk_moe_grouped_gemm_wgrad(const void* dy_bf16, const void* x_bf16, const int
 
 /* Softmax cross entropy of the logits x W^T without the logits in memory: lse[m] = log sum_v exp(x[m] . w[v]) and
  * loss[m] = lse[m] - x[m] . w[label[m]]. x [M, K], w [V, K] bf16; labels [M] int32 (label_type 0) or int64 (1); loss, lse [M]
- * fp32. A label outside [0, V) counts for nothing: loss 0 (lse is written). Requirements: K % 8 == 0, K <= 2^21, M, V < 2^30,
+ * fp32. A label outside [0, V) counts for nothing: loss 0 (lse is written). Requirements: K % 8 == 0, K <= 2^21, M < 2^25, V < 2^30,
  * fewer than 2^23 tiles of 128 x 128 in M x V, M x K and V x K; x and w 16-byte aligned; workspace 16-byte aligned, of
  * hk_linear_cross_entropy_workspace_bytes(M, V, K, 0) bytes (0 for a shape that is refused), nothing in it is kept from one
  * call to the next. */

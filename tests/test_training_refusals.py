@@ -141,3 +141,14 @@ def test_python_boundary_shapes_and_types():
         with pytest.raises(RuntimeError):
             call()
     torch.cuda.synchronize()
+
+
+def test_linear_cross_entropy_rows_of_one_launch(p):
+    """Launches of 64 threads a row, and of a workgroup per eight rows and per 256 classes beside the tiles', hold fewer than
+    2^32 threads: more rows are refused, not left to the launch."""
+    lib = hk.load_library()
+    for M, V in ((1 << 25, 100), (1 << 26, 1), (1 << 27, 100), ((1 << 30) - 1, 8)):
+        assert lib.hk_linear_cross_entropy(p, p, p, 1, p, p, M, V, 8, p, 1 << 60, None) == SHAPE
+        assert lib.hk_linear_cross_entropy_backward(p, p, p, 1, p, p, p, p, 0, M, V, 8, p, 1 << 60, None) == SHAPE
+        assert lib.hk_linear_cross_entropy_workspace_bytes(M, V, 8, 1) == 0
+    assert lib.hk_linear_cross_entropy_workspace_bytes((1 << 25) - 1, 100, 8, 1) > 0
