@@ -262,9 +262,10 @@ __global__ __launch_bounds__(256) void head_dlogits_kernel(const uint16_t* __res
     }
 }
 
-// Both gradients of one piece in one launch: first the items of dx, dl [M, cols] W [cols rows from v0 on], then those of dW,
-// dl^T x. The contraction of dx runs over the piece, a few hundred K-steps for few tiles: with dW's tiles behind it in the same
-// grid CUs that hold no item of dx work on dW from the start, and `splits` cuts it where its items would still outlast the rest.
+// Both gradients of one piece in one launch, the items of dx, dl [M, cols] W [cols rows from v0 on], and those of dW, dl^T x, the
+// longer ones first (65536 x 32000 x 1024 with dx's always first 18501 us, 15444 so, both with pieces of 4096 classes). The contraction of
+// dx runs over the piece, a few hundred K-steps for few tiles: with dW's tiles behind it in the same grid CUs that hold no item of dx
+// work on dW from the start, and `splits` cuts it where its items would still outlast the rest.
 struct HeadPiece {
     const uint16_t *dl, *W, *x;   // x: with zeros for the rows that count for nothing
     float* sums;      // [splits][M][K]: dx so far, when there are several pieces or splits
@@ -275,6 +276,7 @@ struct HeadPiece {
     int M, V, K, v0, cols, pitch;
     int tiles_m, tiles_k, tiles_v, band_dx, band_dw, splits, split_cols;   // splits 0: no dx; tiles_v 0: no dW
     bool first, last, reduce;   // reduce: a launch of its own adds the splits and rounds
+    bool dw_first;    // dW's tiles are the longer ones
 };
 
 template <typename Tile>
@@ -318,13 +320,15 @@ __device__ __forceinline__ void head_dx_item(uint8_t* smem, const HeadPiece& p, 
 template <typename Tile, typename T>
 __global__ __launch_bounds__(256) void head_gradients_kernel(HeadPiece p, T* __restrict__ dw) {
     extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
-    const int dx_items = p.splits * p.tiles_m * p.tiles_k;
-    if ((int)blockIdx.x < dx_items) {
-        head_dx_item<Tile>(smem, p, xcd_chunk_order(blockIdx.x, dx_items, kCuPerXcd));
+    const int dx_items = p.splits * p.tiles_m * p.tiles_k, dw_items = p.tiles_v * p.tiles_k;
+    const int dx_id = (int)blockIdx.x - (p.dw_first ? dw_items : 0);
+    if (dx_id >= 0 && dx_id < dx_items) {
+        head_dx_item<Tile>(smem, p, xcd_chunk_order(dx_id, dx_items, kCuPerXcd));
         return;
     }
     int pm, pn;
-    banded_raster(xcd_chunk_order(blockIdx.x - dx_items, p.tiles_v * p.tiles_k, kCuPerXcd), p.tiles_v, p.tiles_k, head_group(p.band_dw, p.tiles_k), p.band_dw, pm, pn);
+    banded_raster(xcd_chunk_order((int)blockIdx.x - (p.dw_first ? 0 : dx_items), dw_items, kCuPerXcd), p.tiles_v, p.tiles_k,
+                  head_group(p.band_dw, p.tiles_k), p.band_dw, pm, pn);
     const int lane = lane_id(), r = lane & 15, g = lane >> 4;
     const int w = wave_id(), row0 = pm * Tile::kTile, col0 = pn * Tile::kTile;
     const int row = row0 + (w >> 1) * Tile::kPatch, col = col0 + (w & 1) * Tile::kPatch;
@@ -432,8 +436,13 @@ struct HeadBackwardPlan {
     HeadBackwardPlan(int M, int V, int K) {
         // Pieces of 512 MB: a piece's items of dx are the longer and its tiles the more, the fewer pieces there are (backward, us, pieces of
         // 128 / 256 / 512 / 2048 MB: 4096 x 201088 x 2880 11492 / 11737 / 11571 / 11331, 8192 x 129280 x 7168 34150 / 33106 / 32755 /
-        // 33109, 16384 x 50257 x 1024 7282 / 5552 / 4747 / 4644). Rows of at most 4 MB: 32-bit offsets inside a K-step's rows.
-        const long long most = std::min((512ll << 20) / (2ll * M), 1ll << 21) / 256 * 256, all = (long long)tiles_of(V, 256) * 256;
+        // 33109, 16384 x 50257 x 1024 7282 / 5552 / 4747 / 4644). Where that gives dW fewer tiles than CUs (many rows, few columns of x: tiles
+        // of M / 64 K-steps, and the rest of the chip idle), as many classes as fill the CUs, up to 4 GB and half of dl (512 MB / 1 / 2 / 4 GB
+        // at most: 65536 x 32000 x 1024 15444 / 11947 / 11416 / 11394, 262144 x 32000 x 1024 180717 / 104194 / 65851 / 47530).
+        // Rows of at most 4 MB: 32-bit offsets inside a K-step's rows.
+        const long long fill = 256ll * tiles_of(moe_num_compute_units(), tiles_of(K, 256));
+        const long long held = std::max(512ll << 20, std::min({2ll * M * fill, 4ll << 30, 512ll * M * tiles_of(V, 512)}));
+        const long long most = std::min(held / (2ll * M), 1ll << 21) / 256 * 256, all = (long long)tiles_of(V, 256) * 256;
         piece = (int)std::max(256ll, std::min(most, all));
         const int cols = std::min(piece, V);
         logits = head_choice(M, cols, K);
@@ -501,6 +510,7 @@ static int launch_gradients(HeadPiece p, bool dx, T* dw, hipStream_t s) {
     p.band_dx = raster_band(2ll * p.cols * ((long long)p.M + p.K), p.tiles_k);
     p.band_dw = raster_band(2ll * p.M * ((long long)p.cols + p.K), p.tiles_k);
     p.splits = dx ? tiles_of(p.cols, p.split_cols) : 0;
+    p.dw_first = p.M > p.split_cols;
     const long long items = (long long)p.splits * p.tiles_m * p.tiles_k + (long long)p.tiles_v * p.tiles_k;
     return launch_head<Tile>(head_gradients_kernel<Tile, T>, once, items, s, p, dw ? dw + (size_t)p.v0 * p.K : nullptr);
 }
@@ -559,7 +569,7 @@ extern "C" int hk_linear_cross_entropy_backward(const void* x_bf16, const void* 
     int32_t *starts = (int32_t*)(ws + L.starts), *list = (int32_t*)(ws + L.list);
     uint16_t* x0 = (uint16_t*)(ws + L.x);
     HeadPiece p{dl, w, x0, (float*)(ws + L.sums), lab, resid, starts, list, (uint16_t*)dx_bf16_or_null, M, V, K, 0, 0, L.piece, 0, 0, 0, 0, 0, 0, L.split_cols,
-                false, false, L.splits > 1};
+                false, false, L.splits > 1, false};
     for (int v0 = 0; v0 < V; v0 += L.piece) {
         p.v0 = v0;
         p.cols = V - v0 < L.piece ? V - v0 : L.piece;

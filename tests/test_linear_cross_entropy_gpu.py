@@ -218,3 +218,26 @@ def test_pieces_of_the_vocabulary(hk):
         total += dw_r[0]
         bound += dw_r[1] * 5      # 40000 rows' additions instead of 8000
     _within(dw, total, bound, 2**-24)
+
+
+@pytest.mark.parametrize("M,V", [(40000, 30011), (3000, 100003)])
+def test_pieces_by_the_tiles_of_either_gradient(hk, M, V):
+    """Many rows of few columns: pieces larger than for few rows, dw's tiles the longer items of a launch; few rows and many classes:
+    dx's. Both in more than one piece."""
+    K = 64
+    print(f"linear cross entropy, pieces M={M} V={V}", flush=True)
+    x, w, labels, dloss = _case(M, V, K, 7)
+    assert hk.tk_kernel.linear_cross_entropy_workspace_bytes(M, V, K) < 2 * M * V     # not the whole of dl
+    loss, lse, dx, dw = _run(hk, x, w, labels, dloss, torch.float32)
+    total = torch.zeros(V, K, dtype=torch.float64, device=DEV)
+    bound = torch.zeros_like(total)
+    parts = -(-M // 8000)
+    for a in range(0, M, 8000):
+        s = slice(a, a + 8000)
+        lse_r, loss_r, dx_r, dw_r, _ = _reference(x[s], w, labels[s], dloss[s])
+        _within(lse[s], *lse_r)
+        _within(loss[s], *loss_r)
+        _within(dx[s], *dx_r, 2**-8)
+        total += dw_r[0]
+        bound += dw_r[1] * parts   # M rows' additions instead of one part's
+    _within(dw, total, bound, 2**-24)
