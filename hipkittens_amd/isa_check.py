@@ -4,7 +4,7 @@ The kernels issue their vector-memory and matrix instructions from inline assemb
 treats such a statement as opaque: it places what the statement needs in front of it (a scalar
 register restored from a spill slot with v_readlane_b32, a uniform value made scalar with
 v_readfirstlane_b32), schedules its own instructions around it, and does not apply its hazard rules to
-what is inside. gfx950 has no interlock for four cases that matter here, and a fifth check covers the
+what is inside. gfx950 has no interlock for five cases that matter here, and a sixth check covers the
 scalar loads that the kernels issue from inline assembly and wait for later:
 
 * a scalar register written by a vector-ALU instruction and read by a vector-memory instruction
@@ -19,6 +19,9 @@ scalar loads that the kernels issue from inline assembly and wait for later:
   issued); that wait counts;
 * the data registers of a vector-memory store of more than 64 bits must not be written by a vector-ALU
   instruction for two wait states after the store;
+* a register written by a vector-ALU instruction (the compiler's copies of an accumulator around a
+  branch, say) must not be read as the accumulator (C) of a matrix instruction for two wait states: with
+  none in between the matrix instruction has added to the register's previous value;
 * the destination of a scalar load must not be touched before an `s_waitcnt lgkmcnt(0)` (scalar loads
   return out of order): the compiler takes the destination of an inline-assembly statement for
   written when the statement ends and is free to copy it to a spill slot at once.
@@ -47,6 +50,7 @@ from . import build as _build
 VALU_SGPR_TO_VMEM = 5
 M0_TO_LDS_DMA = 1
 WIDE_STORE_TO_VALU_WRITE = 2
+VALU_TO_MFMA = 2
 MFMA_RESULT_EXTRA = 4   # wait states beyond the instruction's passes (what the compiler leaves behind its own)
 
 _VMEM = ("buffer_", "global_", "flat_", "scratch_")
@@ -119,9 +123,11 @@ class _State:
     pipe: int = 0                                # wait states until the matrix pipe takes another instruction
     stored: dict = field(default_factory=dict)   # data register of a wide store -> wait states since the store
     loading: set = field(default_factory=set)    # scalar registers a scalar load may not have written yet
+    written: dict = field(default_factory=dict)  # vector register -> wait states since a vector-ALU write
 
     def copy(self) -> "_State":
-        return _State(dict(self.since), dict(self.pending), self.pipe, dict(self.stored), set(self.loading))
+        return _State(dict(self.since), dict(self.pending), self.pipe, dict(self.stored), set(self.loading),
+                      dict(self.written))
 
     def advance(self, states: int) -> None:
         for key in list(self.since):
@@ -139,6 +145,10 @@ class _State:
             self.stored[key] += states
             if self.stored[key] >= WIDE_STORE_TO_VALU_WRITE:
                 del self.stored[key]
+        for key in list(self.written):
+            self.written[key] += states
+            if self.written[key] >= VALU_TO_MFMA:
+                del self.written[key]
 
     def merge(self, other: "_State") -> "_State":
         """The least favourable of two states (two ways to reach the same place)."""
@@ -151,11 +161,13 @@ class _State:
         for key, value in other.stored.items():
             out.stored[key] = min(out.stored.get(key, _HORIZON), value)
         out.loading |= other.loading
+        for key, value in other.written.items():
+            out.written[key] = min(out.written.get(key, _HORIZON), value)
         return out
 
     def __eq__(self, other) -> bool:
-        return ((self.since, self.pending, self.pipe, self.stored, self.loading) ==
-                (other.since, other.pending, other.pipe, other.stored, other.loading))
+        return ((self.since, self.pending, self.pipe, self.stored, self.loading, self.written) ==
+                (other.since, other.pending, other.pipe, other.stored, other.loading, other.written))
 
 
 def _step(state: _State, instr, function: str, findings: list | None) -> None:
@@ -185,6 +197,11 @@ def _step(state: _State, instr, function: str, findings: list | None) -> None:
             state.loading.update(_sgprs(operands[0]))
     if op.startswith("v_mfma"):
         touches(operands[1:3] + operands[4:6])   # A, B and scale operands (C chains on its own result)
+        if findings is not None:
+            for operand in operands[3:4]:
+                for reg in _vector_registers(operand.split()[0]):
+                    if reg in state.written:
+                        findings.append(Finding(function, number, op, reg, state.written[reg], VALU_TO_MFMA))
         state.advance(state.pipe)                # waits for the pipe
         state.advance(1)
         passes = mfma_passes(op, args)
@@ -211,6 +228,8 @@ def _step(state: _State, instr, function: str, findings: list | None) -> None:
         for reg in _vector_registers(data):
             state.stored[reg] = 0
     if op.startswith("v_") and operands:
+        for reg in _vector_registers(operands[0]):
+            state.written[reg] = 0
         written = _sgprs(operands[0])
         if len(operands) > 1 and _VALU_SECOND_DST.match(op):
             written += _sgprs(operands[1])

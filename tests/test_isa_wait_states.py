@@ -4,7 +4,8 @@ statement reads a register sooner than the hardware allows after the instruction
 The compiler does not apply its hazard rules to inline assembly; hipkittens_amd/isa_check.py states the
 rules checked (vector-ALU write of a scalar register -> vector-memory read: five wait states; scalar
 write of M0 -> global->LDS load: one; result of a matrix instruction -> any other use: its passes + 4;
-data registers of a store of more than 64 bits -> vector-ALU write: two). Compiles every csrc/*.hip to assembly: about two minutes
+data registers of a store of more than 64 bits -> vector-ALU write: two; vector-ALU write -> accumulator of a matrix
+instruction: two). Compiles every csrc/*.hip to assembly: about two minutes
 on eight cores, no GPU needed.
 """
 import shutil
@@ -54,6 +55,25 @@ _Z3barPi:
 	s_endpgm
 """
     assert [(f.register, f.wait_states) for f in isa_check.scan(branch)] == [("s8", 1)]
+
+
+def test_scanner_accumulators_that_vector_instructions_write():
+    # an accumulator copied in front of the matrix instruction that adds to it: two wait states; its A and B operands are interlocked
+    bad = """
+_Z3fooPi:
+	v_accvgpr_write_b32 a0, v70
+	v_accvgpr_write_b32 a3, v73
+	v_mov_b32_e32 v8, v9
+	v_mfma_f32_16x16x32_bf16 a[0:3], v[8:11], v[4:7], a[0:3]
+"""
+    assert [(f.register, f.wait_states, f.needed) for f in isa_check.scan(bad)] == [("a3", 1, 2)]
+    good = """
+_Z3fooPi:
+	v_accvgpr_write_b32 a3, v73
+	s_nop 1
+	v_mfma_f32_16x16x32_bf16 a[0:3], v[8:11], v[4:7], a[0:3]
+"""
+    assert isa_check.scan(good) == []
 
 
 def test_scanner_matrix_results():
