@@ -32,6 +32,8 @@ struct TileOperand {
 // read touches two neighbouring chunks of the eight rows k0 + {0..3, 8..11}: they fall on sixteen different chunks of a
 // 256-byte line, i.e. on every bank once.
 __device__ __forceinline__ uint32_t across_swz(uint32_t k) { return 2u * ((k & 3u) | ((k >> 1) & 4u)); }
+// The same for rows of 128 bytes, two of which share a line: row bit 0 is the half of it.
+__device__ __forceinline__ uint32_t across_swz128(uint32_t k) { return 2u * (((k >> 1) & 1u) | ((k >> 2) & 2u)); }
 
 __device__ __forceinline__ v2i lds_read_tr(uint32_t addr) {
     return __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s_t*)(uintptr_t)addr));

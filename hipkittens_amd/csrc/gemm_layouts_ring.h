@@ -23,7 +23,7 @@ __device__ __forceinline__ void mfma_bf16_acc(v4f& acc, const v4i& x, const v4i&
 }
 
 // Loads and reads of one operand of a tile of TILE rows (columns): TILE / 32 loads a wave. Load i: along, rows 32 i + 8 w .. +8; across,
-// TILE 256, K rows 8 i + 2 w and the next, TILE 128, 16 i + 4 w .. +4.
+// TILE 256, K rows 8 i + 2 w and the next, TILE 128, 16 i + 4 w .. +4, TILE 64, 32 i + 8 w .. +8.
 template <bool ACROSS, int TILE = kRingTile>
 struct RingOperand {
     static constexpr uint32_t kRow = 2 * TILE;   // across: bytes of a K row in LDS
@@ -32,7 +32,7 @@ struct RingOperand {
     uint32_t voff[2];     // even / odd loads (across: the swizzle takes bit 3 of the K row)
     uint32_t round, tail_or;
     uint32_t rd[2];       // along: the lane's two chunks of its row; across: rd[0] = the lane's address in fragment 0
-    static __device__ __forceinline__ int64_t step(uint32_t pitch) { return (int64_t)kLayoutStep * pitch; }
+    static __device__ __forceinline__ uint32_t swz(uint32_t k) { return TILE == 64 ? across_swz128(k) : across_swz(k); }
 
     // `patch`: which half of the tile's rows (columns) this wave reads
     __device__ __forceinline__ void init(const TileOperand& op, int K, int patch, uint32_t lds0) {
@@ -46,11 +46,11 @@ struct RingOperand {
             for (int odd = 0; odd < 2; ++odd) {
                 constexpr uint32_t kChunks = kRow / 16, kLoadRows = 64 / kChunks;   // chunks of a row, rows of a load
                 const uint32_t k = kLoadRows * w + lane / kChunks;
-                voff[odd] = k * pitch + (((lane % kChunks) ^ across_swz(k + 4 * kLoadRows * odd)) * 16u);
+                voff[odd] = k * pitch + (((lane % kChunks) ^ swz(k + 4 * kLoadRows * odd)) * 16u);
                 round = 4u * kLoadRows * pitch;
             }
             const uint32_t k = 8 * g + (r >> 2);
-            rd[0] = lds0 + k * kRow + (((TILE / 16u * patch + ((r >> 1) & 1u)) ^ across_swz(k)) * 16u) + (r & 1u) * 8u;
+            rd[0] = lds0 + k * kRow + (((TILE / 16u * patch + ((r >> 1) & 1u)) ^ swz(k)) * 16u) + (r & 1u) * 8u;
             rd[1] = 0;
         } else {
             const uint32_t R = 8 * w + (lane >> 3), c = swz_chunk(R, lane & 7) * 16u;
@@ -232,29 +232,35 @@ __device__ __forceinline__ void ring_product(uint8_t* smem, const TileOperand& A
     mfma_drain_agpr(acc);
 }
 
-// 128x128 tiles in the same manner, for problems with no more tiles than CUs, where one workgroup has a CU to itself: four LDS
-// stages, three K-steps ahead, the next K-step's fragments read behind the MFMAs of this one (a quarter of the tile and 32
-// MFMAs a wave and K-step). Weight gradient of 16384 rows, 64 tiles of 256 K-steps: 155 us with two stages, 117 here, 31 bytes
-// a clock into each CU, which bounds it (five stages: 116); loss of 100 x 10000 x 4096 52 / 39; 16 rows of 4 experts of 4096 x 4096
-// 45 / 33.
-constexpr int kDeepStages = 4, kDeepStage = 2 * kLayoutTile * 128;
-template <bool A_ACROSS, bool B_ACROSS>
-__device__ __forceinline__ void deep_product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K, v4f (&acc)[4][4]) {
-    constexpr int S = kDeepStages, kLoads = 4;
+// 128x128 and 64x64 tiles in the same manner, for problems with no more tiles than CUs, where one workgroup has a CU to itself: four or
+// eight LDS stages, all but one or two of them ahead, the next fragments read behind the MFMAs of these (a quarter of the tile a wave).
+// Weight gradient of 16384 rows, 1024 x 1024, 64 tiles of 256 K-steps: 155 us with two stages of 128x128, 117 with four, 31 bytes a clock
+// into each CU, which bounds it (five stages: 116); 256 tiles of 64x64 with a barrier every K-step 70, every second 66. A K-step of
+// 64x64 takes 0.23 to 0.25 us, of 128x128 0.45, also where few rows leave most of A's loads without memory behind them: the issue of
+// the loads into LDS bounds a CU, not memory.
+template <int TILE>
+struct DeepStages {
+    static constexpr int kStages = TILE == 128 ? 4 : 8, kBytes = 2 * TILE * 128;
+    static constexpr int kGroup = TILE == 128 ? 1 : 2;   // K-steps from barrier to barrier
+};
+template <int TILE, bool A_ACROSS, bool B_ACROSS>
+__device__ __forceinline__ void deep_product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K,
+                                             v4f (&acc)[TILE / 32][TILE / 32]) {
+    constexpr int S = DeepStages<TILE>::kStages, kStage = DeepStages<TILE>::kBytes, U = DeepStages<TILE>::kGroup, F = TILE / 32, kLoads = TILE / 32;
     const uint32_t lds0 = (uint32_t)(uintptr_t)smem, w = wave_id();
     const uint32_t mine = to_sgpr(lds0 + w * 1024u);
-    RingOperand<A_ACROSS, kLayoutTile> oa;
-    RingOperand<B_ACROSS, kLayoutTile> ob;
+    RingOperand<A_ACROSS, TILE> oa;
+    RingOperand<B_ACROSS, TILE> ob;
     oa.init(A, K, w >> 1, lds0);
-    ob.init(B, K, w & 1, lds0 + kDeepStage / 2);
+    ob.init(B, K, w & 1, lds0 + kStage / 2);
     const int nk = (K + kLayoutStep - 1) / kLayoutStep;
     const uint32_t step_a = A_ACROSS ? to_sgpr(kLayoutStep * A.pitch) : 128u, step_b = B_ACROSS ? to_sgpr(kLayoutStep * B.pitch) : 128u;
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
+    for (int m = 0; m < F; ++m)
 #pragma unroll
-        for (int n = 0; n < 4; ++n) acc[m][n] = v4f{0.f, 0.f, 0.f, 0.f};
+        for (int n = 0; n < F; ++n) acc[m][n] = v4f{0.f, 0.f, 0.f, 0.f};
     struct Frag { v4i lo, hi; };
-    Frag af[2][4], bf[2][4];
+    Frag af[2][U][F], bf[2][U][F];
     v4i da, db;
     uint32_t vor_a = 0, vor_b = 0, rows_a = 0, rows_b = 0;
     auto next_step = [&](int kt) __attribute__((always_inline)) {   // the descriptors' K-step
@@ -267,69 +273,85 @@ __device__ __forceinline__ void deep_product(uint8_t* smem, const TileOperand& A
         oa.advance(step_a);
         ob.advance(step_b);
     };
-    auto load = [&](int i, uint32_t stage) __attribute__((always_inline)) {   // 0 .. 3: A, 4 .. 7: B
+    auto load = [&](int i, uint32_t stage) __attribute__((always_inline)) {   // A's loads of a K-step, then B's
+        auto one = [&]<int I>() __attribute__((always_inline)) {
+            if constexpr (I < kLoads) oa.template load<I>(mine + stage, da, vor_a, rows_a);
+            else if constexpr (I < 2 * kLoads) ob.template load<I - kLoads, kStage / 2>(mine + stage, db, vor_b, rows_b);
+        };
         switch (i) {
-            case 0: oa.template load<0>(mine + stage, da, vor_a, rows_a); break;
-            case 1: oa.template load<1>(mine + stage, da, vor_a, rows_a); break;
-            case 2: oa.template load<2>(mine + stage, da, vor_a, rows_a); break;
-            case 3: oa.template load<3>(mine + stage, da, vor_a, rows_a); break;
-            case 4: ob.template load<0, kDeepStage / 2>(mine + stage, db, vor_b, rows_b); break;
-            case 5: ob.template load<1, kDeepStage / 2>(mine + stage, db, vor_b, rows_b); break;
-            case 6: ob.template load<2, kDeepStage / 2>(mine + stage, db, vor_b, rows_b); break;
-            default: ob.template load<3, kDeepStage / 2>(mine + stage, db, vor_b, rows_b); break;
+            case 0: one.template operator()<0>(); break;
+            case 1: one.template operator()<1>(); break;
+            case 2: one.template operator()<2>(); break;
+            case 3: one.template operator()<3>(); break;
+            case 4: one.template operator()<4>(); break;
+            case 5: one.template operator()<5>(); break;
+            case 6: one.template operator()<6>(); break;
+            default: one.template operator()<7>(); break;
         }
     };
-    // half u (0 .. 15) of a K-step's fragments into register set Q
-    auto read = [&]<int Q>(int u, uint32_t stage) __attribute__((always_inline)) {
-        const int f = u / 4, h = u & 1;
+    // half u (0 .. 4 F U - 1) of a group's fragments into register set Q
+    auto read = [&]<int Q>(int u, uint32_t group) __attribute__((always_inline)) {
+        const int s = u / (4 * F), f = u % (4 * F) / 4, h = u & 1;
+        const uint32_t stage = group + s * kStage;
         if ((u & 2) == 0) {
-            if (h) bf[Q][f].hi = ob.template half<1>(f, stage);
-            else bf[Q][f].lo = ob.template half<0>(f, stage);
+            if (h) bf[Q][s][f].hi = ob.template half<1>(f, stage);
+            else bf[Q][s][f].lo = ob.template half<0>(f, stage);
         } else {
-            if (h) af[Q][f].hi = oa.template half<1>(f, stage);
-            else af[Q][f].lo = oa.template half<0>(f, stage);
+            if (h) af[Q][s][f].hi = oa.template half<1>(f, stage);
+            else af[Q][s][f].lo = oa.template half<0>(f, stage);
         }
     };
 #pragma unroll
     for (int p = 0; p < S; ++p) {
         next_step(p);
 #pragma unroll
-        for (int i = 0; i < 2 * kLoads; ++i) load(i, p * kDeepStage);
+        for (int i = 0; i < 2 * kLoads; ++i) load(i, p * kStage);
     }
-    wait_vmcnt<(S - 1) * 2 * kLoads>();
+    wait_vmcnt<(S - U) * 2 * kLoads>();
     block_barrier();
 #pragma unroll
-    for (int u = 0; u < 16; ++u) read.template operator()<0>(u, 0u);
-    uint32_t at = 0, at1 = kDeepStage;   // stages of K-steps kt and kt + 1
-    auto step = [&]<int P>(int kt) __attribute__((always_inline)) {
-        // this K-step's fragments are here, so its stage is free once everyone says so; the next K-step has landed
+    for (int u = 0; u < 4 * F * U; ++u) read.template operator()<0>(u, 0u);
+    uint32_t at = 0, at1 = U * kStage;   // stages of groups kg and kg + 1
+    auto step = [&]<int P>(int kg) __attribute__((always_inline)) {
+        // this group's fragments are here, so its stages are free once everyone says so; the next group has landed
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        wait_vmcnt<(S - 2) * 2 * kLoads>();
+        wait_vmcnt<(S - 2 * U) * 2 * kLoads>();
         block_barrier();
         __builtin_amdgcn_sched_barrier(0);
-        next_step(kt + S);
+        mfma_enter_agpr(acc);
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
+        for (int s = 0; s < U; ++s) {
+            next_step(kg * U + S + s);
 #pragma unroll
-            for (int pass = 0; pass < 2; ++pass)
+            for (int m = 0; m < F; ++m)
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    if (pass == 0) mfma_bf16_acc(acc[m][n], bf[P][n].lo, af[P][m].lo);
-                    else mfma_bf16_acc(acc[m][n], bf[P][n].hi, af[P][m].hi);
-                    const int q = 8 * m + 4 * pass + n;
-                    if (q < 16) read.template operator()<P ^ 1>(q, at1);
-                    else if (q & 1) load((q - 16) / 2, at);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
+                for (int pass = 0; pass < 2; ++pass)
+#pragma unroll
+                    for (int n = 0; n < F; ++n) {
+                        if (pass == 0) mfma_bf16_acc(acc[m][n], bf[P][s][n].lo, af[P][s][m].lo);
+                        else mfma_bf16_acc(acc[m][n], bf[P][s][n].hi, af[P][s][m].hi);
+                        const int q = F * (2 * m + pass) + n;
+                        if (F == 2) {   // a read behind each, a load behind every second
+                            read.template operator()<P ^ 1>(8 * s + q, at1);
+                            if (q & 1) load(q / 2, at + s * kStage);
+                        } else if (q < 16) {
+                            read.template operator()<P ^ 1>(q, at1);
+                        } else if (q & 1) {
+                            load((q - 16) / 2, at);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+        }
         at = at1;
-        at1 = at1 == (S - 1) * kDeepStage ? 0u : at1 + kDeepStage;
+        at1 = at1 == (S - U) * kStage ? 0u : at1 + U * kStage;
     };
-    int kt = 0;
-    for (; kt + 1 < nk; kt += 2) {
-        step.template operator()<0>(kt);
-        step.template operator()<1>(kt + 1);
+    const int groups = (nk + U - 1) / U;
+    int kg = 0;
+    for (; kg + 1 < groups; kg += 2) {
+        step.template operator()<0>(kg);
+        step.template operator()<1>(kg + 1);
     }
-    if (kt < nk) step.template operator()<0>(kt);
+    if (kg < groups) step.template operator()<0>(kg);
     wait_vmcnt<0>();   // nothing may still be writing LDS when the workgroup retires or uses it otherwise
     mfma_drain_agpr(acc);
 }
@@ -409,17 +431,20 @@ struct LayoutTile256 {
     }
 };
 
-struct LayoutTile128Deep {
-    static constexpr int kTile = kLayoutTile, kPatch = kTile / 2, F = 4, kLds = kDeepStages * kDeepStage;
+template <int TILE>
+struct LayoutTileDeep {
+    static constexpr int kTile = TILE, kPatch = kTile / 2, F = TILE / 32, kLds = DeepStages<TILE>::kStages * DeepStages<TILE>::kBytes;
     template <bool A_ACROSS, bool B_ACROSS>
     static __device__ __forceinline__ void product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K, v4f (&acc)[F][F]) {
-        deep_product<A_ACROSS, B_ACROSS>(smem, A, B, K, acc);
+        deep_product<TILE, A_ACROSS, B_ACROSS>(smem, A, B, K, acc);
     }
     static __device__ __forceinline__ void read_row(const v4f (&acc)[F], v4f (&v)[F]) {
 #pragma unroll
         for (int n = 0; n < F; ++n) v[n] = acc[n];
     }
 };
+typedef LayoutTileDeep<128> LayoutTile128Deep;
+typedef LayoutTileDeep<64> LayoutTile64Deep;
 
 // Whether 256x256 tiles take less time than 128x128 ones: rounds of workgroups over the CUs (one of the large kernel or two of
 // the small one on a CU; a round that is not full is a round, later ones run into each other) times a fixed part and a part per
@@ -431,11 +456,15 @@ inline bool prefer_tile256(double tiles256, double tiles128, double k_steps, int
     auto rounds = [](double tiles, double at_once) { return tiles <= at_once ? 1.0 : tiles / at_once + 0.2; };
     return rounds(tiles256, cus) * (7.0 + 1.43 * k_steps) < rounds(tiles128, 2.0 * cus) * (2.7 + small_step * k_steps);
 }
-// The tile and the number of LDS stages of the small one: four where no CU gets a second workgroup anyway.
-enum LayoutChoice { kLayout256, kLayout128, kLayout128Deep };
-inline LayoutChoice choose_layout(double tiles256, double tiles128, double k_steps, int cus, double small_step = kSmallStepAlong) {
-    if (prefer_tile256(tiles256, tiles128, k_steps, cus, small_step)) return kLayout256;
-    return tiles128 <= cus ? kLayout128Deep : kLayout128;
+// The tile, and for the small ones the number of LDS stages: many where no CU gets a second workgroup anyway, and 64x64 tiles as long as
+// there are no more of them than CUs. (us, 128x128 / 64x64: forward of 16 rows of 4 experts of 4096 x 4096, 256 tiles of 64x64, 32.5 / 23.4;
+// loss of 60 x 14000 x 1024, 219 tiles, 16.6 / 12.5; more tiles than CUs: loss of 128 x 16000 x 2880, 500 tiles, 29 / 35.)
+enum LayoutChoice { kLayout256, kLayout128, kLayout128Deep, kLayout64Deep };
+struct LayoutTiles { double t256, t128, t64; };   // how many tiles of each size there are
+inline LayoutChoice choose_layout(LayoutTiles tiles, double k_steps, int cus, double small_step = kSmallStepAlong) {
+    if (tiles.t64 <= cus) return kLayout64Deep;
+    if (prefer_tile256(tiles.t256, tiles.t128, k_steps, cus, small_step)) return kLayout256;
+    return tiles.t128 <= cus ? kLayout128Deep : kLayout128;
 }
 
 }  // namespace hk

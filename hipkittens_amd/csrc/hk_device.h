@@ -255,6 +255,16 @@ __device__ __forceinline__ void mfma_drain_agpr(v4f (&acc)[M][N]) {
 #pragma unroll
         for (int n = 0; n < N; ++n) asm volatile("" : "+a"(acc[m][n]));
 }
+// In front of asm MFMA statements that a branch leads to: the compiler's copies of accumulators (it may hold them in other registers
+// across the branch) end here, two wait states before a matrix instruction adds to them.
+template <int M, int N>
+__device__ __forceinline__ void mfma_enter_agpr(v4f (&acc)[M][N]) {
+#pragma unroll
+    for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int n = 0; n < N; ++n) asm volatile("" : "+a"(acc[m][n]));
+    asm volatile("s_nop 1");
+}
 template <int M, int N>
 __device__ __forceinline__ void mfma_drain_vgpr(v4f (&acc)[M][N]) {
     mfma_drain();

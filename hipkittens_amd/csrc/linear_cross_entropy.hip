@@ -409,8 +409,8 @@ __global__ __launch_bounds__(256) void head_dx_reduce_kernel(const float* __rest
 static int tiles_of(int n, int tile) { return (n + tile - 1) / tile; }
 static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 static LayoutChoice head_choice(int rows, int cols, int k) {   // a product of rows x cols over k
-    return choose_layout((double)tiles_of(rows, 256) * tiles_of(cols, 256), (double)tiles_of(rows, 128) * tiles_of(cols, 128),
-                         tiles_of(k, kLayoutStep), moe_num_compute_units());
+    auto tiles = [&](int tile) { return (double)tiles_of(rows, tile) * tiles_of(cols, tile); };
+    return choose_layout({tiles(256), tiles(128), tiles(64)}, tiles_of(k, kLayoutStep), moe_num_compute_units());
 }
 
 // forward: label logits, then the partial results
@@ -420,7 +420,7 @@ struct HeadForwardPlan {
     size_t label_logit, partial, bytes;
     HeadForwardPlan(int M, int V, int K) {
         tile = head_choice(M, V, K);
-        blocks = 2 * tiles_of(V, tile == kLayout256 ? 256 : 128);
+        blocks = 2 * tiles_of(V, tile == kLayout256 ? 256 : tile == kLayout64Deep ? 64 : 128);
         label_logit = 0;
         partial = up256((size_t)M * 4);
         bytes = partial + up256((size_t)M * blocks * sizeof(float2));
@@ -538,9 +538,11 @@ extern "C" int hk_linear_cross_entropy(const void* x_bf16, const void* w_bf16, c
     float* label_logit = (float*)((uint8_t*)workspace + L.label_logit);
     const HeadLabels lab{labels, label_type};
     const uint16_t *x = (const uint16_t*)x_bf16, *w = (const uint16_t*)w_bf16;
-    const int st = L.tile == kLayout256   ? launch_logits<LayoutTile256>(x, w, lab, M, V, K, partial, label_logit, s)
-                   : L.tile == kLayout128 ? launch_logits<LayoutTile128>(x, w, lab, M, V, K, partial, label_logit, s)
-                                          : launch_logits<LayoutTile128Deep>(x, w, lab, M, V, K, partial, label_logit, s);
+    auto logits = [&]<typename Tile>() { return launch_logits<Tile>(x, w, lab, M, V, K, partial, label_logit, s); };
+    const int st = L.tile == kLayout256       ? logits.template operator()<LayoutTile256>()
+                   : L.tile == kLayout128     ? logits.template operator()<LayoutTile128>()
+                   : L.tile == kLayout128Deep ? logits.template operator()<LayoutTile128Deep>()
+                                              : logits.template operator()<LayoutTile64Deep>();
     if (st != HK_OK) return st;
     hipLaunchKernelGGL(head_loss_kernel, dim3((M + 15) / 16), dim3(16 * kJoin), 0, s, (const float2*)partial, (const float*)label_logit, lab, M, V,
                        L.blocks, loss, lse);
@@ -577,9 +579,13 @@ extern "C" int hk_linear_cross_entropy_backward(const void* x_bf16, const void* 
         p.last = v0 + p.cols == V;
         const bool first_dw = dw_or_null && v0 == 0;
         const HeadRows rows{starts, list, x0, first_dw ? tiles_of(V, 256) : 0, first_dw ? tiles_of(M, kHeadCopyRows) : 0};
-        int st = L.logits == kLayout256   ? launch_dlogits<LayoutTile256>(x, w, lab, lse, dloss, M, V, K, v0, p.cols, L.piece, dl, resid, rows, s)
-                 : L.logits == kLayout128 ? launch_dlogits<LayoutTile128>(x, w, lab, lse, dloss, M, V, K, v0, p.cols, L.piece, dl, resid, rows, s)
-                                          : launch_dlogits<LayoutTile128Deep>(x, w, lab, lse, dloss, M, V, K, v0, p.cols, L.piece, dl, resid, rows, s);
+        auto dlogits = [&]<typename Tile>() {
+            return launch_dlogits<Tile>(x, w, lab, lse, dloss, M, V, K, v0, p.cols, L.piece, dl, resid, rows, s);
+        };
+        int st = L.logits == kLayout256       ? dlogits.template operator()<LayoutTile256>()
+                 : L.logits == kLayout128     ? dlogits.template operator()<LayoutTile128>()
+                 : L.logits == kLayout128Deep ? dlogits.template operator()<LayoutTile128Deep>()
+                                              : dlogits.template operator()<LayoutTile64Deep>();
         if (st != HK_OK) return st;
         if (dw_type == 0)
             st = L.grads256 ? launch_gradients<LayoutTile256>(p, want_dx, (uint16_t*)dw_or_null, s)

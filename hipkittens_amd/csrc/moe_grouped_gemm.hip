@@ -140,16 +140,19 @@ static int launch_grouped_tile(const void* x, const void* W, const int32_t* offs
 // 20 / 27. The rule's one miss there: 32 experts of 64 rows, small 428, large 359.)
 static LayoutChoice grouped_choice(int R, int E, int in, int out) {
     const double used = R < E ? R : E, mean = R / used;
-    const double m256 = mean / 256 + 0.6, m128 = mean / 128 + 0.6;
-    return choose_layout(used * (m256 > 1 ? m256 : 1) * ((out + 255) / 256), used * (m128 > 1 ? m128 : 1) * ((out + 127) / 128),
-                         (in + kLayoutStep - 1) / kLayoutStep, moe_num_compute_units());
+    auto tiles = [&](int tile) {
+        const double m = mean / tile + 0.6;
+        return used * (m > 1 ? m : 1) * ((out + tile - 1) / tile);
+    };
+    return choose_layout({tiles(256), tiles(128), tiles(64)}, (in + kLayoutStep - 1) / kLayoutStep, moe_num_compute_units());
 }
 template <bool DGRAD>
 static int launch_grouped(const void* x, const void* W, const int32_t* offsets, void* y, int R, int E, int N, int K, hipStream_t s) {
     switch (grouped_choice(R, E, DGRAD ? N : K, DGRAD ? K : N)) {
         case kLayout256: return launch_grouped_tile<LayoutTile256, DGRAD>(x, W, offsets, y, R, E, N, K, s);
         case kLayout128: return launch_grouped_tile<LayoutTile128, DGRAD>(x, W, offsets, y, R, E, N, K, s);
-        default: return launch_grouped_tile<LayoutTile128Deep, DGRAD>(x, W, offsets, y, R, E, N, K, s);
+        case kLayout128Deep: return launch_grouped_tile<LayoutTile128Deep, DGRAD>(x, W, offsets, y, R, E, N, K, s);
+        default: return launch_grouped_tile<LayoutTile64Deep, DGRAD>(x, W, offsets, y, R, E, N, K, s);
     }
 }
 
@@ -179,10 +182,12 @@ static int launch_wgrad(const void* dy, const void* x, const int32_t* offsets, v
         return large < single ? launch_wgrad_tile<LayoutTile256, T>(dy, x, offsets, dW, R, E, N, K, s)
                               : launch_wgrad_tile<LayoutTile128Stages<1>, T>(dy, x, offsets, dW, R, E, N, K, s);
     }
-    switch (choose_layout(e * n256 * k256, e * n128 * k128, steps, cus, kSmallStepAcross)) {
+    const double t64 = e * ((N + 63) / 64) * ((K + 63) / 64);
+    switch (choose_layout({e * n256 * k256, e * n128 * k128, t64}, steps, cus, kSmallStepAcross)) {
         case kLayout256: return launch_wgrad_tile<LayoutTile256, T>(dy, x, offsets, dW, R, E, N, K, s);
         case kLayout128: return launch_wgrad_tile<LayoutTile128, T>(dy, x, offsets, dW, R, E, N, K, s);
-        default: return launch_wgrad_tile<LayoutTile128Deep, T>(dy, x, offsets, dW, R, E, N, K, s);
+        case kLayout128Deep: return launch_wgrad_tile<LayoutTile128Deep, T>(dy, x, offsets, dW, R, E, N, K, s);
+        default: return launch_wgrad_tile<LayoutTile64Deep, T>(dy, x, offsets, dW, R, E, N, K, s);
     }
 }
 

@@ -180,3 +180,10 @@ def test_weight_gradient_of_a_long_expert(hk):
     w[0, -1] = 1.0
     hk.tk_kernel.dispatch_moe_grouped_gemm_dgrad(dy, w, torch.tensor([0, R], dtype=torch.int32, device=DEV), dx)
     assert torch.all(dx[:-1] == 1) and torch.all(dx[-1] == 64)
+
+
+@pytest.mark.parametrize("N,K", [(2056, 1544), (776, 3080), (2056, 8)])
+@pytest.mark.parametrize("rows,unused", [([300, 200, 500], 0), ([700], 3), ([3, 0, 9, 1], 0), ([1500], 0)])
+def test_products_between_the_tile_sizes(hk, rows, unused, N, K):
+    """More tiles of 64x64 than CUs and fewer of 128x128, or just as many of the former, and contractions of one K-step to dozens."""
+    _products_and_gradients(hk, rows, unused, N, K, 5000 + N + K + rows[0])
