@@ -430,7 +430,7 @@ struct HeadForwardPlan {
 struct HeadBackwardPlan {
     int piece;   // columns of a piece, a multiple of 256
     LayoutChoice logits;
-    bool grads256;
+    LayoutChoice grads;
     int splits, split_cols;
     size_t resid, starts, list, x, dl, sums, bytes;
     HeadBackwardPlan(int M, int V, int K) {
@@ -446,19 +446,31 @@ struct HeadBackwardPlan {
         piece = (int)std::max(256ll, std::min(most, all));
         const int cols = std::min(piece, V);
         logits = head_choice(M, cols, K);
-        // dx and dW together: K-steps of all tiles over the workgroups that run at once
-        const int slots = moe_num_compute_units(), steps_v = tiles_of(cols, kLayoutStep), steps_m = tiles_of(M, kLayoutStep);
-        const double dx256 = (double)tiles_of(M, 256) * tiles_of(K, 256), dw256 = (double)tiles_of(cols, 256) * tiles_of(K, 256);
-        const double dx128 = (double)tiles_of(M, 128) * tiles_of(K, 128), dw128 = (double)tiles_of(cols, 128) * tiles_of(K, 128);
-        const double large = (dx256 * (7.0 + 1.43 * steps_v) + dw256 * (7.0 + 1.43 * steps_m)) / slots;
-        const double small = (dx128 * (2.7 + kSmallStepAlong * steps_v) + dw128 * (2.7 + kSmallStepAcross * steps_m)) / (2.0 * slots);
-        grads256 = large < small;
-        const double total = grads256 ? dx256 * steps_v + dw256 * steps_m : dx128 * steps_v + dw128 * steps_m;
-        const double share = total / (grads256 ? slots : 2 * slots);   // K-steps of one workgroup's place
-        const int per_split = std::max(8, (int)std::min((double)steps_v, share));
-        splits = tiles_of(steps_v, per_split);
-        split_cols = tiles_of(steps_v, splits) * kLayoutStep;
-        splits = tiles_of(cols, split_cols);
+        // dx and dW together. dx's contraction is cut to the K-steps that a workgroup's place has (8 at least); the time of a tile's kernel is
+        // that of all K-steps over the places, or of the longest item if that is longer (large: one workgroup a CU; small: two).
+        // (Gradients, us, without regard to the longest item and without LayoutTile128Deep / so: 973 x 1187 x 792 79 / 48, 395 x 1029 x 3552
+        // 59 / 43, 4096 x 4096 x 1024 195 / 143, 1024 x 8192 x 1024 73 / 73.)
+        const int cus = moe_num_compute_units(), steps_v = tiles_of(cols, kLayoutStep), steps_m = tiles_of(M, kLayoutStep);
+        struct Cut { int splits, split_cols; bool deep; double us; };
+        auto cut = [&](int tile) {
+            const double dx = (double)tiles_of(M, tile) * tiles_of(K, tile), dw = (double)tiles_of(cols, tile) * tiles_of(K, tile);
+            const int places = tile == 256 ? cus : 2 * cus;
+            const int per_split = std::max(8, (int)std::min((double)steps_v, (dx * steps_v + dw * steps_m) / places));
+            Cut c;
+            c.split_cols = tiles_of(steps_v, tiles_of(steps_v, per_split)) * kLayoutStep;
+            c.splits = tiles_of(cols, c.split_cols);
+            const double fixed = tile == 256 ? 7.0 : 2.7, items = dx * c.splits + dw;
+            const double along = tile == 256 ? 1.43 : kSmallStepAlong, across = tile == 256 ? 1.43 : kSmallStepAcross;
+            const double longest = std::max(along * std::min(per_split, steps_v), across * steps_m);
+            c.us = std::max((dx * (fixed + along * steps_v) + dw * (fixed + across * steps_m)) / places, fixed + longest);
+            if (tile == 128 && items <= cus) c.us = 2.7 + 0.45 * std::max(std::min(per_split, steps_v), steps_m);   // LayoutTile128Deep
+            c.deep = tile == 128 && items <= cus;
+            return c;
+        };
+        const Cut large = cut(256), small = cut(128);
+        grads = large.us < small.us ? kLayout256 : small.deep ? kLayout128Deep : kLayout128;
+        splits = (grads == kLayout256 ? large : small).splits;
+        split_cols = (grads == kLayout256 ? large : small).split_cols;
         resid = 0;
         list = up256((size_t)M * 4);
         starts = list + up256((size_t)M * 4);
@@ -587,12 +599,13 @@ extern "C" int hk_linear_cross_entropy_backward(const void* x_bf16, const void* 
                  : L.logits == kLayout128Deep ? dlogits.template operator()<LayoutTile128Deep>()
                                               : dlogits.template operator()<LayoutTile64Deep>();
         if (st != HK_OK) return st;
-        if (dw_type == 0)
-            st = L.grads256 ? launch_gradients<LayoutTile256>(p, want_dx, (uint16_t*)dw_or_null, s)
-                            : launch_gradients<LayoutTile128>(p, want_dx, (uint16_t*)dw_or_null, s);
-        else
-            st = L.grads256 ? launch_gradients<LayoutTile256>(p, want_dx, (float*)dw_or_null, s)
-                            : launch_gradients<LayoutTile128>(p, want_dx, (float*)dw_or_null, s);
+        auto gradients = [&]<typename Tile>() {
+            return dw_type == 0 ? launch_gradients<Tile>(p, want_dx, (uint16_t*)dw_or_null, s)
+                                : launch_gradients<Tile>(p, want_dx, (float*)dw_or_null, s);
+        };
+        st = L.grads == kLayout256   ? gradients.template operator()<LayoutTile256>()
+             : L.grads == kLayout128 ? gradients.template operator()<LayoutTile128>()
+                                     : gradients.template operator()<LayoutTile128Deep>();
         if (st != HK_OK) return st;
         if (V - v0 <= L.piece) break;
     }

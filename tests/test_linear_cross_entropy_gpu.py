@@ -241,3 +241,20 @@ def test_pieces_by_the_tiles_of_either_gradient(hk, M, V):
         total += dw_r[0]
         bound += dw_r[1] * parts   # M rows' additions instead of one part's
     _within(dw, total, bound, 2**-24)
+
+
+@pytest.mark.parametrize("M,V,K", [(973, 1187, 792), (311, 2478, 1480), (64, 64, 2056), (130, 6000, 136)])
+@pytest.mark.parametrize("crowded", [False, True])
+def test_few_tiles(hk, M, V, K, crowded):
+    """No more tiles than CUs in the logits, the gradients or both, with labels all over and on a few classes."""
+    print(f"linear cross entropy, few tiles M={M} V={V} K={K} crowded={crowded}", flush=True)
+    x, w, labels, dloss = _case(M, V, K, M + K)
+    if crowded:
+        labels = torch.where(torch.arange(M, device=DEV) % 2 == 0, V // 2 + torch.arange(M, device=DEV) % 17, labels)
+    lse_r, loss_r, dx_r, dw_r, _ = _reference(x, w, labels, dloss)
+    for dw_dtype, half in ((torch.bfloat16, 2**-8), (torch.float32, 2**-24)):
+        loss, lse, dx, dw = _run(hk, x, w, labels, dloss, dw_dtype)
+        _within(lse, *lse_r)
+        _within(loss, *loss_r)
+        _within(dx, *dx_r, 2**-8)
+        _within(dw, *dw_r, half)
