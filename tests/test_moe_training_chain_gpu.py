@@ -208,3 +208,71 @@ def test_native_and_python_dispatchers_agree(hk, monkeypatch):
     step.run()
     for got, w in zip(step.outs, want):
         assert torch.equal(got.view(torch.uint8), w.view(torch.uint8))
+
+
+def test_two_streams_at_once(hk):
+    """The head on two streams side by side, each with its own workspace: the same bits as one after the other."""
+    tk = hk.tk_kernel
+    M, V, K = 311, 2478, 1472
+    print("training chain: two streams", flush=True)
+
+    def case(seed):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        x = torch.randn(M, K, device=DEV, generator=g).to(torch.bfloat16)
+        w = (torch.randn(V, K, device=DEV, generator=g) * K**-0.5).to(torch.bfloat16)
+        labels = torch.randint(0, V, (M,), device=DEV, generator=g)
+        ws = torch.empty(tk.linear_cross_entropy_workspace_bytes(M, V, K), dtype=torch.uint8, device=DEV)
+        rows = [torch.empty(M, device=DEV) for _ in range(2)]
+        return x, w, labels, *rows, torch.full((M,), 1 / M, device=DEV), torch.empty_like(x), torch.empty_like(w), ws
+
+    def run(x, w, labels, loss, lse, dloss, dx, dw, ws):
+        tk.dispatch_linear_cross_entropy(x, w, labels, loss, lse, ws)
+        tk.dispatch_linear_cross_entropy_backward(x, w, labels, lse, dloss, dx, dw, ws)
+
+    cases, streams = [case(1), case(2)], [torch.cuda.Stream() for _ in range(2)]
+    want = []
+    for c in cases:
+        run(*c)
+        want.append([t.clone() for t in c[3:8]])
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for c, s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                run(*c)
+    torch.cuda.synchronize()
+    for c, values in zip(cases, want):
+        assert all(torch.equal(a, b) for a, b in zip(c[3:8], values))
+
+
+def test_a_graph_follows_the_offsets(hk):
+    """The products' tables are read on the device: a captured call serves other numbers of rows per expert."""
+    tk = hk.tk_kernel
+    print("training chain: graph with other offsets", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    x = torch.randn(1500, 520, device=DEV, generator=g).to(torch.bfloat16)
+    w = torch.randn(3, 264, 520, device=DEV, generator=g).to(torch.bfloat16)
+    tables = [torch.tensor(t, dtype=torch.int32, device=DEV) for t in ([0, 1000, 1000, 1500], [0, 10, 900, 1500], [0, 0, 0, 3])]
+    offsets = tables[0].clone()
+    y, dw = torch.zeros(1500, 264, dtype=torch.bfloat16, device=DEV), torch.zeros(3, 264, 520, device=DEV)
+
+    def run():
+        tk.dispatch_moe_grouped_gemm(x, w, offsets, y)
+        tk.dispatch_moe_grouped_gemm_wgrad(y, x, offsets, dw)
+
+    want = []
+    for t in tables:
+        offsets.copy_(t)
+        y.zero_()
+        run()
+        want.append((y.clone(), dw.clone()))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for i in (1, 0, 2, 1, 2, 0):
+        offsets.copy_(tables[i])
+        y.zero_()
+        dw.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[i][0]) and torch.equal(dw, want[i][1])
