@@ -13,7 +13,11 @@
 // is bf16), then dx += dl W in fp32 and dW = dl^T x. The rounding is at most 2^-8 of each term, and a row's largest term is most
 // often its label's, scale (p - 1): that one's remainder, r[m], is kept in fp32 and its products r[m] W[label] and r[m] x[m] are
 // added in the epilogues of dx and dW. (Error of dx and dW against 64 bits, relative, 1111 rows: 0.0024 without the remainder, 0.0031
-// and more for a few rows; 0.0017 with it, which is the rounding of dx and dW themselves.)
+// and more for a few rows; 0.0017 with it, which is the rounding of dx and dW themselves. Before that rounding 1.3e-4 to 1.6e-4
+// with flat logits, 2e-4 to 1.1e-3 where other classes than the label have large shares: up to 1.2 times the error of rounding a
+// bf16 result, which is what holding dl in half the bytes and multiplying it once costs.)
+// For dW in fp32 that would be all its error, so there dl is two numbers of bf16, the value and what is left of it (then 2^-16 of each
+// term), one below the other as 2 M rows, times two copies of x below one another; the label's remainder behind both is kept likewise.
 #include <algorithm>
 
 #include "gemm_layouts_ring.h"
@@ -141,12 +145,13 @@ __device__ __forceinline__ v4f bf16_quad(const uint16_t* p) {
 struct HeadRows {
     int32_t *starts, *list;
     uint16_t* x;          // x with zeros for the rows that count for nothing
+    uint16_t* x_again;    // the same once more, behind the other, or null
     int groups, copies;   // workgroups of 256 classes, of kHeadCopyRows rows of x; 0: not wanted
 };
 constexpr int kHeadCopyRows = 8;
 // Rows of x for dW, whose products with dl's zeros must be zeros whatever a row without a label (padding) holds.
 __device__ __forceinline__ void head_copy_rows(const uint16_t* __restrict__ x, const HeadLabels& labels, int M, int V, int K,
-                                               uint16_t* __restrict__ out, int group) {
+                                               uint16_t* __restrict__ out, uint16_t* __restrict__ again, int group) {
     const int64_t m0 = (int64_t)group * kHeadCopyRows;
     const int chunks = K / 8, n = (int)min((int64_t)kHeadCopyRows, M - m0) * chunks;
     for (int c0 = threadIdx.x; c0 < n; c0 += 8 * 256) {
@@ -159,7 +164,10 @@ __device__ __forceinline__ void head_copy_rows(const uint16_t* __restrict__ x, c
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (c0 + i * 256 < n) *(v4i*)(out + m0 * K + (int64_t)(c0 + i * 256) * 8) = row[i];
+            if (c0 + i * 256 < n) {
+                *(v4i*)(out + m0 * K + (int64_t)(c0 + i * 256) * 8) = row[i];
+                if (again) *(v4i*)(again + m0 * K + (int64_t)(c0 + i * 256) * 8) = row[i];
+            }
     }
 }
 __device__ __forceinline__ void head_label_rows(int* counts, const HeadLabels& labels, int M, int V, const HeadRows& rows, int group) {
@@ -206,19 +214,23 @@ __device__ __forceinline__ void head_label_rows(int* counts, const HeadLabels& l
     });
 }
 
-// dl of the columns [v0, v0 + cols) of the vocabulary; `width` columns of it are written, those behind V as zeros. The last
+// What is left of dl's label terms, in fp32: behind one number of bf16, for dx and dW; and behind two, for dW in fp32.
+struct HeadRemainders { float *one, *two; };
+
+// dl of the columns [v0, v0 + cols) of the vocabulary; `width` columns of it are written, those behind V as zeros; what the rounding
+// leaves of it goes to dl_rest (null: not wanted). The last
 // workgroups copy x and sort the rows by label for the launch behind this one.
 template <typename Tile>
 __global__ __launch_bounds__(256) void head_dlogits_kernel(const uint16_t* __restrict__ x, const uint16_t* __restrict__ W,
                                                            HeadLabels labels, const float* __restrict__ lse,
                                                            const float* __restrict__ dloss, int M, int V, int K, int v0, int width,
                                                            int pitch, int tiles_m, int tiles_n, int band_n,
-                                                           uint16_t* __restrict__ dl,
-                                                           float* __restrict__ resid, HeadRows rows) {
+                                                           uint16_t* __restrict__ dl, uint16_t* __restrict__ dl_rest,
+                                                           HeadRemainders rest, HeadRows rows) {
     extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
     const int extra = (int)blockIdx.x - tiles_m * tiles_n;
     if (extra >= rows.copies) return head_label_rows((int*)smem, labels, M, V, rows, extra - rows.copies);
-    if (extra >= 0) return head_copy_rows(x, labels, M, V, K, rows.x, extra);
+    if (extra >= 0) return head_copy_rows(x, labels, M, V, K, rows.x, rows.x_again, extra);
     int pm, pn;
     banded_raster(xcd_chunk_order(blockIdx.x, tiles_m * tiles_n, kCuPerXcd), tiles_m, tiles_n, head_group(band_n, tiles_n), band_n, pm, pn);
     const int w = wave_id(), row0 = pm * Tile::kTile, col0 = v0 + pn * Tile::kTile;
@@ -240,16 +252,19 @@ __global__ __launch_bounds__(256) void head_dlogits_kernel(const uint16_t* __res
             for (int j = 0; j < 4; ++j) d[n][j] = scale * __builtin_amdgcn_exp2f(__builtin_fmaf(d[n][j], kLog2e, -lse2));
         const bool here = label >= col && label < col + Tile::kPatch && ((label >> 2) & 3) == g;   // among this lane's
         if (__any(here)) {
-            float rest = 0.f;
+            float left_over = 0.f;
 #pragma unroll
             for (int n = 0; n < Tile::F; ++n)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const bool hot = label == col + 16 * n + 4 * g + j;
                     d[n][j] -= hot ? scale : 0.f;
-                    rest = hot ? d[n][j] - bf16_value(d[n][j]) : rest;
+                    left_over = hot ? d[n][j] - bf16_value(d[n][j]) : left_over;
                 }
-            if (here) resid[at] = rest;
+            if (here) {
+                rest.one[at] = left_over;
+                if (dl_rest) rest.two[at] = left_over - bf16_value(left_over);
+            }
         }
         if (left < Tile::kPatch || __any(label < 0)) {   // zeros, not products with zero
 #pragma unroll
@@ -258,6 +273,13 @@ __global__ __launch_bounds__(256) void head_dlogits_kernel(const uint16_t* __res
                 for (int j = 0; j < 4; ++j) d[n][j] = label >= 0 && 16 * n + 4 * g + j < left ? d[n][j] : 0.f;
         }
         store_block_row(d, m, dl + (size_t)row * pitch + (col - v0), pitch, M - row, v0 + width - col);
+        if (dl_rest) {
+#pragma unroll
+            for (int n = 0; n < Tile::F; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) d[n][j] -= bf16_value(d[n][j]);
+            store_block_row(d, m, dl_rest + (size_t)row * pitch + (col - v0), pitch, M - row, v0 + width - col);
+        }
         slot_fence();
     }
 }
@@ -267,13 +289,14 @@ __global__ __launch_bounds__(256) void head_dlogits_kernel(const uint16_t* __res
 // dx runs over the piece, a few hundred K-steps for few tiles: with dW's tiles behind it in the same grid CUs that hold no item of dx
 // work on dW from the start, and `splits` cuts it where its items would still outlast the rest.
 struct HeadPiece {
-    const uint16_t *dl, *W, *x;   // x: with zeros for the rows that count for nothing
+    const uint16_t *dl, *W, *x;   // x: with zeros for the rows that count for nothing; dl and x: dw_rows rows of them for dW
     float* sums;      // [splits][M][K]: dx so far, when there are several pieces or splits
     HeadLabels labels;
-    const float* resid;              // r[m], of the rows whose label lies in this piece or an earlier one
+    const float *dx_rest, *dw_rest;   // r[m], of the rows whose label lies in this piece or an earlier one
     const int32_t *starts, *list;    // rows by their label's block of 16 classes
     uint16_t* dx;
     int M, V, K, v0, cols, pitch;
+    int dw_rows;   // M, or 2 M: dl's values and what is left of them, x twice
     int tiles_m, tiles_k, tiles_v, band_dx, band_dw, splits, split_cols;   // splits 0: no dx; tiles_v 0: no dW
     bool first, last, reduce;   // reduce: a launch of its own adds the splits and rounds
     bool dw_first;    // dW's tiles are the longer ones
@@ -304,7 +327,7 @@ __device__ __forceinline__ void head_dx_item(uint8_t* smem, const HeadPiece& p, 
         if (p.last && !p.reduce) {
             const int label = at < p.M ? p.labels.at(at, p.V) : -1;
             if (label >= 0) {
-                const float rest = p.resid[at];
+                const float rest = p.dx_rest[at];
 #pragma unroll
                 for (int c = 0; c < Tile::F; ++c)
                     if (col + 16 * c + 4 * g < p.K) v[c] += rest * bf16_quad(p.W + (size_t)label * p.K + col + 16 * c + 4 * g);
@@ -342,13 +365,14 @@ __global__ __launch_bounds__(256) void head_gradients_kernel(HeadPiece p, T* __r
         if (first + lane < count) {
             my_row = p.list[begin + first + lane];
             my_label = p.labels.at(my_row, p.V);
-            my_rest = p.resid[my_row];
+            my_rest = p.dw_rest[my_row];
         }
     };
     entries(0);
     asm volatile("" : "+v"(begin), "+v"(count));   // (in vector registers over the product, which needs the scalar ones)
     v4f acc[Tile::F][Tile::F];
-    Tile::template product<true, true>(smem, operand_across(p.dl, 2ull * p.pitch, row0, p.M), operand_across(p.x, 2ull * p.K, col0, p.M), p.M, acc);
+    Tile::template product<true, true>(smem, operand_across(p.dl, 2ull * p.pitch, row0, p.dw_rows),
+                                       operand_across(p.x, 2ull * p.K, col0, p.dw_rows), p.dw_rows, acc);
     begin = to_sgpr(begin);
     count = to_sgpr(count);
     // Their columns of x, 64 rows at a time, in this wave's part of the LDS that the product is done with, several rows
@@ -426,14 +450,14 @@ struct HeadForwardPlan {
         bytes = partial + up256((size_t)M * blocks * sizeof(float2));
     }
 };
-// backward: dl of a piece, then the fp32 sums of dx
+// backward: dl of a piece, then the fp32 sums of dx. parts: the numbers of bf16 that dl is held in, 2 for dW in fp32.
 struct HeadBackwardPlan {
     int piece;   // columns of a piece, a multiple of 256
     LayoutChoice logits;
     LayoutChoice grads;
     int splits, split_cols;
-    size_t resid, starts, list, x, dl, sums, bytes;
-    HeadBackwardPlan(int M, int V, int K) {
+    size_t rest, starts, list, x, dl, sums, bytes;   // rest: `parts` remainders of each row
+    HeadBackwardPlan(int M, int V, int K, int parts) {
         // Pieces of 512 MB: a piece's items of dx are the longer and its tiles the more, the fewer pieces there are (backward, us, pieces of
         // 128 / 256 / 512 / 2048 MB: 4096 x 201088 x 2880 11492 / 11737 / 11571 / 11331, 8192 x 129280 x 7168 34150 / 33106 / 32755 /
         // 33109, 16384 x 50257 x 1024 7282 / 5552 / 4747 / 4644). Where that gives dW fewer tiles than CUs (many rows, few columns of x: tiles
@@ -441,8 +465,11 @@ struct HeadBackwardPlan {
         // at most: 65536 x 32000 x 1024 15444 / 11947 / 11416 / 11394, 262144 x 32000 x 1024 180717 / 104194 / 65851 / 47530).
         // Rows of at most 4 MB: 32-bit offsets inside a K-step's rows.
         const long long fill = 256ll * tiles_of(moe_num_compute_units(), tiles_of(K, 256));
-        const long long held = std::max(512ll << 20, std::min({2ll * M * fill, 4ll << 30, 512ll * M * tiles_of(V, 512)}));
-        const long long most = std::min(held / (2ll * M), 1ll << 21) / 256 * 256, all = (long long)tiles_of(V, 256) * 256;
+        // dl in two parts, and the second copy of x, are held in the same bytes: pieces of half the classes and less.
+        const long long copies = 2ll * M * K * (parts - 1);
+        long long held = std::max(512ll << 20, std::min({2ll * M * fill, 4ll << 30, 512ll * M * tiles_of(V, 512)}));
+        held = std::max(held - copies, held / 4);
+        const long long most = std::min(held / (2ll * parts * M), 1ll << 21) / 256 * 256, all = (long long)tiles_of(V, 256) * 256;
         piece = (int)std::max(256ll, std::min(most, all));
         const int cols = std::min(piece, V);
         logits = head_choice(M, cols, K);
@@ -450,7 +477,7 @@ struct HeadBackwardPlan {
         // that of all K-steps over the places, or of the longest item if that is longer (large: one workgroup a CU; small: two).
         // (Gradients, us, without regard to the longest item and without LayoutTile128Deep / so: 973 x 1187 x 792 79 / 48, 395 x 1029 x 3552
         // 59 / 43, 4096 x 4096 x 1024 195 / 143, 1024 x 8192 x 1024 73 / 73.)
-        const int cus = moe_num_compute_units(), steps_v = tiles_of(cols, kLayoutStep), steps_m = tiles_of(M, kLayoutStep);
+        const int cus = moe_num_compute_units(), steps_v = tiles_of(cols, kLayoutStep), steps_m = tiles_of(parts * M, kLayoutStep);
         struct Cut { int splits, split_cols; bool deep; double us; };
         auto cut = [&](int tile) {
             const double dx = (double)tiles_of(M, tile) * tiles_of(K, tile), dw = (double)tiles_of(cols, tile) * tiles_of(K, tile);
@@ -471,12 +498,12 @@ struct HeadBackwardPlan {
         grads = large.us < small.us ? kLayout256 : small.deep ? kLayout128Deep : kLayout128;
         splits = (grads == kLayout256 ? large : small).splits;
         split_cols = (grads == kLayout256 ? large : small).split_cols;
-        resid = 0;
-        list = up256((size_t)M * 4);
+        rest = 0;
+        list = up256((size_t)M * 4 * parts);
         starts = list + up256((size_t)M * 4);
         x = starts + up256(((size_t)tiles_of(V, 256) * 16 + 1) * 4);
-        dl = x + up256((size_t)M * K * 2);
-        sums = dl + up256((size_t)M * piece * 2);
+        dl = x + up256((size_t)M * K * 2 * parts);
+        sums = dl + up256((size_t)M * piece * 2 * parts);
         bytes = sums + (piece < V || splits > 1 ? up256((size_t)splits * M * K * 4) : 0);
     }
 };
@@ -507,11 +534,11 @@ static int launch_logits(const uint16_t* x, const uint16_t* W, HeadLabels labels
 }
 template <typename Tile>
 static int launch_dlogits(const uint16_t* x, const uint16_t* W, HeadLabels labels, const float* lse, const float* dloss, int M, int V, int K,
-                          int v0, int cols, int pitch, uint16_t* dl, float* resid, HeadRows rows, hipStream_t s) {
+                          int v0, int cols, int pitch, uint16_t* dl, uint16_t* dl_rest, HeadRemainders rest, HeadRows rows, hipStream_t s) {
     static DeviceOnce once;
     const int tm = tiles_of(M, Tile::kTile), tv = tiles_of(cols, Tile::kTile);
     return launch_head<Tile>(head_dlogits_kernel<Tile>, once, (long long)tm * tv + rows.groups + rows.copies, s, x, W, labels, lse, dloss, M, V, K, v0,
-                             (cols + 7) / 8 * 8, pitch, tm, tv, raster_band(2ll * K * ((long long)M + cols), tv), dl, resid, rows);
+                             (cols + 7) / 8 * 8, pitch, tm, tv, raster_band(2ll * K * ((long long)M + cols), tv), dl, dl_rest, rest, rows);
 }
 template <typename Tile, typename T>
 static int launch_gradients(HeadPiece p, bool dx, T* dw, hipStream_t s) {
@@ -520,9 +547,9 @@ static int launch_gradients(HeadPiece p, bool dx, T* dw, hipStream_t s) {
     p.tiles_k = tiles_of(p.K, Tile::kTile);
     p.tiles_v = dw ? tiles_of(p.cols, Tile::kTile) : 0;
     p.band_dx = raster_band(2ll * p.cols * ((long long)p.M + p.K), p.tiles_k);
-    p.band_dw = raster_band(2ll * p.M * ((long long)p.cols + p.K), p.tiles_k);
+    p.band_dw = raster_band(2ll * p.dw_rows * ((long long)p.cols + p.K), p.tiles_k);
     p.splits = dx ? tiles_of(p.cols, p.split_cols) : 0;
-    p.dw_first = p.M > p.split_cols;
+    p.dw_first = p.dw_rows > p.split_cols;
     const long long items = (long long)p.splits * p.tiles_m * p.tiles_k + (long long)p.tiles_v * p.tiles_k;
     return launch_head<Tile>(head_gradients_kernel<Tile, T>, once, items, s, p, dw ? dw + (size_t)p.v0 * p.K : nullptr);
 }
@@ -532,8 +559,8 @@ static int launch_gradients(HeadPiece p, bool dx, T* dw, hipStream_t s) {
 extern "C" size_t hk_linear_cross_entropy_workspace_bytes(int M, int V, int K, int backward) {
     using namespace hk;
     if (head_check(M, V, K) != HK_OK) return 0;
-    const size_t f = HeadForwardPlan(M, V, K).bytes, b = backward ? HeadBackwardPlan(M, V, K).bytes : 0;
-    return f > b ? f : b;
+    const size_t f = HeadForwardPlan(M, V, K).bytes;
+    return backward ? std::max({f, HeadBackwardPlan(M, V, K, 1).bytes, HeadBackwardPlan(M, V, K, 2).bytes}) : f;
 }
 
 extern "C" int hk_linear_cross_entropy(const void* x_bf16, const void* w_bf16, const void* labels, int label_type, float* loss,
@@ -571,18 +598,21 @@ extern "C" int hk_linear_cross_entropy_backward(const void* x_bf16, const void* 
     if ((label_type != 0 && label_type != 1) || (dw_type != 0 && dw_type != 1)) return HK_ERR_UNSUPPORTED;
     if (((uintptr_t)x_bf16 | (uintptr_t)w_bf16 | (uintptr_t)dx_bf16_or_null | (uintptr_t)dw_or_null | (uintptr_t)workspace) & 15u)
         return HK_ERR_BAD_ALIGNMENT;
-    const HeadBackwardPlan L(M, V, K);
+    const int parts = dw_or_null && dw_type == 1 ? 2 : 1;
+    const HeadBackwardPlan L(M, V, K, parts);
     if (!workspace || workspace_bytes < L.bytes) return HK_ERR_WORKSPACE;
     const hipStream_t s = (hipStream_t)stream;
     uint8_t* ws = (uint8_t*)workspace;
     const HeadLabels lab{labels, label_type};
     const uint16_t *x = (const uint16_t*)x_bf16, *w = (const uint16_t*)w_bf16;
     uint16_t* dl = (uint16_t*)(ws + L.dl);
+    uint16_t* dl_rest = parts == 2 ? dl + (size_t)M * L.piece : nullptr;
     const bool want_dx = dx_bf16_or_null != nullptr;
-    float* resid = (float*)(ws + L.resid);
+    const HeadRemainders rest{(float*)(ws + L.rest), (float*)(ws + L.rest) + (parts == 2 ? M : 0)};
     int32_t *starts = (int32_t*)(ws + L.starts), *list = (int32_t*)(ws + L.list);
     uint16_t* x0 = (uint16_t*)(ws + L.x);
-    HeadPiece p{dl, w, x0, (float*)(ws + L.sums), lab, resid, starts, list, (uint16_t*)dx_bf16_or_null, M, V, K, 0, 0, L.piece, 0, 0, 0, 0, 0, 0, L.split_cols,
+    HeadPiece p{dl, w, x0, (float*)(ws + L.sums), lab, rest.one, rest.two, starts, list, (uint16_t*)dx_bf16_or_null, M, V, K, 0, 0, L.piece, parts * M, 0, 0, 0, 0, 0, 0,
+                L.split_cols,
                 false, false, L.splits > 1, false};
     for (int v0 = 0; v0 < V; v0 += L.piece) {
         p.v0 = v0;
@@ -590,9 +620,10 @@ extern "C" int hk_linear_cross_entropy_backward(const void* x_bf16, const void* 
         p.first = v0 == 0;
         p.last = v0 + p.cols == V;
         const bool first_dw = dw_or_null && v0 == 0;
-        const HeadRows rows{starts, list, x0, first_dw ? tiles_of(V, 256) : 0, first_dw ? tiles_of(M, kHeadCopyRows) : 0};
+        const HeadRows rows{starts, list, x0, parts == 2 ? x0 + (size_t)M * K : nullptr, first_dw ? tiles_of(V, 256) : 0,
+                            first_dw ? tiles_of(M, kHeadCopyRows) : 0};
         auto dlogits = [&]<typename Tile>() {
-            return launch_dlogits<Tile>(x, w, lab, lse, dloss, M, V, K, v0, p.cols, L.piece, dl, resid, rows, s);
+            return launch_dlogits<Tile>(x, w, lab, lse, dloss, M, V, K, v0, p.cols, L.piece, dl, dl_rest, rest, rows, s);
         };
         int st = L.logits == kLayout256       ? dlogits.template operator()<LayoutTile256>()
                  : L.logits == kLayout128     ? dlogits.template operator()<LayoutTile128>()
@@ -612,7 +643,7 @@ extern "C" int hk_linear_cross_entropy_backward(const void* x_bf16, const void* 
     if (want_dx && L.splits > 1) {
         const size_t n = (size_t)M * K;
         hipLaunchKernelGGL(head_dx_reduce_kernel, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, s, (const float*)(ws + L.sums),
-                           L.splits, M, V, K, lab, (const float*)resid, w, (uint16_t*)dx_bf16_or_null);
+                           L.splits, M, V, K, lab, (const float*)rest.one, w, (uint16_t*)dx_bf16_or_null);
         if (hipGetLastError() != hipSuccess) return HK_ERR_LAUNCH;
     }
     return HK_OK;

@@ -513,8 +513,9 @@ int hk_linear_cross_entropy(const void* x_bf16, const void* w_bf16, const void* 
 /* Its gradients for dloss [M] fp32 (the gradient of each row's loss; for a mean 1 / rows that count) and the forward's lse:
  * dl[m,v] = dloss[m] * (exp(x[m] . w[v] - lse[m]) - [v = label[m]]), 0 for a row whose label counts for nothing (whatever its
  * dloss and lse are); dx [M, K] = bf16(dl w), dw [V, K] = dl^T x in bf16 (dw_type 0) or fp32 (1). Either of dx and dw may be
- * NULL. Goes over the vocabulary in pieces; dl of a piece is held in bf16 (its label's term with an fp32 remainder). A row that counts for
- * nothing takes no part, whatever its x holds. workspace: hk_linear_cross_entropy_workspace_bytes(M, V, K, 1) bytes (enough for
+ * NULL. Goes over the vocabulary in pieces; dl of a piece is held in bf16, its label's term with an fp32 remainder: for a bf16 dw and for dx
+ * (an error of at most 2^-8 of each other term, before the rounding to bf16). For an fp32 dw in two numbers of bf16 (2^-16 of each term),
+ * which takes a third to two thirds longer. A row that counts for nothing takes no part, whatever its x holds. workspace: hk_linear_cross_entropy_workspace_bytes(M, V, K, 1) bytes (enough for
  * the forward too). */
 int hk_linear_cross_entropy_backward(const void* x_bf16, const void* w_bf16, const void* labels, int label_type,
                                      const float* lse, const float* dloss, void* dx_bf16_or_null, void* dw_or_null, int dw_type,

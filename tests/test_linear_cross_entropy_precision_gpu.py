@@ -1,0 +1,64 @@
+"""Digits of the head's results where single precision or bf16 could lose them: logits that fp32 holds exactly (operands are
+small multiples of 1/8), so that every difference from the definitions in 64 bits is the epilogues' and the gradients' own."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def _exact_case(M, V, K, seed, size=8, ignored=0.1):
+    """x and w: multiples of 1/8 up to size / 8; logits: multiples of 1/64 below 2^18 / 64. Every other row's label is its largest logit."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    eighths = lambda *s: (torch.randint(-size, size + 1, s, device=DEV, generator=g) / 8).to(torch.bfloat16)
+    x, w = eighths(M, K), eighths(V, K)
+    l = x.double() @ w.double().t().contiguous()
+    assert float(l.abs().max()) < 2**12
+    labels = torch.randint(0, V, (M,), device=DEV, generator=g)
+    labels = torch.where(torch.arange(M, device=DEV) % 2 == 0, l.argmax(dim=1), labels)
+    labels[torch.rand(M, device=DEV, generator=g) < ignored] = -100
+    return x, w, l, labels, torch.randn(M, device=DEV, generator=g)
+
+
+def _gradients(hk, x, w, labels, lse, dloss, dw_dtype):
+    tk = hk.tk_kernel
+    (M, K), V = x.shape, w.shape[0]
+    ws = torch.full((tk.linear_cross_entropy_workspace_bytes(M, V, K),), 0xFF, dtype=torch.uint8, device=DEV)
+    dx, dw = torch.empty_like(x), torch.full((V + 1, K), 777.0, dtype=dw_dtype, device=DEV)
+    tk.dispatch_linear_cross_entropy_backward(x, w, labels, lse, dloss, dx, dw[:V], ws)
+    assert torch.all(dw[V] == 777.0)
+    return dx, dw[:V]
+
+
+def _dl(l, labels, lse, dloss):
+    """dl for the lse that the call is given, |dl| and the error of |dl| before it is rounded to fewer bits: the exponential's argument
+    in fp32 (half a step of lse log2 e and of the difference), the instruction by a step, the products and the difference by half of one."""
+    counts = labels >= 0
+    hot = torch.zeros_like(l)
+    hot[counts, labels[counts]] = 1.0
+    scale = torch.where(counts, dloss.double(), 0.0)[:, None]
+    lse = lse.double()[:, None]
+    p = torch.exp(l - lse)
+    arg = (lse.abs() + (l - lse).abs()) * 2**-23
+    return scale * (p - hot), scale.abs() * (p * (arg + 2**-21) + (p + hot) * 2**-22) + (scale.abs() + 1) * 2.0**-126
+
+
+@pytest.mark.parametrize("M,V,K", [(45, 333, 8), (130, 1000, 64), (700, 3000, 64), (973, 1187, 792), (2000, 9001, 264), (40000, 7777, 64)])
+def test_weight_gradient_in_fp32_has_more_digits_than_bf16(hk, M, V, K):
+    print(f"linear cross entropy, fp32 dw M={M} V={V} K={K}", flush=True)
+    x, w, l, labels, dloss = _exact_case(M, V, K, M + K)
+    lse = torch.logsumexp(l, dim=1).float()
+    _, dw = _gradients(hk, x, w, labels, lse, dloss, torch.float32)
+    want, err, size = (torch.zeros(V, K, dtype=torch.float64, device=DEV) for _ in range(3))
+    for a in range(0, M, 8000):
+        s = slice(a, a + 8000)
+        dl, d = _dl(l[s], labels[s], lse[s], dloss[s])
+        xd = x[s].double()
+        want += dl.t().contiguous() @ xd
+        # what is left of dl behind two numbers of bf16: half a step of half a step
+        err += (d + (dl.abs() + d) * 2**-16).t().contiguous() @ xd.abs()
+        size += dl.abs().t().contiguous() @ xd.abs()
+    # 2 M products added in fp32, a step each, doubled for what a matrix instruction does inside; the smallest number of bf16 and fp32
+    err += size * 2 * (2 * M + 8) * 2**-24 + 2 * (M + 1) * 2.0**-126
+    bad = (dw.double() - want).abs() > err + want.abs() * 2**-24
+    assert not bad.any(), (int(bad.sum()), float((dw.double() - want).norm() / want.norm()))
