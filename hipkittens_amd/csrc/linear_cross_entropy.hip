@@ -437,7 +437,8 @@ static LayoutChoice head_choice(int rows, int cols, int k) {   // a product of r
     return choose_layout({tiles(256), tiles(128), tiles(64)}, tiles_of(k, kLayoutStep), moe_num_compute_units());
 }
 
-// forward: label logits, then the partial results
+// forward: label logits, then the partial results. bytes: what any number of rows up to M takes, so that a workspace for the largest batch
+// serves the smaller ones, whose tiles may be smaller and their partial results more.
 struct HeadForwardPlan {
     LayoutChoice tile;
     int blocks;   // columns of a partial result: a wave's patch
@@ -447,7 +448,8 @@ struct HeadForwardPlan {
         blocks = 2 * tiles_of(V, tile == kLayout256 ? 256 : tile == kLayout64Deep ? 64 : 128);
         label_logit = 0;
         partial = up256((size_t)M * 4);
-        bytes = partial + up256((size_t)M * blocks * sizeof(float2));
+        const size_t rows64 = std::min(M, 64 * (moe_num_compute_units() / tiles_of(V, 64)));   // most that 64x64 tiles are taken for
+        bytes = partial + up256(std::max((size_t)M * tiles_of(V, 128), rows64 * tiles_of(V, 64)) * 2 * sizeof(float2));
     }
 };
 // backward: dl of a piece, then the fp32 sums of dx. parts: the numbers of bf16 that dl is held in, 2 for dW in fp32.
@@ -457,6 +459,27 @@ struct HeadBackwardPlan {
     LayoutChoice grads;
     int splits, split_cols;
     size_t rest, starts, list, x, dl, sums, bytes;   // rest: `parts` remainders of each row
+    // Bytes of dl and the second copy of x, which are held together. Neither grows when there are fewer rows.
+    static long long held_for_dl(long long M, int V, int K) {
+        const long long fill = 256ll * tiles_of(moe_num_compute_units(), tiles_of(K, 256));
+        return std::max(512ll << 20, std::min({2 * M * fill, 4ll << 30, 512 * M * tiles_of(V, 512)}));
+    }
+    // What any number of rows up to M takes, with either type of dW. Fewer rows than `cut` have dx tiles for less than the CUs' places, and up to
+    // 1 + 9/8 places / tiles sums of dx (per_split below is at least 8/9 of all K-steps over the places): bounded by the places' tiles.
+    static size_t bytes_up_to(int M, int V, int K) {
+        const long long all = (long long)tiles_of(V, 256) * 256, cus = moe_num_compute_units();
+        auto uncut = [&](long long m) {
+            const long long held = held_for_dl(m, V, K), copy = 2 * m * K;
+            const long long one = std::min(std::max(held, 512 * m), 2 * m * all);
+            const long long two = std::min(std::max({held - copy, held / 4, 1024 * m}), 4 * m * all) + copy;
+            return up256((size_t)m * 8) + up256((size_t)m * 4) + up256(((size_t)tiles_of(V, 256) * 16 + 1) * 4) + up256((size_t)copy) +
+                   up256((size_t)std::max(one, two)) + up256((size_t)m * K * 4) + 1024;
+        };
+        const long long cut = std::min((long long)M, std::max(256 * ((cus - 1) / tiles_of(K, 256)), 128 * ((2 * cus - 1) / tiles_of(K, 128))));
+        auto tile_bytes = [&](long long t) { return 4 * std::min(t, cut) * std::min<long long>(t, K); };
+        const long long sums = std::min(4 * cut * K * tiles_of(tiles_of(V, kLayoutStep), 8), std::max(cus * tile_bytes(256), 2 * cus * tile_bytes(128)) * 9 / 8);
+        return std::max(uncut(M), uncut(cut) + up256((size_t)sums));
+    }
     HeadBackwardPlan(int M, int V, int K, int parts) {
         // Pieces of 512 MB: a piece's items of dx are the longer and its tiles the more, the fewer pieces there are (backward, us, pieces of
         // 128 / 256 / 512 / 2048 MB: 4096 x 201088 x 2880 11492 / 11737 / 11571 / 11331, 8192 x 129280 x 7168 34150 / 33106 / 32755 /
@@ -464,10 +487,9 @@ struct HeadBackwardPlan {
         // of M / 64 K-steps, and the rest of the chip idle), as many classes as fill the CUs, up to 4 GB and half of dl (512 MB / 1 / 2 / 4 GB
         // at most: 65536 x 32000 x 1024 15444 / 11947 / 11416 / 11394, 262144 x 32000 x 1024 180717 / 104194 / 65851 / 47530).
         // Rows of at most 4 MB: 32-bit offsets inside a K-step's rows.
-        const long long fill = 256ll * tiles_of(moe_num_compute_units(), tiles_of(K, 256));
         // dl in two parts, and the second copy of x, are held in the same bytes: pieces of half the classes and less.
         const long long copies = 2ll * M * K * (parts - 1);
-        long long held = std::max(512ll << 20, std::min({2ll * M * fill, 4ll << 30, 512ll * M * tiles_of(V, 512)}));
+        long long held = held_for_dl(M, V, K);
         held = std::max(held - copies, held / 4);
         const long long most = std::min(held / (2ll * parts * M), 1ll << 21) / 256 * 256, all = (long long)tiles_of(V, 256) * 256;
         piece = (int)std::max(256ll, std::min(most, all));
@@ -504,7 +526,7 @@ struct HeadBackwardPlan {
         x = starts + up256(((size_t)tiles_of(V, 256) * 16 + 1) * 4);
         dl = x + up256((size_t)M * K * 2 * parts);
         sums = dl + up256((size_t)M * piece * 2 * parts);
-        bytes = sums + (piece < V || splits > 1 ? up256((size_t)splits * M * K * 4) : 0);
+        bytes = std::max(bytes_up_to(M, V, K), sums + (piece < V || splits > 1 ? up256((size_t)splits * M * K * 4) : 0));
     }
 };
 

@@ -505,8 +505,8 @@ int hk_moe_grouped_gemm_wgrad(const void* dy_bf16, const void* x_bf16, const int
  * loss[m] = lse[m] - x[m] . w[label[m]]. x [M, K], w [V, K] bf16; labels [M] int32 (label_type 0) or int64 (1); loss, lse [M]
  * fp32. A label outside [0, V) counts for nothing: loss 0 (lse is written). Requirements: K % 8 == 0, K <= 2^21, M < 2^25, V < 2^30,
  * fewer than 2^23 tiles of 128 x 128 in M x V, M x K and V x K; x and w 16-byte aligned; workspace 16-byte aligned, of
- * hk_linear_cross_entropy_workspace_bytes(M, V, K, 0) bytes (0 for a shape that is refused), nothing in it is kept from one
- * call to the next. */
+ * hk_linear_cross_entropy_workspace_bytes(M, V, K, 0) bytes (0 for a shape that is refused; never less for a larger M), nothing in
+ * it is kept from one call to the next. */
 size_t hk_linear_cross_entropy_workspace_bytes(int M, int V, int K, int backward);
 int hk_linear_cross_entropy(const void* x_bf16, const void* w_bf16, const void* labels, int label_type, float* loss, float* lse,
                             int M, int V, int K, void* workspace, size_t workspace_bytes, void* stream);
