@@ -26,7 +26,7 @@
 
 namespace hk {
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f;
 
 // Tile rows of a raster group, as the BF16 GEMM takes them: bands where the operands do not fit the memory-side cache (us, without /
 // with: forward 8192 x 129280 x 7168 10957 / 10600, 4096 x 201088 x 2880 3555 / 3522, backward of the first 33689 / 32919).
@@ -125,9 +125,14 @@ __global__ __launch_bounds__(16 * kJoin) void head_loss_kernel(const float2* __r
         if (seg < off) part[seg][r] = all = join(all, part[seg + off][r]);
     }
     if (seg == 0 && m < M) {
-        const float l = (all.x + log2f(all.y)) * kLn2;
-        lse[m] = l;
-        loss[m] = labels.at(m, V) >= 0 ? l - label_logit[m] : 0.f;
+        // lse is rounded once. The loss does not come from it: for a confident row it is far smaller than a step of lse, but the label's distance
+        // from the largest logit and the logarithm of the sum are of its own size. (No loss is negative; a rounding of the sum, 1 or more, may be.)
+        constexpr double kToNatural = 1.0 / (double)kLog2e;
+        const float sum2 = log2f(all.y);
+        lse[m] = (float)(((double)all.x + (double)sum2) * kToNatural);
+        float l = 0.f;
+        if (labels.at(m, V) >= 0) l = (sum2 - __builtin_fmaf(label_logit[m], kLog2e, -all.x)) * (float)kToNatural;
+        loss[m] = l < 0.f ? 0.f : l;
     }
 }
 

@@ -62,3 +62,28 @@ def test_weight_gradient_in_fp32_has_more_digits_than_bf16(hk, M, V, K):
     err += size * 2 * (2 * M + 8) * 2**-24 + 2 * (M + 1) * 2.0**-126
     bad = (dw.double() - want).abs() > err + want.abs() * 2**-24
     assert not bad.any(), (int(bad.sum()), float((dw.double() - want).norm() / want.norm()))
+
+
+def test_loss_of_confident_rows_and_large_logits(hk):
+    """Logits of hundreds: the loss is the sum's logarithm over the label's term and does not carry the rounding of lse, which is
+    a hundred times larger than the loss of a confident row; no loss is negative. lse is rounded once."""
+    M, V, K = 500, 777, 64
+    print("linear cross entropy, loss of large logits", flush=True)
+    x, w, l, labels, _ = _exact_case(M, V, K, 3, size=64)
+    l0 = l.max(dim=1).values
+    tk = hk.tk_kernel
+    ws = torch.full((tk.linear_cross_entropy_workspace_bytes(M, V, K, backward=False),), 0xFF, dtype=torch.uint8, device=DEV)
+    loss, lse = torch.empty(M, device=DEV), torch.empty(M, device=DEV)
+    tk.dispatch_linear_cross_entropy(x, w, labels, loss, lse, ws)
+    counts = labels >= 0
+    want = torch.logsumexp(l, dim=1)
+    mine = l.gather(1, labels.clamp(min=0)[:, None]).squeeze(1)
+    # the sum relative to the largest term: at most 100 additions in a row, each half a step, the exponentials' arguments and
+    # the instruction a few steps more
+    total = 2**-17
+    assert ((lse.double() - want).abs() <= want.abs() * 2**-24 + total).all()
+    want_loss = torch.where(counts, torch.log(torch.exp(l - mine[:, None]).sum(dim=1)), 0.0)
+    want_loss = torch.where(counts & (l0 - mine > 300), want - mine, want_loss)
+    # the label's distance from the largest logit times log2 e and ln 2: three roundings of what is at most the loss
+    assert ((loss.double() - want_loss).abs() <= total + want_loss * 2**-22).all(), float((loss.double() - want_loss).abs().max())
+    assert (loss >= 0).all() and torch.all(loss[~counts] == 0)
