@@ -248,13 +248,15 @@ __global__ __launch_bounds__(256) void head_dlogits_kernel(const uint16_t* __res
     for (int m = 0; m < Tile::F; ++m) {
         const int at = row + 16 * m + r;
         const int label = at < M ? labels.at(at, V) : -1;
-        const float scale = label >= 0 ? dloss[at] : 0.f, lse2 = label >= 0 ? lse[at] * kLog2e : 0.f;
+        const float scale = label >= 0 ? dloss[at] : 0.f, own = label >= 0 ? lse[at] : 0.f, lse2 = own * kLog2e;
+        // what the rounding of lse2 leaves (of lse2 = 500 up to 2^-16, more than a confident row's p - 1) goes into the exponentials' factor
+        const float part = fabsf(lse2) < INFINITY ? scale * __builtin_amdgcn_exp2f(-__builtin_fmaf(own, kLog2e, -lse2)) : scale;
         v4f d[Tile::F];
         Tile::read_row(acc[m], d);
 #pragma unroll
         for (int n = 0; n < Tile::F; ++n)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) d[n][j] = scale * __builtin_amdgcn_exp2f(__builtin_fmaf(d[n][j], kLog2e, -lse2));
+            for (int j = 0; j < 4; ++j) d[n][j] = part * __builtin_amdgcn_exp2f(__builtin_fmaf(d[n][j], kLog2e, -lse2));
         const bool here = label >= col && label < col + Tile::kPatch && ((label >> 2) & 3) == g;   // among this lane's
         if (__any(here)) {
             float left_over = 0.f;

@@ -87,3 +87,39 @@ def test_loss_of_confident_rows_and_large_logits(hk):
     # the label's distance from the largest logit times log2 e and ln 2: three roundings of what is at most the loss
     assert ((loss.double() - want_loss).abs() <= total + want_loss * 2**-22).all(), float((loss.double() - want_loss).abs().max())
     assert (loss >= 0).all() and torch.all(loss[~counts] == 0)
+
+
+def test_gradients_of_confident_rows_and_large_logits(hk):
+    """p - 1 of a confident row is far smaller than a rounding of lse log2 e where lse is several hundred: that rounding is not added."""
+    M, V, K = 64, 777, 64
+    print("linear cross entropy, gradients of confident rows", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(4)
+    x, w, _, _, dloss = _exact_case(M, V, K, 4, size=64, ignored=0.0)
+    # rows of three classes within a few units of one another at the top of some hundred logits
+    at = torch.randint(0, V - 3, (M,), device=DEV, generator=g)
+    w[1::3], w[2::3] = w[0::3][: w[1::3].shape[0]], w[0::3][: w[2::3].shape[0]]
+    top = at // 3 * 3
+    x = w[top].clone()
+    x[:, 0] = 8.0
+    w[:, 0] = ((torch.arange(V, device=DEV) % 3 == 0).float() * 0.875).to(torch.bfloat16)   # 7 ahead of its copies: p - 1 about -2e-3
+    l = x.double() @ w.double().t().contiguous()
+    lse = torch.logsumexp(l, dim=1).float()
+    labels = top.clone()
+    dx, dw = _gradients(hk, x, w, labels, lse, dloss, torch.float32)
+    hot = torch.zeros_like(l)
+    hot[torch.arange(M, device=DEV), labels] = 1.0
+    p = torch.exp(l - lse.double()[:, None])
+    assert float((1 - p.gather(1, labels[:, None])).max()) < 0.01 and float(lse.abs().min()) > 300
+    scale = dloss.double()[:, None]
+    dl = scale * (p - hot)
+    # as in _dl, without a rounding of lse: the argument's own, which counts where the exponential does (|a| e^a < 1)
+    d = scale.abs() * (2**-22 + p * 2**-21 + (p + hot) * 2**-22) + (scale.abs() + 1) * 2.0**-126
+    d = torch.where((l - lse.double()[:, None]) < -60, scale.abs() * 2**-60, d)
+    half = (dl.abs() + d) * 2**-8 * (1 - hot)
+    dx_err = (d + half) @ w.double().abs() + (dl.abs() @ w.double().abs()) * 2 * (V + 8) * 2**-24
+    bad = (dx.double() - dl @ w.double()).abs() > dx_err * (1 + 2**-8) + (dl @ w.double()).abs() * 2**-8
+    assert not bad.any(), int(bad.sum())
+    want = dl.t().contiguous() @ x.double()
+    dw_err = ((d + (dl.abs() + d) * 2**-16).t().contiguous() + dl.abs().t().contiguous() * 2 * (2 * M + 8) * 2**-24) @ x.double().abs()
+    bad = (dw.double() - want).abs() > dw_err + want.abs() * 2**-24
+    assert not bad.any(), (int(bad.sum()), float((dw.double() - want).norm() / want.norm()))
