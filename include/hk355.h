@@ -490,7 +490,7 @@ int hk_moe_unpermute_backward(const void* dy_bf16, const void* o_bf16, const flo
 /* The experts' products in bf16: y[r, :] = bf16(x[r, :] W[e]^T) for the rows r of [expert_offsets[e], expert_offsets[e+1]).
  * x [R, K], w [E, N, K], y [R, N]; expert_offsets [E+1] int32 on the device, ascending, the last at most R. Rows behind it
  * are neither read nor written, and an expert's result depends on its own rows only. (Offsets are held inside [0, R] and in
- * order whatever they hold.) Requirements: N % 8 == 0, K % 8 == 0, both at most 2^21, E <= 512, R < 2^30, fewer than 2^24
+ * order whatever they hold, by a running maximum: no row belongs to two experts.) Requirements: N % 8 == 0, K % 8 == 0, both at most 2^21, E <= 512, R < 2^30, fewer than 2^24
  * tiles of 128 x 128 in all; x, w and y 16-byte aligned; no workspace. */
 int hk_moe_grouped_gemm(const void* x_bf16, const void* w_bf16, const int32_t* expert_offsets, void* y_bf16, int R, int E,
                         int N, int K, void* stream);
