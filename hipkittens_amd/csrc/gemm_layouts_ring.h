@@ -143,6 +143,7 @@ __device__ __forceinline__ void ring_product(uint8_t* smem, const TileOperand& A
     uint32_t off1 = kRingSlot, off2 = 2 * kRingSlot;
 
     auto step = [&]<int P>(int kt) __attribute__((always_inline)) {
+        mfma_enter_agpr(acc);   // (the loop's tail is a branch of its own; no difference in time)
         oa.advance(oa.opaque(step_a));   // (else multiples of it are held for the unrolled K-steps)
         ob.advance(ob.opaque(step_b));
         const bool more = kt + 2 < nk;
