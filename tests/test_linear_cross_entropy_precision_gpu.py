@@ -123,3 +123,61 @@ def test_gradients_of_confident_rows_and_large_logits(hk):
     dw_err = ((d + (dl.abs() + d) * 2**-16).t().contiguous() + dl.abs().t().contiguous() * 2 * (2 * M + 8) * 2**-24) @ x.double().abs()
     bad = (dw.double() - want).abs() > dw_err + want.abs() * 2**-24
     assert not bad.any(), (int(bad.sum()), float((dw.double() - want).norm() / want.norm()))
+
+
+@pytest.mark.parametrize("M,V,K", [(5000, 2, 72), (3001, 17, 264), (4000, 130, 1032), (2500, 40, 8), (6000, 1000, 520)])
+@pytest.mark.parametrize("kind", ["spread", "sorted", "one"])
+@pytest.mark.parametrize("dw_dtype", [torch.bfloat16, torch.float32])
+def test_many_rows_of_each_class(hk, M, V, K, kind, dw_dtype):
+    """Hundreds to thousands of rows with a label among the classes of one wave, in the order of the classes or mixed, or all of one
+    class: the label's remainder is added for each of them."""
+    print(f"linear cross entropy, many rows a class M={M} V={V} K={K} {kind} {dw_dtype}", flush=True)
+    x, w, l, labels, dloss = _exact_case(M, V, K, M + V)
+    if kind == "sorted":
+        labels = labels.sort().values
+    elif kind == "one":
+        labels = torch.where(labels >= 0, V - 1, labels)
+    lse = torch.logsumexp(l, dim=1).float()
+    dx, dw = _gradients(hk, x, w, labels, lse, dloss, dw_dtype)
+    dl, d = _dl(l, labels, lse, dloss)
+    hot = torch.zeros_like(l)
+    hot[labels >= 0, labels[labels >= 0]] = 1.0
+    xd, wd = x.double(), w.double()
+    half = (dl.abs() + d) * 2**-8 * (1 - hot)   # one number of bf16, but for the label's term
+    dlt = dl.t().contiguous()
+    want = dlt @ xd
+    err = (d + (half if dw_dtype == torch.bfloat16 else (dl.abs() + d) * 2**-16)).t().contiguous() @ xd.abs()
+    err += (dlt.abs() @ xd.abs()) * 2 * (2 * M + 8) * 2**-24 + 2 * (M + 1) * 2.0**-126
+    step = 2**-8 if dw_dtype == torch.bfloat16 else 2**-24
+    bad = (dw.double() - want).abs() > err * (1 + step) + want.abs() * step
+    assert not bad.any(), (int(bad.sum()), float((dw.double() - want).norm() / want.norm()))
+    want = dl @ wd
+    err = (d + half) @ wd.abs() + (dl.abs() @ wd.abs()) * 2 * (V + 8) * 2**-24 + 2 * (V + 1) * 2.0**-126
+    bad = (dx.double() - want).abs() > err * (1 + 2**-8) + want.abs() * 2**-8
+    assert not bad.any(), int(bad.sum())
+
+
+@pytest.mark.parametrize("M,V,K", [(600, 5, 200), (1500, 40, 504), (2000, 2, 1000)])
+@pytest.mark.parametrize("kind", ["spread", "one"])
+def test_each_rows_label_term_of_many(hk, M, V, K, kind):
+    """Rows of x with one element other than 0: an element of dw is the sum of three rows' products, in which one row's missing or
+    misplaced remainder shows."""
+    print(f"linear cross entropy, rows of one element M={M} V={V} K={K} {kind}", flush=True)
+    g = torch.Generator(device=DEV).manual_seed(M + K)
+    _, w, _, labels, dloss = _exact_case(M, V, K, M + V)
+    x = torch.zeros(M, K, dtype=torch.bfloat16, device=DEV)
+    x[torch.arange(M, device=DEV), torch.arange(M, device=DEV) % K] = (torch.randint(1, 9, (M,), device=DEV, generator=g) / 8).to(torch.bfloat16)
+    if kind == "one":
+        labels = torch.where(labels >= 0, V // 2, labels)
+    l = x.double() @ w.double().t().contiguous()
+    lse = torch.logsumexp(l, dim=1).float()
+    _, dw = _gradients(hk, x, w, labels, lse, dloss, torch.float32)
+    dl, d = _dl(l, labels, lse, dloss)
+    hot = torch.zeros_like(l)
+    hot[labels >= 0, labels[labels >= 0]] = 1.0
+    xd, dlt = x.double(), dl.t().contiguous()
+    # two numbers of bf16 and the remainder's two: at most 12 products other than 0, half a step of fp32 each, doubled
+    err = (d + (dl.abs() + d) * 2**-16 * (1 - hot)).t().contiguous() @ xd + (dlt.abs() @ xd) * 24 * 2**-24 + 24 * 2.0**-126
+    want = dlt @ xd
+    bad = (dw.double() - want).abs() > err + want.abs() * 2**-24
+    assert not bad.any(), (int(bad.sum()), float((dw.double() - want).norm() / want.norm()))
