@@ -40,8 +40,8 @@ __device__ __forceinline__ v2i lds_read_tr(uint32_t addr) {
 }
 
 // Tile product of four waves, each a quarter (TILE / 2 square) of TILE x TILE. Two LDS stages: the next K-step is loaded while this
-// one is multiplied, two workgroups on a CU. One: each K-step in turn, four workgroups on a CU, for contractions of a few K-steps. acc[m][n] holds, for tile row 16 m + lane % 16 of the wave's quarter, its columns
-// 16 n + 4 (lane / 16) .. +4.
+// one is multiplied, two workgroups on a CU. One: each K-step in turn, four workgroups on a CU, for contractions of a few K-steps.
+// acc[m][n] holds, for tile row 16 m + lane % 16 of the wave's quarter, its columns 16 n + 4 (lane / 16) .. +4.
 constexpr int kLayoutTile = 128;
 constexpr int kLayoutStageBytes = 2 * kLayoutTile * 128;
 

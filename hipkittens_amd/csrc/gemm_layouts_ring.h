@@ -452,10 +452,11 @@ typedef LayoutTileDeep<64> LayoutTile64Deep;
 // K-step, us. The constants are fits to 32 experts of 4096 x 7168: 65536 rows forward 2873 large / 4130 small, gradient of the
 // weights with 3, 9 and 33 K-steps 660, 1167, 3013 / 628, 1290, 3738; small_step: the small kernel's K-step, which the gradient of
 // the weights (both operands in runs of 256 bytes) takes faster than the others.
-constexpr double kSmallStepAlong = 1.1, kSmallStepAcross = 0.945;
+constexpr double kLargeFixed = 7.0, kLargeStep = 1.43, kSmallFixed = 2.7, kSmallStepAlong = 1.1, kSmallStepAcross = 0.945;
+constexpr double kDeepStep = 0.45;   // LayoutTile128Deep, alone on its CU
 inline bool prefer_tile256(double tiles256, double tiles128, double k_steps, int cus, double small_step = kSmallStepAlong) {
     auto rounds = [](double tiles, double at_once) { return tiles <= at_once ? 1.0 : tiles / at_once + 0.2; };
-    return rounds(tiles256, cus) * (7.0 + 1.43 * k_steps) < rounds(tiles128, 2.0 * cus) * (2.7 + small_step * k_steps);
+    return rounds(tiles256, cus) * (kLargeFixed + kLargeStep * k_steps) < rounds(tiles128, 2.0 * cus) * (kSmallFixed + small_step * k_steps);
 }
 // The tile, and for the small ones the number of LDS stages: many where no CU gets a second workgroup anyway, and 64x64 tiles as long as
 // there are no more of them than CUs. (us, 128x128 / 64x64: forward of 16 rows of 4 experts of 4096 x 4096, 256 tiles of 64x64, 32.5 / 23.4;

@@ -96,7 +96,7 @@ __global__ __launch_bounds__(256) void head_logits_kernel(const uint16_t* __rest
 }
 
 // Joins the partial results (exponents of 2) of a row: 16 rows a workgroup, 64 threads each, thread i the blocks i, 64 + i, .., eight loads
-// at a time; then pair by pair. (Forward of 60 x 100000 x 600, 1564 blocks: 66 us with 16 threads a row and a load at a time, now 42.)
+// at a time; then pair by pair. (Forward of 60 x 100000 x 600, 1564 blocks: 66 us with 16 threads a row and a load at a time, now 39.)
 constexpr int kJoin = 64;
 __global__ __launch_bounds__(16 * kJoin) void head_loss_kernel(const float2* __restrict__ partial, const float* __restrict__ label_logit,
                                                                HeadLabels labels, int M, int V, int blocks, float* __restrict__ loss,
@@ -540,11 +540,11 @@ struct HeadBackwardPlan {
             Cut c;
             c.split_cols = tiles_of(steps_v, tiles_of(steps_v, per_split)) * kLayoutStep;
             c.splits = tiles_of(cols, c.split_cols);
-            const double fixed = tile == 256 ? 7.0 : 2.7, items = dx * c.splits + dw;
-            const double along = tile == 256 ? 1.43 : kSmallStepAlong, across = tile == 256 ? 1.43 : kSmallStepAcross;
+            const double fixed = tile == 256 ? kLargeFixed : kSmallFixed, items = dx * c.splits + dw;
+            const double along = tile == 256 ? kLargeStep : kSmallStepAlong, across = tile == 256 ? kLargeStep : kSmallStepAcross;
             const double longest = std::max(along * std::min(per_split, steps_v), across * steps_m);
             c.us = std::max((dx * (fixed + along * steps_v) + dw * (fixed + across * steps_m)) / places, fixed + longest);
-            if (tile == 128 && items <= cus) c.us = 2.7 + 0.45 * std::max(std::min(per_split, steps_v), steps_m);   // LayoutTile128Deep
+            if (tile == 128 && items <= cus) c.us = kSmallFixed + kDeepStep * std::max(std::min(per_split, steps_v), steps_m);   // LayoutTile128Deep
             c.deep = tile == 128 && items <= cus;
             return c;
         };

@@ -212,7 +212,7 @@ static int launch_wgrad(const void* dy, const void* x, const int32_t* offsets, v
     // 128 634 / 635 / 565, 256 800 / 874 / 784, 384 936 / 1092 / 962; 128 experts of 2880 x 2880, 128 rows, fp32 1090 / 1117 / 1017;
     // fewer tiles, 8 experts of 1024 x 1024: 24 / 14 / 18.)
     if (e * n128 * k128 >= 4.0 * cus) {
-        const double large = e * n256 * k256 / cus * (7.0 + 1.43 * steps), single = e * n128 * k128 / (4.0 * cus) * (3.8 + 2.08 * steps);
+        const double large = e * n256 * k256 / cus * (kLargeFixed + kLargeStep * steps), single = e * n128 * k128 / (4.0 * cus) * (3.8 + 2.08 * steps);
         return large < single ? launch_wgrad_tile<LayoutTile256, T>(dy, x, offsets, dW, R, E, N, K, s)
                               : launch_wgrad_tile<LayoutTile128Stages<1>, T>(dy, x, offsets, dW, R, E, N, K, s);
     }
