@@ -502,8 +502,8 @@ int hk_moe_grouped_gemm_wgrad(const void* dy_bf16, const void* x_bf16, const int
                               int R, int E, int N, int K, void* stream);
 
 /* Softmax cross entropy of the logits x W^T without the logits in memory: lse[m] = log sum_v exp(x[m] . w[v]) and
- * loss[m] = lse[m] - x[m] . w[label[m]] (from the sums, not from the rounded lse; never negative). x [M, K], w [V, K] bf16; labels [M] int32 (label_type 0) or int64 (1); loss, lse [M]
- * fp32. A label outside [0, V) counts for nothing: loss 0 (lse is written). Requirements: K % 8 == 0, K <= 2^21, M < 2^25, V < 2^30,
+ * loss[m] = lse[m] - x[m] . w[label[m]] (from the sums, not from the rounded lse; never negative). x [M, K], w [V, K] bf16;
+ * labels [M] int32 (label_type 0) or int64 (1); loss, lse [M] fp32. A label outside [0, V) counts for nothing: loss 0 (lse is written). Requirements: K % 8 == 0, K <= 2^21, M < 2^25, V < 2^30,
  * fewer than 2^23 tiles of 128 x 128 in M x V, M x K and V x K; x and w 16-byte aligned; workspace 16-byte aligned, of
  * hk_linear_cross_entropy_workspace_bytes(M, V, K, 0) bytes (0 for a shape that is refused; never less for a larger M), nothing in
  * it is kept from one call to the next. */
@@ -516,8 +516,8 @@ int hk_linear_cross_entropy(const void* x_bf16, const void* w_bf16, const void* 
  * dloss and lse are); dx [M, K] = bf16(dl w), dw [V, K] = dl^T x in bf16 (dw_type 0) or fp32 (1). Either of dx and dw may be
  * NULL. Goes over the vocabulary in pieces; dl of a piece is held in bf16, its label's term with an fp32 remainder: for a bf16 dw and for dx
  * (an error of at most 2^-8 of each other term, before the rounding to bf16). For an fp32 dw in two numbers of bf16 (2^-16 of each term),
- * which takes a third to four fifths longer. A row that counts for nothing takes no part, whatever its x holds. workspace: hk_linear_cross_entropy_workspace_bytes(M, V, K, 1) bytes (enough for
- * the forward too). */
+ * which takes a third to four fifths longer. A row that counts for nothing takes no part, whatever its x holds. workspace:
+ * hk_linear_cross_entropy_workspace_bytes(M, V, K, 1) bytes (enough for the forward too). */
 int hk_linear_cross_entropy_backward(const void* x_bf16, const void* w_bf16, const void* labels, int label_type,
                                      const float* lse, const float* dloss, void* dx_bf16_or_null, void* dw_or_null, int dw_type,
                                      int M, int V, int K, void* workspace, size_t workspace_bytes, void* stream);
