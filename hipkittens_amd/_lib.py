@@ -113,6 +113,10 @@ SIGNATURES = {
                                 [c_void_p, c_size_t, c_void_p]),
     "hk_linear_cross_entropy_backward": (c_int, [c_void_p] * 3 + [c_int] + [c_void_p] * 4 + [c_int] * 4 +
                                          [c_void_p, c_size_t, c_void_p]),
+    "hk_gated_gemm": (c_int, [c_void_p] * 5 + [c_int] * 6 + [c_float] * 2 + [c_void_p]),
+    "hk_gated_gemm_dgrad": (c_int, [c_void_p] * 6 + [c_int] * 6 + [c_float] * 2 + [c_void_p]),
+    "hk_bf16_gemm_dgrad": (c_int, [c_void_p] * 3 + [c_int] * 3 + [c_void_p]),
+    "hk_bf16_gemm_wgrad": (c_int, [c_void_p] * 3 + [c_int] * 4 + [c_void_p]),
 }
 
 

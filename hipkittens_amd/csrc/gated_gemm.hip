@@ -1,0 +1,234 @@
+// The gated feed-forward block in bf16: both projections, the activation and the product in one kernel, and the way back through the
+// down projection and the activation in another. Rows of a dense block, or grouped by expert (expert_offsets [E+1], on the device).
+//
+//   forward    g[r, c] = x[r] . Wg[c], u[r, c] = x[r] . Wu[c], h = (u' + b) g' s(a g') with g' = min(g, l), u' = clamp(u, -l, l),
+//              s the logistic function: SiLU(g) u is a = 1, l = inf, b = 0, the clamped form b = 1 with its a and l
+//   backward   dh = dy W2, dg = [g <= l] dh (u' + b) s (1 + a g' (1 - s)), du = [|u| <= l] dh g' s, and h again, for dW2 = dy^T h
+//
+// What follows the backward kernel are products: dx = dgu W13, dW13 = dgu^T x. g and u are kept in bf16 (gate_up [R, 2I], in the
+// order of W13's rows), each rounded once; h in the forward pass comes from the unrounded values.
+//
+// fp32 accumulation and activation, one rounding. The products are those of gemm_layouts_ring.h, which bound both kernels; in the forward one
+// every 32 rows of the weight tile in LDS are 16 gate rows and the 16 up rows of the same columns (kPairs), so that both values of
+// an element are in one lane's accumulators and the activation needs no exchange between lanes.
+#include "moe_grouped.h"
+#include "../../include/hk355.h"
+
+namespace hk {
+
+struct Gate {
+    float alpha, limit, beta;
+    __device__ __forceinline__ float top(float g) const { return g > limit ? limit : g; }   // (a NaN stays one)
+    __device__ __forceinline__ float lin(float u) const { return (u > limit ? limit : u < -limit ? -limit : u) + beta; }
+    __device__ __forceinline__ float sig(float g) const {   // of a clamped g
+        return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * (alpha * -1.4426950408889634f)));
+    }
+    __device__ __forceinline__ float value(float g, float u) const {
+        const float t = top(g);
+        return lin(u) * (t * sig(t));
+    }
+    // h of (g, u), and from dh the gradients of both
+    __device__ __forceinline__ float gradients(float g, float u, float dh, float& dg, float& du) const {
+        const float t = top(g), v = lin(u), s = sig(t), ts = t * s;
+        dg = g > limit ? 0.f : dh * v * (s * (1.0f + alpha * t * (1.0f - s)));
+        du = u > limit || u < -limit ? 0.f : dh * ts;
+        return v * ts;
+    }
+};
+
+struct GatedForward {
+    const uint16_t *x, *w13;
+    const int32_t* offsets;   // null: dense
+    uint16_t *h, *gate_up;    // gate_up null: not wanted
+    int R, E, I, K, tiles_n, interleaved;
+    Gate gate;
+};
+
+// One row of blocks of gate and up values (or their gradients) to gate_up: `at` the patch's first row, `col` its first column of I.
+template <int F>
+__device__ __forceinline__ void store_gate_up(const v4f (&g)[F], const v4f (&u)[F], int m, uint16_t* at, int col, int I, int interleaved,
+                                              int rows) {
+    if (!interleaved) {
+        store_block_row(g, m, at + col, 2 * (int64_t)I, rows, I - col);
+        store_block_row(u, m, at + I + col, 2 * (int64_t)I, rows, I - col);
+        return;
+    }
+    const int r = lane_id() & 15, q = lane_id() >> 4, row = 16 * m + r;
+#pragma unroll
+    for (int n = 0; n < F; ++n) {
+        const int c = col + 16 * n + 4 * q;
+        if (row < rows && c < I)
+            *(v4i*)(at + 2 * (int64_t)I * row + 2 * c) = v4i{(int)pack_bf16(g[n].x, u[n].x), (int)pack_bf16(g[n].y, u[n].y),
+                                                             (int)pack_bf16(g[n].z, u[n].z), (int)pack_bf16(g[n].w, u[n].w)};
+    }
+}
+template <int F>
+__device__ __forceinline__ void load_gate_up(v4f (&g)[F], v4f (&u)[F], int m, const uint16_t* at, int col, int I, int interleaved, int rows) {
+    if (!interleaved) {
+        load_block_row(g, m, at + col, 2 * (int64_t)I, rows, I - col);
+        load_block_row(u, m, at + I + col, 2 * (int64_t)I, rows, I - col);
+        return;
+    }
+    const int r = lane_id() & 15, q = lane_id() >> 4, row = 16 * m + r;
+#pragma unroll
+    for (int n = 0; n < F; ++n) {
+        const int c = col + 16 * n + 4 * q;
+        v4i in{0, 0, 0, 0};
+        if (row < rows && c < I) in = *(const v4i*)(at + 2 * (int64_t)I * row + 2 * c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            g[n][j] = __uint_as_float((uint32_t)in[j] << 16);
+            u[n][j] = __uint_as_float((uint32_t)in[j] & 0xffff0000u);
+        }
+    }
+}
+
+// A tile of kTile rows takes kTile / 2 columns of h.
+template <typename Tile>
+__global__ __launch_bounds__(256) void gated_gemm_kernel(GatedForward p) {
+    extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
+    const GroupedTile t = grouped_tile(p.offsets, p.E, p.R, Tile::kTile, p.tiles_n, p.K, 2 * p.I, xcd_chunk_order(blockIdx.x, gridDim.x, kCuPerXcd));
+    if (t.expert < 0) return;
+    const int col0 = t.tile_n * (Tile::kTile / 2);
+    const uint16_t* w = p.w13 + (size_t)t.expert * 2 * p.I * p.K;
+    const size_t pitch = 2ull * p.K;   // bytes
+    v4f acc[Tile::F][Tile::F];
+    Tile::template product<kAlong, kPairs>(
+        smem, operand_along(p.x, pitch, t.row0, t.row0 + t.rows, p.K),
+        operand_pairs(w, w + (p.interleaved ? (size_t)p.K : (size_t)p.I * p.K), p.interleaved ? 2 * pitch : pitch, col0, p.I, p.K), p.K, acc);
+    constexpr int B = Tile::F / 2;   // blocks of 16 columns of h
+    const int wv = wave_id(), row = (wv >> 1) * Tile::kPatch, col = col0 + (wv & 1) * (Tile::kPatch / 2), rows = t.rows - row;
+    const size_t first = (size_t)(t.row0 + row);
+#pragma unroll
+    for (int m = 0; m < Tile::F; ++m) {
+        v4f v[Tile::F], g[B], u[B], h[B];
+        Tile::read_row(acc[m], v);
+#pragma unroll
+        for (int n = 0; n < B; ++n) {
+            g[n] = v[2 * n];
+            u[n] = v[2 * n + 1];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) h[n][j] = p.gate.value(g[n][j], u[n][j]);
+        }
+        store_block_row(h, m, p.h + first * p.I + col, p.I, rows, p.I - col);
+        if (p.gate_up) store_gate_up(g, u, m, p.gate_up + first * 2 * p.I, col, p.I, p.interleaved, rows);
+        slot_fence();
+    }
+}
+
+struct GatedBackward {
+    const uint16_t *dy, *w2;
+    const int32_t* offsets;
+    const uint16_t* gate_up;
+    uint16_t *dgate_up, *h;   // dgate_up may be gate_up; h null: not wanted
+    int R, E, N, I, tiles_n, interleaved;
+    Gate gate;
+};
+
+template <typename Tile>
+__global__ __launch_bounds__(256) void gated_dgrad_kernel(GatedBackward p) {
+    extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
+    const GroupedTile t = grouped_tile(p.offsets, p.E, p.R, Tile::kTile, p.tiles_n, p.N, p.I, xcd_chunk_order(blockIdx.x, gridDim.x, kCuPerXcd));
+    if (t.expert < 0) return;
+    const int col0 = t.tile_n * Tile::kTile;
+    v4f acc[Tile::F][Tile::F];
+    Tile::template product<kAlong, kAcross>(smem, operand_along(p.dy, 2ull * p.N, t.row0, t.row0 + t.rows, p.N),
+                                            operand_across(p.w2 + (size_t)t.expert * p.N * p.I, 2ull * p.I, col0, p.N), p.N, acc);
+    const int w = wave_id(), row = (w >> 1) * Tile::kPatch, col = col0 + (w & 1) * Tile::kPatch, rows = t.rows - row;
+    const size_t first = (size_t)(t.row0 + row);
+#pragma unroll
+    for (int m = 0; m < Tile::F; ++m) {
+        v4f dh[Tile::F], g[Tile::F], u[Tile::F], dg[Tile::F], du[Tile::F];
+        load_gate_up(g, u, m, p.gate_up + first * 2 * p.I, col, p.I, p.interleaved, rows);
+        Tile::read_row(acc[m], dh);
+#pragma unroll
+        for (int n = 0; n < Tile::F; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float a, b;
+                dh[n][j] = p.gate.gradients(g[n][j], u[n][j], dh[n][j], a, b);
+                dg[n][j] = a;
+                du[n][j] = b;
+            }
+        store_gate_up(dg, du, m, p.dgate_up + first * 2 * p.I, col, p.I, p.interleaved, rows);
+        if (p.h) store_block_row(dh, m, p.h + first * p.I + col, p.I, rows, p.I - col);
+        slot_fence();
+    }
+}
+
+// alpha, limit of the clamped form (1); SiLU (0) has its own
+static int make_gate(int activation, float alpha, float limit, Gate& g) {
+    if (activation == 0) {
+        g = Gate{1.0f, __builtin_inff(), 0.0f};
+        return HK_OK;
+    }
+    if (activation != 1 || !(limit > 0.f) || !(__builtin_fabsf(alpha) < __builtin_inff())) return HK_ERR_UNSUPPORTED;
+    g = Gate{alpha, limit, 1.0f};
+    return HK_OK;
+}
+
+// wide: the length of the rows that are not I or 2 I
+static int gated_check(int R, int E, int I, int wide, const int32_t* offsets) {
+    if (R <= 0 || R >= (1 << 30) || E <= 0 || E > kGroupedMaxE || I <= 0 || wide <= 0 || (I % 8) != 0 || (wide % 8) != 0 || I > (1 << 20) ||
+        wide > (1 << 21) || (!offsets && E != 1))
+        return HK_ERR_BAD_SHAPE;
+    return HK_OK;
+}
+
+template <typename Tile, typename P>
+static int launch_gated_tile(void (*kern)(P), DeviceOnce& once, P p, int out, hipStream_t s) {
+    p.tiles_n = (out + Tile::kTile - 1) / Tile::kTile;
+    const long long grid = grouped_tiles_m(p.R, p.E, Tile::kTile) * p.tiles_n;
+    if (grid >= kMaxWorkgroups) return HK_ERR_BAD_SHAPE;
+    if (!set_lds_limit_once((const void*)kern, Tile::kLds, once)) return HK_ERR_LAUNCH;
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), Tile::kLds, s, p);
+    return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
+}
+template <typename Tile>
+static int launch_gated(const GatedForward& p, hipStream_t s) {
+    static DeviceOnce once;
+    return launch_gated_tile<Tile>(gated_gemm_kernel<Tile>, once, p, 2 * p.I, s);
+}
+template <typename Tile>
+static int launch_gated(const GatedBackward& p, hipStream_t s) {
+    static DeviceOnce once;
+    return launch_gated_tile<Tile>(gated_dgrad_kernel<Tile>, once, p, p.I, s);
+}
+template <typename P>
+static int launch_gated_choice(const P& p, int in, int out, hipStream_t s) {
+    switch (grouped_choice(p.R, p.E, in, out, !p.offsets)) {
+        case kLayout256: return launch_gated<LayoutTile256>(p, s);
+        case kLayout128: return launch_gated<LayoutTile128>(p, s);
+        case kLayout128Deep: return launch_gated<LayoutTile128Deep>(p, s);
+        default: return launch_gated<LayoutTile64Deep>(p, s);
+    }
+}
+
+}  // namespace hk
+
+extern "C" int hk_gated_gemm(const void* x_bf16, const void* w13_bf16, const int32_t* expert_offsets_or_null, void* h_bf16,
+                             void* gate_up_bf16_or_null, int R, int E, int I, int K, int interleaved, int activation, float alpha,
+                             float limit, void* stream) {
+    using namespace hk;
+    if (!x_bf16 || !w13_bf16 || !h_bf16) return HK_ERR_NULL_POINTER;
+    if (const int st = gated_check(R, E, I, K, expert_offsets_or_null)) return st;
+    if (((uintptr_t)x_bf16 | (uintptr_t)w13_bf16 | (uintptr_t)h_bf16 | (uintptr_t)gate_up_bf16_or_null) & 15u) return HK_ERR_BAD_ALIGNMENT;
+    GatedForward p{(const uint16_t*)x_bf16, (const uint16_t*)w13_bf16, expert_offsets_or_null, (uint16_t*)h_bf16, (uint16_t*)gate_up_bf16_or_null,
+                   R, E, I, K, 0, interleaved != 0, {}};
+    if (const int st = make_gate(activation, alpha, limit, p.gate)) return st;
+    return launch_gated_choice(p, K, 2 * I, (hipStream_t)stream);
+}
+
+extern "C" int hk_gated_gemm_dgrad(const void* dy_bf16, const void* w2_bf16, const int32_t* expert_offsets_or_null, const void* gate_up_bf16,
+                                   void* dgate_up_bf16, void* h_bf16_or_null, int R, int E, int N, int I, int interleaved, int activation,
+                                   float alpha, float limit, void* stream) {
+    using namespace hk;
+    if (!dy_bf16 || !w2_bf16 || !gate_up_bf16 || !dgate_up_bf16) return HK_ERR_NULL_POINTER;
+    if (const int st = gated_check(R, E, I, N, expert_offsets_or_null)) return st;
+    if (((uintptr_t)dy_bf16 | (uintptr_t)w2_bf16 | (uintptr_t)gate_up_bf16 | (uintptr_t)dgate_up_bf16 | (uintptr_t)h_bf16_or_null) & 15u)
+        return HK_ERR_BAD_ALIGNMENT;
+    GatedBackward p{(const uint16_t*)dy_bf16, (const uint16_t*)w2_bf16, expert_offsets_or_null, (const uint16_t*)gate_up_bf16,
+                    (uint16_t*)dgate_up_bf16, (uint16_t*)h_bf16_or_null, R, E, N, I, 0, interleaved != 0, {}};
+    if (const int st = make_gate(activation, alpha, limit, p.gate)) return st;
+    return launch_gated_choice(p, N, I, (hipStream_t)stream);
+}

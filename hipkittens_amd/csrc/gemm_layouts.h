@@ -19,6 +19,13 @@ typedef __bf16 v8bf_t __attribute__((ext_vector_type(8)));
 
 constexpr int kLayoutStep = 64;   // elements of the contraction per K-step
 
+// How an operand lies in memory. kPairs: contracted along its rows, every 32 rows of the tile are 16 of one matrix and the 16 of the same
+// places of another (the gate and up rows of the same columns): waves 0 and 1 load the first half, 2 and 3 the second, each from its
+// own base, so that a lane ends up with both values of a column.
+enum OperandOrder : int { kAlong = 0, kAcross = 1, kPairs = 2 };
+// rows of the operand's matrix per load of the workgroup
+template <int ORDER> constexpr uint32_t order_rows() { return ORDER == kPairs ? 16u : 32u; }
+
 // One operand of a tile product. across = false: `rows` rows of `pitch` bytes, contraction along them. across = true: the
 // rows run along the contraction and the tile takes the columns from `base` on.
 // bytes: from `base` to the end of what may be read (the last row's last element): loads beyond it give zeros.
@@ -45,9 +52,10 @@ __device__ __forceinline__ v2i lds_read_tr(uint32_t addr) {
 constexpr int kLayoutTile = 128;
 constexpr int kLayoutStageBytes = 2 * kLayoutTile * 128;
 
-template <bool ACROSS>
+template <int ORDER>
 struct TileLoader {
     static constexpr int TILE = kLayoutTile;
+    static constexpr bool ACROSS = ORDER == kAcross;
     v4i srd;
     uint64_t base, left;
     uint32_t voff, pitch, k_bytes, round;
@@ -63,8 +71,8 @@ struct TileLoader {
             round = 16u * pitch;
         } else {
             const uint32_t R = 8 * w + (lane >> 3);                   // + 32 per load
-            voff = R * pitch + swz_chunk(R, lane & 7) * 16u;
-            round = 32u * pitch;
+            voff = R % order_rows<ORDER>() * pitch + swz_chunk(R, lane & 7) * 16u;
+            round = order_rows<ORDER>() * pitch;
         }
     }
     // K-step kt into the LDS tile at dst (this wave's first KiB of it). The descriptor starts at the K-step (64-bit base),
@@ -103,13 +111,13 @@ __device__ __forceinline__ Frag4 tile_fragment(uint32_t tile, int first, int f) 
     return out;
 }
 
-template <bool A_ACROSS, bool B_ACROSS, int STAGES>
+template <int A_ORDER, int B_ORDER, int STAGES>
 __device__ __forceinline__ void tile_product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K,
                                              v4f (&acc)[4][4]) {
     constexpr uint32_t kOperand = kLayoutTile * 128, kStage = 2 * kOperand;
     const int w = wave_id(), wm = w >> 1, wn = w & 1;
-    const TileLoader<A_ACROSS> la(A, K);
-    const TileLoader<B_ACROSS> lb(B, K);
+    const TileLoader<A_ORDER> la(A, K);
+    const TileLoader<B_ORDER> lb(B, K);
     const uint32_t lds0 = (uint32_t)(uintptr_t)smem, mine = to_sgpr(lds0 + (uint32_t)w * 1024u);
 #pragma unroll
     for (int m = 0; m < 4; ++m)
@@ -138,10 +146,10 @@ __device__ __forceinline__ void tile_product(uint8_t* smem, const TileOperand& A
         const uint32_t at = lds0 + (STAGES == 2 ? (uint32_t)(kt & 1) * kStage : 0u);
         Frag4 b[4];
 #pragma unroll
-        for (int n = 0; n < 4; ++n) b[n] = tile_fragment<B_ACROSS>(at + kOperand, wn * 64, n);
+        for (int n = 0; n < 4; ++n) b[n] = tile_fragment<B_ORDER == kAcross>(at + kOperand, wn * 64, n);
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
-            const Frag4 a = tile_fragment<A_ACROSS>(at, wm * 64, m);
+            const Frag4 a = tile_fragment<A_ORDER == kAcross>(at, wm * 64, m);
 #pragma unroll
             for (int n = 0; n < 4; ++n) {
                 acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf_t, b[n].lo),
@@ -170,6 +178,11 @@ __device__ __forceinline__ TileOperand operand_across(const void* p, uint64_t pi
     o.bytes = all > 2ull * (uint64_t)col0 ? all - 2ull * (uint64_t)col0 : 0;
     o.pitch = (uint32_t)pitch;
     return o;
+}
+
+// ... or rows [row0, rows) of the gate matrix and of the up matrix beside it (kPairs): this wave's half.
+__device__ __forceinline__ TileOperand operand_pairs(const void* gate, const void* up, uint64_t pitch, int64_t row0, int64_t rows, int K) {
+    return operand_along(wave_id() < 2 ? gate : up, pitch, row0, rows, K);
 }
 
 }  // namespace hk

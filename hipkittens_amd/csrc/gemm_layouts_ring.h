@@ -24,8 +24,9 @@ __device__ __forceinline__ void mfma_bf16_acc(v4f& acc, const v4i& x, const v4i&
 
 // Loads and reads of one operand of a tile of TILE rows (columns): TILE / 32 loads a wave. Load i: along, rows 32 i + 8 w .. +8; across,
 // TILE 256, K rows 8 i + 2 w and the next, TILE 128, 16 i + 4 w .. +4, TILE 64, 32 i + 8 w .. +8.
-template <bool ACROSS, int TILE = kRingTile>
+template <int ORDER, int TILE = kRingTile>
 struct RingOperand {
+    static constexpr bool ACROSS = ORDER == kAcross;
     static constexpr uint32_t kRow = 2 * TILE;   // across: bytes of a K row in LDS
     uint64_t base;        // descriptor of the K-step that is loaded next
     int64_t left;
@@ -54,8 +55,8 @@ struct RingOperand {
             rd[1] = 0;
         } else {
             const uint32_t R = 8 * w + (lane >> 3), c = swz_chunk(R, lane & 7) * 16u;
-            voff[0] = voff[1] = R * pitch + c;
-            round = 32u * pitch;
+            voff[0] = voff[1] = R % order_rows<ORDER>() * pitch + c;
+            round = order_rows<ORDER>() * pitch;
             const int nk = (K + kLayoutStep - 1) / kLayoutStep;
             tail_or = (int)c >= 2 * (K - (nk - 1) * kLayoutStep) ? 0x80000000u : 0u;
             rd[0] = lds0 + (TILE / 2u * patch + r) * 128u + swz_chunk(r, g) * 16u;
@@ -95,17 +96,17 @@ struct RingOperand {
 };
 
 // acc of this wave's 128x128 patch (wave w: rows 128 (w / 2), columns 128 (w % 2) of the tile). K > 0.
-template <bool A_ACROSS, bool B_ACROSS>
+template <int A_ORDER, int B_ORDER>
 __device__ __forceinline__ void ring_product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K, v4f (&acc)[8][8]) {
     constexpr int MT = 8, NT = 8, PG = 4, kLoads = 8;
     const uint32_t lds0 = (uint32_t)(uintptr_t)smem, w = wave_id();
     const uint32_t mine_a = to_sgpr(lds0 + w * 1024u), mine_b = to_sgpr(lds0 + 2 * kRingSlot + w * 1024u);
-    RingOperand<A_ACROSS> oa;
-    RingOperand<B_ACROSS> ob;
+    RingOperand<A_ORDER> oa;
+    RingOperand<B_ORDER> ob;
     oa.init(A, K, w >> 1, lds0);
     ob.init(B, K, w & 1, lds0 + 2 * kRingSlot);
     const int nk = (K + kLayoutStep - 1) / kLayoutStep;
-    const uint32_t step_a = A_ACROSS ? to_sgpr(kLayoutStep * A.pitch) : 128u, step_b = B_ACROSS ? to_sgpr(kLayoutStep * B.pitch) : 128u;
+    const uint32_t step_a = A_ORDER == kAcross ? to_sgpr(kLayoutStep * A.pitch) : 128u, step_b = B_ORDER == kAcross ? to_sgpr(kLayoutStep * B.pitch) : 128u;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -244,18 +245,18 @@ struct DeepStages {
     static constexpr int kStages = TILE == 128 ? 4 : 8, kBytes = 2 * TILE * 128;
     static constexpr int kGroup = TILE == 128 ? 1 : 2;   // K-steps from barrier to barrier
 };
-template <int TILE, bool A_ACROSS, bool B_ACROSS>
+template <int TILE, int A_ORDER, int B_ORDER>
 __device__ __forceinline__ void deep_product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K,
                                              v4f (&acc)[TILE / 32][TILE / 32]) {
     constexpr int S = DeepStages<TILE>::kStages, kStage = DeepStages<TILE>::kBytes, U = DeepStages<TILE>::kGroup, F = TILE / 32, kLoads = TILE / 32;
     const uint32_t lds0 = (uint32_t)(uintptr_t)smem, w = wave_id();
     const uint32_t mine = to_sgpr(lds0 + w * 1024u);
-    RingOperand<A_ACROSS, TILE> oa;
-    RingOperand<B_ACROSS, TILE> ob;
+    RingOperand<A_ORDER, TILE> oa;
+    RingOperand<B_ORDER, TILE> ob;
     oa.init(A, K, w >> 1, lds0);
     ob.init(B, K, w & 1, lds0 + kStage / 2);
     const int nk = (K + kLayoutStep - 1) / kLayoutStep;
-    const uint32_t step_a = A_ACROSS ? to_sgpr(kLayoutStep * A.pitch) : 128u, step_b = B_ACROSS ? to_sgpr(kLayoutStep * B.pitch) : 128u;
+    const uint32_t step_a = A_ORDER == kAcross ? to_sgpr(kLayoutStep * A.pitch) : 128u, step_b = B_ORDER == kAcross ? to_sgpr(kLayoutStep * B.pitch) : 128u;
 #pragma unroll
     for (int m = 0; m < F; ++m)
 #pragma unroll
@@ -385,6 +386,33 @@ __device__ __forceinline__ void store_block_row(const v4f (&v)[F], int m, T* __r
             const int col = 32 * p + 8 * (g >> 1) + 16 * (g & 1);
             if (row < rows && col < cols) *(v4i*)(at + col) = out;
         }
+        if constexpr (F % 2 == 1) {   // the last block on its own, four columns a lane
+            const v4f a = v[F - 1];
+            const int col = 16 * (F - 1) + 4 * g;
+            if (row < rows && col < cols) *(v2i*)(at + col) = v2i{(int)pack_bf16(a.x, a.y), (int)pack_bf16(a.z, a.w)};
+        }
+    }
+}
+// The reverse for bf16: the values of C in the places that store_block_row takes them from; zeros where there is no C.
+template <int F>
+__device__ __forceinline__ void load_block_row(v4f (&v)[F], int m, const uint16_t* C, int64_t ldc, int64_t rows, int64_t cols) {
+    static_assert(F % 2 == 0);
+    const int r = lane_id() & 15, g = lane_id() >> 4, row = 16 * m + r;
+    const uint16_t* at = C + row * ldc;
+#pragma unroll
+    for (int p = 0; p < F / 2; ++p) {
+        const int col = 32 * p + 8 * (g >> 1) + 16 * (g & 1);
+        v4i in{0, 0, 0, 0};
+        if (row < rows && col < cols) in = *(const v4i*)(at + col);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const auto s = __builtin_amdgcn_permlane16_swap((uint32_t)in[h], (uint32_t)in[2 + h], false, false);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                v[2 * p + q][2 * h] = __uint_as_float((uint32_t)s[q] << 16);
+                v[2 * p + q][2 * h + 1] = __uint_as_float((uint32_t)s[q] & 0xffff0000u);
+            }
+        }
     }
 }
 // The whole patch. (A fence behind every row block: without it the compiler holds more of them in registers than there are.)
@@ -402,9 +430,9 @@ __device__ __forceinline__ void store_patch(const v4f (&acc)[F][F], T* __restric
 template <int STAGES>
 struct LayoutTile128Stages {
     static constexpr int kTile = kLayoutTile, kPatch = kTile / 2, F = 4, kLds = STAGES * kLayoutStageBytes;
-    template <bool A_ACROSS, bool B_ACROSS>
+    template <int A_ORDER, int B_ORDER>
     static __device__ __forceinline__ void product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K, v4f (&acc)[F][F]) {
-        tile_product<A_ACROSS, B_ACROSS, STAGES>(smem, A, B, K, acc);
+        tile_product<A_ORDER, B_ORDER, STAGES>(smem, A, B, K, acc);
     }
     static __device__ __forceinline__ void read_row(const v4f (&acc)[F], v4f (&v)[F]) {
 #pragma unroll
@@ -414,9 +442,9 @@ struct LayoutTile128Stages {
 typedef LayoutTile128Stages<2> LayoutTile128;
 struct LayoutTile256 {
     static constexpr int kTile = kRingTile, kPatch = kTile / 2, F = 8, kLds = kRingLdsBytes;
-    template <bool A_ACROSS, bool B_ACROSS>
+    template <int A_ORDER, int B_ORDER>
     static __device__ __forceinline__ void product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K, v4f (&acc)[F][F]) {
-        ring_product<A_ACROSS, B_ACROSS>(smem, A, B, K, acc);
+        ring_product<A_ORDER, B_ORDER>(smem, A, B, K, acc);
     }
     // One row of blocks out of the accumulation registers, here and no sooner: an epilogue with branches otherwise has the
     // compiler move all 256 into vector registers at once, and spill.
@@ -435,9 +463,9 @@ struct LayoutTile256 {
 template <int TILE>
 struct LayoutTileDeep {
     static constexpr int kTile = TILE, kPatch = kTile / 2, F = TILE / 32, kLds = DeepStages<TILE>::kStages * DeepStages<TILE>::kBytes;
-    template <bool A_ACROSS, bool B_ACROSS>
+    template <int A_ORDER, int B_ORDER>
     static __device__ __forceinline__ void product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K, v4f (&acc)[F][F]) {
-        deep_product<TILE, A_ACROSS, B_ACROSS>(smem, A, B, K, acc);
+        deep_product<TILE, A_ORDER, B_ORDER>(smem, A, B, K, acc);
     }
     static __device__ __forceinline__ void read_row(const v4f (&acc)[F], v4f (&v)[F]) {
 #pragma unroll

@@ -883,3 +883,95 @@ def dispatch_linear_cross_entropy_backward(x, w, labels, lse, dloss, dx, dw, wor
             dx.data_ptr() if dx is not None else None, dw.data_ptr() if dw is not None else None,
             int(dw is not None and dw.dtype == torch.float32), M, V, K, workspace.data_ptr(), workspace.numel(), _stream(x))
     _lib.check(st, "dispatch_linear_cross_entropy_backward")
+
+
+# ------------------------------------------------------------ training: gated feed-forward blocks
+def _check_gated(rows_wide, name_wide, w, name_w, w_shape, gate_up, name_gate_up, rows_i, name_i, expert_offsets, activation):
+    """-> (R, E, I, activation code) of rows_wide [R, .], w (w_shape(I) behind an expert's index where there are experts), gate_up [R, 2I] or
+    None and rows_i [R, I] or None"""
+    if activation not in _ACTIVATIONS:
+        raise RuntimeError(f"activation must be one of {sorted(_ACTIVATIONS)}")
+    _check_tensor(rows_wide, name_wide, _BF16, 2)
+    _check_tensor(w, name_w, _BF16, 2 if expert_offsets is None else 3)
+    R = rows_wide.shape[0]
+    E = 1 if expert_offsets is None else w.shape[0]
+    for t, name in ((gate_up, name_gate_up), (rows_i, name_i)):
+        if t is not None:
+            _check_tensor(t, name, _BF16, 2)
+    I = rows_i.shape[1] if rows_i is not None else gate_up.shape[1] // 2
+    if expert_offsets is not None:
+        _check_tensor(expert_offsets, "expert_offsets", _I32, 1)
+        if expert_offsets.shape[0] != E + 1:
+            raise RuntimeError(f"expert_offsets must be [{E + 1}], got {tuple(expert_offsets.shape)}")
+    if (tuple(w.shape[-2:]) != w_shape(I) or (gate_up is not None and tuple(gate_up.shape) != (R, 2 * I)) or
+            (rows_i is not None and rows_i.shape[0] != R)):
+        raise RuntimeError("shape mismatch: " + ", ".join(f"{n} {tuple(t.shape)}" for t, n in (
+            (rows_wide, name_wide), (w, name_w), (gate_up, name_gate_up), (rows_i, name_i)) if t is not None))
+    _same_device(rows_wide, w, gate_up, rows_i, expert_offsets)
+    return R, E, I, _ACTIVATIONS[activation]
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def dispatch_gated_gemm(x, w13, h, gate_up=None, expert_offsets=None, interleaved: bool = False, activation: str = "silu",
+                        alpha: float = 1.702, limit: float = 7.0) -> None:
+    """First half of a gated feed-forward block: h [R,I] = act(x Wg^T, x Wu^T) for x [R,K] and w13 [2I,K] (gate rows, then up rows; alternating
+    with `interleaved`), activation "silu" or "swiglu_oai" (alpha, limit). gate_up [R,2I]: both projections, in the order of w13's rows, for
+    dispatch_gated_gemm_dgrad. With expert_offsets [E+1] (dispatch_moe_sort): w13 [E,2I,K], rows grouped by expert; rows behind the last
+    offset are left alone. The second half is dispatch_bf16_gemm or dispatch_moe_grouped_gemm."""
+    R, E, I, act = _check_gated(x, "x", w13, "w13", lambda i: (2 * i, x.shape[1]), gate_up, "gate_up", h, "h", expert_offsets, activation)
+    with torch.cuda.device(x.device):
+        st = _lib.load_library().hk_gated_gemm(x.data_ptr(), w13.data_ptr(), _ptr(expert_offsets), h.data_ptr(), _ptr(gate_up), R, E, I,
+                                               x.shape[1], int(bool(interleaved)), act, float(alpha), float(limit), _stream(x))
+    _lib.check(st, "dispatch_gated_gemm")
+
+
+def dispatch_gated_gemm_dgrad(dy, w2, gate_up, dgate_up, h=None, expert_offsets=None, interleaved: bool = False,
+                              activation: str = "silu", alpha: float = 1.702, limit: float = 7.0) -> None:
+    """Backward of a gated feed-forward block through its down projection w2 [N,I] ([E,N,I] with expert_offsets) and its activation: dgate_up
+    [R,2I] from dy [R,N] and the forward's gate_up [R,2I] (it may be gate_up itself), and h [R,I], the activation's value again, if given. What is
+    left are dispatch_bf16_gemm_dgrad / _wgrad or dispatch_moe_grouped_gemm_dgrad / _wgrad: dx = dgate_up W13, dW13 = dgate_up^T x,
+    dW2 = dy^T h."""
+    if gate_up is None or dgate_up is None:
+        raise RuntimeError("gate_up and dgate_up: expected a torch.Tensor")
+    R, E, I, act = _check_gated(dy, "dy", w2, "w2", lambda i: (dy.shape[1], i), gate_up, "gate_up", h, "h", expert_offsets, activation)
+    _check_tensor(dgate_up, "dgate_up", _BF16, 2)
+    if tuple(dgate_up.shape) != (R, 2 * I):
+        raise RuntimeError("dgate_up must have the shape of gate_up")
+    _same_device(dy, dgate_up)
+    with torch.cuda.device(dy.device):
+        st = _lib.load_library().hk_gated_gemm_dgrad(dy.data_ptr(), w2.data_ptr(), _ptr(expert_offsets), gate_up.data_ptr(), dgate_up.data_ptr(),
+                                                     _ptr(h), R, E, dy.shape[1], I, int(bool(interleaved)), act, float(alpha), float(limit),
+                                                     _stream(dy))
+    _lib.check(st, "dispatch_gated_gemm_dgrad")
+
+
+def _check_product(rows_n, name_n, rows_k, name_k, w, name_w, w_types):
+    """-> (M, N, K) of rows_n [M,N], rows_k [M,K] and w [N,K]"""
+    _check_tensor(rows_n, name_n, _BF16, 2)
+    _check_tensor(rows_k, name_k, _BF16, 2)
+    _check_tensor(w, name_w, w_types, 2)
+    (M, N), K = rows_n.shape, rows_k.shape[1]
+    if rows_k.shape[0] != M or tuple(w.shape) != (N, K):
+        raise RuntimeError(f"shape mismatch: {name_n} {tuple(rows_n.shape)}, {name_k} {tuple(rows_k.shape)}, {name_w} {tuple(w.shape)}")
+    _same_device(rows_n, rows_k, w)
+    return M, N, K
+
+
+def dispatch_bf16_gemm_dgrad(dy, w, dx) -> None:
+    """Gradient of y = x @ w.T (dispatch_bf16_gemm) in x: dx [M,K] = dy [M,N] @ w [N,K], bf16."""
+    M, N, K = _check_product(dy, "dy", dx, "dx", w, "w", _BF16)
+    with torch.cuda.device(dy.device):
+        st = _lib.load_library().hk_bf16_gemm_dgrad(dy.data_ptr(), w.data_ptr(), dx.data_ptr(), M, N, K, _stream(dy))
+    _lib.check(st, "dispatch_bf16_gemm_dgrad")
+
+
+def dispatch_bf16_gemm_wgrad(dy, x, dw) -> None:
+    """Gradient of y = x @ w.T (dispatch_bf16_gemm) in w: dw [N,K] = dy [M,N].T @ x [M,K], in bf16 or fp32."""
+    M, N, K = _check_product(dy, "dy", x, "x", dw, "dw", _BF16 + _F32)
+    with torch.cuda.device(dy.device):
+        st = _lib.load_library().hk_bf16_gemm_wgrad(dy.data_ptr(), x.data_ptr(), dw.data_ptr(), int(dw.dtype == torch.float32), M, N, K,
+                                                    _stream(dy))
+    _lib.check(st, "dispatch_bf16_gemm_wgrad")

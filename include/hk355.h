@@ -522,6 +522,33 @@ int hk_linear_cross_entropy_backward(const void* x_bf16, const void* w_bf16, con
                                      const float* lse, const float* dloss, void* dx_bf16_or_null, void* dw_or_null, int dw_type,
                                      int M, int V, int K, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------ training: gated feed-forward blocks
+ * In the manner of the entry points above. Dense (expert_offsets NULL, E = 1) or over the experts' rows.
+ */
+
+/* Both projections of a gated feed-forward block, its activation and the product: h[r, c] = act(x[r] . Wg[c], x[r] . Wu[c]).
+ * x [R, K], w13 [E, 2I, K] (gate rows 0 .. I-1, then up rows; interleaved != 0: gate and up rows of column c are rows 2c and 2c + 1),
+ * h [R, I], gate_up [R, 2I] or NULL: both projections in the order of w13's rows, rounded to bf16, for the backward pass (h comes from the
+ * unrounded ones). activation 0: silu(g) u (alpha and limit are not used); 1: (clamp(u, -limit, limit) + 1) g' / (1 + exp(-alpha g')) with
+ * g' = min(g, limit), limit > 0, alpha finite. A NaN stays one. Rows, offsets and rows behind the last as for hk_moe_grouped_gemm.
+ * Requirements: I % 8 == 0, I <= 2^20, K % 8 == 0, K <= 2^21, E <= 512, R < 2^30, fewer than 2^24 tiles of 128 x 128 of [R, 2I]; everything
+ * 16-byte aligned; no workspace. */
+int hk_gated_gemm(const void* x_bf16, const void* w13_bf16, const int32_t* expert_offsets_or_null, void* h_bf16,
+                  void* gate_up_bf16_or_null, int R, int E, int I, int K, int interleaved, int activation, float alpha, float limit,
+                  void* stream);
+/* The way back through the down projection and the activation: with dh = dy W2 (dy [R, N], w2 [E, N, I], in fp32) and gate_up from the forward
+ * pass, dgate_up [R, 2I] = the gradients of the gate and up values, in their order (0 where a clamp holds the value), and h [R, I] or
+ * NULL = the activation's value again (from the rounded gate_up), for dW2 = dy^T h. dgate_up may be gate_up itself. What is left are products:
+ * dx = dgate_up W13 and dW13 = dgate_up^T x. Same requirements, with N in K's place, tiles of [R, I]. */
+int hk_gated_gemm_dgrad(const void* dy_bf16, const void* w2_bf16, const int32_t* expert_offsets_or_null, const void* gate_up_bf16,
+                        void* dgate_up_bf16, void* h_bf16_or_null, int R, int E, int N, int I, int interleaved, int activation,
+                        float alpha, float limit, void* stream);
+
+/* The gradients of hk_bf16_gemm's product y = x W^T (x [M, K], w [N, K], dy [M, N]): dx [M, K] = bf16(dy W); dw [N, K] = dy^T x in bf16
+ * (dw_type 0) or fp32 (1). The kernels of the experts' products with all rows in one group: same requirements with R = M, E = 1. */
+int hk_bf16_gemm_dgrad(const void* dy_bf16, const void* w_bf16, void* dx_bf16, int M, int N, int K, void* stream);
+int hk_bf16_gemm_wgrad(const void* dy_bf16, const void* x_bf16, void* dw, int dw_type, int M, int N, int K, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
