@@ -79,7 +79,7 @@ def test_python_boundary():
     with pytest.raises(RuntimeError, match="GPU"):
         tk.dispatch_gated_gemm(bf(4, 64), bf(128, 64), bf(4, 64))
     with pytest.raises(RuntimeError, match="Tensor"):
-        tk.dispatch_gated_gemm(bf(4, 64), None, bf(4, 64))
+        tk.dispatch_gated_gemm([1], bf(128, 64), bf(4, 64))
     with pytest.raises(RuntimeError, match="Tensor"):
         tk.dispatch_gated_gemm(None, bf(128, 64), bf(4, 64))
     with pytest.raises(RuntimeError, match="activation"):
