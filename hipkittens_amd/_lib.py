@@ -3,7 +3,7 @@ from __future__ import annotations
 
 import ctypes
 import importlib.util
-from ctypes import c_float, c_int, c_size_t, c_void_p
+from ctypes import c_float, c_int, c_int64, c_size_t, c_void_p
 from pathlib import Path
 
 _LIB_PATH = Path(__file__).resolve().parent / "libhk355.so"
@@ -117,6 +117,14 @@ SIGNATURES = {
     "hk_gated_gemm_dgrad": (c_int, [c_void_p] * 6 + [c_int] * 6 + [c_float] * 2 + [c_void_p]),
     "hk_bf16_gemm_dgrad": (c_int, [c_void_p] * 3 + [c_int] * 3 + [c_void_p]),
     "hk_bf16_gemm_wgrad": (c_int, [c_void_p] * 3 + [c_int] * 4 + [c_void_p]),
+    "hk_embedding": (c_int, [c_void_p, c_int, c_void_p, c_int, c_void_p] + [c_int] * 3 + [c_float, c_void_p]),
+    "hk_embedding_backward_workspace_bytes": (c_size_t, [c_int] * 3),
+    "hk_embedding_backward": (c_int, [c_void_p, c_int, c_void_p, c_void_p, c_void_p] + [c_int] * 4 + [c_float, c_void_p, c_size_t, c_void_p]),
+    "hk_grad_list_bytes": (c_size_t, [c_int]),
+    "hk_grad_list_fill": (c_int, [c_void_p] * 5 + [c_int, c_void_p, c_size_t, ctypes.POINTER(c_int64)]),
+    "hk_grad_norm_workspace_bytes": (c_size_t, []),
+    "hk_grad_norm": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "hk_grad_clip": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_float, c_void_p]),
 }
 
 

@@ -1,0 +1,485 @@
+// The embedding in front of a model's blocks: rows of a table [V, H] by token, times a scale, and the table's gradient.
+//
+//   forward    out[t] = scale table[id[t]]; zeros for an id outside [0, V)
+//   backward   dtable[v] = add[v] + scale sum_{t: id[t] = v} dout[t]
+//
+// Both move rows, and HBM bounds them. The gradient needs every row's tokens together and in an order of their own: the tokens are sorted by id
+// (stable, digit by digit from the lowest), and blocks of the sorted list are summed in order, so that results are the same on every call and
+// no value goes through an atomic. All rows get zeros (or a copy of `add`) first, in the launches that sort, whose few workgroups
+// would leave the chip idle: rows with tokens are then written a second time, at most one row per token. A row whose tokens are
+// spread over several blocks leaves fp32 partial sums, which the last launch joins in order.
+#include <algorithm>
+
+#include "hk_device.h"
+#include "hk_host.h"
+#include "../../include/hk355.h"
+
+namespace hk {
+
+struct Ids {
+    const void* p;
+    int is64;
+    // the id of token t, -1 outside [0, V)
+    __device__ __forceinline__ int at(int64_t t, int V) const {
+        const int64_t l = is64 ? ((const int64_t*)p)[t] : (int64_t)((const int32_t*)p)[t];
+        return l >= 0 && l < V ? (int)l : -1;
+    }
+};
+
+// A wave takes kEmbedLoads times 64 pieces of eight columns of one token (gridDim.y: the pieces of a row), all of its loads in flight together.
+constexpr int kEmbedLoads = 4;
+template <typename T>
+__global__ __launch_bounds__(256) void embedding_kernel(Ids ids, const T* __restrict__ table, uint16_t* __restrict__ out, int tokens, int V,
+                                                        int H, float scale) {
+    const int64_t t = (int64_t)blockIdx.x * 4 + wave_id();
+    if (t >= tokens) return;
+    const int id = to_sgpr(ids.at(t, V)), pieces = H / 8;
+    const int first = blockIdx.y * (64 * kEmbedLoads) + lane_id();
+    Row8 r[kEmbedLoads];
+#pragma unroll
+    for (int i = 0; i < kEmbedLoads; ++i) {
+        r[i] = Row8{};
+        if (id >= 0 && first + 64 * i < pieces) r[i] = load8(table + (int64_t)id * H + (int64_t)(first + 64 * i) * 8);
+    }
+#pragma unroll
+    for (int i = 0; i < kEmbedLoads; ++i) {
+        if (first + 64 * i >= pieces) break;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[i].v[j] = id >= 0 ? r[i].v[j] * scale : 0.f;
+        store8(out + t * H + (int64_t)(first + 64 * i) * 8, r[i]);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ sort
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64, kSortIter = 4;
+constexpr int kSortChunk = kSortThreads * kSortIter;   // tokens of a workgroup
+constexpr int kMaxDigitBits = 9, kMaxDigits = 1 << kMaxDigitBits;
+
+// What the sorting launches write besides: `out`'s 16-byte pieces [from, to), from `add` or zeros.
+struct Fill {
+    v4i* out;
+    const v4i* add;   // null: zeros
+    size_t from, to;
+    int groups;
+};
+__device__ __forceinline__ void fill(const Fill& f, int group) {
+    const size_t step = (size_t)f.groups * kSortThreads;
+    size_t i = f.from + (size_t)group * kSortThreads + threadIdx.x;
+    for (; i + 3 * step < f.to; i += 4 * step) {
+        v4i v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = f.add ? f.add[i + j * step] : v4i{0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f.out[i + j * step] = v[j];
+    }
+    for (; i < f.to; i += step) f.out[i] = f.add ? f.add[i] : v4i{0, 0, 0, 0};
+}
+
+struct Digit {
+    int shift, bits;
+    __device__ __forceinline__ int of(int key) const { return (key >> shift) & ((1 << bits) - 1); }
+    __host__ __device__ __forceinline__ int count() const { return 1 << bits; }
+};
+
+// The lanes whose `value` (of `bits` bits) is this lane's, among those of `live`.
+__device__ __forceinline__ uint64_t same_value(int value, int bits, uint64_t live) {
+    uint64_t same = live;
+    for (int b = 0; b < bits; ++b) {
+        const bool one = value >> b & 1;
+        const uint64_t ones = __ballot(one);
+        same &= one ? ones : ~ones;
+    }
+    return same;
+}
+
+struct SortLds {
+    int count[kSortWaves][kMaxDigits];   // of a wave's items; then where its first item of a digit goes
+    int base[kMaxDigits];
+    int wave_sum[kMaxDigits / 64];
+};
+// Exclusive prefix of the counts of `digits` digits (thread d holds digit d's) to lds.base, their sum returned. One call per pass.
+__device__ __forceinline__ int scan_digits(SortLds& lds, int mine, int digits) {
+    const int tid = threadIdx.x, lane = lane_id();
+    int upto = tid < digits ? mine : 0;
+    const int own = upto;
+    for (int d = 1; d < 64; d <<= 1) {
+        const int u = __shfl_up(upto, d, 64);
+        if (lane >= d) upto += u;
+    }
+    if (tid < kMaxDigits && lane == 63) lds.wave_sum[tid / 64] = upto;
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < kMaxDigits / 64; ++w) {
+        before += w < tid / 64 ? lds.wave_sum[w] : 0;
+        all += lds.wave_sum[w];
+    }
+    if (tid < digits) lds.base[tid] = before + upto - own;
+    return all;
+}
+
+// A workgroup's items (key -1: none) in the order of wave, iteration and lane: rank[i] = how many of the wave's items before this one have its
+// digit; lds.count then holds the waves' counts. lds.count must be zero and everyone past that.
+__device__ __forceinline__ void rank_items(SortLds& lds, const int (&key)[kSortIter], Digit digit, int (&rank)[kSortIter]) {
+    int* count = lds.count[wave_id()];
+    const uint64_t below = (1ull << lane_id()) - 1;
+#pragma unroll
+    for (int i = 0; i < kSortIter; ++i) {
+        const bool live = key[i] >= 0;
+        const int d = live ? digit.of(key[i]) : 0;
+        const uint64_t same = same_value(d, digit.bits, __ballot(live));
+        const int before = __popcll(same & below);
+        rank[i] = live ? count[d] + before : 0;
+        slot_fence();   // (every lane has read before one of them writes, and the next iteration reads behind that)
+        if (live && before == 0) count[d] += __popcll(same);
+        slot_fence();
+    }
+}
+// lds.count of wave w and digit d: where the wave's first item of the digit goes. Behind a barrier on count and base; ends with one.
+__device__ __forceinline__ void place_waves(SortLds& lds, int digits, int base) {
+    if ((int)threadIdx.x < digits) {
+        int at = base;
+#pragma unroll
+        for (int w = 0; w < kSortWaves; ++w) {
+            const int n = lds.count[w][threadIdx.x];
+            lds.count[w][threadIdx.x] = at;
+            at += n;
+        }
+    }
+    __syncthreads();
+}
+__device__ __forceinline__ void clear_counts(SortLds& lds) {
+    for (int i = threadIdx.x; i < kSortWaves * kMaxDigits; i += kSortThreads) (&lds.count[0][0])[i] = 0;
+    __syncthreads();
+}
+
+// Tokens of one workgroup: all passes at once, the items in LDS in between.
+__global__ __launch_bounds__(kSortThreads) void embedding_sort_one_kernel(Ids ids, int T, int V, int passes, int bits, int2* __restrict__ sorted,
+                                                                          int* __restrict__ length, Fill f) {
+    if (blockIdx.x > 0) return fill(f, blockIdx.x - 1);
+    __shared__ SortLds lds;
+    __shared__ int2 items[kSortChunk];
+    int key[kSortIter], token[kSortIter], rank[kSortIter];
+#pragma unroll
+    for (int i = 0; i < kSortIter; ++i) {
+        token[i] = (wave_id() * kSortIter + i) * 64 + lane_id();
+        key[i] = token[i] < T ? ids.at(token[i], V) : -1;
+    }
+    for (int pass = 0; pass < passes; ++pass) {
+        const Digit digit{pass * bits, bits};
+        clear_counts(lds);
+        rank_items(lds, key, digit, rank);
+        __syncthreads();
+        int total = 0;
+        if ((int)threadIdx.x < digit.count())
+            for (int w = 0; w < kSortWaves; ++w) total += lds.count[w][threadIdx.x];
+        const int all = scan_digits(lds, total, digit.count());
+        place_waves(lds, digit.count(), (int)threadIdx.x < digit.count() ? lds.base[threadIdx.x] : 0);
+        int2* out = pass + 1 < passes ? items : sorted;
+#pragma unroll
+        for (int i = 0; i < kSortIter; ++i)
+            if (key[i] >= 0) out[lds.count[wave_id()][digit.of(key[i])] + rank[i]] = make_int2(key[i], token[i]);
+        if (threadIdx.x == 0) *length = all;
+        if (pass + 1 == passes) break;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kSortIter; ++i) {
+            const int at = (wave_id() * kSortIter + i) * 64 + lane_id();
+            const int2 item = at < all ? items[at] : make_int2(-1, 0);
+            key[i] = item.x;
+            token[i] = item.y;
+        }
+    }
+}
+
+// How often every digit of the first pass occurs in each chunk; the counts of the passes behind it start at zero.
+__global__ __launch_bounds__(kSortThreads) void embedding_count_kernel(Ids ids, int T, int V, int chunks, Digit digit, int* __restrict__ counts,
+                                                                       int passes, Fill f) {
+    if ((int)blockIdx.x >= chunks) return fill(f, blockIdx.x - chunks);
+    __shared__ int count[kMaxDigits];
+    const int digits = digit.count();
+    if ((int)threadIdx.x < digits) count[threadIdx.x] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kSortIter; ++i) {
+        const int64_t t = (int64_t)blockIdx.x * kSortChunk + i * kSortThreads + threadIdx.x;
+        const int key = t < T ? ids.at(t, V) : -1;
+        if (key >= 0) atomicAdd(&count[digit.of(key)], 1);
+    }
+    __syncthreads();
+    for (int p = 0; p < passes; ++p)
+        if ((int)threadIdx.x < digits) counts[((size_t)p * chunks + blockIdx.x) * digits + threadIdx.x] = p == 0 ? count[threadIdx.x] : 0;
+}
+
+// One pass: the items of a chunk to their places. The first reads the ids, and drops what is no row; the others `in`. The counts of the
+// next pass's chunks are made on the way (sums of integers: their order does not matter).
+__global__ __launch_bounds__(kSortThreads) void embedding_scatter_kernel(Ids ids, const int2* __restrict__ in, int T, int V, int chunks, Digit digit,
+                                                                         const int* __restrict__ counts, int* __restrict__ next_counts,
+                                                                         int2* __restrict__ out, int* __restrict__ length, Fill f) {
+    if ((int)blockIdx.x >= chunks) return fill(f, blockIdx.x - chunks);
+    __shared__ SortLds lds;
+    const int digits = digit.count(), c = blockIdx.x;
+    int total = 0, before = 0;
+    if ((int)threadIdx.x < digits) {
+#pragma unroll 8
+        for (int i = 0; i < chunks; ++i) {
+            const int n = counts[(size_t)i * digits + threadIdx.x];
+            total += n;
+            before += i < c ? n : 0;
+        }
+    }
+    const int all = scan_digits(lds, total, digits);
+    if (c == 0 && threadIdx.x == 0) *length = all;
+    int key[kSortIter], token[kSortIter], rank[kSortIter];
+#pragma unroll
+    for (int i = 0; i < kSortIter; ++i) {
+        const int64_t at = (int64_t)c * kSortChunk + (wave_id() * kSortIter + i) * 64 + lane_id();
+        if (in) {
+            const int2 item = at < all ? in[at] : make_int2(-1, 0);
+            key[i] = item.x;
+            token[i] = item.y;
+        } else {
+            key[i] = at < T ? ids.at(at, V) : -1;
+            token[i] = (int)at;
+        }
+    }
+    clear_counts(lds);
+    rank_items(lds, key, digit, rank);
+    __syncthreads();
+    place_waves(lds, digits, (int)threadIdx.x < digits ? lds.base[threadIdx.x] + before : 0);
+    const Digit next{digit.shift + digit.bits, digit.bits};
+    const int chunk_bits = 32 - __clz(chunks - 1);
+#pragma unroll
+    for (int i = 0; i < kSortIter; ++i) {
+        const bool live = key[i] >= 0;
+        const int pos = live ? lds.count[wave_id()][digit.of(key[i])] + rank[i] : 0;
+        if (live) out[pos] = make_int2(key[i], token[i]);
+        if (next_counts) {   // one addition per chunk and digit of the wave's
+            const int at = live ? (pos / kSortChunk) * digits + next.of(key[i]) : 0;
+            const uint64_t same = same_value(at, digit.bits + chunk_bits, __ballot(live));
+            if (live && (same & ((1ull << lane_id()) - 1)) == 0) atomicAdd(next_counts + at, __popcll(same));
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ sums
+struct EmbedSums {
+    const int2* sorted;   // (row, token), ascending
+    const int* length;
+    const uint16_t* dout;
+    float* partial;       // [blocks][2][H]: of a row whose tokens began in an earlier block, of one whose tokens go on in the next
+    int H, block;         // block: tokens of a block, 64 at most
+    float scale;
+};
+template <typename T>
+__device__ __forceinline__ void write_row(const EmbedSums& p, const T* add, T* dtable, int row, int col, Row8 r) {
+    const size_t at = (size_t)row * p.H + col;
+    Row8 a{};
+    if (add) a = load8(add + at);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) r.v[j] = add ? __builtin_fmaf(p.scale, r.v[j], a.v[j]) : p.scale * r.v[j];
+    store8(dtable + at, r);
+}
+
+// A wave: the tokens of one block, in order, 512 columns of them, eight rows in flight.
+template <typename T>
+__global__ __launch_bounds__(256) void embedding_sum_kernel(EmbedSums p, const T* add, T* dtable) {
+    constexpr int kAhead = 8;
+    const int length = *p.length, lane = lane_id();
+    const int64_t b = (int64_t)blockIdx.x * 4 + wave_id(), first = b * p.block;
+    if (first >= length) return;
+    const int n = (int)min((int64_t)p.block, length - first);
+    const int2 item = lane < n ? p.sorted[first + lane] : make_int2(-1, 0);
+    const int before = first > 0 ? p.sorted[first - 1].x : -1, behind = first + n < length ? p.sorted[first + n].x : -1;
+    const int col = blockIdx.y * 512 + lane * 8;
+    const bool mine = col < p.H;
+    Row8 sum{};
+    bool head = __builtin_amdgcn_readlane(item.x, 0) == to_sgpr(before);   // the run that is summed began in an earlier block
+    for (int i0 = 0; i0 < n; i0 += kAhead) {
+        Row8 r[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            r[i] = Row8{};
+            if (i0 + i < n && mine) r[i] = load8(p.dout + (size_t)__builtin_amdgcn_readlane(item.y, min(i0 + i, 63)) * p.H + col);
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            if (i0 + i >= n) break;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum.v[j] += r[i].v[j];
+            const int row = __builtin_amdgcn_readlane(item.x, i0 + i);
+            const bool last = i0 + i == n - 1;
+            const int next = last ? to_sgpr(behind) : __builtin_amdgcn_readlane(item.x, min(i0 + i + 1, 63));
+            if (row == next && !last) continue;
+            if (head || row == next) {
+                if (mine) store8(p.partial + ((size_t)b * 2 + (head ? 0 : 1)) * p.H + col, sum);
+            } else if (mine) {
+                write_row(p, add, dtable, row, col, sum);
+            }
+            head = false;
+            sum = Row8{};
+        }
+    }
+}
+
+// Rows whose tokens are spread over several blocks: the workgroup of the block in which they begin adds the partial sums, each wave a
+// run of the blocks behind it, then the waves' in order.
+template <typename T>
+__global__ __launch_bounds__(256) void embedding_join_kernel(EmbedSums p, const T* add, T* dtable) {
+    __shared__ float part[4][64][9];
+    const int length = *p.length, lane = lane_id(), w = wave_id();
+    const int64_t b = blockIdx.x, end = (b + 1) * p.block;   // the next block's first token
+    if (end >= length) return;
+    const int row = p.sorted[end].x;
+    if (p.sorted[end - 1].x != row) return;
+    if (b > 0 && p.sorted[b * p.block - 1].x == row) return;   // it began earlier
+    // blocks behind this one that begin with the row
+    const int64_t blocks = (length + p.block - 1) / p.block;
+    int64_t lo = b + 1, hi = blocks;   // block lo begins with it; block hi does not, or is none
+    while (hi - lo > 1) {
+        const int64_t mid = (lo + hi) / 2;
+        if (p.sorted[mid * p.block].x == row) lo = mid;
+        else hi = mid;
+    }
+    const int col = blockIdx.y * 512 + lane * 8;
+    const bool mine = col < p.H;
+    const int64_t count = hi - b, from = count * w / 4, to = count * (w + 1) / 4;   // of blocks b, b + 1, .. hi - 1
+    Row8 sum{};
+    if (mine) {
+        for (int64_t i = from; i < to; i += 8) {
+            Row8 r[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                r[k] = Row8{};
+                if (i + k < to) r[k] = load8(p.partial + ((size_t)(b + i + k) * 2 + (i + k == 0 ? 1 : 0)) * p.H + col);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum.v[j] += r[k].v[j];
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) part[w][lane][j] = sum.v[j];
+    __syncthreads();
+    if (w == 0 && mine) {
+#pragma unroll
+        for (int v = 1; v < 4; ++v)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) sum.v[j] += part[v][lane][j];
+        write_row(p, add, dtable, row, col, sum);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+static int embed_check(int T, int V, int H) {
+    if (T <= 0 || V <= 0 || H <= 0 || (H % 8) != 0 || T >= (1 << 24) || V >= (1 << 30) || H > (1 << 21)) return HK_ERR_BAD_SHAPE;
+    return HK_OK;
+}
+static size_t embed_up(size_t n) { return (n + 255) / 256 * 256; }
+
+// Tokens of a block of the sums: fewer where there are few, so that the chip has waves enough.
+static int embed_block(long long T, int H) {
+    const long long waves = T * ((H + 511) / 512);
+    return waves >= 64 * 4096 ? 64 : waves >= 32 * 4096 ? 32 : waves >= 16 * 4096 ? 16 : 8;
+}
+struct EmbedPlan {
+    int passes, bits, chunks, block;
+    size_t counts, a, b, partial, bytes;   // offsets; the list's length stands in front
+    EmbedPlan(int T, int V, int H) {
+        int all = 1;
+        while (all < 30 && (1ll << all) < V) ++all;
+        passes = (all + kMaxDigitBits - 1) / kMaxDigitBits;
+        bits = (all + passes - 1) / passes;
+        chunks = (T + kSortChunk - 1) / kSortChunk;
+        block = embed_block(T, H);
+        counts = 256;
+        a = counts + embed_up((size_t)passes * chunks * sizeof(int) << bits);
+        b = a + embed_up((size_t)T * sizeof(int2));
+        partial = b + embed_up((size_t)T * sizeof(int2));
+        // two partial sums a block; fewer tokens may have more blocks: at most those of the largest number that blocks of 8, 16 or 32 are taken for
+        size_t blocks = (T + block - 1) / block;
+        const long long slabs = (H + 511) / 512;
+        for (int small = 8; small < block; small *= 2) blocks = std::max(blocks, (size_t)((2 * 4096 * small + slabs - 1) / slabs / small + 1));
+        bytes = partial + embed_up(blocks * 2 * H * sizeof(float));
+    }
+};
+
+template <typename T>
+static int launch_embedding(Ids ids, const void* table, void* out, int tokens, int V, int H, float scale, hipStream_t s) {
+    const dim3 grid((unsigned)((tokens + 3) / 4), (unsigned)((H / 8 + 64 * kEmbedLoads - 1) / (64 * kEmbedLoads)));
+    hipLaunchKernelGGL(embedding_kernel<T>, grid, dim3(256), 0, s, ids, (const T*)table, (uint16_t*)out, tokens, V, H, scale);
+    return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
+}
+
+template <typename T>
+static int launch_embedding_backward(Ids ids, const void* dout, const void* add, void* dtable, int tokens, int V, int H, float scale, uint8_t* ws,
+                                     hipStream_t s) {
+    const EmbedPlan L(tokens, V, H);
+    int* length = (int*)ws;
+    int* counts = (int*)(ws + L.counts);
+    int2 *a = (int2*)(ws + L.a), *b = (int2*)(ws + L.b);
+    const size_t pieces = add == dtable ? 0 : (size_t)V * H * sizeof(T) / 16;
+    const int launches = L.chunks == 1 ? 1 : 1 + L.passes;
+    auto part = [&](int launch) {
+        Fill f{(v4i*)dtable, (const v4i*)add, pieces * launch / launches, pieces * (launch + 1) / launches, 0};
+        f.groups = (int)std::min<size_t>(512, (f.to - f.from + 4 * kSortThreads - 1) / (4 * kSortThreads));
+        return f;
+    };
+    const int2* sorted = a;
+    if (L.chunks == 1) {
+        const Fill f = part(0);
+        hipLaunchKernelGGL(embedding_sort_one_kernel, dim3(1 + f.groups), dim3(kSortThreads), 0, s, ids, tokens, V, L.passes, L.bits, a, length, f);
+    } else {
+        const Fill f = part(0);
+        hipLaunchKernelGGL(embedding_count_kernel, dim3(L.chunks + f.groups), dim3(kSortThreads), 0, s, ids, tokens, V, L.chunks, Digit{0, L.bits},
+                           counts, L.passes, f);
+        const int2* in = nullptr;
+        for (int p = 0; p < L.passes; ++p) {
+            const Fill g = part(1 + p);
+            int2* out = p % 2 == 0 ? a : b;
+            const size_t row = (size_t)L.chunks << L.bits;
+            hipLaunchKernelGGL(embedding_scatter_kernel, dim3(L.chunks + g.groups), dim3(kSortThreads), 0, s, ids, in, tokens, V, L.chunks,
+                               Digit{p * L.bits, L.bits}, (const int*)(counts + p * row), p + 1 < L.passes ? counts + (p + 1) * row : nullptr, out,
+                               length, g);
+            sorted = in = out;
+        }
+    }
+    if (hipGetLastError() != hipSuccess) return HK_ERR_LAUNCH;
+    const EmbedSums p{sorted, length, (const uint16_t*)dout, (float*)(ws + L.partial), H, L.block, scale};
+    const unsigned blocks = (unsigned)((tokens + L.block - 1) / L.block), slabs = (unsigned)((H + 511) / 512);
+    hipLaunchKernelGGL(embedding_sum_kernel<T>, dim3((blocks + 3) / 4, slabs), dim3(256), 0, s, p, (const T*)add, (T*)dtable);
+    if (blocks > 1) hipLaunchKernelGGL(embedding_join_kernel<T>, dim3(blocks - 1, slabs), dim3(256), 0, s, p, (const T*)add, (T*)dtable);
+    return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
+}
+
+}  // namespace hk
+
+extern "C" int hk_embedding(const void* ids, int id_type, const void* table, int table_type, void* out_bf16, int T, int V, int H, float scale,
+                            void* stream) {
+    using namespace hk;
+    if (!ids || !table || !out_bf16) return HK_ERR_NULL_POINTER;
+    if (const int st = embed_check(T, V, H)) return st;
+    if ((id_type != 0 && id_type != 1) || (table_type != 0 && table_type != 1)) return HK_ERR_UNSUPPORTED;
+    if (((uintptr_t)table | (uintptr_t)out_bf16) & 15u) return HK_ERR_BAD_ALIGNMENT;
+    const Ids at{ids, id_type};
+    return table_type == 0 ? launch_embedding<uint16_t>(at, table, out_bf16, T, V, H, scale, (hipStream_t)stream)
+                           : launch_embedding<float>(at, table, out_bf16, T, V, H, scale, (hipStream_t)stream);
+}
+
+extern "C" size_t hk_embedding_backward_workspace_bytes(int T, int V, int H) {
+    return hk::embed_check(T, V, H) == HK_OK ? hk::EmbedPlan(T, V, H).bytes : 0;
+}
+
+extern "C" int hk_embedding_backward(const void* ids, int id_type, const void* dout_bf16, const void* add_or_null, void* dtable, int table_type,
+                                     int T, int V, int H, float scale, void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace hk;
+    if (!ids || !dout_bf16 || !dtable) return HK_ERR_NULL_POINTER;
+    if (const int st = embed_check(T, V, H)) return st;
+    if ((id_type != 0 && id_type != 1) || (table_type != 0 && table_type != 1)) return HK_ERR_UNSUPPORTED;
+    if (((uintptr_t)dout_bf16 | (uintptr_t)add_or_null | (uintptr_t)dtable | (uintptr_t)workspace) & 15u) return HK_ERR_BAD_ALIGNMENT;
+    if (!workspace || workspace_bytes < EmbedPlan(T, V, H).bytes) return HK_ERR_WORKSPACE;
+    const Ids at{ids, id_type};
+    return table_type == 0 ? launch_embedding_backward<uint16_t>(at, dout_bf16, add_or_null, dtable, T, V, H, scale, (uint8_t*)workspace, (hipStream_t)stream)
+                           : launch_embedding_backward<float>(at, dout_bf16, add_or_null, dtable, T, V, H, scale, (uint8_t*)workspace, (hipStream_t)stream);
+}

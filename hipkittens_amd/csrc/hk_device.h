@@ -281,6 +281,30 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return __builtin_bit_cast(uint32_t, h);
 }
 
+// Eight neighbouring elements of bf16 or fp32 at 16-byte aligned addresses, in fp32.
+struct Row8 { float v[8]; };
+__device__ __forceinline__ Row8 load8(const uint16_t* p) {
+    const v4i q = *(const v4i*)p;
+    Row8 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        r.v[2 * i] = __uint_as_float((uint32_t)q[i] << 16);
+        r.v[2 * i + 1] = __uint_as_float((uint32_t)q[i] & 0xffff0000u);
+    }
+    return r;
+}
+__device__ __forceinline__ Row8 load8(const float* p) {
+    const v4f a = ((const v4f*)p)[0], b = ((const v4f*)p)[1];
+    return Row8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
+}
+__device__ __forceinline__ void store8(uint16_t* p, const Row8& r) {
+    *(v4i*)p = v4i{(int)pack_bf16(r.v[0], r.v[1]), (int)pack_bf16(r.v[2], r.v[3]), (int)pack_bf16(r.v[4], r.v[5]), (int)pack_bf16(r.v[6], r.v[7])};
+}
+__device__ __forceinline__ void store8(float* p, const Row8& r) {
+    ((v4f*)p)[0] = v4f{r.v[0], r.v[1], r.v[2], r.v[3]};
+    ((v4f*)p)[1] = v4f{r.v[4], r.v[5], r.v[6], r.v[7]};
+}
+
 // Workgroup order. Hardware hands consecutive workgroup ids to the 8 XCDs round
 // robin. `xcd_chunk_order` regroups ids so that each XCD (own L2) owns runs of
 // `chunk` consecutive logical ids (cf. chiplet_transform_chunked,

@@ -11,6 +11,7 @@ stream (the reference uses the null stream).
 """
 from __future__ import annotations
 
+import ctypes
 import warnings
 
 import torch
@@ -975,3 +976,129 @@ def dispatch_bf16_gemm_wgrad(dy, x, dw) -> None:
         st = _lib.load_library().hk_bf16_gemm_wgrad(dy.data_ptr(), x.data_ptr(), dw.data_ptr(), int(dw.dtype == torch.float32), M, N, K,
                                                     _stream(dy))
     _lib.check(st, "dispatch_bf16_gemm_wgrad")
+
+
+# ------------------------------------------------------------ training: embedding, gradient norm and clipping
+_TABLE = (torch.bfloat16, torch.float32)
+
+
+def embedding_backward_workspace_bytes(T: int, V: int, H: int) -> int:
+    """Bytes of workspace of dispatch_embedding_backward; never less for a larger T."""
+    return int(_lib.load_library().hk_embedding_backward_workspace_bytes(int(T), int(V), int(H)))
+
+
+def _check_embedding(ids, rows, name_rows, table, name_table):
+    """-> (T, V, H) of ids [T], rows [T,H] and table [V,H]"""
+    _check_tensor(ids, "ids", _LABELS, 1)
+    _check_tensor(rows, name_rows, _BF16, 2)
+    _check_tensor(table, name_table, _TABLE, 2)
+    T, (V, H) = ids.shape[0], table.shape
+    if tuple(rows.shape) != (T, H):
+        raise RuntimeError(f"shape mismatch: ids {tuple(ids.shape)}, {name_rows} {tuple(rows.shape)}, {name_table} {tuple(table.shape)}")
+    _same_device(ids, rows, table)
+    return T, V, H
+
+
+def dispatch_embedding(ids, table, out, scale: float = 1.0) -> None:
+    """Rows of a table by token: out[t] = scale * table[ids[t]], zeros for an id outside [0, V); ids [T] int32 or int64, table [V,H] bf16 or
+    fp32, out [T,H] bf16."""
+    T, V, H = _check_embedding(ids, out, "out", table, "table")
+    with torch.cuda.device(ids.device):
+        st = _lib.load_library().hk_embedding(ids.data_ptr(), int(ids.dtype == torch.int64), table.data_ptr(), int(table.dtype == torch.float32),
+                                              out.data_ptr(), T, V, H, float(scale), _stream(ids))
+    _lib.check(st, "dispatch_embedding")
+
+
+def dispatch_embedding_backward(ids, dout, dtable, workspace, scale: float = 1.0, add=None) -> None:
+    """Gradient of dispatch_embedding in the table: dtable[v] = add[v] + scale * (sum of dout[t] over the tokens with ids[t] = v); dout [T,H] bf16,
+    dtable and add [V,H] bf16 or fp32, every row written (zeros without tokens and `add`). add may be dtable itself, e.g. the head's
+    gradient of a tied table: then only rows with tokens are touched. workspace: embedding_backward_workspace_bytes(T, V, H) bytes."""
+    T, V, H = _check_embedding(ids, dout, "dout", dtable, "dtable")
+    _check_tensor(workspace, "workspace", _U8, 1)
+    if add is not None:
+        _check_tensor(add, "add", (dtable.dtype,), 2)
+        if tuple(add.shape) != (V, H):
+            raise RuntimeError("add must have the shape of dtable")
+    _same_device(ids, workspace, add)
+    with torch.cuda.device(ids.device):
+        st = _lib.load_library().hk_embedding_backward(
+            ids.data_ptr(), int(ids.dtype == torch.int64), dout.data_ptr(), _ptr(add), dtable.data_ptr(), int(dtable.dtype == torch.float32),
+            T, V, H, float(scale), workspace.data_ptr(), workspace.numel(), _stream(ids))
+    _lib.check(st, "dispatch_embedding_backward")
+
+
+class GradTensors:
+    """Gradients that are clipped together: bf16 and fp32 tensors of any shape on one device, contiguous, none overlapping another. `outs`: where
+    the scaled ones go, tensor by tensor, of the same numbers of elements in bf16 or fp32 (None: in place). The tensors are kept, and a
+    table of them on the device, made once (a host copy, outside a captured graph): make another where gradients move to new memory."""
+
+    def __init__(self, grads, outs=None):
+        self.grads = list(grads)
+        self.outs = self.grads if outs is None else list(outs)
+        if not self.grads:
+            raise RuntimeError("grads: expected at least one tensor")
+        if len(self.outs) != len(self.grads):
+            raise RuntimeError(f"{len(self.grads)} gradients, {len(self.outs)} outputs")
+        spans = []
+        for name, tensors in (("grads", self.grads),) + ((("outs", self.outs),) if outs is not None else ()):
+            for i, t in enumerate(tensors):
+                if isinstance(t, torch.Tensor) and t.dim() > 4:
+                    t = t.detach().view(-1) if t.is_contiguous() else t   # (any number of dimensions)
+                _check_tensor(t, f"{name}[{i}]", _TABLE)
+                if name == "outs" and t.numel() != self.grads[i].numel():
+                    raise RuntimeError(f"outs[{i}] has {t.numel()} elements, grads[{i}] {self.grads[i].numel()}")
+                if name == "outs" and t.data_ptr() == self.grads[i].data_ptr() and t.dtype == self.grads[i].dtype:
+                    continue   # in place
+                if t.numel():
+                    spans.append((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), f"{name}[{i}]"))
+        spans.sort()
+        for (_, end, a), (start, _, b) in zip(spans, spans[1:]):
+            if start < end:
+                raise RuntimeError(f"{a} and {b} overlap")
+        _same_device(*self.grads, *self.outs)
+        self.device = self.grads[0].device
+        n = len(self.grads)
+        lib = _lib.load_library()
+        host = torch.empty(int(lib.hk_grad_list_bytes(n)), dtype=torch.uint8)
+        pointers = lambda ts: (ctypes.c_void_p * n)(*(t.data_ptr() for t in ts))
+        types = lambda ts: (ctypes.c_int32 * n)(*(int(t.dtype == torch.float32) for t in ts))
+        chunks = ctypes.c_int64()
+        _lib.check(lib.hk_grad_list_fill(pointers(self.grads), pointers(self.outs), (ctypes.c_int64 * n)(*(t.numel() for t in self.grads)),
+                                         types(self.grads), types(self.outs), n, host.data_ptr(), host.numel(), ctypes.byref(chunks)),
+                   "GradTensors")
+        self.n, self.chunks, self.list = n, chunks.value, host.to(self.device)
+
+
+def grad_norm_workspace_bytes() -> int:
+    """Bytes of workspace of dispatch_grad_norm."""
+    return int(_lib.load_library().hk_grad_norm_workspace_bytes())
+
+
+def _check_norm(grads, norm):
+    if not isinstance(grads, GradTensors):
+        raise RuntimeError("grads: expected a GradTensors")
+    _check_tensor(norm, "norm", _F32, 1)
+    if norm.shape[0] != 1:
+        raise RuntimeError("norm must be [1]")
+    _same_device(grads.list, norm)
+
+
+def dispatch_grad_norm(grads, norm, workspace) -> None:
+    """norm [1] fp32 = the square root of the sum of the squares of all of `grads` (a GradTensors), added in 64 bits. workspace:
+    grad_norm_workspace_bytes() bytes."""
+    _check_norm(grads, norm)
+    _check_tensor(workspace, "workspace", _U8, 1)
+    _same_device(norm, workspace)
+    with torch.cuda.device(norm.device):
+        st = _lib.load_library().hk_grad_norm(grads.list.data_ptr(), grads.n, grads.chunks, norm.data_ptr(), workspace.data_ptr(),
+                                              workspace.numel(), _stream(norm))
+    _lib.check(st, "dispatch_grad_norm")
+
+
+def dispatch_grad_clip(grads, norm, max_norm: float) -> None:
+    """Every gradient of `grads` times min(1, max_norm / (norm + 1e-6)), in place or into its outs; norm [1] of dispatch_grad_norm, or of
+    all ranks together."""
+    _check_norm(grads, norm)
+    with torch.cuda.device(norm.device):
+        st = _lib.load_library().hk_grad_clip(grads.list.data_ptr(), grads.n, grads.chunks, norm.data_ptr(), float(max_norm), _stream(norm))
+    _lib.check(st, "dispatch_grad_clip")

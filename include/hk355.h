@@ -549,6 +549,39 @@ int hk_gated_gemm_dgrad(const void* dy_bf16, const void* w2_bf16, const int32_t*
 int hk_bf16_gemm_dgrad(const void* dy_bf16, const void* w_bf16, void* dx_bf16, int M, int N, int K, void* stream);
 int hk_bf16_gemm_wgrad(const void* dy_bf16, const void* x_bf16, void* dw, int dw_type, int M, int N, int K, void* stream);
 
+/* ------------------------------------------------------------------ training: embedding, gradient norm and clipping
+ */
+
+/* Rows of a table by token: out[t, :] = bf16(scale * table[ids[t], :]), zeros for an id outside [0, V). ids [T] int32 (id_type 0) or int64 (1);
+ * table [V, H] bf16 (table_type 0) or fp32 (1); out [T, H]. Requirements: H % 8 == 0, H <= 2^21, T < 2^24, V < 2^30; table and out 16-byte
+ * aligned. */
+int hk_embedding(const void* ids, int id_type, const void* table, int table_type, void* out_bf16, int T, int V, int H, float scale,
+                 void* stream);
+/* Its gradient: dtable[v, :] = add[v, :] + scale * sum over the tokens t with ids[t] = v of dout[t, :] (fp32 sums in an order that depends on
+ * the ids alone, one rounding), every row written; add NULL: zeros in its place. dout [T, H] bf16; dtable and add [V, H] of table_type. add may be
+ * dtable itself: then rows without tokens are neither read nor written (the gradient of a tied table is added to the head's). An id
+ * outside [0, V) has no gradient, whatever its dout holds. Same requirements, dout, add, dtable and workspace 16-byte aligned; workspace of
+ * hk_embedding_backward_workspace_bytes(T, V, H) bytes (0 for a shape that is refused; never less for a larger T), nothing in it is kept. */
+size_t hk_embedding_backward_workspace_bytes(int T, int V, int H);
+int hk_embedding_backward(const void* ids, int id_type, const void* dout_bf16, const void* add_or_null, void* dtable, int table_type,
+                          int T, int V, int H, float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* A list of gradients for hk_grad_norm and hk_grad_clip: hk_grad_list_fill writes a table of hk_grad_list_bytes(n) bytes to host memory (8-byte
+ * aligned) and how many chunks of work it holds; the caller copies it to the device once and keeps it while the tensors stay where they are.
+ * grads[i] (device) holds counts[i] elements (0 or more, below 2^40) of type types[i] (0 bf16, 1 fp32), aligned to its element; outs[i] takes
+ * the scaled ones, in out_types[i]; outs NULL: in place. 1 <= n <= 2^20. No tensor may overlap another, but outs[i] may be grads[i]
+ * (of the same type). */
+size_t hk_grad_list_bytes(int n);
+int hk_grad_list_fill(const void* const* grads, void* const* outs_or_null, const int64_t* counts, const int32_t* types,
+                      const int32_t* out_types_or_null, int n, void* list, size_t list_bytes, int64_t* chunks);
+/* norm[0] = sqrt(sum of the squares of all gradients), added in 64 bits in an order that depends on the list alone, rounded to fp32. list: on the
+ * device, n and chunks of hk_grad_list_fill. workspace: 16-byte aligned, hk_grad_norm_workspace_bytes() bytes. */
+size_t hk_grad_norm_workspace_bytes(void);
+int hk_grad_norm(const void* list, int n, int64_t chunks, float* norm, void* workspace, size_t workspace_bytes, void* stream);
+/* outs = grads * min(1, max_norm / (norm[0] + 1e-6)) with norm on the device (of hk_grad_norm, or of all ranks together); in place and with a
+ * factor of 1 nothing is written. A norm that is not a number makes all of them so. max_norm >= 0. */
+int hk_grad_clip(const void* list, int n, int64_t chunks, const float* norm, float max_norm, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
