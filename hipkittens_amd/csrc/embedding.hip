@@ -26,23 +26,22 @@ struct Ids {
     }
 };
 
-// A wave takes kEmbedLoads times 64 pieces of eight columns of one token (gridDim.y: the pieces of a row), all of its loads in flight together.
-constexpr int kEmbedLoads = 4;
-template <typename T>
+// A wave takes LOADS times 64 pieces of eight columns of one token (gridDim.y: the parts of a row), all of its loads in flight together.
+template <typename T, int LOADS>
 __global__ __launch_bounds__(256) void embedding_kernel(Ids ids, const T* __restrict__ table, uint16_t* __restrict__ out, int tokens, int V,
                                                         int H, float scale) {
     const int64_t t = (int64_t)blockIdx.x * 4 + wave_id();
     if (t >= tokens) return;
     const int id = to_sgpr(ids.at(t, V)), pieces = H / 8;
-    const int first = blockIdx.y * (64 * kEmbedLoads) + lane_id();
-    Row8 r[kEmbedLoads];
+    const int first = blockIdx.y * (64 * LOADS) + lane_id();
+    Row8 r[LOADS];
 #pragma unroll
-    for (int i = 0; i < kEmbedLoads; ++i) {
+    for (int i = 0; i < LOADS; ++i) {
         r[i] = Row8{};
         if (id >= 0 && first + 64 * i < pieces) r[i] = load8(table + (int64_t)id * H + (int64_t)(first + 64 * i) * 8);
     }
 #pragma unroll
-    for (int i = 0; i < kEmbedLoads; ++i) {
+    for (int i = 0; i < LOADS; ++i) {
         if (first + 64 * i >= pieces) break;
 #pragma unroll
         for (int j = 0; j < 8; ++j) r[i].v[j] = id >= 0 ? r[i].v[j] * scale : 0.f;
@@ -55,24 +54,40 @@ constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64, kSortIter = 4
 constexpr int kSortChunk = kSortThreads * kSortIter;   // tokens of a workgroup
 constexpr int kMaxDigitBits = 9, kMaxDigits = 1 << kMaxDigitBits;
 
+constexpr size_t kSortFillBytes = (size_t)48 << 20;
 // What the sorting launches write besides: `out`'s 16-byte pieces [from, to), from `add` or zeros.
 struct Fill {
     v4i* out;
     const v4i* add;   // null: zeros
     size_t from, to;
     int groups;
+    int stream;   // more than the memory-side cache holds: past it
 };
-__device__ __forceinline__ void fill(const Fill& f, int group) {
+template <bool STREAM>
+__device__ __forceinline__ void fill_pieces(const Fill& f, int group) {
+    auto get = [&](size_t i) {
+        if (!f.add) return v4i{0, 0, 0, 0};
+        if constexpr (STREAM) return __builtin_nontemporal_load(f.add + i);
+        else return f.add[i];
+    };
+    auto put = [&](size_t i, v4i v) {
+        if constexpr (STREAM) __builtin_nontemporal_store(v, f.out + i);
+        else f.out[i] = v;
+    };
     const size_t step = (size_t)f.groups * kSortThreads;
     size_t i = f.from + (size_t)group * kSortThreads + threadIdx.x;
     for (; i + 3 * step < f.to; i += 4 * step) {
         v4i v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = f.add ? f.add[i + j * step] : v4i{0, 0, 0, 0};
+        for (int j = 0; j < 4; ++j) v[j] = get(i + j * step);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) f.out[i + j * step] = v[j];
+        for (int j = 0; j < 4; ++j) put(i + j * step, v[j]);
     }
-    for (; i < f.to; i += step) f.out[i] = f.add ? f.add[i] : v4i{0, 0, 0, 0};
+    for (; i < f.to; i += step) put(i, get(i));
+}
+__device__ __forceinline__ void fill(const Fill& f, int group) {
+    if (f.stream) fill_pieces<true>(f, group);
+    else fill_pieces<false>(f, group);
 }
 
 struct Digit {
@@ -211,6 +226,9 @@ __global__ __launch_bounds__(kSortThreads) void embedding_count_kernel(Ids ids, 
         if ((int)threadIdx.x < digits) counts[((size_t)p * chunks + blockIdx.x) * digits + threadIdx.x] = p == 0 ? count[threadIdx.x] : 0;
 }
 
+// Counts of the next pass that a workgroup gathers in LDS; more (many chunks) go to memory wave by wave. (65536 tokens of 1000 rows, 16 chunks:
+// 22.6 us wave by wave, every wave's frequent ids at the same counts.)
+constexpr int kNextCounts = 8192;
 // One pass: the items of a chunk to their places. The first reads the ids, and drops what is no row; the others `in`. The counts of the
 // next pass's chunks are made on the way (sums of integers: their order does not matter).
 __global__ __launch_bounds__(kSortThreads) void embedding_scatter_kernel(Ids ids, const int2* __restrict__ in, int T, int V, int chunks, Digit digit,
@@ -218,7 +236,11 @@ __global__ __launch_bounds__(kSortThreads) void embedding_scatter_kernel(Ids ids
                                                                          int2* __restrict__ out, int* __restrict__ length, Fill f) {
     if ((int)blockIdx.x >= chunks) return fill(f, blockIdx.x - chunks);
     __shared__ SortLds lds;
+    __shared__ int next_here[kNextCounts];
     const int digits = digit.count(), c = blockIdx.x;
+    const bool gather = next_counts && chunks * digits <= kNextCounts;
+    if (gather)
+        for (int i = threadIdx.x; i < chunks * digits; i += kSortThreads) next_here[i] = 0;   // (barriers behind it: scan_digits')
     int total = 0, before = 0;
     if ((int)threadIdx.x < digits) {
 #pragma unroll 8
@@ -254,11 +276,18 @@ __global__ __launch_bounds__(kSortThreads) void embedding_scatter_kernel(Ids ids
         const bool live = key[i] >= 0;
         const int pos = live ? lds.count[wave_id()][digit.of(key[i])] + rank[i] : 0;
         if (live) out[pos] = make_int2(key[i], token[i]);
-        if (next_counts) {   // one addition per chunk and digit of the wave's
-            const int at = live ? (pos / kSortChunk) * digits + next.of(key[i]) : 0;
+        const int at = live ? (pos / kSortChunk) * digits + next.of(key[i]) : 0;
+        if (gather) {
+            if (live) atomicAdd(&next_here[at], 1);
+        } else if (next_counts) {   // one addition per chunk and digit of the wave's
             const uint64_t same = same_value(at, digit.bits + chunk_bits, __ballot(live));
             if (live && (same & ((1ull << lane_id()) - 1)) == 0) atomicAdd(next_counts + at, __popcll(same));
         }
+    }
+    if (gather) {
+        __syncthreads();
+        for (int i = threadIdx.x; i < chunks * digits; i += kSortThreads)
+            if (next_here[i]) atomicAdd(next_counts + i, next_here[i]);
     }
 }
 
@@ -272,49 +301,105 @@ struct EmbedSums {
     float scale;
 };
 template <typename T>
-__device__ __forceinline__ void write_row(const EmbedSums& p, const T* add, T* dtable, int row, int col, Row8 r) {
-    const size_t at = (size_t)row * p.H + col;
-    Row8 a{};
-    if (add) a = load8(add + at);
+__device__ __forceinline__ void write_row(const EmbedSums& p, T* dtable, int row, int col, bool add, const Row8& a, Row8 r) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) r.v[j] = add ? __builtin_fmaf(p.scale, r.v[j], a.v[j]) : p.scale * r.v[j];
-    store8(dtable + at, r);
+    store8(dtable + (size_t)row * p.H + col, r);
 }
 
-// A wave: the tokens of one block, in order, 512 columns of them, eight rows in flight.
-template <typename T>
-__global__ __launch_bounds__(256) void embedding_sum_kernel(EmbedSums p, const T* add, T* dtable) {
+// Rows [from, to) without tokens: zeros, or a copy of `add`; a workgroup takes kRestRows of them, a thread finds out whether its row has tokens, a
+// wave writes a row.
+struct EmbedRest {
+    int from, to, rows;   // rows of a workgroup
+    int stream;           // more than the memory-side cache holds: past it
+};
+constexpr int kRestRows = 256;
+template <bool STREAM, typename T>
+__device__ __forceinline__ void rest_rows(const EmbedSums& p, const EmbedRest& rest, int group, int length, const T* add, T* dtable) {
+    __shared__ uint8_t has[kRestRows];
+    const int row0 = rest.from + group * rest.rows, n = min(rest.rows, rest.to - row0);
+    if ((int)threadIdx.x < n) {
+        const int row = row0 + threadIdx.x;
+        int lo = 0, hi = length;   // the first item of the row or behind it
+        while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (p.sorted[mid].x < row) lo = mid + 1;
+            else hi = mid;
+        }
+        has[threadIdx.x] = lo < length && p.sorted[lo].x == row;
+    }
+    __syncthreads();
+    const int pieces = p.H * (int)sizeof(T) / 16;
+    for (int r = wave_id(); r < n; r += 4) {
+        if (has[r]) continue;
+        const v4i* in = (const v4i*)(add + (size_t)(row0 + r) * p.H);
+        v4i* out = (v4i*)(dtable + (size_t)(row0 + r) * p.H);
+        for (int i = lane_id(); i < pieces; i += 4 * 64) {
+            v4i v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                v[k] = v4i{0, 0, 0, 0};
+                if (add && i + 64 * k < pieces) v[k] = STREAM ? __builtin_nontemporal_load(in + i + 64 * k) : in[i + 64 * k];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (i + 64 * k < pieces) {
+                    if (STREAM) __builtin_nontemporal_store(v[k], out + i + 64 * k);
+                    else out[i + 64 * k] = v[k];
+                }
+        }
+    }
+}
+
+// A wave: the tokens of one block, in order, 512 columns of them, eight rows in flight, and with them what is added to the rows that
+// end among them. The workgroups behind those of the sums write the rows without tokens.
+template <typename T, bool ADD>
+__global__ __launch_bounds__(256) void embedding_sum_kernel(EmbedSums p, EmbedRest rest, int groups, int slabs, const T* add, T* dtable) {
     constexpr int kAhead = 8;
-    const int length = *p.length, lane = lane_id();
-    const int64_t b = (int64_t)blockIdx.x * 4 + wave_id(), first = b * p.block;
+    const int length = *p.length, lane = lane_id(), group = blockIdx.x;
+    if (group >= groups * slabs) {
+        if (rest.stream) rest_rows<true>(p, rest, group - groups * slabs, length, ADD ? add : (const T*)nullptr, dtable);
+        else rest_rows<false>(p, rest, group - groups * slabs, length, ADD ? add : (const T*)nullptr, dtable);
+        return;
+    }
+    const int at = group / slabs, slab = group - at * slabs;   // (a row's slabs side by side: it is read in one go)
+    const int64_t b = (int64_t)at * 4 + wave_id(), first = b * p.block;
     if (first >= length) return;
     const int n = (int)min((int64_t)p.block, length - first);
     const int2 item = lane < n ? p.sorted[first + lane] : make_int2(-1, 0);
-    const int before = first > 0 ? p.sorted[first - 1].x : -1, behind = first + n < length ? p.sorted[first + n].x : -1;
-    const int col = blockIdx.y * 512 + lane * 8;
+    const int before = to_sgpr(first > 0 ? p.sorted[first - 1].x : -1), behind = to_sgpr(first + n < length ? p.sorted[first + n].x : -1);
+    const int col = slab * 512 + lane * 8;
     const bool mine = col < p.H;
+    // bit i: token i is its row's last
+    const int below = __shfl_down(item.x, 1, 64);   // (with every lane taking part)
+    const uint64_t ends = __ballot(lane < n && (lane < n - 1 ? below : behind) != item.x);
     Row8 sum{};
-    bool head = __builtin_amdgcn_readlane(item.x, 0) == to_sgpr(before);   // the run that is summed began in an earlier block
+    bool head = __builtin_amdgcn_readlane(item.x, 0) == before;   // the run that is summed began in an earlier block
     for (int i0 = 0; i0 < n; i0 += kAhead) {
-        Row8 r[kAhead];
+        v4i r[kAhead];   // (as they are in memory)
+        Row8 a[kAhead];
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            r[i] = Row8{};
-            if (i0 + i < n && mine) r[i] = load8(p.dout + (size_t)__builtin_amdgcn_readlane(item.y, min(i0 + i, 63)) * p.H + col);
+            r[i] = v4i{0, 0, 0, 0};
+            a[i] = Row8{};
+            if (i0 + i < n && mine) r[i] = *(const v4i*)(p.dout + (size_t)__builtin_amdgcn_readlane(item.y, min(i0 + i, 63)) * p.H + col);
+            if (ADD && i0 + i < n && mine && (ends >> (i0 + i) & 1))
+                a[i] = load8(add + (size_t)__builtin_amdgcn_readlane(item.x, min(i0 + i, 63)) * p.H + col);
         }
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             if (i0 + i >= n) break;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum.v[j] += r[i].v[j];
-            const int row = __builtin_amdgcn_readlane(item.x, i0 + i);
-            const bool last = i0 + i == n - 1;
-            const int next = last ? to_sgpr(behind) : __builtin_amdgcn_readlane(item.x, min(i0 + i + 1, 63));
-            if (row == next && !last) continue;
-            if (head || row == next) {
+            for (int j = 0; j < 4; ++j) {
+                sum.v[2 * j] += __uint_as_float((uint32_t)r[i][j] << 16);
+                sum.v[2 * j + 1] += __uint_as_float((uint32_t)r[i][j] & 0xffff0000u);
+            }
+            const bool last = i0 + i == n - 1, end = ends >> (i0 + i) & 1;
+            if (!end && !last) continue;
+            if (head || !end) {
                 if (mine) store8(p.partial + ((size_t)b * 2 + (head ? 0 : 1)) * p.H + col, sum);
             } else if (mine) {
-                write_row(p, add, dtable, row, col, sum);
+                write_row(p, dtable, __builtin_amdgcn_readlane(item.x, i0 + i), col, ADD, a[i], sum);
             }
             head = false;
             sum = Row8{};
@@ -367,13 +452,16 @@ __global__ __launch_bounds__(256) void embedding_join_kernel(EmbedSums p, const 
         for (int v = 1; v < 4; ++v)
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum.v[j] += part[v][lane][j];
-        write_row(p, add, dtable, row, col, sum);
+        write_row(p, dtable, row, col, add != nullptr, add ? load8(add + (size_t)row * p.H + col) : Row8{}, sum);
     }
 }
 
 // ------------------------------------------------------------------------------------------------ host
 static int embed_check(int T, int V, int H) {
-    if (T <= 0 || V <= 0 || H <= 0 || (H % 8) != 0 || T >= (1 << 24) || V >= (1 << 30) || H > (1 << 21)) return HK_ERR_BAD_SHAPE;
+    // (2^38 elements of rows or of the table: workgroups of every launch below 2^24)
+    if (T <= 0 || V <= 0 || H <= 0 || (H % 8) != 0 || T >= (1 << 24) || V >= (1 << 30) || H > (1 << 21) || (long long)T * H >= (1ll << 38) ||
+        (long long)V * H >= (1ll << 38))
+        return HK_ERR_BAD_SHAPE;
     return HK_OK;
 }
 static size_t embed_up(size_t n) { return (n + 255) / 256 * 256; }
@@ -405,11 +493,29 @@ struct EmbedPlan {
     }
 };
 
+// Loads of a wave: a row in as few waves as hold it with eight each, evenly (2880 columns: one of six; 7168: two of seven); in waves of two
+// where that gives the chip fewer waves than it holds.
 template <typename T>
 static int launch_embedding(Ids ids, const void* table, void* out, int tokens, int V, int H, float scale, hipStream_t s) {
-    const dim3 grid((unsigned)((tokens + 3) / 4), (unsigned)((H / 8 + 64 * kEmbedLoads - 1) / (64 * kEmbedLoads)));
-    hipLaunchKernelGGL(embedding_kernel<T>, grid, dim3(256), 0, s, ids, (const T*)table, (uint16_t*)out, tokens, V, H, scale);
-    return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
+    const int parts64 = (H / 8 + 63) / 64;
+    int waves = (parts64 + 7) / 8, loads = (parts64 + waves - 1) / waves;
+    if ((long long)tokens * waves < 4096) loads = std::min(loads, 2);
+    waves = (parts64 + loads - 1) / loads;
+    auto launch = [&]<int LOADS>() {
+        hipLaunchKernelGGL((embedding_kernel<T, LOADS>), dim3((unsigned)((tokens + 3) / 4), (unsigned)waves), dim3(256), 0, s, ids, (const T*)table,
+                           (uint16_t*)out, tokens, V, H, scale);
+        return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
+    };
+    switch (loads) {
+        case 1: return launch.template operator()<1>();
+        case 2: return launch.template operator()<2>();
+        case 3: return launch.template operator()<3>();
+        case 4: return launch.template operator()<4>();
+        case 5: return launch.template operator()<5>();
+        case 6: return launch.template operator()<6>();
+        case 7: return launch.template operator()<7>();
+        default: return launch.template operator()<8>();
+    }
 }
 
 template <typename T>
@@ -419,10 +525,15 @@ static int launch_embedding_backward(Ids ids, const void* dout, const void* add,
     int* length = (int*)ws;
     int* counts = (int*)(ws + L.counts);
     int2 *a = (int2*)(ws + L.a), *b = (int2*)(ws + L.b);
-    const size_t pieces = add == dtable ? 0 : (size_t)V * H * sizeof(T) / 16;
+    // The launches that sort write the first rows, as many as take them about their time, whether these have tokens or not; the launch that sums
+    // writes the others, where there are no tokens.
     const int launches = L.chunks == 1 ? 1 : 1 + L.passes;
+    const size_t row_bytes = (size_t)H * sizeof(T), all_bytes = V * row_bytes;
+    const int blind = add == dtable ? 0 : (int)std::min<size_t>(V, launches * (add ? kSortFillBytes / 2 : kSortFillBytes) / row_bytes);
+    const size_t pieces = blind * row_bytes / 16;
+    EmbedRest rest{blind, add == dtable ? blind : V, (int)std::min<size_t>(kRestRows, std::max<size_t>(4, (128u << 10) / row_bytes)), all_bytes > (256u << 20)};
     auto part = [&](int launch) {
-        Fill f{(v4i*)dtable, (const v4i*)add, pieces * launch / launches, pieces * (launch + 1) / launches, 0};
+        Fill f{(v4i*)dtable, (const v4i*)add, pieces * launch / launches, pieces * (launch + 1) / launches, 0, rest.stream};
         f.groups = (int)std::min<size_t>(512, (f.to - f.from + 4 * kSortThreads - 1) / (4 * kSortThreads));
         return f;
     };
@@ -448,7 +559,10 @@ static int launch_embedding_backward(Ids ids, const void* dout, const void* add,
     if (hipGetLastError() != hipSuccess) return HK_ERR_LAUNCH;
     const EmbedSums p{sorted, length, (const uint16_t*)dout, (float*)(ws + L.partial), H, L.block, scale};
     const unsigned blocks = (unsigned)((tokens + L.block - 1) / L.block), slabs = (unsigned)((H + 511) / 512);
-    hipLaunchKernelGGL(embedding_sum_kernel<T>, dim3((blocks + 3) / 4, slabs), dim3(256), 0, s, p, (const T*)add, (T*)dtable);
+    const unsigned groups = (blocks + 3) / 4;
+    const unsigned grid = groups * slabs + (unsigned)((rest.to - rest.from + rest.rows - 1) / rest.rows);
+    if (add) hipLaunchKernelGGL((embedding_sum_kernel<T, true>), dim3(grid), dim3(256), 0, s, p, rest, (int)groups, (int)slabs, (const T*)add, (T*)dtable);
+    else hipLaunchKernelGGL((embedding_sum_kernel<T, false>), dim3(grid), dim3(256), 0, s, p, rest, (int)groups, (int)slabs, (const T*)nullptr, (T*)dtable);
     if (blocks > 1) hipLaunchKernelGGL(embedding_join_kernel<T>, dim3(blocks - 1, slabs), dim3(256), 0, s, p, (const T*)add, (T*)dtable);
     return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
 }

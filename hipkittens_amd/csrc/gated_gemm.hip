@@ -11,6 +11,7 @@
 // fp32 accumulation and activation, one rounding. The products are those of gemm_layouts_ring.h, which bound both kernels; in the forward one
 // every 32 rows of the weight tile in LDS are 16 gate rows and the 16 up rows of the same columns (kPairs), so that both values of
 // an element are in one lane's accumulators and the activation needs no exchange between lanes.
+#include "gemm_skinny.h"
 #include "moe_grouped.h"
 #include "../../include/hk355.h"
 
@@ -116,6 +117,43 @@ __global__ __launch_bounds__(256) void gated_gemm_kernel(GatedForward p) {
     }
 }
 
+// Few rows of a dense block (decode): one pass over the weights at HBM speed, the skinny kernel with gate and up rows in its two halves.
+struct GatedMma {
+    static constexpr bool kScaled = false;
+    static __device__ __forceinline__ void mma(v4f& acc, const v8i& b, const v8i& a) {
+        auto half = [](const v8i& v, int h) { return __builtin_bit_cast(v8bf_t, h ? __builtin_shufflevector(v, v, 4, 5, 6, 7) : __builtin_shufflevector(v, v, 0, 1, 2, 3)); };
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(half(b, 0), half(a, 0), acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(half(b, 1), half(a, 1), acc, 0, 0, 0);
+    }
+};
+struct GatedSkinnyOut {
+    static constexpr bool kPairs = true;
+    GatedForward p;
+    __device__ __forceinline__ uint32_t pitch() const { return (uint32_t)p.K * (p.interleaved ? 4u : 2u); }
+    __device__ __forceinline__ const uint8_t* other() const { return (const uint8_t*)(p.w13 + (p.interleaved ? (size_t)p.K : (size_t)p.I * p.K)); }
+    // columns c .. c + 4 of h
+    __device__ __forceinline__ void store(int row, int c, const v4f& g, const v4f& u) const {
+        float h[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[j] = p.gate.value(g[j], u[j]);
+        *(v2i*)(p.h + (size_t)row * p.I + c) = v2i{(int)pack_bf16(h[0], h[1]), (int)pack_bf16(h[2], h[3])};
+        if (!p.gate_up) return;
+        uint16_t* at = p.gate_up + (size_t)row * 2 * p.I;
+        if (p.interleaved) {
+            *(v4i*)(at + 2 * c) = v4i{(int)pack_bf16(g.x, u.x), (int)pack_bf16(g.y, u.y), (int)pack_bf16(g.z, u.z), (int)pack_bf16(g.w, u.w)};
+        } else {
+            *(v2i*)(at + c) = v2i{(int)pack_bf16(g.x, g.y), (int)pack_bf16(g.z, g.w)};
+            *(v2i*)(at + p.I + c) = v2i{(int)pack_bf16(u.x, u.y), (int)pack_bf16(u.z, u.w)};
+        }
+    }
+};
+template <int R, int NW, int D, int NF, bool NT>
+__global__ __launch_bounds__(64 * NW) void gated_skinny_kernel(GatedForward p) {
+    extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
+    gemm_skinny_body<GatedMma, R, NW, D, NF, NT>(smem, (const uint8_t*)p.x, (const uint8_t*)p.w13, nullptr, p.R, p.I, 2 * p.K, 1.0f,
+                                                 SkinnyScales{nullptr, nullptr, 0, 0, 0}, GatedSkinnyOut{p});
+}
+
 struct GatedBackward {
     const uint16_t *dy, *w2;
     const int32_t* offsets;
@@ -194,6 +232,46 @@ static int launch_gated(const GatedBackward& p, hipStream_t s) {
     static DeviceOnce once;
     return launch_gated_tile<Tile>(gated_dgrad_kernel<Tile>, once, p, p.I, s);
 }
+template <int R, int NW, int D, int NF, bool NT>
+static int launch_gated_skinny_kernel(const GatedForward& p, hipStream_t s) {
+    auto kern = gated_skinny_kernel<R, NW, D, NF, NT>;
+    constexpr int lds_bytes = skinny_lds_bytes(R, NW, D, false, NF);
+    static_assert(lds_bytes <= 160 * 1024, "LDS of one CU");
+    static DeviceOnce configured;
+    if (!set_lds_limit_once((const void*)kern, lds_bytes, configured)) return HK_ERR_LAUNCH;
+    hipLaunchKernelGGL(kern, dim3((p.I + 8 * NF - 1) / (8 * NF)), dim3(64 * NW), lds_bytes, s, p);
+    return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
+}
+// R: 16 rows of x each. Rows of the weights a workgroup: 16 (NF = 1) while 32 would leave half of the CUs without one; 64 (NF = 4, three waves of
+// three stages) where their rounds over the CUs, one workgroup each, take in fewer bytes than those of 32 (NF = 2, four waves): x is loaded once
+// a workgroup, and a CU's loads into LDS, not HBM, bound more than 16 rows. (us from HBM, 32 / 64 rows of weights a workgroup / 64-tile kernel:
+// 48 rows, I = 14336, K = 4096 55.7 / 43.6 / 55.0; 32 rows 47.5 / 40.4 / 55.2; 32 rows, I = 9216, K = 8192 65.8 / 68.2 / 74.1; with 16 rows
+// and 32 a workgroup 41.1 / - / 55.1, one row 38.9. 1 row, I = 2048, K = 7168: 11.2 / - / 30.2.)
+template <int R, int D1, int D2>
+static int launch_gated_skinny_rows(const GatedForward& p, hipStream_t s) {
+    const int cus = moe_num_compute_units();
+    const bool nt = 4ll * p.I * p.K >= kSkinnyNtBytes;
+    auto launch = [&]<int W, int D, int NF>() {
+        return nt ? launch_gated_skinny_kernel<R, W, D, NF, true>(p, s) : launch_gated_skinny_kernel<R, W, D, NF, false>(p, s);
+    };
+    auto rounds = [&](int cols) { return ((p.I + cols - 1) / cols + cus - 1) / cus; };
+    if (2ll * ((p.I + 15) / 16) <= cus) return launch.template operator()<4, D1, 1>();
+    if constexpr (R > 1)
+        if (rounds(32) * (64 + 16 * R) < rounds(16) * (32 + 16 * R)) return launch.template operator()<3, 3, 4>();
+    return launch.template operator()<4, D2, 2>();
+}
+// Not for short rows of many columns, where a wave has few K-steps of its own (16 rows, skinny / 64-tile kernel, us: I = 57344, K = 512 35.4 / 27.9;
+// I = 100000, K = 1024 89.4 / 88.9, 64 rows 105 / 95; I = 28672, K = 2048, 64 rows 52.9 / 59.9).
+static bool use_gated_skinny(int R, int I, int K) {
+    if (R > kSkinnyMaxM) return false;
+    return (I + 15) / 16 <= moe_num_compute_units() || K >= (R <= 32 ? 1024 : 2048);
+}
+static int launch_gated_skinny(const GatedForward& p, hipStream_t s) {
+    if (p.R <= 16) return launch_gated_skinny_rows<1, 4, 4>(p, s);
+    if (p.R <= 32) return launch_gated_skinny_rows<2, 3, 3>(p, s);
+    if (p.R <= 48) return launch_gated_skinny_rows<3, 4, 4>(p, s);
+    return launch_gated_skinny_rows<4, 3, 3>(p, s);
+}
 template <typename P>
 static int launch_gated_choice(const P& p, int in, int out, hipStream_t s) {
     switch (grouped_choice(p.R, p.E, in, out, !p.offsets)) {
@@ -216,6 +294,7 @@ extern "C" int hk_gated_gemm(const void* x_bf16, const void* w13_bf16, const int
     GatedForward p{(const uint16_t*)x_bf16, (const uint16_t*)w13_bf16, expert_offsets_or_null, (uint16_t*)h_bf16, (uint16_t*)gate_up_bf16_or_null,
                    R, E, I, K, 0, interleaved != 0, {}};
     if (const int st = make_gate(activation, alpha, limit, p.gate)) return st;
+    if (!p.offsets && use_gated_skinny(R, I, K)) return launch_gated_skinny(p, (hipStream_t)stream);
     return launch_gated_choice(p, K, 2 * I, (hipStream_t)stream);
 }
 

@@ -45,22 +45,33 @@ __device__ __forceinline__ v2i scale_bytes_direct(v4i srd, uint32_t off) {
 struct SkinnyScales {
     const uint8_t* SA; const uint8_t* SB; int sa_pitch, sb_pitch, row_bytes;
 };
-template <typename MMA, int R, int NW, int D, int NF = 2, bool NT = false>
+// OUT: what the sums become. SkinnyPlain: C. With kPairs, B is one half of the operand and out.other() the other, each in rows of out.pitch()
+// bytes: a workgroup owns rows n0 .. n0 + 8 NF of both (NF / 2 fragments of the one, then of the other; NF = 1: the two halves of one), and
+// out.store(row, n, first, second) takes both sums of rows n .. n + 4 of them (N % 4 == 0).
+struct SkinnyPlain { static constexpr bool kPairs = false; };
+template <typename MMA, int R, int NW, int D, int NF = 2, bool NT = false, typename OUT = SkinnyPlain>
 __device__ __forceinline__ void gemm_skinny_body(
     uint8_t* smem, const uint8_t* __restrict__ A, const uint8_t* __restrict__ B, uint16_t* __restrict__ C,
-    int M, int N, int K, float alpha, SkinnyScales sc = SkinnyScales{nullptr, nullptr, 0, 0, 0}) {
-    constexpr bool kScaled = MMA::kScaled;
-    constexpr int kRowsB = 16 * NF;   // rows of B per workgroup
-    constexpr int kWBytes = kRowsB * BK, kStage = kWBytes + 16 * R * BK, kRegion = (D + (kScaled ? 2 : 0)) * kStage;
+    int M, int N, int K, float alpha, SkinnyScales sc = SkinnyScales{nullptr, nullptr, 0, 0, 0}, const OUT& out_pairs = OUT{}) {
+    constexpr bool kScaled = MMA::kScaled, kPairs = OUT::kPairs;
+    static_assert(!(kPairs && kScaled));
+    constexpr int kRowsB = (kPairs ? 8 : 16) * NF;   // rows of B (of each half) per workgroup
+    constexpr int kWBytes = 16 * NF * BK, kStage = kWBytes + 16 * R * BK, kRegion = (D + (kScaled ? 2 : 0)) * kStage;
     constexpr int LPT = 2 * NF + 2 * R;   // loads per K-step (and per tile of scales)
     static_assert(D >= 2 && (D - 1 + (kScaled ? 1 : 0)) * LPT < 64, "vmcnt range");
-    static_assert(NF == 1 || NF == 2, "one or two fragments of B per workgroup");
+    static_assert(NF == 1 || NF == 2 || (kPairs && NF == 4), "fragments of B per workgroup");
     static_assert(NW * R * NF * 1024 <= NW * kRegion, "the partial sums reuse the stages");
     const int lane = lane_id(), w = wave_id();
     const uint32_t r = lane & 15, g = lane >> 4;
     const int n0 = blockIdx.x * kRowsB;
     const int rows_b = N - n0 < kRowsB ? N - n0 : kRowsB;
-    const v4i srd_b = make_srd(B + (size_t)n0 * K, (uint32_t)rows_b * (uint32_t)K);
+    uint32_t pitch_b = (uint32_t)K;
+    v4i srd_other = {0, 0, 0, 0};
+    if constexpr (kPairs) {
+        pitch_b = out_pairs.pitch();
+        srd_other = make_srd(out_pairs.other() + (size_t)n0 * pitch_b, (uint32_t)(rows_b - 1) * pitch_b + (uint32_t)K);
+    }
+    const v4i srd_b = make_srd(B + (size_t)n0 * pitch_b, (uint32_t)(rows_b - 1) * pitch_b + (uint32_t)K);
     const v4i srd_a = make_srd(A, (uint32_t)M * (uint32_t)K);
     const int nk = (K + BK - 1) / BK;
     const int s0 = (int)((long long)nk * w / NW), n = (int)((long long)nk * (w + 1) / NW) - s0;
@@ -68,11 +79,13 @@ __device__ __forceinline__ void gemm_skinny_body(
     // load i of a tile covers its rows 8 i .. 8 i + 7: lane l fetches, for LDS position l & 7 of row
     // 8 i + l / 8, the 16-byte chunk that the swizzle puts there
     uint32_t voff[2], tail_or[2];   // even / odd i (the swizzle of row 8 i + y depends on i's parity only)
+    uint32_t voff_pairs[2] = {0, 0};   // load i of halves' rows: NF loads of the first, then NF of the second
 #pragma unroll
     for (int par = 0; par < 2; ++par) {
         const uint32_t row = 8u * par + (lane >> 3);
         const uint32_t c = swz_chunk(row, lane & 7);
         voff[par] = row * (uint32_t)K + c * 16u;
+        if constexpr (kPairs) voff_pairs[par] = (row - (NF == 1 ? 8u * par : 0u)) * pitch_b + c * 16u;
         tail_or[par] = (int)(c * 16u) >= K - (nk - 1) * BK ? 0x80000000u : 0u;
     }
     const uint32_t lds0 = (uint32_t)(uintptr_t)smem;
@@ -94,9 +107,10 @@ __device__ __forceinline__ void gemm_skinny_body(
         const bool last = kt == nk - 1;
 #pragma unroll
         for (int i = 0; i < 2 * NF; ++i) {
-            const uint32_t vo = (voff[i & 1] + (uint32_t)(i >> 1) * 16u * (uint32_t)K) | (last ? tail_or[i & 1] : 0u);
-            if constexpr (NT) dma16_nt(srd_b, dst + i * 1024, vo, k0);
-            else dma16(srd_b, dst + i * 1024, vo, k0);
+            const uint32_t vo = (kPairs ? voff_pairs[i & 1] + (uint32_t)(i % NF >> 1) * 16u * pitch_b : voff[i & 1] + (uint32_t)(i >> 1) * 16u * (uint32_t)K) | (last ? tail_or[i & 1] : 0u);
+            const v4i srd = kPairs && i >= NF ? srd_other : srd_b;
+            if constexpr (NT) dma16_nt(srd, dst + i * 1024, vo, k0);
+            else dma16(srd, dst + i * 1024, vo, k0);
         }
 #pragma unroll
         for (int i = 0; i < 2 * R; ++i)
@@ -225,6 +239,21 @@ __device__ __forceinline__ void gemm_skinny_body(
 #pragma unroll
         for (int f = 0; f < NF; ++f) red[((w * R + i) * NF + f) * 64 + lane] = acc[i][f];
     __syncthreads();
+    if constexpr (kPairs) {
+        for (int t = threadIdx.x; t < R * NF * 32; t += 64 * NW) {
+            const int l = t % (32 * NF), i = t / (32 * NF);   // (l over the first half's fragments, or half a fragment)
+            const int first = i * NF * 64 + l, second = first + 32 * NF;
+            v4f a = red[first], b = red[second];
+#pragma unroll
+            for (int ww = 1; ww < NW; ++ww) {
+                a += red[ww * R * NF * 64 + first];
+                b += red[ww * R * NF * 64 + second];
+            }
+            const int row = 16 * i + (l & 15), n = n0 + 4 * (l >> 4);
+            if (row < M && n < N) out_pairs.store(row, n, a, b);
+        }
+        return;
+    }
     for (int t = threadIdx.x; t < R * NF * 64; t += 64 * NW) {
         const int l = t & 63;
         v4f sum = red[t];

@@ -4,7 +4,7 @@
 //
 // HBM bounds both: the gradients are read once for the norm and once to be scaled. A list is any number of bf16 and fp32 tensors of any length
 // and alignment, described by a table on the device that a program makes once: one launch goes over all of them. Work is cut into
-// chunks of kClipChunk elements; a workgroup takes a run of chunks, so that it looks its first tensor up once and then walks. Squares are added
+// chunks of kClipChunk elements, which a workgroup looks up in the table. Squares are added
 // in 64 bits (a square of fp32 does not leave their range, and the sum of 2^30 of them keeps fp32's digits), in an order that depends on the
 // list alone.
 #include <algorithm>
@@ -26,25 +26,36 @@ struct GradEntry {
 };
 static_assert(sizeof(GradEntry) == 40);
 
-// The workgroup's run of chunks, tensor by tensor: f(entry, from, to) for each piece of one tensor.
+// The workgroup's chunks: f(entry, from, to). Neighbouring workgroups have neighbouring chunks, so that the launch goes through memory front to
+// back (each workgroup a run of its own instead: norm of 2.4 GB 458 us, so 385).
 template <typename F>
-__device__ __forceinline__ void for_pieces(const GradEntry* __restrict__ list, int n, int64_t chunks, F&& f) {
-    int64_t c = chunks * blockIdx.x / gridDim.x;
-    const int64_t end = chunks * (blockIdx.x + 1) / gridDim.x;
-    if (c >= end) return;
-    int lo = 0, hi = n;   // the last tensor whose chunks begin at c or in front of it (tensors without elements have none)
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (list[mid].chunk0 <= c) lo = mid;
-        else hi = mid;
+__device__ __forceinline__ void for_chunks(const GradEntry* __restrict__ list, int n, int64_t chunks, F&& f) {
+    int at = 0;
+    for (int64_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+        int hi = n;   // the last tensor whose chunks begin at c or in front of it (tensors without elements have none)
+        while (hi - at > 1) {
+            const int mid = (at + hi) / 2;
+            if (list[mid].chunk0 <= c) at = mid;
+            else hi = mid;
+        }
+        const GradEntry e = list[at];
+        const int64_t from = (c - e.chunk0) * kClipChunk;
+        f(e, from, min(e.count, from + kClipChunk));
     }
-    for (; c < end && lo < n; ++lo) {
-        const GradEntry e = list[lo];
-        const int64_t stop = min(end, e.chunk0 + (e.count + kClipChunk - 1) / kClipChunk);
-        if (stop <= c) continue;
-        f(e, (c - e.chunk0) * kClipChunk, min(e.count, (stop - e.chunk0) * kClipChunk));
-        c = stop;
-    }
+}
+
+// Lists that do not fit the memory-side cache together (256 MB) go past it: with the non-temporal hint the norm of 2.4 GB takes 342 us instead of
+// 385, the clip 879 instead of 913; smaller ones are still there for the clip when the norm has read them.
+constexpr int64_t kClipStreamChunks = (256ll << 20) / (2 * kClipChunk);
+template <bool NT>
+__device__ __forceinline__ v4i load_piece(const v4i* p) {
+    if constexpr (NT) return __builtin_nontemporal_load(p);
+    else return *p;
+}
+template <bool NT>
+__device__ __forceinline__ void store_piece(v4i* p, v4i v) {
+    if constexpr (NT) __builtin_nontemporal_store(v, p);
+    else *p = v;
 }
 
 // Elements [from, to) of a tensor at `p`: one(i) for those in front of the first and behind the last 16-byte piece, piece(i) for the pieces,
@@ -61,17 +72,18 @@ __device__ __forceinline__ void for_elements(uint64_t p, int64_t from, int64_t t
 
 __device__ __forceinline__ float bf16_at(uint64_t p, int64_t i) { return __uint_as_float((uint32_t)((const uint16_t*)p)[i] << 16); }
 
+template <bool NT>
 __global__ __launch_bounds__(256) void grad_square_sum_kernel(const GradEntry* __restrict__ list, int n, int64_t chunks, double* __restrict__ partial) {
     constexpr int kAhead = 4;
     double sum[2] = {0.0, 0.0};
     auto add = [&](float x, int which) { sum[which] = __builtin_fma((double)x, (double)x, sum[which]); };
-    for_pieces(list, n, chunks, [&](const GradEntry& e, int64_t from, int64_t to) {
+    for_chunks(list, n, chunks, [&](const GradEntry& e, int64_t from, int64_t to) {
         auto pieces = [&](int64_t first, int64_t count, int size) {
             const v4i* at = (const v4i*)(e.src + first * size);
             for (int64_t i = threadIdx.x; i < count; i += kAhead * 256) {
                 v4i q[kAhead];
 #pragma unroll
-                for (int k = 0; k < kAhead; ++k) q[k] = i + k * 256 < count ? at[i + k * 256] : v4i{0, 0, 0, 0};
+                for (int k = 0; k < kAhead; ++k) q[k] = i + k * 256 < count ? load_piece<NT>(at + i + k * 256) : v4i{0, 0, 0, 0};
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k)
 #pragma unroll
@@ -111,10 +123,11 @@ __global__ __launch_bounds__(1024) void grad_norm_kernel(const double* __restric
     }
 }
 
+template <bool NT>
 __global__ __launch_bounds__(256) void grad_clip_kernel(const GradEntry* __restrict__ list, int n, int64_t chunks, const float* __restrict__ norm,
                                                         float max_norm) {
     const float ratio = max_norm / (norm[0] + 1e-6f), factor = ratio >= 1.0f ? 1.0f : ratio;   // (a NaN stays one)
-    for_pieces(list, n, chunks, [&](const GradEntry& e, int64_t from, int64_t to) {
+    for_chunks(list, n, chunks, [&](const GradEntry& e, int64_t from, int64_t to) {
         if (factor == 1.0f && e.src == e.dst) return;   // in place, nothing to scale
         auto get = [&](int64_t i) { return e.src_fp32 ? ((const float*)e.src)[i] : bf16_at(e.src, i); };
         auto put = [&](int64_t i, float v) {
@@ -157,7 +170,7 @@ __global__ __launch_bounds__(256) void grad_clip_kernel(const GradEntry* __restr
             for (int64_t i = threadIdx.x; i < count; i += kAhead * 256) {
                 v4i q[kAhead];
 #pragma unroll
-                for (int k = 0; k < kAhead; ++k) q[k] = i + k * 256 < count ? at[i + k * 256] : v4i{0, 0, 0, 0};
+                for (int k = 0; k < kAhead; ++k) q[k] = i + k * 256 < count ? load_piece<NT>(at + i + k * 256) : v4i{0, 0, 0, 0};
 #pragma unroll
                 for (int k = 0; k < kAhead; ++k) {
 #pragma unroll
@@ -166,7 +179,7 @@ __global__ __launch_bounds__(256) void grad_clip_kernel(const GradEntry* __restr
                         else q[k][j] = (int)pack_bf16(__uint_as_float((uint32_t)q[k][j] << 16) * factor,
                                                       __uint_as_float((uint32_t)q[k][j] & 0xffff0000u) * factor);
                     }
-                    if (i + k * 256 < count) out[i + k * 256] = q[k];
+                    if (i + k * 256 < count) store_piece<NT>(out + i + k * 256, q[k]);
                 }
             }
         };
@@ -216,7 +229,7 @@ extern "C" int hk_grad_norm(const void* list, int n, int64_t chunks, float* norm
     const hipStream_t s = (hipStream_t)stream;
     const int groups = clip_groups(chunks);
     if (groups > 0)
-        hipLaunchKernelGGL(grad_square_sum_kernel, dim3(groups), dim3(256), 0, s, (const GradEntry*)list, n, chunks, (double*)workspace);
+        hipLaunchKernelGGL(chunks > kClipStreamChunks ? grad_square_sum_kernel<true> : grad_square_sum_kernel<false>, dim3(groups), dim3(256), 0, s, (const GradEntry*)list, n, chunks, (double*)workspace);
     hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(1024), 0, s, (const double*)workspace, groups, norm);
     return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
 }
@@ -229,6 +242,6 @@ extern "C" int hk_grad_clip(const void* list, int n, int64_t chunks, const float
     if (!(max_norm >= 0.f)) return HK_ERR_UNSUPPORTED;
     const int groups = clip_groups(chunks);
     if (groups == 0) return HK_OK;
-    hipLaunchKernelGGL(grad_clip_kernel, dim3(groups), dim3(256), 0, (hipStream_t)stream, (const GradEntry*)list, n, chunks, norm, max_norm);
+    hipLaunchKernelGGL(chunks > kClipStreamChunks ? grad_clip_kernel<true> : grad_clip_kernel<false>, dim3(groups), dim3(256), 0, (hipStream_t)stream, (const GradEntry*)list, n, chunks, norm, max_norm);
     return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
 }

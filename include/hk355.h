@@ -553,8 +553,8 @@ int hk_bf16_gemm_wgrad(const void* dy_bf16, const void* x_bf16, void* dw, int dw
  */
 
 /* Rows of a table by token: out[t, :] = bf16(scale * table[ids[t], :]), zeros for an id outside [0, V). ids [T] int32 (id_type 0) or int64 (1);
- * table [V, H] bf16 (table_type 0) or fp32 (1); out [T, H]. Requirements: H % 8 == 0, H <= 2^21, T < 2^24, V < 2^30; table and out 16-byte
- * aligned. */
+ * table [V, H] bf16 (table_type 0) or fp32 (1); out [T, H]. Requirements: H % 8 == 0, H <= 2^21, T < 2^24, V < 2^30, T H and V H
+ * below 2^38; table and out 16-byte aligned. */
 int hk_embedding(const void* ids, int id_type, const void* table, int table_type, void* out_bf16, int T, int V, int H, float scale,
                  void* stream);
 /* Its gradient: dtable[v, :] = add[v, :] + scale * sum over the tokens t with ids[t] = v of dout[t, :] (fp32 sums in an order that depends on
