@@ -12,7 +12,8 @@ _DISPATCH_PATH = Path(__file__).resolve().parent / "_dispatch.so"
 _DISPATCH_ENTRIES = ("fp8_gemm", "fp8_gemm_ws", "bf16_gemm", "bf16_gemm_ws", "mxfp4_gemm", "mxfp4_gemm_ws",
                      "mxfp4_gemm_pitched", "mxfp4_quantize_rows", "moe_permute", "moe_permute_backward",
                      "moe_unpermute_backward", "moe_grouped_gemm", "moe_grouped_gemm_dgrad", "moe_grouped_gemm_wgrad",
-                     "linear_cross_entropy", "linear_cross_entropy_backward")   # the order of csrc/dispatch.cpp's Entries
+                     "linear_cross_entropy", "linear_cross_entropy_backward", "gated_gemm", "gated_gemm_dgrad",
+                     "bf16_gemm_dgrad", "bf16_gemm_wgrad", "embedding", "embedding_backward", "grad_norm", "grad_clip")   # the order of csrc/dispatch.cpp's Entries
 _dispatch = None
 
 # name -> (restype, argtypes); one entry per symbol declared in include/hk355.h

@@ -1,4 +1,4 @@
-// The dispatchers' argument checks and launches (GEMMs; the MoE layers' rows and products and the output head in training)
+// The dispatchers' argument checks and launches (GEMMs; the operators of training)
 // for ordinary arguments, as a CPython module (`_dispatch`).
 //
 // A launch takes the runtime about 3 us; the same checks in Python, a call through ctypes and the attribute reads for it
@@ -42,6 +42,14 @@ struct Entries {
     decltype(&hk_moe_grouped_gemm_wgrad) grouped_wgrad;
     decltype(&hk_linear_cross_entropy) head_loss;
     decltype(&hk_linear_cross_entropy_backward) head_gradients;
+    decltype(&hk_gated_gemm) gated;
+    decltype(&hk_gated_gemm_dgrad) gated_dgrad;
+    decltype(&hk_bf16_gemm_dgrad) dense_dgrad;
+    decltype(&hk_bf16_gemm_wgrad) dense_wgrad;
+    decltype(&hk_embedding) embedding;
+    decltype(&hk_embedding_backward) embedding_backward;
+    decltype(&hk_grad_norm) grad_norm;
+    decltype(&hk_grad_clip) grad_clip;
 };
 Entries entries{};
 PyTypeObject* parameter_type = nullptr;
@@ -326,6 +334,157 @@ PyObject* linear_cross_entropy_backward(PyObject*, PyObject* const* args, Py_ssi
     });
 }
 
+struct Gated {
+    Operand wide, w, gate_up{}, h{}, offsets{};
+    int E, interleaved, act;
+    float alpha, limit;
+};
+// rows [R, wide], w ([E,] .., ..), gate_up [R, 2 I] or None, h [R, I] or None, expert_offsets [E + 1] or None, interleaved, activation, alpha, limit
+bool gated(PyObject* wide, PyObject* w, PyObject* gate_up, PyObject* h, PyObject* const* rest, Gated& g) {
+    const bool experts = rest[0] != Py_None;
+    if (!operand(wide, kBf16, 2, g.wide) || !operand(w, kBf16, experts ? 3 : 2, g.w) || (gate_up != Py_None && !operand(gate_up, kBf16, 2, g.gate_up)) ||
+        (h != Py_None && !operand(h, kBf16, 2, g.h)) || (experts && !operand(rest[0], kI32, 1, g.offsets)) || !PyBool_Check(rest[1]) ||
+        !PyLong_CheckExact(rest[2]) || !number(rest[3], g.alpha) || !number(rest[4], g.limit))
+        return false;
+    g.interleaved = rest[1] == Py_True;
+    g.act = (int)PyLong_AsLong(rest[2]);
+    g.E = (int)g.w.outer;
+    for (const Operand* t : {&g.w, &g.gate_up, &g.h, &g.offsets})
+        if (t->data && t->device != g.wide.device) return false;
+    return (!g.gate_up.data || (g.gate_up.rows == g.wide.rows && g.gate_up.cols % 2 == 0)) && (!g.h.data || g.h.rows == g.wide.rows) &&
+           (!experts || g.offsets.cols == g.w.outer + 1) && current(g.wide.device);
+}
+// (x, w13, h, gate_up or None, expert_offsets or None, interleaved, activation, alpha, limit)
+PyObject* gated_gemm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Gated g;
+        if (n != 9 || args[2] == Py_None || !gated(args[0], args[1], args[3], args[2], args + 4, g) || g.w.cols != g.wide.cols ||
+            g.w.rows != 2 * g.h.cols || (g.gate_up.data && g.gate_up.cols != g.w.rows))
+            Py_RETURN_NONE;
+        void* s = stream_of(g.wide.device);
+        return launch([&] {
+            return entries.gated(g.wide.data, g.w.data, (const int32_t*)g.offsets.data, g.h.data, g.gate_up.data, (int)g.wide.rows, g.E, (int)g.h.cols,
+                                 (int)g.wide.cols, g.interleaved, g.act, g.alpha, g.limit, s);
+        });
+    });
+}
+// (dy, w2, gate_up, dgate_up, h or None, expert_offsets or None, interleaved, activation, alpha, limit)
+PyObject* gated_gemm_dgrad(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Gated g;
+        Operand d;
+        if (n != 10 || args[2] == Py_None || !gated(args[0], args[1], args[2], args[4], args + 5, g) || !operand(args[3], kBf16, 2, d) ||
+            g.w.rows != g.wide.cols || g.gate_up.cols != 2 * g.w.cols || (g.h.data && g.h.cols != g.w.cols) || d.rows != g.wide.rows ||
+            d.cols != g.gate_up.cols || d.device != g.wide.device)
+            Py_RETURN_NONE;
+        void* s = stream_of(g.wide.device);
+        return launch([&] {
+            return entries.gated_dgrad(g.wide.data, g.w.data, (const int32_t*)g.offsets.data, g.gate_up.data, d.data, g.h.data, (int)g.wide.rows, g.E,
+                                       (int)g.wide.cols, (int)g.w.cols, g.interleaved, g.act, g.alpha, g.limit, s);
+        });
+    });
+}
+// (dy, w, dx)
+PyObject* bf16_gemm_dgrad(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Operand dy, w, dx;
+        if (n != 3 || !operand(args[0], kBf16, 2, dy) || !operand(args[1], kBf16, 2, w) || !operand(args[2], kBf16, 2, dx) || w.rows != dy.cols ||
+            dx.rows != dy.rows || dx.cols != w.cols || w.device != dy.device || dx.device != dy.device || !current(dy.device))
+            Py_RETURN_NONE;
+        void* s = stream_of(dy.device);
+        return launch([&] { return entries.dense_dgrad(dy.data, w.data, dx.data, (int)dy.rows, (int)dy.cols, (int)w.cols, s); });
+    });
+}
+// (dy, x, dw)
+PyObject* bf16_gemm_wgrad(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Operand dy, x, dw;
+        if (n != 3 || !operand(args[0], kBf16, 2, dy) || !operand(args[1], kBf16, 2, x)) Py_RETURN_NONE;
+        const bool fp32 = operand(args[2], kF32, 2, dw);
+        if ((!fp32 && !operand(args[2], kBf16, 2, dw)) || x.rows != dy.rows || dw.rows != dy.cols || dw.cols != x.cols || x.device != dy.device ||
+            dw.device != dy.device || !current(dy.device))
+            Py_RETURN_NONE;
+        void* s = stream_of(dy.device);
+        return launch([&] { return entries.dense_wgrad(dy.data, x.data, dw.data, fp32 ? 1 : 0, (int)dy.rows, (int)dy.cols, (int)x.cols, s); });
+    });
+}
+
+struct Embedding {
+    Operand ids, rows, table;
+    int id_type, table_type;
+    float scale;
+};
+// ids [T], rows [T, H], table [V, H]
+bool embedding_operands(PyObject* ids, PyObject* rows, PyObject* table, PyObject* scale, Embedding& e) {
+    e.id_type = operand(ids, {at::kLong}, 1, e.ids) ? 1 : 0;
+    if (!e.id_type && !operand(ids, kI32, 1, e.ids)) return false;
+    e.table_type = operand(table, kF32, 2, e.table) ? 1 : 0;
+    if ((!e.table_type && !operand(table, kBf16, 2, e.table)) || !operand(rows, kBf16, 2, e.rows) || !number(scale, e.scale)) return false;
+    return e.rows.rows == e.ids.cols && e.rows.cols == e.table.cols && e.rows.device == e.ids.device && e.table.device == e.ids.device &&
+           current(e.ids.device);
+}
+// (ids, table, out, scale)
+PyObject* embedding(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Embedding e;
+        if (n != 4 || !embedding_operands(args[0], args[2], args[1], args[3], e)) Py_RETURN_NONE;
+        void* s = stream_of(e.ids.device);
+        return launch([&] {
+            return entries.embedding(e.ids.data, e.id_type, e.table.data, e.table_type, e.rows.data, (int)e.rows.rows, (int)e.table.rows,
+                                     (int)e.table.cols, e.scale, s);
+        });
+    });
+}
+// (ids, dout, dtable, workspace, scale, add or None)
+PyObject* embedding_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Embedding e;
+        Operand ws, add{};
+        if (n != 6 || !embedding_operands(args[0], args[1], args[2], args[4], e) || !operand(args[3], kByte, 1, ws) || ws.device != e.ids.device ||
+            (args[5] != Py_None && ((e.table_type ? !operand(args[5], kF32, 2, add) : !operand(args[5], kBf16, 2, add)) || add.rows != e.table.rows ||
+                                    add.cols != e.table.cols || add.device != e.ids.device)))
+            Py_RETURN_NONE;
+        void* s = stream_of(e.ids.device);
+        return launch([&] {
+            return entries.embedding_backward(e.ids.data, e.id_type, e.rows.data, add.data, e.table.data, e.table_type, (int)e.rows.rows,
+                                              (int)e.table.rows, (int)e.table.cols, e.scale, ws.data, (size_t)ws.cols, s);
+        });
+    });
+}
+
+struct GradList {
+    Operand list, norm;
+    int n;
+    int64_t chunks;
+};
+// a GradTensors' list, n and chunks, and norm [1]
+bool grad_list(PyObject* const* args, PyObject* norm, GradList& g) {
+    if (!operand(args[0], kByte, 1, g.list) || !PyLong_CheckExact(args[1]) || !PyLong_CheckExact(args[2]) || !operand(norm, kF32, 1, g.norm)) return false;
+    g.n = (int)PyLong_AsLong(args[1]);
+    g.chunks = PyLong_AsLongLong(args[2]);
+    return g.norm.cols == 1 && g.norm.device == g.list.device && current(g.list.device);
+}
+// (list, n, chunks, norm, workspace)
+PyObject* grad_norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        GradList g;
+        Operand ws;
+        if (n != 5 || !grad_list(args, args[3], g) || !operand(args[4], kByte, 1, ws) || ws.device != g.list.device) Py_RETURN_NONE;
+        void* s = stream_of(g.list.device);
+        return launch([&] { return entries.grad_norm(g.list.data, g.n, g.chunks, (float*)g.norm.data, ws.data, (size_t)ws.cols, s); });
+    });
+}
+// (list, n, chunks, norm, max_norm)
+PyObject* grad_clip(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        GradList g;
+        float max_norm;
+        if (n != 5 || !grad_list(args, args[3], g) || !number(args[4], max_norm)) Py_RETURN_NONE;
+        void* s = stream_of(g.list.device);
+        return launch([&] { return entries.grad_clip(g.list.data, g.n, g.chunks, (const float*)g.norm.data, max_norm, s); });
+    });
+}
+
 // The library's functions by address, in the order of Entries.
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
     constexpr int kCount = sizeof(Entries) / sizeof(void*);
@@ -345,7 +504,9 @@ PyMethodDef methods[] = {HK_METHOD(bind), HK_METHOD(fp8_gemm), HK_METHOD(bf16_ge
                          HK_METHOD(mxfp4_quantize_rows), HK_METHOD(moe_permute), HK_METHOD(moe_permute_backward),
                          HK_METHOD(moe_unpermute_backward), HK_METHOD(moe_grouped_gemm), HK_METHOD(moe_grouped_gemm_dgrad),
                          HK_METHOD(moe_grouped_gemm_wgrad), HK_METHOD(linear_cross_entropy),
-                         HK_METHOD(linear_cross_entropy_backward), {nullptr, nullptr, 0, nullptr}};
+                         HK_METHOD(linear_cross_entropy_backward), HK_METHOD(gated_gemm), HK_METHOD(gated_gemm_dgrad),
+                         HK_METHOD(bf16_gemm_dgrad), HK_METHOD(bf16_gemm_wgrad), HK_METHOD(embedding), HK_METHOD(embedding_backward),
+                         HK_METHOD(grad_norm), HK_METHOD(grad_clip), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_dispatch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -59,6 +59,8 @@ class _NoNative:
     moe_permute = moe_permute_backward = moe_unpermute_backward = fp8_gemm
     moe_grouped_gemm = moe_grouped_gemm_dgrad = moe_grouped_gemm_wgrad = fp8_gemm
     linear_cross_entropy = linear_cross_entropy_backward = fp8_gemm
+    gated_gemm = gated_gemm_dgrad = bf16_gemm_dgrad = bf16_gemm_wgrad = fp8_gemm
+    embedding = embedding_backward = grad_norm = grad_clip = fp8_gemm
 
 
 def _load_native():
@@ -922,6 +924,9 @@ def dispatch_gated_gemm(x, w13, h, gate_up=None, expert_offsets=None, interleave
     with `interleaved`), activation "silu" or "swiglu_oai" (alpha, limit). gate_up [R,2I]: both projections, in the order of w13's rows, for
     dispatch_gated_gemm_dgrad. With expert_offsets [E+1] (dispatch_moe_sort): w13 [E,2I,K], rows grouped by expert; rows behind the last
     offset are left alone. The second half is dispatch_bf16_gemm or dispatch_moe_grouped_gemm."""
+    st = (_native or _load_native()).gated_gemm(x, w13, h, gate_up, expert_offsets, interleaved, _ACTIVATIONS.get(activation), alpha, limit)
+    if st is not None:
+        return _lib.check(st, "dispatch_gated_gemm")
     R, E, I, act = _check_gated(x, "x", w13, "w13", lambda i: (2 * i, x.shape[1]), gate_up, "gate_up", h, "h", expert_offsets, activation)
     with torch.cuda.device(x.device):
         st = _lib.load_library().hk_gated_gemm(x.data_ptr(), w13.data_ptr(), _ptr(expert_offsets), h.data_ptr(), _ptr(gate_up), R, E, I,
@@ -935,6 +940,10 @@ def dispatch_gated_gemm_dgrad(dy, w2, gate_up, dgate_up, h=None, expert_offsets=
     [R,2I] from dy [R,N] and the forward's gate_up [R,2I] (it may be gate_up itself), and h [R,I], the activation's value again, if given. What is
     left are dispatch_bf16_gemm_dgrad / _wgrad or dispatch_moe_grouped_gemm_dgrad / _wgrad: dx = dgate_up W13, dW13 = dgate_up^T x,
     dW2 = dy^T h."""
+    st = (_native or _load_native()).gated_gemm_dgrad(dy, w2, gate_up, dgate_up, h, expert_offsets, interleaved,
+                                                     _ACTIVATIONS.get(activation), alpha, limit)
+    if st is not None:
+        return _lib.check(st, "dispatch_gated_gemm_dgrad")
     if gate_up is None or dgate_up is None:
         raise RuntimeError("gate_up and dgate_up: expected a torch.Tensor")
     R, E, I, act = _check_gated(dy, "dy", w2, "w2", lambda i: (dy.shape[1], i), gate_up, "gate_up", h, "h", expert_offsets, activation)
@@ -963,6 +972,9 @@ def _check_product(rows_n, name_n, rows_k, name_k, w, name_w, w_types):
 
 def dispatch_bf16_gemm_dgrad(dy, w, dx) -> None:
     """Gradient of y = x @ w.T (dispatch_bf16_gemm) in x: dx [M,K] = dy [M,N] @ w [N,K], bf16."""
+    st = (_native or _load_native()).bf16_gemm_dgrad(dy, w, dx)
+    if st is not None:
+        return _lib.check(st, "dispatch_bf16_gemm_dgrad")
     M, N, K = _check_product(dy, "dy", dx, "dx", w, "w", _BF16)
     with torch.cuda.device(dy.device):
         st = _lib.load_library().hk_bf16_gemm_dgrad(dy.data_ptr(), w.data_ptr(), dx.data_ptr(), M, N, K, _stream(dy))
@@ -971,6 +983,9 @@ def dispatch_bf16_gemm_dgrad(dy, w, dx) -> None:
 
 def dispatch_bf16_gemm_wgrad(dy, x, dw) -> None:
     """Gradient of y = x @ w.T (dispatch_bf16_gemm) in w: dw [N,K] = dy [M,N].T @ x [M,K], in bf16 or fp32."""
+    st = (_native or _load_native()).bf16_gemm_wgrad(dy, x, dw)
+    if st is not None:
+        return _lib.check(st, "dispatch_bf16_gemm_wgrad")
     M, N, K = _check_product(dy, "dy", x, "x", dw, "dw", _BF16 + _F32)
     with torch.cuda.device(dy.device):
         st = _lib.load_library().hk_bf16_gemm_wgrad(dy.data_ptr(), x.data_ptr(), dw.data_ptr(), int(dw.dtype == torch.float32), M, N, K,
@@ -1002,6 +1017,9 @@ def _check_embedding(ids, rows, name_rows, table, name_table):
 def dispatch_embedding(ids, table, out, scale: float = 1.0) -> None:
     """Rows of a table by token: out[t] = scale * table[ids[t]], zeros for an id outside [0, V); ids [T] int32 or int64, table [V,H] bf16 or
     fp32, out [T,H] bf16."""
+    st = (_native or _load_native()).embedding(ids, table, out, scale)
+    if st is not None:
+        return _lib.check(st, "dispatch_embedding")
     T, V, H = _check_embedding(ids, out, "out", table, "table")
     with torch.cuda.device(ids.device):
         st = _lib.load_library().hk_embedding(ids.data_ptr(), int(ids.dtype == torch.int64), table.data_ptr(), int(table.dtype == torch.float32),
@@ -1013,6 +1031,9 @@ def dispatch_embedding_backward(ids, dout, dtable, workspace, scale: float = 1.0
     """Gradient of dispatch_embedding in the table: dtable[v] = add[v] + scale * (sum of dout[t] over the tokens with ids[t] = v); dout [T,H] bf16,
     dtable and add [V,H] bf16 or fp32, every row written (zeros without tokens and `add`). add may be dtable itself, e.g. the head's
     gradient of a tied table: then only rows with tokens are touched. workspace: embedding_backward_workspace_bytes(T, V, H) bytes."""
+    st = (_native or _load_native()).embedding_backward(ids, dout, dtable, workspace, scale, add)
+    if st is not None:
+        return _lib.check(st, "dispatch_embedding_backward")
     T, V, H = _check_embedding(ids, dout, "dout", dtable, "dtable")
     _check_tensor(workspace, "workspace", _U8, 1)
     if add is not None:
@@ -1086,6 +1107,10 @@ def _check_norm(grads, norm):
 def dispatch_grad_norm(grads, norm, workspace) -> None:
     """norm [1] fp32 = the square root of the sum of the squares of all of `grads` (a GradTensors), added in 64 bits. workspace:
     grad_norm_workspace_bytes() bytes."""
+    if type(grads) is GradTensors:
+        st = (_native or _load_native()).grad_norm(grads.list, grads.n, grads.chunks, norm, workspace)
+        if st is not None:
+            return _lib.check(st, "dispatch_grad_norm")
     _check_norm(grads, norm)
     _check_tensor(workspace, "workspace", _U8, 1)
     _same_device(norm, workspace)
@@ -1098,6 +1123,10 @@ def dispatch_grad_norm(grads, norm, workspace) -> None:
 def dispatch_grad_clip(grads, norm, max_norm: float) -> None:
     """Every gradient of `grads` times min(1, max_norm / (norm + 1e-6)), in place or into its outs; norm [1] of dispatch_grad_norm, or of
     all ranks together."""
+    if type(grads) is GradTensors:
+        st = (_native or _load_native()).grad_clip(grads.list, grads.n, grads.chunks, norm, max_norm)
+        if st is not None:
+            return _lib.check(st, "dispatch_grad_clip")
     _check_norm(grads, norm)
     with torch.cuda.device(norm.device):
         st = _lib.load_library().hk_grad_clip(grads.list.data_ptr(), grads.n, grads.chunks, norm.data_ptr(), float(max_norm), _stream(norm))
