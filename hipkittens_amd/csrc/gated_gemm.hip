@@ -11,28 +11,40 @@
 // fp32 accumulation and activation, one rounding. The products are those of gemm_layouts_ring.h, which bound both kernels; in the forward one
 // every 32 rows of the weight tile in LDS are 16 gate rows and the 16 up rows of the same columns (kPairs), so that both values of
 // an element are in one lane's accumulators and the activation needs no exchange between lanes.
+#include <utility>
+
 #include "gemm_skinny.h"
 #include "moe_grouped.h"
 #include "../../include/hk355.h"
 
 namespace hk {
 
+// The activation. SiLU has a form of its own: the backward kernel's epilogue, 256 elements a lane, is bound by their instructions (65536 rows of 32
+// experts, N = 7168, I = 2048, in one form for both 1780 us). A NaN stays one: the clamps are IEEE's minimum and maximum.
+struct GateArgs { float alpha, limit; };
+template <bool CLAMPED>
 struct Gate {
-    float alpha, limit, beta;
-    __device__ __forceinline__ float top(float g) const { return g > limit ? limit : g; }   // (a NaN stays one)
-    __device__ __forceinline__ float lin(float u) const { return (u > limit ? limit : u < -limit ? -limit : u) + beta; }
-    __device__ __forceinline__ float sig(float g) const {   // of a clamped g
-        return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * (alpha * -1.4426950408889634f)));
+    GateArgs a;
+    __device__ __forceinline__ static float sig(float z) {
+        return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
+    }
+    __device__ __forceinline__ float top(float g) const { return CLAMPED ? __builtin_elementwise_minimum(g, a.limit) : g; }
+    __device__ __forceinline__ float lin(float u) const {
+        return CLAMPED ? __builtin_elementwise_maximum(__builtin_elementwise_minimum(u, a.limit), -a.limit) + 1.0f : u;
     }
     __device__ __forceinline__ float value(float g, float u) const {
         const float t = top(g);
-        return lin(u) * (t * sig(t));
+        return lin(u) * (t * sig(CLAMPED ? a.alpha * t : t));
     }
     // h of (g, u), and from dh the gradients of both
     __device__ __forceinline__ float gradients(float g, float u, float dh, float& dg, float& du) const {
-        const float t = top(g), v = lin(u), s = sig(t), ts = t * s;
-        dg = g > limit ? 0.f : dh * v * (s * (1.0f + alpha * t * (1.0f - s)));
-        du = u > limit || u < -limit ? 0.f : dh * ts;
+        const float t = top(g), v = lin(u), z = CLAMPED ? a.alpha * t : t, s = sig(z), ts = t * s;
+        dg = dh * v * __builtin_fmaf(z * s, 1.0f - s, s);   // s (1 + z (1 - s))
+        du = dh * ts;
+        if (CLAMPED) {
+            dg = g > a.limit ? 0.f : dg;
+            du = __builtin_fabsf(u) > a.limit ? 0.f : du;
+        }
         return v * ts;
     }
 };
@@ -41,15 +53,14 @@ struct GatedForward {
     const uint16_t *x, *w13;
     const int32_t* offsets;   // null: dense
     uint16_t *h, *gate_up;    // gate_up null: not wanted
-    int R, E, I, K, tiles_n, interleaved;
-    Gate gate;
+    int R, E, I, K, tiles_n, interleaved, clamped;
+    GateArgs gate;
 };
 
 // One row of blocks of gate and up values (or their gradients) to gate_up: `at` the patch's first row, `col` its first column of I.
-template <int F>
-__device__ __forceinline__ void store_gate_up(const v4f (&g)[F], const v4f (&u)[F], int m, uint16_t* at, int col, int I, int interleaved,
-                                              int rows) {
-    if (!interleaved) {
+template <bool INTERLEAVED, int F>
+__device__ __forceinline__ void store_gate_up(const v4f (&g)[F], const v4f (&u)[F], int m, uint16_t* at, int col, int I, int rows) {
+    if constexpr (!INTERLEAVED) {
         store_block_row(g, m, at + col, 2 * (int64_t)I, rows, I - col);
         store_block_row(u, m, at + I + col, 2 * (int64_t)I, rows, I - col);
         return;
@@ -63,29 +74,66 @@ __device__ __forceinline__ void store_gate_up(const v4f (&g)[F], const v4f (&u)[
                                                              (int)pack_bf16(g[n].z, u[n].z), (int)pack_bf16(g[n].w, u[n].w)};
     }
 }
-template <int F>
-__device__ __forceinline__ void load_gate_up(v4f (&g)[F], v4f (&u)[F], int m, const uint16_t* at, int col, int I, int interleaved, int rows) {
-    if (!interleaved) {
-        load_block_row(g, m, at + col, 2 * (int64_t)I, rows, I - col);
-        load_block_row(u, m, at + I + col, 2 * (int64_t)I, rows, I - col);
-        return;
+// The kept gate and up values of a wave's patch, row block by row block (16 rows) through its share of the LDS that the product is done with: as many
+// blocks as that holds are under way at once. Rows of LDS hold 16-byte chunk c of row r at c ^ swz(r): a read of a column block touches
+// every bank once. (Read straight into registers, a block at a time: 1864 us where this takes 1780, with the activation in one form.)
+template <typename Tile, bool INTERLEAVED>
+struct GateUpLoads {
+    static constexpr int F = Tile::F, kBlockBytes = Tile::kPatch * 64, kLoads = kBlockBytes / 1024;
+    static constexpr int kSlots = Tile::kLds / 4 / kBlockBytes < F ? Tile::kLds / 4 / kBlockBytes : F;
+    static_assert(kSlots >= 1 && (kSlots - 1) * kLoads < 64);
+    // 16-byte chunks of a row of LDS: of its gate or of its up values, or of both where they alternate; rows of a load
+    static constexpr uint32_t kChunks = INTERLEAVED ? Tile::kPatch / 4 : Tile::kPatch / 8, kLoadRows = 64 / kChunks;
+    v4i srd;
+    uint32_t lds, voff, pitch, half;   // voff: the lane's place in an even load's first row; half: bytes between a row's gate and up values
+
+    __device__ __forceinline__ static uint32_t swz(uint32_t r) { return kChunks >= 16 ? r & 15u : (r / (16u / kChunks)) & (kChunks - 1); }
+    // at: the patch's first row; col: its first column of I; rows: what is left of the rows (none: everything reads as zeros)
+    __device__ __forceinline__ GateUpLoads(uint8_t* smem, const uint16_t* at, int col, int I, int rows) {
+        pitch = to_sgpr(4u * (uint32_t)I);
+        half = 2u * (uint32_t)I;
+        srd = make_srd(at, rows > 0 ? (uint32_t)rows * pitch : 0u);   // (at most 256 rows of 4 MB)
+        lds = to_sgpr((uint32_t)(uintptr_t)smem + wave_id() * (Tile::kLds / 4));
+        voff = lane_id() / kChunks * pitch + (uint32_t)col * (INTERLEAVED ? 4u : 2u);
     }
-    const int r = lane_id() & 15, q = lane_id() >> 4, row = 16 * m + r;
+    __device__ __forceinline__ void issue(int m) const {
+        const uint32_t lane = lane_id(), dst = lds + m % kSlots * kBlockBytes;
 #pragma unroll
-    for (int n = 0; n < F; ++n) {
-        const int c = col + 16 * n + 4 * q;
-        v4i in{0, 0, 0, 0};
-        if (row < rows && c < I) in = *(const v4i*)(at + 2 * (int64_t)I * row + 2 * c);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            g[n][j] = __uint_as_float((uint32_t)in[j] << 16);
-            u[n][j] = __uint_as_float((uint32_t)in[j] & 0xffff0000u);
+        for (int i = 0; i < kLoads; ++i) {   // the gate values' loads, then the up values'
+            const uint32_t k = INTERLEAVED ? i : i % (kLoads / 2);
+            const uint32_t row = k * kLoadRows + lane / kChunks;
+            const uint32_t at = voff + (16 * m + k * kLoadRows) * pitch + ((lane % kChunks) ^ swz(row)) * 16u + (!INTERLEAVED && i >= kLoads / 2 ? half : 0u);
+            dma16(srd, to_sgpr(dst + i * 1024), at, 0u);
         }
     }
-}
+    __device__ __forceinline__ void read(int m, v4f (&g)[F], v4f (&u)[F]) const {
+        const uint32_t r = lane_id() & 15, q = lane_id() >> 4, at = lds + m % kSlots * kBlockBytes + r * (kChunks * 16);
+#pragma unroll
+        for (int n = 0; n < F; ++n) {
+            if constexpr (INTERLEAVED) {
+                const v4i in = *(lds_v4i_t*)(uintptr_t)(at + ((4 * n + q) ^ swz(r)) * 16);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    g[n][j] = __uint_as_float((uint32_t)in[j] << 16);
+                    u[n][j] = __uint_as_float((uint32_t)in[j] & 0xffff0000u);
+                }
+            } else {
+                const uint32_t p = at + ((2 * n + (q >> 1)) ^ swz(r)) * 16 + (q & 1) * 8;
+                const v2i a = *(lds_v2i_t*)(uintptr_t)p, b = *(lds_v2i_t*)(uintptr_t)(p + kBlockBytes / 2);
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    g[n][2 * j] = __uint_as_float((uint32_t)a[j] << 16);
+                    g[n][2 * j + 1] = __uint_as_float((uint32_t)a[j] & 0xffff0000u);
+                    u[n][2 * j] = __uint_as_float((uint32_t)b[j] << 16);
+                    u[n][2 * j + 1] = __uint_as_float((uint32_t)b[j] & 0xffff0000u);
+                }
+            }
+        }
+    }
+};
 
 // A tile of kTile rows takes kTile / 2 columns of h.
-template <typename Tile>
+template <typename Tile, bool CLAMPED, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void gated_gemm_kernel(GatedForward p) {
     extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
     const GroupedTile t = grouped_tile(p.offsets, p.E, p.R, Tile::kTile, p.tiles_n, p.K, 2 * p.I, xcd_chunk_order(blockIdx.x, gridDim.x, kCuPerXcd));
@@ -96,7 +144,8 @@ __global__ __launch_bounds__(256) void gated_gemm_kernel(GatedForward p) {
     v4f acc[Tile::F][Tile::F];
     Tile::template product<kAlong, kPairs>(
         smem, operand_along(p.x, pitch, t.row0, t.row0 + t.rows, p.K),
-        operand_pairs(w, w + (p.interleaved ? (size_t)p.K : (size_t)p.I * p.K), p.interleaved ? 2 * pitch : pitch, col0, p.I, p.K), p.K, acc);
+        operand_pairs(w, w + (INTERLEAVED ? (size_t)p.K : (size_t)p.I * p.K), INTERLEAVED ? 2 * pitch : pitch, col0, p.I, p.K), p.K, acc);
+    const Gate<CLAMPED> gate{p.gate};
     constexpr int B = Tile::F / 2;   // blocks of 16 columns of h
     const int wv = wave_id(), row = (wv >> 1) * Tile::kPatch, col = col0 + (wv & 1) * (Tile::kPatch / 2), rows = t.rows - row;
     const size_t first = (size_t)(t.row0 + row);
@@ -109,10 +158,10 @@ __global__ __launch_bounds__(256) void gated_gemm_kernel(GatedForward p) {
             g[n] = v[2 * n];
             u[n] = v[2 * n + 1];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) h[n][j] = p.gate.value(g[n][j], u[n][j]);
+            for (int j = 0; j < 4; ++j) h[n][j] = gate.value(g[n][j], u[n][j]);
         }
         store_block_row(h, m, p.h + first * p.I + col, p.I, rows, p.I - col);
-        if (p.gate_up) store_gate_up(g, u, m, p.gate_up + first * 2 * p.I, col, p.I, p.interleaved, rows);
+        if (p.gate_up) store_gate_up<INTERLEAVED>(g, u, m, p.gate_up + first * 2 * p.I, col, p.I, rows);
         slot_fence();
     }
 }
@@ -135,7 +184,7 @@ struct GatedSkinnyOut {
     __device__ __forceinline__ void store(int row, int c, const v4f& g, const v4f& u) const {
         float h[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) h[j] = p.gate.value(g[j], u[j]);
+        for (int j = 0; j < 4; ++j) h[j] = p.clamped ? Gate<true>{p.gate}.value(g[j], u[j]) : Gate<false>{p.gate}.value(g[j], u[j]);
         *(v2i*)(p.h + (size_t)row * p.I + c) = v2i{(int)pack_bf16(h[0], h[1]), (int)pack_bf16(h[2], h[3])};
         if (!p.gate_up) return;
         uint16_t* at = p.gate_up + (size_t)row * 2 * p.I;
@@ -159,11 +208,11 @@ struct GatedBackward {
     const int32_t* offsets;
     const uint16_t* gate_up;
     uint16_t *dgate_up, *h;   // dgate_up may be gate_up; h null: not wanted
-    int R, E, N, I, tiles_n, interleaved;
-    Gate gate;
+    int R, E, N, I, tiles_n, interleaved, clamped;
+    GateArgs gate;
 };
 
-template <typename Tile>
+template <typename Tile, bool CLAMPED, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void gated_dgrad_kernel(GatedBackward p) {
     extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
     const GroupedTile t = grouped_tile(p.offsets, p.E, p.R, Tile::kTile, p.tiles_n, p.N, p.I, xcd_chunk_order(blockIdx.x, gridDim.x, kCuPerXcd));
@@ -174,35 +223,45 @@ __global__ __launch_bounds__(256) void gated_dgrad_kernel(GatedBackward p) {
                                             operand_across(p.w2 + (size_t)t.expert * p.N * p.I, 2ull * p.I, col0, p.N), p.N, acc);
     const int w = wave_id(), row = (w >> 1) * Tile::kPatch, col = col0 + (w & 1) * Tile::kPatch, rows = t.rows - row;
     const size_t first = (size_t)(t.row0 + row);
+    block_barrier();   // everyone is done with the product's LDS
+    typedef GateUpLoads<Tile, INTERLEAVED> Loads;
+    const Loads kept(smem, p.gate_up + first * 2 * p.I, col, p.I, rows);
+    const Gate<CLAMPED> gate{p.gate};
 #pragma unroll
-    for (int m = 0; m < Tile::F; ++m) {
+    for (int m = 0; m < Loads::kSlots; ++m) kept.issue(m);
+    auto block = [&]<int m>() __attribute__((always_inline)) {
         v4f dh[Tile::F], g[Tile::F], u[Tile::F], dg[Tile::F], du[Tile::F];
-        load_gate_up(g, u, m, p.gate_up + first * 2 * p.I, col, p.I, p.interleaved, rows);
+        // the block has landed: no more is under way than the loads issued behind its own (stores in between only make this wait longer)
+        constexpr int last = m + Loads::kSlots < Tile::F ? m + Loads::kSlots : Tile::F;
+        wait_vmcnt<(last - 1 - m) * Loads::kLoads>();
+        kept.read(m, g, u);
+        if constexpr (m + Loads::kSlots < Tile::F) {
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // ... and has been read
+            kept.issue(m + Loads::kSlots);
+        }
         Tile::read_row(acc[m], dh);
 #pragma unroll
         for (int n = 0; n < Tile::F; ++n)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float a, b;
-                dh[n][j] = p.gate.gradients(g[n][j], u[n][j], dh[n][j], a, b);
+                dh[n][j] = gate.gradients(g[n][j], u[n][j], dh[n][j], a, b);
                 dg[n][j] = a;
                 du[n][j] = b;
             }
-        store_gate_up(dg, du, m, p.dgate_up + first * 2 * p.I, col, p.I, p.interleaved, rows);
+        store_gate_up<INTERLEAVED>(dg, du, m, p.dgate_up + first * 2 * p.I, col, p.I, rows);
         if (p.h) store_block_row(dh, m, p.h + first * p.I + col, p.I, rows, p.I - col);
         slot_fence();
-    }
+    };
+    [&]<int... m>(std::integer_sequence<int, m...>) __attribute__((always_inline)) {
+        (block.template operator()<m>(), ...);
+    }(std::make_integer_sequence<int, Tile::F>());
 }
 
-// alpha, limit of the clamped form (1); SiLU (0) has its own
-static int make_gate(int activation, float alpha, float limit, Gate& g) {
-    if (activation == 0) {
-        g = Gate{1.0f, __builtin_inff(), 0.0f};
-        return HK_OK;
-    }
-    if (activation != 1 || !(limit > 0.f) || !(__builtin_fabsf(alpha) < __builtin_inff())) return HK_ERR_UNSUPPORTED;
-    g = Gate{alpha, limit, 1.0f};
-    return HK_OK;
+// alpha and limit of the clamped form (1); SiLU (0) has none
+static int check_gate(int activation, const GateArgs& g) {
+    if (activation == 0) return HK_OK;
+    return activation == 1 && g.limit > 0.f && __builtin_fabsf(g.alpha) < __builtin_inff() ? HK_OK : HK_ERR_UNSUPPORTED;
 }
 
 // wide: the length of the rows that are not I or 2 I
@@ -222,15 +281,20 @@ static int launch_gated_tile(void (*kern)(P), DeviceOnce& once, P p, int out, hi
     hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), Tile::kLds, s, p);
     return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
 }
-template <typename Tile>
+template <typename Tile, bool CLAMPED, bool INTERLEAVED>
 static int launch_gated(const GatedForward& p, hipStream_t s) {
     static DeviceOnce once;
-    return launch_gated_tile<Tile>(gated_gemm_kernel<Tile>, once, p, 2 * p.I, s);
+    return launch_gated_tile<Tile>(gated_gemm_kernel<Tile, CLAMPED, INTERLEAVED>, once, p, 2 * p.I, s);
 }
-template <typename Tile>
+template <typename Tile, bool CLAMPED, bool INTERLEAVED>
 static int launch_gated(const GatedBackward& p, hipStream_t s) {
     static DeviceOnce once;
-    return launch_gated_tile<Tile>(gated_dgrad_kernel<Tile>, once, p, p.I, s);
+    return launch_gated_tile<Tile>(gated_dgrad_kernel<Tile, CLAMPED, INTERLEAVED>, once, p, p.I, s);
+}
+template <typename Tile, typename P>
+static int launch_gated_form(const P& p, hipStream_t s) {
+    if (p.clamped) return p.interleaved ? launch_gated<Tile, true, true>(p, s) : launch_gated<Tile, true, false>(p, s);
+    return p.interleaved ? launch_gated<Tile, false, true>(p, s) : launch_gated<Tile, false, false>(p, s);
 }
 template <int R, int NW, int D, int NF, bool NT>
 static int launch_gated_skinny_kernel(const GatedForward& p, hipStream_t s) {
@@ -275,10 +339,10 @@ static int launch_gated_skinny(const GatedForward& p, hipStream_t s) {
 template <typename P>
 static int launch_gated_choice(const P& p, int in, int out, hipStream_t s) {
     switch (grouped_choice(p.R, p.E, in, out, !p.offsets)) {
-        case kLayout256: return launch_gated<LayoutTile256>(p, s);
-        case kLayout128: return launch_gated<LayoutTile128>(p, s);
-        case kLayout128Deep: return launch_gated<LayoutTile128Deep>(p, s);
-        default: return launch_gated<LayoutTile64Deep>(p, s);
+        case kLayout256: return launch_gated_form<LayoutTile256>(p, s);
+        case kLayout128: return launch_gated_form<LayoutTile128>(p, s);
+        case kLayout128Deep: return launch_gated_form<LayoutTile128Deep>(p, s);
+        default: return launch_gated_form<LayoutTile64Deep>(p, s);
     }
 }
 
@@ -292,8 +356,8 @@ extern "C" int hk_gated_gemm(const void* x_bf16, const void* w13_bf16, const int
     if (const int st = gated_check(R, E, I, K, expert_offsets_or_null)) return st;
     if (((uintptr_t)x_bf16 | (uintptr_t)w13_bf16 | (uintptr_t)h_bf16 | (uintptr_t)gate_up_bf16_or_null) & 15u) return HK_ERR_BAD_ALIGNMENT;
     GatedForward p{(const uint16_t*)x_bf16, (const uint16_t*)w13_bf16, expert_offsets_or_null, (uint16_t*)h_bf16, (uint16_t*)gate_up_bf16_or_null,
-                   R, E, I, K, 0, interleaved != 0, {}};
-    if (const int st = make_gate(activation, alpha, limit, p.gate)) return st;
+                   R, E, I, K, 0, interleaved != 0, activation == 1, {alpha, limit}};
+    if (const int st = check_gate(activation, p.gate)) return st;
     if (!p.offsets && use_gated_skinny(R, I, K)) return launch_gated_skinny(p, (hipStream_t)stream);
     return launch_gated_choice(p, K, 2 * I, (hipStream_t)stream);
 }
@@ -307,7 +371,7 @@ extern "C" int hk_gated_gemm_dgrad(const void* dy_bf16, const void* w2_bf16, con
     if (((uintptr_t)dy_bf16 | (uintptr_t)w2_bf16 | (uintptr_t)gate_up_bf16 | (uintptr_t)dgate_up_bf16 | (uintptr_t)h_bf16_or_null) & 15u)
         return HK_ERR_BAD_ALIGNMENT;
     GatedBackward p{(const uint16_t*)dy_bf16, (const uint16_t*)w2_bf16, expert_offsets_or_null, (const uint16_t*)gate_up_bf16,
-                    (uint16_t*)dgate_up_bf16, (uint16_t*)h_bf16_or_null, R, E, N, I, 0, interleaved != 0, {}};
-    if (const int st = make_gate(activation, alpha, limit, p.gate)) return st;
+                    (uint16_t*)dgate_up_bf16, (uint16_t*)h_bf16_or_null, R, E, N, I, 0, interleaved != 0, activation == 1, {alpha, limit}};
+    if (const int st = check_gate(activation, p.gate)) return st;
     return launch_gated_choice(p, N, I, (hipStream_t)stream);
 }
