@@ -57,23 +57,83 @@ struct GatedForward {
     GateArgs gate;
 };
 
-// One row of blocks of gate and up values (or their gradients) to gate_up: `at` the patch's first row, `col` its first column of I.
-template <bool INTERLEAVED, int F>
-__device__ __forceinline__ void store_gate_up(const v4f (&g)[F], const v4f (&u)[F], int m, uint16_t* at, int col, int I, int rows) {
-    if constexpr (!INTERLEAVED) {
-        store_block_row(g, m, at + col, 2 * (int64_t)I, rows, I - col);
-        store_block_row(u, m, at + I + col, 2 * (int64_t)I, rows, I - col);
-        return;
-    }
-    const int r = lane_id() & 15, q = lane_id() >> 4, row = 16 * m + r;
+// Stores of a wave's patch into rows of bf16, sixteen rows at a time, through a buffer descriptor that ends behind the last row (its range
+// check takes the scalar offset, which holds the row block, with it): a lane has one offset for each piece of 16 bytes, out of range where the row
+// ends in front of it, and a store is one instruction. (Through pointers, a test and an address for each, a sixth of the backward kernel's
+// epilogue were those.) Written as statements of their own: behind a store of 16 bytes with a scalar offset its data may not be overwritten for
+// two wait states, which the compiler does not keep here.
+constexpr uint32_t kOutside = 0x80000000u;
+template <int PIECES>
+struct PatchRows {
+    v4i srd;
+    uint32_t pitch, at[PIECES];
+    // first: the patch's first row; rows: what is left of them; column(i): the first column of the lane's piece i, of `cols` columns of `bytes` bytes
+    template <typename C>
+    __device__ __forceinline__ PatchRows(uint16_t* first, uint32_t pitch_bytes, int rows, int cols, uint32_t bytes, C&& column) {
+        pitch = to_sgpr(pitch_bytes);
+        srd = make_srd(first, rows > 0 ? (uint32_t)min(rows, kRingTile) * pitch_bytes : 0u);   // (at most 256 rows of 4 MB)
 #pragma unroll
-    for (int n = 0; n < F; ++n) {
-        const int c = col + 16 * n + 4 * q;
-        if (row < rows && c < I)
-            *(v4i*)(at + 2 * (int64_t)I * row + 2 * c) = v4i{(int)pack_bf16(g[n].x, u[n].x), (int)pack_bf16(g[n].y, u[n].y),
-                                                             (int)pack_bf16(g[n].z, u[n].z), (int)pack_bf16(g[n].w, u[n].w)};
+        for (int i = 0; i < PIECES; ++i) {
+            const int c = column(i);
+            at[i] = c < cols ? (lane_id() & 15) * pitch_bytes + (uint32_t)c * bytes : kOutside;
+        }
     }
-}
+    __device__ __forceinline__ void store(v4i v, int i, int m, uint32_t more = 0) const {
+        asm volatile("buffer_store_dwordx4 %0, %1, %2, %3 offen\n\ts_nop 1" ::"v"(v), "v"(at[i]), "s"(srd), "s"(to_sgpr(16 * m * pitch + more)) : "memory");
+    }
+    __device__ __forceinline__ void store(v2i v, int i, int m, uint32_t more = 0) const {
+        asm volatile("buffer_store_dwordx2 %0, %1, %2, %3 offen" ::"v"(v), "v"(at[i]), "s"(srd), "s"(to_sgpr(16 * m * pitch + more)) : "memory");
+    }
+};
+// One matrix of F column blocks, in store_block_row's places.
+template <int F>
+struct PatchMatrix {
+    PatchRows<(F + 1) / 2> rows;
+    __device__ __forceinline__ PatchMatrix(uint16_t* first, uint32_t pitch_bytes, int n, int col, int cols)
+        : rows(first, pitch_bytes, n, cols, 2, [&](int i) {
+              const int q = lane_id() >> 4;
+              return col + 32 * i + (2 * i + 1 < F ? 8 * (q >> 1) + 16 * (q & 1) : 4 * q);
+          }) {}
+    // more: bytes from the matrix's columns to those that are written
+    __device__ __forceinline__ void store(const v4f (&v)[F], int m, uint32_t more = 0) const {
+#pragma unroll
+        for (int i = 0; i < F / 2; ++i) {
+            v4i out;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const v4f a = v[2 * i], b = v[2 * i + 1];
+                const auto s = __builtin_amdgcn_permlane16_swap(pack_bf16(a[2 * h], a[2 * h + 1]), pack_bf16(b[2 * h], b[2 * h + 1]), false, false);
+                out[h] = (int)s[0];
+                out[2 + h] = (int)s[1];
+            }
+            rows.store(out, i, m, more);
+        }
+        if constexpr (F % 2 == 1) rows.store(v2i{(int)pack_bf16(v[F - 1].x, v[F - 1].y), (int)pack_bf16(v[F - 1].z, v[F - 1].w)}, F / 2, m, more);
+    }
+};
+// Gate and up values, or their gradients: the one's columns behind the other's, or alternating.
+template <int F, bool INTERLEAVED>
+struct PatchPairs {
+    PatchMatrix<F> rows;
+    uint32_t half;
+    __device__ __forceinline__ PatchPairs(uint16_t* first, int n, int col, int I) : rows(first, 4u * I, n, col, I), half(to_sgpr(2u * I)) {}
+    __device__ __forceinline__ void store(const v4f (&g)[F], const v4f (&u)[F], int m) const {
+        rows.store(g, m);
+        rows.store(u, m, half);
+    }
+};
+template <int F>
+struct PatchPairs<F, true> {
+    PatchRows<F> rows;
+    __device__ __forceinline__ PatchPairs(uint16_t* first, int n, int col, int I)
+        : rows(first, 4u * I, n, I, 4, [&](int i) { return col + 16 * i + 4 * (lane_id() >> 4); }) {}
+    __device__ __forceinline__ void store(const v4f (&g)[F], const v4f (&u)[F], int m) const {
+#pragma unroll
+        for (int n = 0; n < F; ++n)
+            rows.store(v4i{(int)pack_bf16(g[n].x, u[n].x), (int)pack_bf16(g[n].y, u[n].y), (int)pack_bf16(g[n].z, u[n].z), (int)pack_bf16(g[n].w, u[n].w)}, n, m);
+    }
+};
+
 // The kept gate and up values of a wave's patch, row block by row block (16 rows) through its share of the LDS that the product is done with: as many
 // blocks as that holds are under way at once. Rows of LDS hold 16-byte chunk c of row r at c ^ swz(r): a read of a column block touches
 // every bank once. (Read straight into registers, a block at a time: 1864 us where this takes 1780, with the activation in one form.)
@@ -149,6 +209,8 @@ __global__ __launch_bounds__(256) void gated_gemm_kernel(GatedForward p) {
     constexpr int B = Tile::F / 2;   // blocks of 16 columns of h
     const int wv = wave_id(), row = (wv >> 1) * Tile::kPatch, col = col0 + (wv & 1) * (Tile::kPatch / 2), rows = t.rows - row;
     const size_t first = (size_t)(t.row0 + row);
+    const PatchMatrix<B> out(p.h + first * p.I, 2u * p.I, rows, col, p.I);
+    const PatchPairs<B, INTERLEAVED> pairs(p.gate_up + first * 2 * p.I, p.gate_up ? rows : 0, col, p.I);
 #pragma unroll
     for (int m = 0; m < Tile::F; ++m) {
         v4f v[Tile::F], g[B], u[B], h[B];
@@ -160,8 +222,8 @@ __global__ __launch_bounds__(256) void gated_gemm_kernel(GatedForward p) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) h[n][j] = gate.value(g[n][j], u[n][j]);
         }
-        store_block_row(h, m, p.h + first * p.I + col, p.I, rows, p.I - col);
-        if (p.gate_up) store_gate_up<INTERLEAVED>(g, u, m, p.gate_up + first * 2 * p.I, col, p.I, rows);
+        out.store(h, m);
+        if (p.gate_up) pairs.store(g, u, m);
         slot_fence();
     }
 }
@@ -227,6 +289,8 @@ __global__ __launch_bounds__(256) void gated_dgrad_kernel(GatedBackward p) {
     typedef GateUpLoads<Tile, INTERLEAVED> Loads;
     const Loads kept(smem, p.gate_up + first * 2 * p.I, col, p.I, rows);
     const Gate<CLAMPED> gate{p.gate};
+    const PatchMatrix<Tile::F> out(p.h + first * p.I, 2u * p.I, p.h ? rows : 0, col, p.I);
+    const PatchPairs<Tile::F, INTERLEAVED> pairs(p.dgate_up + first * 2 * p.I, rows, col, p.I);
 #pragma unroll
     for (int m = 0; m < Loads::kSlots; ++m) kept.issue(m);
     auto block = [&]<int m>() __attribute__((always_inline)) {
@@ -249,8 +313,8 @@ __global__ __launch_bounds__(256) void gated_dgrad_kernel(GatedBackward p) {
                 dg[n][j] = a;
                 du[n][j] = b;
             }
-        store_gate_up<INTERLEAVED>(dg, du, m, p.dgate_up + first * 2 * p.I, col, p.I, rows);
-        if (p.h) store_block_row(dh, m, p.h + first * p.I + col, p.I, rows, p.I - col);
+        pairs.store(dg, du, m);
+        if (p.h) out.store(dh, m);
         slot_fence();
     };
     [&]<int... m>(std::integer_sequence<int, m...>) __attribute__((always_inline)) {
