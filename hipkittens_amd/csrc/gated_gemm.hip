@@ -11,6 +11,8 @@
 // fp32 accumulation and activation, one rounding. The products are those of gemm_layouts_ring.h, which bound both kernels; in the forward one
 // every 32 rows of the weight tile in LDS are 16 gate rows and the 16 up rows of the same columns (kPairs), so that both values of
 // an element are in one lane's accumulators and the activation needs no exchange between lanes.
+#include <algorithm>
+#include <type_traits>
 #include <utility>
 
 #include "gemm_skinny.h"
@@ -139,11 +141,11 @@ struct PatchPairs<F, true> {
 // every bank once. (Read straight into registers, a block at a time: 1864 us where this takes 1780, with the activation in one form.)
 template <typename Tile, bool INTERLEAVED>
 struct GateUpLoads {
-    static constexpr int F = Tile::F, kBlockBytes = Tile::kPatch * 64, kLoads = kBlockBytes / 1024;
-    static constexpr int kSlots = Tile::kLds / 4 / kBlockBytes < F ? Tile::kLds / 4 / kBlockBytes : F;
+    static constexpr int F = Tile::FC, kBlocks = Tile::F, kBlockBytes = Tile::kPatchCols * 64, kLoads = kBlockBytes / 1024;
+    static constexpr int kSlots = Tile::kLds / 4 / kBlockBytes < kBlocks ? Tile::kLds / 4 / kBlockBytes : kBlocks;
     static_assert(kSlots >= 1 && (kSlots - 1) * kLoads < 64);
     // 16-byte chunks of a row of LDS: of its gate or of its up values, or of both where they alternate; rows of a load
-    static constexpr uint32_t kChunks = INTERLEAVED ? Tile::kPatch / 4 : Tile::kPatch / 8, kLoadRows = 64 / kChunks;
+    static constexpr uint32_t kChunks = INTERLEAVED ? Tile::kPatchCols / 4 : Tile::kPatchCols / 8, kLoadRows = 64 / kChunks;
     v4i srd;
     uint32_t lds, voff, pitch, half;   // voff: the lane's place in an even load's first row; half: bytes between a row's gate and up values
 
@@ -192,28 +194,28 @@ struct GateUpLoads {
     }
 };
 
-// A tile of kTile rows takes kTile / 2 columns of h.
+// A tile takes kTileCols / 2 columns of h.
 template <typename Tile, bool CLAMPED, bool INTERLEAVED>
 __global__ __launch_bounds__(256) void gated_gemm_kernel(GatedForward p) {
     extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
     const GroupedTile t = grouped_tile(p.offsets, p.E, p.R, Tile::kTile, p.tiles_n, p.K, 2 * p.I, xcd_chunk_order(blockIdx.x, gridDim.x, kCuPerXcd));
     if (t.expert < 0) return;
-    const int col0 = t.tile_n * (Tile::kTile / 2);
+    const int col0 = t.tile_n * (Tile::kTileCols / 2);
     const uint16_t* w = p.w13 + (size_t)t.expert * 2 * p.I * p.K;
     const size_t pitch = 2ull * p.K;   // bytes
-    v4f acc[Tile::F][Tile::F];
+    v4f acc[Tile::F][Tile::FC];
     Tile::template product<kAlong, kPairs>(
         smem, operand_along(p.x, pitch, t.row0, t.row0 + t.rows, p.K),
         operand_pairs(w, w + (INTERLEAVED ? (size_t)p.K : (size_t)p.I * p.K), INTERLEAVED ? 2 * pitch : pitch, col0, p.I, p.K), p.K, acc);
     const Gate<CLAMPED> gate{p.gate};
-    constexpr int B = Tile::F / 2;   // blocks of 16 columns of h
-    const int wv = wave_id(), row = (wv >> 1) * Tile::kPatch, col = col0 + (wv & 1) * (Tile::kPatch / 2), rows = t.rows - row;
+    constexpr int B = Tile::FC / 2;   // blocks of 16 columns of h
+    const int wv = wave_id(), row = (wv >> 1) * Tile::kPatch, col = col0 + (wv & 1) * (Tile::kPatchCols / 2), rows = t.rows - row;
     const size_t first = (size_t)(t.row0 + row);
     const PatchMatrix<B> out(p.h + first * p.I, 2u * p.I, rows, col, p.I);
     const PatchPairs<B, INTERLEAVED> pairs(p.gate_up + first * 2 * p.I, p.gate_up ? rows : 0, col, p.I);
 #pragma unroll
     for (int m = 0; m < Tile::F; ++m) {
-        v4f v[Tile::F], g[B], u[B], h[B];
+        v4f v[Tile::FC], g[B], u[B], h[B];
         Tile::read_row(acc[m], v);
 #pragma unroll
         for (int n = 0; n < B; ++n) {
@@ -279,22 +281,22 @@ __global__ __launch_bounds__(256) void gated_dgrad_kernel(GatedBackward p) {
     extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
     const GroupedTile t = grouped_tile(p.offsets, p.E, p.R, Tile::kTile, p.tiles_n, p.N, p.I, xcd_chunk_order(blockIdx.x, gridDim.x, kCuPerXcd));
     if (t.expert < 0) return;
-    const int col0 = t.tile_n * Tile::kTile;
-    v4f acc[Tile::F][Tile::F];
+    const int col0 = t.tile_n * Tile::kTileCols;
+    v4f acc[Tile::F][Tile::FC];
     Tile::template product<kAlong, kAcross>(smem, operand_along(p.dy, 2ull * p.N, t.row0, t.row0 + t.rows, p.N),
                                             operand_across(p.w2 + (size_t)t.expert * p.N * p.I, 2ull * p.I, col0, p.N), p.N, acc);
-    const int w = wave_id(), row = (w >> 1) * Tile::kPatch, col = col0 + (w & 1) * Tile::kPatch, rows = t.rows - row;
+    const int w = wave_id(), row = (w >> 1) * Tile::kPatch, col = col0 + (w & 1) * Tile::kPatchCols, rows = t.rows - row;
     const size_t first = (size_t)(t.row0 + row);
     block_barrier();   // everyone is done with the product's LDS
     typedef GateUpLoads<Tile, INTERLEAVED> Loads;
     const Loads kept(smem, p.gate_up + first * 2 * p.I, col, p.I, rows);
     const Gate<CLAMPED> gate{p.gate};
-    const PatchMatrix<Tile::F> out(p.h + first * p.I, 2u * p.I, p.h ? rows : 0, col, p.I);
-    const PatchPairs<Tile::F, INTERLEAVED> pairs(p.dgate_up + first * 2 * p.I, rows, col, p.I);
+    const PatchMatrix<Tile::FC> out(p.h + first * p.I, 2u * p.I, p.h ? rows : 0, col, p.I);
+    const PatchPairs<Tile::FC, INTERLEAVED> pairs(p.dgate_up + first * 2 * p.I, rows, col, p.I);
 #pragma unroll
     for (int m = 0; m < Loads::kSlots; ++m) kept.issue(m);
     auto block = [&]<int m>() __attribute__((always_inline)) {
-        v4f dh[Tile::F], g[Tile::F], u[Tile::F], dg[Tile::F], du[Tile::F];
+        v4f dh[Tile::FC], g[Tile::FC], u[Tile::FC], dg[Tile::FC], du[Tile::FC];
         // the block has landed: no more is under way than the loads issued behind its own (stores in between only make this wait longer)
         constexpr int last = m + Loads::kSlots < Tile::F ? m + Loads::kSlots : Tile::F;
         wait_vmcnt<(last - 1 - m) * Loads::kLoads>();
@@ -305,7 +307,7 @@ __global__ __launch_bounds__(256) void gated_dgrad_kernel(GatedBackward p) {
         }
         Tile::read_row(acc[m], dh);
 #pragma unroll
-        for (int n = 0; n < Tile::F; ++n)
+        for (int n = 0; n < Tile::FC; ++n)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float a, b;
@@ -338,7 +340,7 @@ static int gated_check(int R, int E, int I, int wide, const int32_t* offsets) {
 
 template <typename Tile, typename P>
 static int launch_gated_tile(void (*kern)(P), DeviceOnce& once, P p, int out, hipStream_t s) {
-    p.tiles_n = (out + Tile::kTile - 1) / Tile::kTile;
+    p.tiles_n = (out + Tile::kTileCols - 1) / Tile::kTileCols;
     const long long grid = grouped_tiles_m(p.R, p.E, Tile::kTile) * p.tiles_n;
     if (grid >= kMaxWorkgroups) return HK_ERR_BAD_SHAPE;
     if (!set_lds_limit_once((const void*)kern, Tile::kLds, once)) return HK_ERR_LAUNCH;
@@ -400,8 +402,28 @@ static int launch_gated_skinny(const GatedForward& p, hipStream_t s) {
     if (p.R <= 48) return launch_gated_skinny_rows<3, 4, 4>(p, s);
     return launch_gated_skinny_rows<4, 3, 3>(p, s);
 }
+// Whether the forward product over experts' rows takes tiles of 128 rows and 256 columns: by rounds over the CUs times a fixed part and a part per
+// K-step, us, with the tiles of rows that an expert has on average (a round begun counts whole between one and two), where there are tiles enough
+// that no kernel with many LDS stages is taken. (us, 128x128 or 256x256, whichever was chosen / 128x256: 128 experts of 2880 x 2880, 64 rows
+// each 870 / 841, 128 rows 1008 / 990, 192 1148 / 1251; 32 of 2048 x 7168, 128 rows 492 / 425; 64 of 1536 x 4096, 150 rows 435 / 386; 8 of 4096 x
+// 4096, 128 rows 203 / 158; the rule's worst, 64 of 768 x 2048, 128 rows 131 / 141. Not in the backward pass, whose epilogue is the longer.)
+static bool use_wide_tile(const GatedForward& p) {
+    if (!p.offsets) return false;
+    const int cus = moe_num_compute_units(), out = 2 * p.I;
+    const LayoutChoice other = grouped_choice(p.R, p.E, p.K, out);
+    if (other == kLayout64Deep || other == kLayout128Deep) return false;
+    const double used = p.R < p.E ? p.R : p.E, mean = p.R / used, steps = (p.K + kLayoutStep - 1) / kLayoutStep;
+    auto tiles_m = [&](int tile) { return used * std::max(1.0, mean / tile + 0.7); };
+    auto rounds = [](double t) { return t <= 1 ? 1.0 : std::max(t + 0.2, std::min(2.0, t + 0.65)); };
+    const double cols = (out + 255) / 256, wide = rounds(tiles_m(128) * cols / cus) * (6.0 + 0.92 * steps);
+    const double small = rounds(tiles_m(128) * ((out + 127) / 128) / (2.0 * cus)) * (kSmallFixed + kSmallStepAlong * steps);
+    return wide < small && wide < rounds(tiles_m(256) * cols / cus) * (kLargeFixed + kLargeStep * steps);
+}
+
 template <typename P>
 static int launch_gated_choice(const P& p, int in, int out, hipStream_t s) {
+    if constexpr (std::is_same_v<P, GatedForward>)
+        if (use_wide_tile(p)) return launch_gated_form<LayoutTileWide>(p, s);
     switch (grouped_choice(p.R, p.E, in, out, !p.offsets)) {
         case kLayout256: return launch_gated_form<LayoutTile256>(p, s);
         case kLayout128: return launch_gated_form<LayoutTile128>(p, s);

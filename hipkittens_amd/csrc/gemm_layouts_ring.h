@@ -358,6 +358,115 @@ __device__ __forceinline__ void deep_product(uint8_t* smem, const TileOperand& A
     mfma_drain_agpr(acc);
 }
 
+// 128x256 tiles in the same manner with three LDS stages: for experts with rows for half a 256x256 tile, whose other half's products would be
+// empty. A wave has 64 rows and 128 columns. A K-step is 64 matrix instructions a wave, behind the first 24 of which it reads the next
+// K-step's fragments, then issues its twelve loads of the K-step after the next two, one behind every third.
+constexpr int kWideRows = 128, kWideCols = 256, kWideStages = 3, kWideStage = (kWideRows + kWideCols) * 128;
+template <int A_ORDER, int B_ORDER>
+__device__ __forceinline__ void wide_product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K, v4f (&acc)[4][8]) {
+    constexpr int FA = 4, FB = 8, kLoads = FA + FB;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)smem, w = wave_id();
+    const uint32_t mine = to_sgpr(lds0 + w * 1024u);
+    RingOperand<A_ORDER, kWideRows> oa;
+    RingOperand<B_ORDER, kWideCols> ob;
+    oa.init(A, K, w >> 1, lds0);
+    ob.init(B, K, w & 1, lds0 + kWideRows * 128);
+    const int nk = (K + kLayoutStep - 1) / kLayoutStep;
+    const uint32_t step_a = A_ORDER == kAcross ? to_sgpr(kLayoutStep * A.pitch) : 128u, step_b = B_ORDER == kAcross ? to_sgpr(kLayoutStep * B.pitch) : 128u;
+#pragma unroll
+    for (int m = 0; m < FA; ++m)
+#pragma unroll
+        for (int n = 0; n < FB; ++n) acc[m][n] = v4f{0.f, 0.f, 0.f, 0.f};
+    struct Frag { v4i lo, hi; };
+    Frag af[2][FA], bf[2][FB];
+    v4i da, db;
+    uint32_t vor_a = 0, vor_b = 0, rows_a = 0, rows_b = 0;
+    auto next_step = [&](int kt) __attribute__((always_inline)) {   // the descriptors' K-step
+        da = oa.srd(kt < nk);
+        db = ob.srd(kt < nk);
+        vor_a = kt == nk - 1 ? oa.tail_or : 0u;
+        vor_b = kt == nk - 1 ? ob.tail_or : 0u;
+        rows_a = oa.opaque(oa.round);
+        rows_b = ob.opaque(ob.round);
+        oa.advance(step_a);
+        ob.advance(step_b);
+    };
+    auto load = [&](int i, uint32_t stage) __attribute__((always_inline)) {   // B's loads of a K-step, then A's
+        auto one = [&]<int I>() __attribute__((always_inline)) {
+            if constexpr (I < FB) ob.template load<I, kWideRows * 128>(mine + stage, db, vor_b, rows_b);
+            else oa.template load<I - FB>(mine + stage, da, vor_a, rows_a);
+        };
+        switch (i) {
+            case 0: one.template operator()<0>(); break;
+            case 1: one.template operator()<1>(); break;
+            case 2: one.template operator()<2>(); break;
+            case 3: one.template operator()<3>(); break;
+            case 4: one.template operator()<4>(); break;
+            case 5: one.template operator()<5>(); break;
+            case 6: one.template operator()<6>(); break;
+            case 7: one.template operator()<7>(); break;
+            case 8: one.template operator()<8>(); break;
+            case 9: one.template operator()<9>(); break;
+            case 10: one.template operator()<10>(); break;
+            default: one.template operator()<11>(); break;
+        }
+    };
+    // half u (0 .. 23) of a K-step's fragments into register set Q: B's, then A's
+    auto read = [&]<int Q>(int u, uint32_t stage) __attribute__((always_inline)) {
+        const int f = u / 2;
+        if (f < FB) {
+            if (u & 1) bf[Q][f].hi = ob.template half<1>(f, stage);
+            else bf[Q][f].lo = ob.template half<0>(f, stage);
+        } else {
+            if (u & 1) af[Q][f - FB].hi = oa.template half<1>(f - FB, stage);
+            else af[Q][f - FB].lo = oa.template half<0>(f - FB, stage);
+        }
+    };
+#pragma unroll
+    for (int p = 0; p < kWideStages; ++p) {
+        next_step(p);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) load(i, p * kWideStage);
+    }
+    wait_vmcnt<(kWideStages - 1) * kLoads>();
+    block_barrier();
+#pragma unroll
+    for (int u = 0; u < 2 * kLoads; ++u) read.template operator()<0>(u, 0u);
+    uint32_t at = 0, at1 = kWideStage;   // stages of K-steps kt and kt + 1
+    auto step = [&]<int P>(int kt) __attribute__((always_inline)) {
+        // this K-step's fragments are here, so its stage is free once everyone says so; the next K-step has landed
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        wait_vmcnt<(kWideStages - 2) * kLoads>();
+        block_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        mfma_enter_agpr(acc);
+        next_step(kt + kWideStages);
+#pragma unroll
+        for (int pass = 0; pass < 2; ++pass)
+#pragma unroll
+            for (int m = 0; m < FA; ++m)
+#pragma unroll
+                for (int n = 0; n < FB; ++n) {
+                    if (pass == 0) mfma_bf16_acc(acc[m][n], bf[P][n].lo, af[P][m].lo);
+                    else mfma_bf16_acc(acc[m][n], bf[P][n].hi, af[P][m].hi);
+                    const int q = FB * (FA * pass + m) + n;
+                    if (q < 2 * kLoads) read.template operator()<P ^ 1>(q, at1);
+                    else if ((q - 2 * kLoads) % 3 == 0 && (q - 2 * kLoads) / 3 < kLoads) load((q - 2 * kLoads) / 3, at);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+        at = at1;
+        at1 = at1 == (kWideStages - 1) * kWideStage ? 0u : at1 + kWideStage;
+    };
+    int kt = 0;
+    for (; kt + 1 < nk; kt += 2) {
+        step.template operator()<0>(kt);
+        step.template operator()<1>(kt + 1);
+    }
+    if (kt < nk) step.template operator()<0>(kt);
+    wait_vmcnt<0>();   // nothing may still be writing LDS when the workgroup retires or uses it otherwise
+    mfma_drain_agpr(acc);
+}
+
 // One 16-row block of a wave's patch (row block m, v[n]: its F column blocks) to C rows of `ldc` elements, C at the patch (rows,
 // cols: what is left of C there, cols a multiple of 8). bf16: neighbouring lane groups swap their halves of two column
 // blocks, so that a lane stores eight columns in one piece: groups 0 and 2 columns 0..7 and 8..15 of the pair's 32, groups
@@ -426,10 +535,12 @@ __device__ __forceinline__ void store_patch(const v4f (&acc)[F][F], T* __restric
 }
 
 // The two tiles as the kernels take them: product() leaves acc[F][F] of 16x16 blocks of the wave's patch, rows
-// kPatch (w / 2) and columns kPatch (w % 2) of the tile; read_row() gives an epilogue one row of blocks.
+// kPatch (w / 2) and columns kPatch (w % 2) of the tile; read_row() gives an epilogue one row of blocks. (kTileCols, kPatchCols, FC: the columns'
+// where they may differ from the rows'.)
 template <int STAGES>
 struct LayoutTile128Stages {
     static constexpr int kTile = kLayoutTile, kPatch = kTile / 2, F = 4, kLds = STAGES * kLayoutStageBytes;
+    static constexpr int kTileCols = kTile, kPatchCols = kPatch, FC = F;
     template <int A_ORDER, int B_ORDER>
     static __device__ __forceinline__ void product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K, v4f (&acc)[F][F]) {
         tile_product<A_ORDER, B_ORDER, STAGES>(smem, A, B, K, acc);
@@ -442,6 +553,7 @@ struct LayoutTile128Stages {
 typedef LayoutTile128Stages<2> LayoutTile128;
 struct LayoutTile256 {
     static constexpr int kTile = kRingTile, kPatch = kTile / 2, F = 8, kLds = kRingLdsBytes;
+    static constexpr int kTileCols = kTile, kPatchCols = kPatch, FC = F;
     template <int A_ORDER, int B_ORDER>
     static __device__ __forceinline__ void product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K, v4f (&acc)[F][F]) {
         ring_product<A_ORDER, B_ORDER>(smem, A, B, K, acc);
@@ -463,6 +575,7 @@ struct LayoutTile256 {
 template <int TILE>
 struct LayoutTileDeep {
     static constexpr int kTile = TILE, kPatch = kTile / 2, F = TILE / 32, kLds = DeepStages<TILE>::kStages * DeepStages<TILE>::kBytes;
+    static constexpr int kTileCols = kTile, kPatchCols = kPatch, FC = F;
     template <int A_ORDER, int B_ORDER>
     static __device__ __forceinline__ void product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K, v4f (&acc)[F][F]) {
         deep_product<TILE, A_ORDER, B_ORDER>(smem, A, B, K, acc);
@@ -470,6 +583,18 @@ struct LayoutTileDeep {
     static __device__ __forceinline__ void read_row(const v4f (&acc)[F], v4f (&v)[F]) {
 #pragma unroll
         for (int n = 0; n < F; ++n) v[n] = acc[n];
+    }
+};
+struct LayoutTileWide {
+    static constexpr int kTile = kWideRows, kTileCols = kWideCols, kPatch = kWideRows / 2, kPatchCols = kWideCols / 2, F = 4, FC = 8;
+    static constexpr int kLds = kWideStages * kWideStage;
+    template <int A_ORDER, int B_ORDER>
+    static __device__ __forceinline__ void product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K, v4f (&acc)[F][FC]) {
+        wide_product<A_ORDER, B_ORDER>(smem, A, B, K, acc);
+    }
+    static __device__ __forceinline__ void read_row(const v4f (&acc)[FC], v4f (&v)[FC]) {
+#pragma unroll
+        for (int n = 0; n < FC; ++n) v[n] = acc[n];
     }
 };
 typedef LayoutTileDeep<128> LayoutTile128Deep;

@@ -325,3 +325,20 @@ def test_captured_and_on_another_stream(hk):
         torch.cuda.synchronize()
         for a, b in zip(out, want):
             assert torch.equal(a.view(torch.int16), b.view(torch.int16)), i
+
+
+@pytest.mark.parametrize("act,interleaved", [("silu", False), ("silu", True), ("swiglu_oai", False), ("swiglu_oai", True)])
+def test_about_half_a_large_tile_of_rows_per_expert(hk, act, interleaved):
+    """The forward kernel of 128 rows and 256 columns: rows on both sides of its tile, columns that end in its halves, K-steps on both sides of its
+    three stages."""
+    rows = [100, 0, 64, 65, 127, 128, 129, 191, 1, 257] * 3 + [90, 110]
+    for I, K in ((1032, 1800), (1160, 1672), (2056, 840)):
+        _run(hk, rows, 5, I, K, act, interleaved, I + K, False)
+
+
+@pytest.mark.parametrize("act,interleaved", [("silu", True), ("swiglu_oai", False)])
+@pytest.mark.parametrize("R", [1, 16, 17, 32, 33, 48, 49, 64])
+def test_few_rows_of_wide_blocks(hk, R, act, interleaved):
+    """Decode: every number of row fragments, with 16, 32 and 64 rows of weights a workgroup, K that ends inside a K-step, kept values or not."""
+    for I, K, keep in ((8, 2056, True), (1032, 136, True), (4104, 1096, False), (9000, 2120, R % 2 == 0)):
+        _run(hk, [R], 0, I, K, act, interleaved, R + I, True, keep=keep)
