@@ -27,7 +27,8 @@ struct Ids {
 };
 
 // A wave takes LOADS times 64 pieces of eight columns of one token (gridDim.y: the parts of a row), all of its loads in flight together.
-template <typename T, int LOADS>
+// STREAM: the stores go past the caches.
+template <typename T, int LOADS, bool STREAM>
 __global__ __launch_bounds__(256) void embedding_kernel(Ids ids, const T* __restrict__ table, uint16_t* __restrict__ out, int tokens, int V,
                                                         int H, float scale) {
     const int64_t t = (int64_t)blockIdx.x * 4 + wave_id();
@@ -45,7 +46,9 @@ __global__ __launch_bounds__(256) void embedding_kernel(Ids ids, const T* __rest
         if (first + 64 * i >= pieces) break;
 #pragma unroll
         for (int j = 0; j < 8; ++j) r[i].v[j] = id >= 0 ? r[i].v[j] * scale : 0.f;
-        store8(out + t * H + (int64_t)(first + 64 * i) * 8, r[i]);
+        uint16_t* at = out + t * H + (int64_t)(first + 64 * i) * 8;
+        if constexpr (STREAM) __builtin_nontemporal_store(pack8(r[i]), (v4i*)at);
+        else *(v4i*)at = pack8(r[i]);
     }
 }
 
@@ -501,8 +504,11 @@ static int launch_embedding(Ids ids, const void* table, void* out, int tokens, i
     int waves = (parts64 + 7) / 8, loads = (parts64 + waves - 1) / waves;
     if ((long long)tokens * waves < 4096) loads = std::min(loads, 2);
     waves = (parts64 + loads - 1) / loads;
+    // an output of 96 MB or more would push everything else out of the memory-side cache before it is read (us: 32768 tokens of 2880 columns 60 so, with
+    // the hint 53; 65536 of 1024 43 / 27)
+    const bool stream = 2ll * tokens * H >= (96ll << 20);
     auto launch = [&]<int LOADS>() {
-        hipLaunchKernelGGL((embedding_kernel<T, LOADS>), dim3((unsigned)((tokens + 3) / 4), (unsigned)waves), dim3(256), 0, s, ids, (const T*)table,
+        hipLaunchKernelGGL((stream ? embedding_kernel<T, LOADS, true> : embedding_kernel<T, LOADS, false>), dim3((unsigned)((tokens + 3) / 4), (unsigned)waves), dim3(256), 0, s, ids, (const T*)table,
                            (uint16_t*)out, tokens, V, H, scale);
         return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
     };

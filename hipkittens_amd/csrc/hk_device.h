@@ -297,9 +297,10 @@ __device__ __forceinline__ Row8 load8(const float* p) {
     const v4f a = ((const v4f*)p)[0], b = ((const v4f*)p)[1];
     return Row8{{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w}};
 }
-__device__ __forceinline__ void store8(uint16_t* p, const Row8& r) {
-    *(v4i*)p = v4i{(int)pack_bf16(r.v[0], r.v[1]), (int)pack_bf16(r.v[2], r.v[3]), (int)pack_bf16(r.v[4], r.v[5]), (int)pack_bf16(r.v[6], r.v[7])};
+__device__ __forceinline__ v4i pack8(const Row8& r) {
+    return v4i{(int)pack_bf16(r.v[0], r.v[1]), (int)pack_bf16(r.v[2], r.v[3]), (int)pack_bf16(r.v[4], r.v[5]), (int)pack_bf16(r.v[6], r.v[7])};
 }
+__device__ __forceinline__ void store8(uint16_t* p, const Row8& r) { *(v4i*)p = pack8(r); }
 __device__ __forceinline__ void store8(float* p, const Row8& r) {
     ((v4f*)p)[0] = v4f{r.v[0], r.v[1], r.v[2], r.v[3]};
     ((v4f*)p)[1] = v4f{r.v[4], r.v[5], r.v[6], r.v[7]};

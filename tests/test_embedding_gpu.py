@@ -168,6 +168,21 @@ def test_lookup(hk, T, V, H, dtype, id_type):
     assert torch.isnan(out[:T]).all()
 
 
+def test_outputs_beyond_the_caches(hk):
+    """A lookup of more than 96 MB and gradients of a table of more than 256 MB, whose stores go past the caches."""
+    print("embedding beyond the caches", flush=True)
+    tk, T, V, H = hk.tk_kernel, 20011, 3000, 2600
+    g = torch.Generator(device=DEV).manual_seed(1)
+    ids, table = _ids("outside", T, V, g), torch.randn(V, H, device=DEV, generator=g).bfloat16()
+    out = torch.full((T + 1, H), 777.0, dtype=torch.bfloat16, device=DEV)
+    tk.dispatch_embedding(ids, table, out[:T], scale=3.0)
+    live = ((ids >= 0) & (ids < V))[:, None]
+    want = torch.where(live, table[ids.clamp(0, V - 1)].double() * 3.0, 0.0)
+    assert ((out[:T].double() - want).abs() <= want.abs() * (2**-8 + 2**-23)).all() and torch.all(out[T] == 777.0)
+    for add in ("no", "yes", "in place"):
+        _backward(hk, 5000, 40000, 2056, "frequent", torch.float32, torch.int64, add, 0.5, 9)
+
+
 def test_a_table_that_passes_32_bits(hk):
     """Rows behind 2^32 bytes of the table, in both directions (fp32: 4.4 GB)."""
     print("embedding of a large table", flush=True)
