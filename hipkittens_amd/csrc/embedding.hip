@@ -55,9 +55,10 @@ __global__ __launch_bounds__(256) void embedding_kernel(Ids ids, const T* __rest
 // ------------------------------------------------------------------------------------------------ sort
 constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64, kSortIter = 4;
 constexpr int kSortChunk = kSortThreads * kSortIter;   // tokens of a workgroup
+constexpr int kSortAlone = 2 * kSortChunk;             // most that one workgroup sorts by itself
 constexpr int kMaxDigitBits = 9, kMaxDigits = 1 << kMaxDigitBits;
 
-constexpr size_t kSortFillBytes = (size_t)48 << 20;
+constexpr size_t kSortFillBytes = (size_t)128 << 20;
 // What the sorting launches write besides: `out`'s 16-byte pieces [from, to), from `add` or zeros.
 struct Fill {
     v4i* out;
@@ -138,11 +139,12 @@ __device__ __forceinline__ int scan_digits(SortLds& lds, int mine, int digits) {
 
 // A workgroup's items (key -1: none) in the order of wave, iteration and lane: rank[i] = how many of the wave's items before this one have its
 // digit; lds.count then holds the waves' counts. lds.count must be zero and everyone past that.
-__device__ __forceinline__ void rank_items(SortLds& lds, const int (&key)[kSortIter], Digit digit, int (&rank)[kSortIter]) {
+template <int ITER>
+__device__ __forceinline__ void rank_items(SortLds& lds, const int (&key)[ITER], Digit digit, int (&rank)[ITER]) {
     int* count = lds.count[wave_id()];
     const uint64_t below = (1ull << lane_id()) - 1;
 #pragma unroll
-    for (int i = 0; i < kSortIter; ++i) {
+    for (int i = 0; i < ITER; ++i) {
         const bool live = key[i] >= 0;
         const int d = live ? digit.of(key[i]) : 0;
         const uint64_t same = same_value(d, digit.bits, __ballot(live));
@@ -171,16 +173,18 @@ __device__ __forceinline__ void clear_counts(SortLds& lds) {
     __syncthreads();
 }
 
-// Tokens of one workgroup: all passes at once, the items in LDS in between.
+// Tokens of one workgroup, ITER a thread: all passes at once, the items in LDS in between. (8192 tokens of 50257 rows: in one workgroup 35 us for the
+// whole gradient of 1024 columns, in two by launches 42.)
+template <int ITER>
 __global__ __launch_bounds__(kSortThreads) void embedding_sort_one_kernel(Ids ids, int T, int V, int passes, int bits, int2* __restrict__ sorted,
                                                                           int* __restrict__ length, Fill f) {
     if (blockIdx.x > 0) return fill(f, blockIdx.x - 1);
     __shared__ SortLds lds;
-    __shared__ int2 items[kSortChunk];
-    int key[kSortIter], token[kSortIter], rank[kSortIter];
+    __shared__ int2 items[ITER * kSortThreads];
+    int key[ITER], token[ITER], rank[ITER];
 #pragma unroll
-    for (int i = 0; i < kSortIter; ++i) {
-        token[i] = (wave_id() * kSortIter + i) * 64 + lane_id();
+    for (int i = 0; i < ITER; ++i) {
+        token[i] = (wave_id() * ITER + i) * 64 + lane_id();
         key[i] = token[i] < T ? ids.at(token[i], V) : -1;
     }
     for (int pass = 0; pass < passes; ++pass) {
@@ -195,14 +199,14 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_one_kernel(Ids id
         place_waves(lds, digit.count(), (int)threadIdx.x < digit.count() ? lds.base[threadIdx.x] : 0);
         int2* out = pass + 1 < passes ? items : sorted;
 #pragma unroll
-        for (int i = 0; i < kSortIter; ++i)
+        for (int i = 0; i < ITER; ++i)
             if (key[i] >= 0) out[lds.count[wave_id()][digit.of(key[i])] + rank[i]] = make_int2(key[i], token[i]);
         if (threadIdx.x == 0) *length = all;
         if (pass + 1 == passes) break;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < kSortIter; ++i) {
-            const int at = (wave_id() * kSortIter + i) * 64 + lane_id();
+        for (int i = 0; i < ITER; ++i) {
+            const int at = (wave_id() * ITER + i) * 64 + lane_id();
             const int2 item = at < all ? items[at] : make_int2(-1, 0);
             key[i] = item.x;
             token[i] = item.y;
@@ -533,7 +537,7 @@ static int launch_embedding_backward(Ids ids, const void* dout, const void* add,
     int2 *a = (int2*)(ws + L.a), *b = (int2*)(ws + L.b);
     // The launches that sort write the first rows, as many as take them about their time, whether these have tokens or not; the launch that sums
     // writes the others, where there are no tokens.
-    const int launches = L.chunks == 1 ? 1 : 1 + L.passes;
+    const int launches = tokens <= kSortAlone ? 1 : 1 + L.passes;
     const size_t row_bytes = (size_t)H * sizeof(T), all_bytes = V * row_bytes;
     const int blind = add == dtable ? 0 : (int)std::min<size_t>(V, launches * (add ? kSortFillBytes / 2 : kSortFillBytes) / row_bytes);
     const size_t pieces = blind * row_bytes / 16;
@@ -544,9 +548,10 @@ static int launch_embedding_backward(Ids ids, const void* dout, const void* add,
         return f;
     };
     const int2* sorted = a;
-    if (L.chunks == 1) {
+    if (tokens <= kSortAlone) {
         const Fill f = part(0);
-        hipLaunchKernelGGL(embedding_sort_one_kernel, dim3(1 + f.groups), dim3(kSortThreads), 0, s, ids, tokens, V, L.passes, L.bits, a, length, f);
+        hipLaunchKernelGGL(tokens <= kSortChunk ? embedding_sort_one_kernel<kSortIter> : embedding_sort_one_kernel<2 * kSortIter>, dim3(1 + f.groups),
+                           dim3(kSortThreads), 0, s, ids, tokens, V, L.passes, L.bits, a, length, f);
     } else {
         const Fill f = part(0);
         hipLaunchKernelGGL(embedding_count_kernel, dim3(L.chunks + f.groups), dim3(kSortThreads), 0, s, ids, tokens, V, L.chunks, Digit{0, L.bits},

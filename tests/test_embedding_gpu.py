@@ -78,7 +78,7 @@ def test_gradient(hk, T, V, H):
 
 
 @pytest.mark.parametrize("kind", ["one", "different", "falling", "frequent", "outside", "none"])
-@pytest.mark.parametrize("T,V,H", [(4097, 100, 64), (9001, 50257, 136), (20000, 70000, 24), (12288, 1 << 19, 8), (9000, 300, 8200), (8500, 700, 16400)])
+@pytest.mark.parametrize("T,V,H", [(4097, 100, 64), (9001, 50257, 136), (20000, 70000, 24), (12288, 1 << 19, 8), (9000, 300, 8200), (8500, 700, 16400), (8192, 777, 72), (8193, 777, 72)])
 def test_gradient_over_several_workgroups(hk, T, V, H, kind):
     n = T + V + len(kind)
     _backward(hk, T, V, H, kind, (torch.bfloat16, torch.float32)[n % 2], (torch.int64, torch.int32)[n // 2 % 2], ("no", "yes", "in place")[n % 3],
