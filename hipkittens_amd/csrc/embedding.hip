@@ -586,7 +586,7 @@ extern "C" int hk_embedding(const void* ids, int id_type, const void* table, int
     if (!ids || !table || !out_bf16) return HK_ERR_NULL_POINTER;
     if (const int st = embed_check(T, V, H)) return st;
     if ((id_type != 0 && id_type != 1) || (table_type != 0 && table_type != 1)) return HK_ERR_UNSUPPORTED;
-    if (((uintptr_t)table | (uintptr_t)out_bf16) & 15u) return HK_ERR_BAD_ALIGNMENT;
+    if ((((uintptr_t)table | (uintptr_t)out_bf16) & 15u) || ((uintptr_t)ids & (id_type ? 7u : 3u))) return HK_ERR_BAD_ALIGNMENT;
     const Ids at{ids, id_type};
     return table_type == 0 ? launch_embedding<uint16_t>(at, table, out_bf16, T, V, H, scale, (hipStream_t)stream)
                            : launch_embedding<float>(at, table, out_bf16, T, V, H, scale, (hipStream_t)stream);
@@ -602,7 +602,8 @@ extern "C" int hk_embedding_backward(const void* ids, int id_type, const void* d
     if (!ids || !dout_bf16 || !dtable) return HK_ERR_NULL_POINTER;
     if (const int st = embed_check(T, V, H)) return st;
     if ((id_type != 0 && id_type != 1) || (table_type != 0 && table_type != 1)) return HK_ERR_UNSUPPORTED;
-    if (((uintptr_t)dout_bf16 | (uintptr_t)add_or_null | (uintptr_t)dtable | (uintptr_t)workspace) & 15u) return HK_ERR_BAD_ALIGNMENT;
+    if ((((uintptr_t)dout_bf16 | (uintptr_t)add_or_null | (uintptr_t)dtable | (uintptr_t)workspace) & 15u) || ((uintptr_t)ids & (id_type ? 7u : 3u)))
+        return HK_ERR_BAD_ALIGNMENT;
     if (!workspace || workspace_bytes < EmbedPlan(T, V, H).bytes) return HK_ERR_WORKSPACE;
     const Ids at{ids, id_type};
     return table_type == 0 ? launch_embedding_backward<uint16_t>(at, dout_bf16, add_or_null, dtable, T, V, H, scale, (uint8_t*)workspace, (hipStream_t)stream)

@@ -324,6 +324,159 @@ __global__ __launch_bounds__(256) void gated_dgrad_kernel(GatedBackward p) {
     }(std::make_integer_sequence<int, Tile::F>());
 }
 
+// Few rows of a dense block in the backward pass: one pass over W2, whose rows the contraction crosses. A workgroup owns NC columns of h and all rows
+// of dy; its four waves take a quarter of the K-steps each, on their own: 64 rows of NC columns of W2 and as many elements of every row of dy
+// into a ring of D stages of LDS that belongs to the wave, W2's read with the transposing loads (gemm_layouts.h). The four partial sums
+// meet in LDS, in order, and the activation's gradients follow from what was kept, which the threads have loaded at the start.
+// R: 16 rows of dy each.
+template <int R, int NC, int D>
+struct SkinnyAcross {
+    static constexpr int kWaves = 4, kRow = 2 * NC, kW = 64 * kRow, kStage = kW + R * 2048, kRegion = D * kStage, kLds = kWaves * kRegion;
+    static constexpr int kChunks = kRow / 16, kLoadRows = 64 / kChunks, kLoads = kW / 1024, kAll = kLoads + 2 * R, F = NC / 16;
+    static_assert(kLds <= 160 * 1024 && (D - 1) * kAll < 64 && R * F * 1024 <= kRegion);
+    // 16-byte chunk c of LDS row k lies at c ^ swz(k) (rows of 64 bytes: four share a line of the banks)
+    static __device__ __forceinline__ uint32_t swz(uint32_t k) { return NC == 64 ? across_swz128(k) : 2u * ((k >> 3) & 1u); }
+};
+template <int R, int NC, int D, bool NT>
+__global__ __launch_bounds__(256) void gated_dgrad_skinny_kernel(GatedBackward p) {
+    typedef SkinnyAcross<R, NC, D> S;
+    extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
+    const uint32_t lane = lane_id(), w = wave_id(), r = lane & 15, g = lane >> 4;
+    const int col0 = xcd_chunk_order(blockIdx.x, gridDim.x, kCuPerXcd) * NC;
+    const int nk = (p.N + kLayoutStep - 1) / kLayoutStep;
+    const int s0 = nk * (int)w / S::kWaves, n = nk * ((int)w + 1) / S::kWaves - s0;
+
+    // this thread's elements of the result: four columns of a row each, and their kept values
+    constexpr int kItems = (R * S::F * 64 + 255) / 256;
+    v2i kept_g[kItems], kept_u[kItems];
+    auto place = [&](int i, int& row, int& col) {
+        const int t = i * 256 + threadIdx.x, l = t & 63;
+        row = t / (S::F * 64) * 16 + (l & 15);
+        col = col0 + (t >> 6) % S::F * 16 + 4 * (l >> 4);
+        return t < R * S::F * 64 && row < p.R && col < p.I;
+    };
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+        int row, col;
+        kept_g[i] = kept_u[i] = v2i{0, 0};
+        if (!place(i, row, col)) continue;
+        const uint16_t* at = p.gate_up + (size_t)row * 2 * p.I;
+        if (p.interleaved) {
+            const v4i both = *(const v4i*)(at + 2 * col);
+            kept_g[i] = v2i{both.x, both.y};
+            kept_u[i] = v2i{both.z, both.w};
+        } else {
+            kept_g[i] = *(const v2i*)(at + col);
+            kept_u[i] = *(const v2i*)(at + p.I + col);
+        }
+    }
+
+    const uint32_t pitch = to_sgpr(2u * (uint32_t)p.I), dy_pitch = to_sgpr(2u * (uint32_t)p.N);
+    const uint64_t base = (uint64_t)(p.w2 + col0);
+    const int64_t bytes = 2 * ((int64_t)p.N * p.I - col0);
+    const v4i srd_dy = make_srd(p.dy, (uint32_t)p.R * dy_pitch);
+    uint32_t voff_w[2], voff_dy[2], tail_or[2];   // even / odd loads (the swizzles take the load's parity)
+#pragma unroll
+    for (int odd = 0; odd < 2; ++odd) {
+        const uint32_t k = lane / S::kChunks;
+        voff_w[odd] = k * pitch + ((lane % S::kChunks) ^ S::swz(k + S::kLoadRows * odd)) * 16u;
+        const uint32_t row = 8u * odd + (lane >> 3), c = swz_chunk(row, lane & 7) * 16u;
+        voff_dy[odd] = row * dy_pitch + c;
+        tail_or[odd] = (int)c >= 2 * (p.N - (nk - 1) * kLayoutStep) ? kOutside : 0u;
+    }
+    const uint32_t lds0 = (uint32_t)(uintptr_t)smem, region = to_sgpr(lds0 + w * S::kRegion);
+    auto issue = [&](int stage, int at) {
+        const int kt = s0 + at;
+        const uint32_t dst = region + (uint32_t)stage * S::kStage;
+        const int64_t skip = (int64_t)kt * kLayoutStep * pitch, left = bytes - skip;
+        const v4i srd = make_srd((const void*)(base + skip), (uint32_t)(left < 0x7fffffff ? (left > 0 ? left : 0) : 0x7fffffff));
+#pragma unroll
+        for (int i = 0; i < S::kLoads; ++i) {
+            const uint32_t so = to_sgpr(i * S::kLoadRows * pitch);
+            if constexpr (NT) dma16_nt(srd, to_sgpr(dst + i * 1024), voff_w[i & 1], so);
+            else dma16(srd, to_sgpr(dst + i * 1024), voff_w[i & 1], so);
+        }
+        const bool last = kt == nk - 1;
+#pragma unroll
+        for (int i = 0; i < 2 * R; ++i)
+            dma16(srd_dy, to_sgpr(dst + S::kW + i * 1024), (voff_dy[i & 1] + (uint32_t)(i >> 1) * 16u * dy_pitch) | (last ? tail_or[i & 1] : 0u),
+                  to_sgpr((uint32_t)kt * 128u));
+    };
+    v4f acc[R][S::F];
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int f = 0; f < S::F; ++f) acc[i][f] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < D - 1; ++s)
+        if (s < n) issue(s, s);
+    const uint32_t k0 = 8 * g + (r >> 2);
+    const uint32_t rd_w = region + k0 * S::kRow + (((r >> 1) & 1u) ^ S::swz(k0)) * 16u + (r & 1u) * 8u;
+    const uint32_t rd_lo = region + S::kW + r * 128u + swz_chunk(r, g) * 16u, rd_hi = region + S::kW + r * 128u + swz_chunk(r, g + 4) * 16u;
+    int st = 0;
+    for (int kt = 0; kt < n; ++kt) {
+        // K-step kt has landed: no more of the K-steps behind it are under way than were issued
+        switch (min(n - 1 - kt, D - 2)) {
+            case 0: wait_vmcnt<0>(); break;
+            case 1: wait_vmcnt<S::kAll>(); break;
+            case 2: wait_vmcnt<(D > 3 ? 2 : 1) * S::kAll>(); break;
+            case 3: wait_vmcnt<(D > 4 ? 3 : 1) * S::kAll>(); break;
+            default: wait_vmcnt<(D > 5 ? 4 : 1) * S::kAll>(); break;
+        }
+        static_assert(D >= 2 && D <= 6);
+        if (kt + D - 1 < n) issue(st == 0 ? D - 1 : st - 1, kt + D - 1);   // (that stage's reads were waited for before its products)
+        const uint32_t so = (uint32_t)st * S::kStage;
+        v8i wf[S::F];
+#pragma unroll
+        for (int f = 0; f < S::F; ++f) {
+            const uint32_t at = (rd_w ^ (32u * f)) + so;
+            const v2i a = lds_read_tr(at), b = lds_read_tr(at + 4 * S::kRow), c = lds_read_tr(at + 32 * S::kRow), d = lds_read_tr(at + 36 * S::kRow);
+            wf[f] = v8i{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+        }
+#pragma unroll
+        for (int i = 0; i < R; ++i) {
+            const v8i af = lds_frag(rd_lo + so, rd_hi + so, i * 2048);
+#pragma unroll
+            for (int f = 0; f < S::F; ++f) GatedMma::mma(acc[i][f], wf[f], af);
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // this stage's reads are done before a later load may overwrite it
+        st = st == D - 1 ? 0 : st + 1;
+    }
+    __syncthreads();   // every wave is done with its stages
+    v4f* red = (v4f*)smem;   // [waves][R][F][64]
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+#pragma unroll
+        for (int f = 0; f < S::F; ++f) red[((w * R + i) * S::F + f) * 64 + lane] = acc[i][f];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+        int row, col;
+        if (!place(i, row, col)) continue;
+        v4f dh = red[i * 256 + threadIdx.x];
+#pragma unroll
+        for (int v = 1; v < S::kWaves; ++v) dh += red[v * R * S::F * 64 + i * 256 + threadIdx.x];
+        float dg[4], du[4], h[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            // (alternating: words 2 j .. of both halves hold a pair each; stacked: two gate values a word)
+            const uint32_t pair = (uint32_t)(j < 2 ? kept_g[i][j] : kept_u[i][j - 2]);
+            const uint32_t two_g = (uint32_t)kept_g[i][j / 2], two_u = (uint32_t)kept_u[i][j / 2];
+            const float gv = __uint_as_float(p.interleaved ? pair << 16 : j & 1 ? two_g & 0xffff0000u : two_g << 16);
+            const float uv = __uint_as_float(p.interleaved ? pair & 0xffff0000u : j & 1 ? two_u & 0xffff0000u : two_u << 16);
+            h[j] = p.clamped ? Gate<true>{p.gate}.gradients(gv, uv, dh[j], dg[j], du[j]) : Gate<false>{p.gate}.gradients(gv, uv, dh[j], dg[j], du[j]);
+        }
+        uint16_t* at = p.dgate_up + (size_t)row * 2 * p.I;
+        if (p.interleaved) {
+            *(v4i*)(at + 2 * col) = v4i{(int)pack_bf16(dg[0], du[0]), (int)pack_bf16(dg[1], du[1]), (int)pack_bf16(dg[2], du[2]), (int)pack_bf16(dg[3], du[3])};
+        } else {
+            *(v2i*)(at + col) = v2i{(int)pack_bf16(dg[0], dg[1]), (int)pack_bf16(dg[2], dg[3])};
+            *(v2i*)(at + p.I + col) = v2i{(int)pack_bf16(du[0], du[1]), (int)pack_bf16(du[2], du[3])};
+        }
+        if (p.h) *(v2i*)(p.h + (size_t)row * p.I + col) = v2i{(int)pack_bf16(h[0], h[1]), (int)pack_bf16(h[2], h[3])};
+    }
+}
+
 // alpha and limit of the clamped form (1); SiLU (0) has none
 static int check_gate(int activation, const GateArgs& g) {
     if (activation == 0) return HK_OK;
@@ -402,20 +555,44 @@ static int launch_gated_skinny(const GatedForward& p, hipStream_t s) {
     if (p.R <= 48) return launch_gated_skinny_rows<3, 4, 4>(p, s);
     return launch_gated_skinny_rows<4, 3, 3>(p, s);
 }
-// Whether the forward product over experts' rows takes tiles of 128 rows and 256 columns: by rounds over the CUs times a fixed part and a part per
-// K-step, us, with the tiles of rows that an expert has on average (a round begun counts whole between one and two), where there are tiles enough
-// that no kernel with many LDS stages is taken. (us, 128x128 or 256x256, whichever was chosen / 128x256: 128 experts of 2880 x 2880, 64 rows
-// each 870 / 841, 128 rows 1008 / 990, 192 1148 / 1251; 32 of 2048 x 7168, 128 rows 492 / 425; 64 of 1536 x 4096, 150 rows 435 / 386; 8 of 4096 x
-// 4096, 128 rows 203 / 158; the rule's worst, 64 of 768 x 2048, 128 rows 131 / 141. Not in the backward pass, whose epilogue is the longer.)
+template <int R, int NC, int D>
+static int launch_gated_dgrad_skinny_kernel(const GatedBackward& p, hipStream_t s) {
+    const bool nt = 2ll * p.I * p.N >= kSkinnyNtBytes;
+    auto kern = nt ? gated_dgrad_skinny_kernel<R, NC, D, true> : gated_dgrad_skinny_kernel<R, NC, D, false>;
+    constexpr int lds_bytes = SkinnyAcross<R, NC, D>::kLds;
+    static DeviceOnce configured[2];
+    if (!set_lds_limit_once((const void*)kern, lds_bytes, configured[nt])) return HK_ERR_LAUNCH;
+    hipLaunchKernelGGL(kern, dim3((p.I + NC - 1) / NC), dim3(256), lds_bytes, s, p);
+    return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
+}
+// 32 columns a workgroup while that gives no CU a second one (rows of W2 in pieces of 64 bytes: what a CU has under way is counted in
+// pieces, so that half as many workgroups of 64 columns are no faster); more columns in pieces of 64 up to 32 rows, and the 64-tile kernel beyond.
+// (us from HBM, 64-tile kernel / 32 columns / 64: one row, I = 2048, N = 7168 32.5 / 24.8 / 29.4; I = 912, N = 3728 19.6 / 12.7 / 17.0;
+// I = 14336, N = 4096 25.9 / 35.4 / 24.4; 64 rows of it 32.6 / 51.5 / 33.4, of I = 8192, N = 2048 17.1 / 15.8 / 17.8.)
+static bool use_gated_dgrad_skinny(int R, int I) {
+    return R <= 32 || (R <= kSkinnyMaxM && (I + 31) / 32 <= moe_num_compute_units());
+}
+static int launch_gated_dgrad_skinny(const GatedBackward& p, hipStream_t s) {
+    const bool narrow = (p.I + 31) / 32 <= moe_num_compute_units();
+    if (p.R <= 16) return narrow ? launch_gated_dgrad_skinny_kernel<1, 32, 6>(p, s) : launch_gated_dgrad_skinny_kernel<1, 64, 4>(p, s);
+    if (p.R <= 32) return narrow ? launch_gated_dgrad_skinny_kernel<2, 32, 5>(p, s) : launch_gated_dgrad_skinny_kernel<2, 64, 3>(p, s);
+    return launch_gated_dgrad_skinny_kernel<4, 32, 3>(p, s);
+}
+
+// Whether the forward product takes tiles of 128 rows and 256 columns: by rounds over the CUs times a fixed part and a part per K-step, us (a
+// round begun counts whole between one and two), where there are tiles enough that no kernel with many LDS stages is taken. (us, 128x128 or
+// 256x256, whichever would be chosen / 128x256: 32 experts of 2048 x 7168, 128 rows each 492 / 425; 128 of 2880 x 2880, 64 rows 870 / 841,
+// 128 rows 1008 / 990; 64 of 1536 x 4096, 150 rows 435 / 386; 8 of 4096 x 4096, 128 rows 203 / 158, but 64 of 768 x 2048, 128 rows 131 / 141.
+// On 4300 drawn shapes, time over the best kernel's on average: dense blocks 1.020 without it, 1.014 with it, the tenth with the
+// worst choice 1.063 and 1.01; experts 1.030, 1.027. Not in the backward pass, whose epilogue is the longer.)
 static bool use_wide_tile(const GatedForward& p) {
-    if (!p.offsets) return false;
     const int cus = moe_num_compute_units(), out = 2 * p.I;
-    const LayoutChoice other = grouped_choice(p.R, p.E, p.K, out);
+    const LayoutChoice other = grouped_choice(p.R, p.E, p.K, out, !p.offsets);
     if (other == kLayout64Deep || other == kLayout128Deep) return false;
     const double used = p.R < p.E ? p.R : p.E, mean = p.R / used, steps = (p.K + kLayoutStep - 1) / kLayoutStep;
-    auto tiles_m = [&](int tile) { return used * std::max(1.0, mean / tile + 0.7); };
+    auto tiles_m = [&](int tile) { return p.offsets ? used * std::max(1.0, mean / tile + 0.6) : (p.R + tile - 1) / tile; };
     auto rounds = [](double t) { return t <= 1 ? 1.0 : std::max(t + 0.2, std::min(2.0, t + 0.65)); };
-    const double cols = (out + 255) / 256, wide = rounds(tiles_m(128) * cols / cus) * (6.0 + 0.92 * steps);
+    const double cols = (out + 255) / 256, wide = rounds(tiles_m(128) * cols / cus) * (6.0 + 0.97 * steps);
     const double small = rounds(tiles_m(128) * ((out + 127) / 128) / (2.0 * cus)) * (kSmallFixed + kSmallStepAlong * steps);
     return wide < small && wide < rounds(tiles_m(256) * cols / cus) * (kLargeFixed + kLargeStep * steps);
 }
@@ -459,5 +636,6 @@ extern "C" int hk_gated_gemm_dgrad(const void* dy_bf16, const void* w2_bf16, con
     GatedBackward p{(const uint16_t*)dy_bf16, (const uint16_t*)w2_bf16, expert_offsets_or_null, (const uint16_t*)gate_up_bf16,
                     (uint16_t*)dgate_up_bf16, (uint16_t*)h_bf16_or_null, R, E, N, I, 0, interleaved != 0, activation == 1, {alpha, limit}};
     if (const int st = check_gate(activation, p.gate)) return st;
+    if (!p.offsets && use_gated_dgrad_skinny(R, I)) return launch_gated_dgrad_skinny(p, (hipStream_t)stream);
     return launch_gated_choice(p, N, I, (hipStream_t)stream);
 }

@@ -40,6 +40,8 @@ def test_embedding(p):
         args = [p, 0, p, p, p, 0, 4, 100, 64, 1.0, p, big, None]
         args[at] = p + 8
         assert lib.hk_embedding_backward(*args) == ALIGN
+    assert lib.hk_embedding(p + 2, 0, p, 0, p, 4, 100, 64, 1.0, None) == ALIGN and lib.hk_embedding(p + 4, 1, p, 0, p, 4, 100, 64, 1.0, None) == ALIGN
+    assert lib.hk_embedding_backward(p + 4, 1, p, p, p, 0, 4, 100, 64, 1.0, p, big, None) == ALIGN
     need = lib.hk_embedding_backward_workspace_bytes(4, 100, 64)
     assert lib.hk_embedding_backward(p, 0, p, p, p, 0, 4, 100, 64, 1.0, p, need - 1, None) == WORKSPACE
     assert lib.hk_embedding_backward(p, 0, p, p, p, 0, 4, 100, 64, 1.0, None, need, None) == WORKSPACE

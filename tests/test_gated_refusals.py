@@ -113,6 +113,8 @@ def test_python_boundary_shapes_and_types():
                  lambda: tk.dispatch_gated_gemm(bf(4, 64), bf(2, 128, 64), bf(4, 64), expert_offsets=f32(3)),
                  lambda: tk.dispatch_gated_gemm(bf(4, 60), bf(128, 60), bf(4, 64)),
                  lambda: tk.dispatch_gated_gemm(bf(4, 64), bf(128, 64), bf(4, 64), activation="swiglu_oai", limit=-1.0),
+                 lambda: tk.dispatch_gated_gemm(bf(4, 64), bf(128, 64), None),
+                 lambda: tk.dispatch_gated_gemm(bf(4, 64), bf(128, 64), None, bf(4, 128)),
                  lambda: tk.dispatch_gated_gemm(bf(0, 64), bf(128, 64), bf(0, 64)),
                  lambda: tk.dispatch_gated_gemm_dgrad(bf(4, 64), bf(64, 72), bf(4, 128), bf(4, 128)),
                  lambda: tk.dispatch_gated_gemm_dgrad(bf(4, 64), bf(64, 64), bf(4, 128), bf(4, 64)),
