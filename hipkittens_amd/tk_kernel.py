@@ -927,7 +927,8 @@ def dispatch_gated_gemm(x, w13, h, gate_up=None, expert_offsets=None, interleave
     st = (_native or _load_native()).gated_gemm(x, w13, h, gate_up, expert_offsets, interleaved, _ACTIVATIONS.get(activation), alpha, limit)
     if st is not None:
         return _lib.check(st, "dispatch_gated_gemm")
-    _check_tensor(h, "h", _BF16, 2)
+    if h is None:
+        raise RuntimeError("h: expected a torch.Tensor")
     R, E, I, act = _check_gated(x, "x", w13, "w13", lambda i: (2 * i, x.shape[1]), gate_up, "gate_up", h, "h", expert_offsets, activation)
     with torch.cuda.device(x.device):
         st = _lib.load_library().hk_gated_gemm(x.data_ptr(), w13.data_ptr(), _ptr(expert_offsets), h.data_ptr(), _ptr(gate_up), R, E, I,
