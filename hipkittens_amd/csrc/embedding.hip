@@ -5,9 +5,10 @@
 //
 // Both move rows, and HBM bounds them. The gradient needs every row's tokens together and in an order of their own: the tokens are sorted by id
 // (stable, digit by digit from the lowest), and blocks of the sorted list are summed in order, so that results are the same on every call and
-// no value goes through an atomic. All rows get zeros (or a copy of `add`) first, in the launches that sort, whose few workgroups
-// would leave the chip idle: rows with tokens are then written a second time, at most one row per token. A row whose tokens are
-// spread over several blocks leaves fp32 partial sums, which the last launch joins in order.
+// no value goes through an atomic. Rows without tokens get zeros (or a copy of `add`): the first rows, whether they have tokens or not, in
+// the launches that sort, whose few workgroups would leave the chip idle (those with tokens are then written a second time); the
+// others beside the sums, where a search of the sorted list finds no token. A row whose tokens are spread over several blocks
+// leaves fp32 partial sums, which the last launch joins in order.
 #include <algorithm>
 
 #include "hk_device.h"
@@ -58,7 +59,7 @@ constexpr int kSortChunk = kSortThreads * kSortIter;   // tokens of a workgroup
 constexpr int kSortAlone = 2 * kSortChunk;             // most that one workgroup sorts by itself
 constexpr int kMaxDigitBits = 9, kMaxDigits = 1 << kMaxDigitBits;
 
-constexpr size_t kSortFillBytes = (size_t)128 << 20;
+constexpr size_t kSortFillBytes = (size_t)128 << 20;   // that a sorting launch writes besides (half of it where it is read first)
 // What the sorting launches write besides: `out`'s 16-byte pieces [from, to), from `add` or zeros.
 struct Fill {
     v4i* out;
@@ -512,8 +513,9 @@ static int launch_embedding(Ids ids, const void* table, void* out, int tokens, i
     // the hint 53; 65536 of 1024 43 / 27)
     const bool stream = 2ll * tokens * H >= (96ll << 20);
     auto launch = [&]<int LOADS>() {
-        hipLaunchKernelGGL((stream ? embedding_kernel<T, LOADS, true> : embedding_kernel<T, LOADS, false>), dim3((unsigned)((tokens + 3) / 4), (unsigned)waves), dim3(256), 0, s, ids, (const T*)table,
-                           (uint16_t*)out, tokens, V, H, scale);
+        hipLaunchKernelGGL((stream ? embedding_kernel<T, LOADS, true> : embedding_kernel<T, LOADS, false>),
+                           dim3((unsigned)((tokens + 3) / 4), (unsigned)waves), dim3(256), 0, s, ids, (const T*)table, (uint16_t*)out, tokens, V, H,
+                           scale);
         return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
     };
     switch (loads) {

@@ -495,33 +495,6 @@ __device__ __forceinline__ void store_block_row(const v4f (&v)[F], int m, T* __r
             const int col = 32 * p + 8 * (g >> 1) + 16 * (g & 1);
             if (row < rows && col < cols) *(v4i*)(at + col) = out;
         }
-        if constexpr (F % 2 == 1) {   // the last block on its own, four columns a lane
-            const v4f a = v[F - 1];
-            const int col = 16 * (F - 1) + 4 * g;
-            if (row < rows && col < cols) *(v2i*)(at + col) = v2i{(int)pack_bf16(a.x, a.y), (int)pack_bf16(a.z, a.w)};
-        }
-    }
-}
-// The reverse for bf16: the values of C in the places that store_block_row takes them from; zeros where there is no C.
-template <int F>
-__device__ __forceinline__ void load_block_row(v4f (&v)[F], int m, const uint16_t* C, int64_t ldc, int64_t rows, int64_t cols) {
-    static_assert(F % 2 == 0);
-    const int r = lane_id() & 15, g = lane_id() >> 4, row = 16 * m + r;
-    const uint16_t* at = C + row * ldc;
-#pragma unroll
-    for (int p = 0; p < F / 2; ++p) {
-        const int col = 32 * p + 8 * (g >> 1) + 16 * (g & 1);
-        v4i in{0, 0, 0, 0};
-        if (row < rows && col < cols) in = *(const v4i*)(at + col);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const auto s = __builtin_amdgcn_permlane16_swap((uint32_t)in[h], (uint32_t)in[2 + h], false, false);
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                v[2 * p + q][2 * h] = __uint_as_float((uint32_t)s[q] << 16);
-                v[2 * p + q][2 * h + 1] = __uint_as_float((uint32_t)s[q] & 0xffff0000u);
-            }
-        }
     }
 }
 // The whole patch. (A fence behind every row block: without it the compiler holds more of them in registers than there are.)

@@ -3,10 +3,9 @@
 //   norm = sqrt(sum_i sum_j g_ij^2),   out_ij = g_ij min(1, max_norm / (norm + 1e-6))
 //
 // HBM bounds both: the gradients are read once for the norm and once to be scaled. A list is any number of bf16 and fp32 tensors of any length
-// and alignment, described by a table on the device that a program makes once: one launch goes over all of them. Work is cut into
-// chunks of kClipChunk elements, which a workgroup looks up in the table. Squares are added
-// in 64 bits (a square of fp32 does not leave their range, and the sum of 2^30 of them keeps fp32's digits), in an order that depends on the
-// list alone.
+// and alignment, described by a table on the device that a program makes once: one launch goes over all of them. Work is cut into chunks of
+// kClipChunk elements, which a workgroup looks up in the table. Squares are added in 64 bits (a square of fp32 does not leave their range,
+// and the sum of 2^30 of them keeps fp32's digits), in an order that depends on the list alone.
 #include <algorithm>
 
 #include "hk_device.h"
@@ -26,14 +25,15 @@ struct GradEntry {
 };
 static_assert(sizeof(GradEntry) == 40);
 
-// The workgroup's chunks: f(entry, from, to), or with REVERSE from the last one to the first. Neighbouring workgroups have neighbouring chunks, so that the launch goes through memory front to
-// back (each workgroup a run of its own instead: norm of 2.4 GB 458 us, so 385).
+// The workgroup's chunks: f(entry, from, to), or with REVERSE from the last one to the first. Neighbouring workgroups have neighbouring
+// chunks, so that the launch goes through memory front to back (each workgroup a run of its own instead: norm of 2.4 GB 458 us, so 385).
 template <bool REVERSE, typename F>
 __device__ __forceinline__ void for_chunks(const GradEntry* __restrict__ list, int n, int64_t chunks, F&& f) {
     int at = REVERSE ? n : 0;   // of the chunk before: where the search ends, or begins
     for (int64_t i = blockIdx.x; i < chunks; i += gridDim.x) {
         const int64_t c = REVERSE ? chunks - 1 - i : i;
-        int lo = REVERSE ? 0 : at, hi = REVERSE ? at : n;   // the last tensor whose chunks begin at c or in front of it (tensors without elements have none)
+        // the last tensor whose chunks begin at c or in front of it (tensors without elements have none)
+        int lo = REVERSE ? 0 : at, hi = REVERSE ? at : n;
         while (hi - lo > 1) {
             const int mid = (lo + hi) / 2;
             if (list[mid].chunk0 <= c) lo = mid;
@@ -232,7 +232,8 @@ extern "C" int hk_grad_norm(const void* list, int n, int64_t chunks, float* norm
     const hipStream_t s = (hipStream_t)stream;
     const int groups = clip_groups(chunks);
     if (groups > 0)
-        hipLaunchKernelGGL(chunks > kClipStreamChunks ? grad_square_sum_kernel<true> : grad_square_sum_kernel<false>, dim3(groups), dim3(256), 0, s, (const GradEntry*)list, n, chunks, (double*)workspace);
+        hipLaunchKernelGGL(chunks > kClipStreamChunks ? grad_square_sum_kernel<true> : grad_square_sum_kernel<false>, dim3(groups), dim3(256), 0, s,
+                           (const GradEntry*)list, n, chunks, (double*)workspace);
     hipLaunchKernelGGL(grad_norm_kernel, dim3(1), dim3(1024), 0, s, (const double*)workspace, groups, norm);
     return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
 }
@@ -245,6 +246,7 @@ extern "C" int hk_grad_clip(const void* list, int n, int64_t chunks, const float
     if (!(max_norm >= 0.f)) return HK_ERR_UNSUPPORTED;
     const int groups = clip_groups(chunks);
     if (groups == 0) return HK_OK;
-    hipLaunchKernelGGL(chunks > kClipStreamChunks ? grad_clip_kernel<true> : grad_clip_kernel<false>, dim3(groups), dim3(256), 0, (hipStream_t)stream, (const GradEntry*)list, n, chunks, norm, max_norm);
+    hipLaunchKernelGGL(chunks > kClipStreamChunks ? grad_clip_kernel<true> : grad_clip_kernel<false>, dim3(groups), dim3(256), 0,
+                       (hipStream_t)stream, (const GradEntry*)list, n, chunks, norm, max_norm);
     return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
 }

@@ -889,6 +889,13 @@ def dispatch_linear_cross_entropy_backward(x, w, labels, lse, dloss, dx, dw, wor
 
 
 # ------------------------------------------------------------ training: gated feed-forward blocks
+def _check_sizes(*tensors):
+    """The entry points count in 32 bits: a longer dimension would reach them cut short."""
+    for t, name in tensors:
+        if t is not None and max(t.shape) >= 2 ** 31:
+            raise RuntimeError(f"{name} {tuple(t.shape)}: a dimension of 2^31 or more")
+
+
 def _check_gated(rows_wide, name_wide, w, name_w, w_shape, gate_up, name_gate_up, rows_i, name_i, expert_offsets, activation):
     """-> (R, E, I, activation code) of rows_wide [R, .], w (w_shape(I) behind an expert's index where there are experts), gate_up [R, 2I] or
     None and rows_i [R, I] or None"""
@@ -910,6 +917,7 @@ def _check_gated(rows_wide, name_wide, w, name_w, w_shape, gate_up, name_gate_up
             (rows_i is not None and rows_i.shape[0] != R)):
         raise RuntimeError("shape mismatch: " + ", ".join(f"{n} {tuple(t.shape)}" for t, n in (
             (rows_wide, name_wide), (w, name_w), (gate_up, name_gate_up), (rows_i, name_i)) if t is not None))
+    _check_sizes((rows_wide, name_wide), (w, name_w))
     _same_device(rows_wide, w, gate_up, rows_i, expert_offsets)
     return R, E, I, _ACTIVATIONS[activation]
 
@@ -968,6 +976,7 @@ def _check_product(rows_n, name_n, rows_k, name_k, w, name_w, w_types):
     (M, N), K = rows_n.shape, rows_k.shape[1]
     if rows_k.shape[0] != M or tuple(w.shape) != (N, K):
         raise RuntimeError(f"shape mismatch: {name_n} {tuple(rows_n.shape)}, {name_k} {tuple(rows_k.shape)}, {name_w} {tuple(w.shape)}")
+    _check_sizes((rows_n, name_n), (w, name_w))
     _same_device(rows_n, rows_k, w)
     return M, N, K
 
@@ -1000,7 +1009,9 @@ _TABLE = (torch.bfloat16, torch.float32)
 
 
 def embedding_backward_workspace_bytes(T: int, V: int, H: int) -> int:
-    """Bytes of workspace of dispatch_embedding_backward; never less for a larger T."""
+    """Bytes of workspace of dispatch_embedding_backward, 0 for a shape that it refuses; never less for a larger T."""
+    if max(T, V, H) >= 2 ** 31:
+        return 0
     return int(_lib.load_library().hk_embedding_backward_workspace_bytes(int(T), int(V), int(H)))
 
 
@@ -1012,6 +1023,7 @@ def _check_embedding(ids, rows, name_rows, table, name_table):
     T, (V, H) = ids.shape[0], table.shape
     if tuple(rows.shape) != (T, H):
         raise RuntimeError(f"shape mismatch: ids {tuple(ids.shape)}, {name_rows} {tuple(rows.shape)}, {name_table} {tuple(table.shape)}")
+    _check_sizes((ids, "ids"), (table, name_table))
     _same_device(ids, rows, table)
     return T, V, H
 
