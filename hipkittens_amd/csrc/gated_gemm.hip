@@ -12,6 +12,7 @@
 // every 32 rows of the weight tile in LDS are 16 gate rows and the 16 up rows of the same columns (kPairs), so that both values of
 // an element are in one lane's accumulators and the activation needs no exchange between lanes.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 #include <utility>
 
@@ -230,7 +231,7 @@ __global__ __launch_bounds__(256) void gated_gemm_kernel(GatedForward p) {
     }
 }
 
-// Few rows of a dense block (decode): one pass over the weights at HBM speed, the skinny kernel with gate and up rows in its two halves.
+// Few rows of a dense block or an expert (decode): one pass over the weights at HBM speed, the skinny kernel with gate and up rows in its two halves.
 struct GatedMma {
     static constexpr bool kScaled = false;
     static __device__ __forceinline__ void mma(v4f& acc, const v8i& b, const v8i& a) {
@@ -242,6 +243,8 @@ struct GatedMma {
 struct GatedSkinnyOut {
     static constexpr bool kPairs = true;
     GatedForward p;
+    int col0;
+    __device__ __forceinline__ int first() const { return col0; }
     __device__ __forceinline__ uint32_t pitch() const { return (uint32_t)p.K * (p.interleaved ? 4u : 2u); }
     __device__ __forceinline__ const uint8_t* other() const { return (const uint8_t*)(p.w13 + (p.interleaved ? (size_t)p.K : (size_t)p.I * p.K)); }
     // columns c .. c + 4 of h
@@ -260,11 +263,22 @@ struct GatedSkinnyOut {
         }
     }
 };
-template <int R, int NW, int D, int NF, bool NT>
+template <int R, int NW, int D, int NF, bool NT, bool EXPERTS>
 __global__ __launch_bounds__(64 * NW) void gated_skinny_kernel(GatedForward p) {
     extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
+    int col0 = blockIdx.x * (8 * NF);
+    if constexpr (EXPERTS) {   // up to 16 R of an expert's rows
+        const GroupedTile t = grouped_tile(p.offsets, p.E, p.R, 16 * R, p.tiles_n, p.K, 2 * p.I, xcd_chunk_order(blockIdx.x, gridDim.x, kCuPerXcd));
+        if (t.expert < 0) return;
+        col0 = t.tile_n * (8 * NF);
+        p.x += (size_t)t.row0 * p.K;
+        p.w13 += (size_t)t.expert * 2 * p.I * p.K;
+        p.h += (size_t)t.row0 * p.I;
+        if (p.gate_up) p.gate_up += (size_t)t.row0 * 2 * p.I;
+        p.R = t.rows;
+    }
     gemm_skinny_body<GatedMma, R, NW, D, NF, NT>(smem, (const uint8_t*)p.x, (const uint8_t*)p.w13, nullptr, p.R, p.I, 2 * p.K, 1.0f,
-                                                 SkinnyScales{nullptr, nullptr, 0, 0, 0}, GatedSkinnyOut{p});
+                                                 SkinnyScales{nullptr, nullptr, 0, 0, 0}, GatedSkinnyOut{p, col0});
 }
 
 struct GatedBackward {
@@ -324,33 +338,45 @@ __global__ __launch_bounds__(256) void gated_dgrad_kernel(GatedBackward p) {
     }(std::make_integer_sequence<int, Tile::F>());
 }
 
-// Few rows of a dense block in the backward pass: one pass over W2, whose rows the contraction crosses. A workgroup owns NC columns of h and all rows
-// of dy; its four waves take a quarter of the K-steps each, on their own: 64 rows of NC columns of W2 and as many elements of every row of dy
-// into a ring of D stages of LDS that belongs to the wave, W2's read with the transposing loads (gemm_layouts.h). The four partial sums
-// meet in LDS, in order, and the activation's gradients follow from what was kept, which the threads have loaded at the start.
+// Few rows of a dense block or an expert in the backward pass: one pass over W2, whose rows the contraction crosses. A workgroup owns NC columns of
+// h and all rows of dy; its W waves take a part of the K-steps each, on their own: 64 rows of NC columns of W2 and as many elements of every
+// row of dy into a ring of D stages of LDS that belongs to the wave, W2's read with the transposing loads (gemm_layouts.h). The waves' partial
+// sums meet in LDS, in order, and the activation's gradients follow from what was kept, which the threads have loaded at the start.
 // R: 16 rows of dy each.
-template <int R, int NC, int D>
+template <int R, int W, int NC, int D>
 struct SkinnyAcross {
-    static constexpr int kWaves = 4, kRow = 2 * NC, kW = 64 * kRow, kStage = kW + R * 2048, kRegion = D * kStage, kLds = kWaves * kRegion;
+    static constexpr int kWaves = W, kRow = 2 * NC, kW = 64 * kRow, kStage = kW + R * 2048, kRegion = D * kStage, kLds = kWaves * kRegion;
     static constexpr int kChunks = kRow / 16, kLoadRows = 64 / kChunks, kLoads = kW / 1024, kAll = kLoads + 2 * R, F = NC / 16;
     static_assert(kLds <= 160 * 1024 && (D - 1) * kAll < 64 && R * F * 1024 <= kRegion);
     // 16-byte chunk c of LDS row k lies at c ^ swz(k) (rows of 64 bytes: four share a line of the banks)
     static __device__ __forceinline__ uint32_t swz(uint32_t k) { return NC == 64 ? across_swz128(k) : 2u * ((k >> 3) & 1u); }
 };
-template <int R, int NC, int D, bool NT>
-__global__ __launch_bounds__(256) void gated_dgrad_skinny_kernel(GatedBackward p) {
-    typedef SkinnyAcross<R, NC, D> S;
+template <int R, int W, int NC, int D, bool NT, bool EXPERTS>
+__global__ __launch_bounds__(64 * W) void gated_dgrad_skinny_kernel(GatedBackward p) {
+    typedef SkinnyAcross<R, W, NC, D> S;
+    constexpr int kThreads = 64 * W;
     extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
     const uint32_t lane = lane_id(), w = wave_id(), r = lane & 15, g = lane >> 4;
-    const int col0 = xcd_chunk_order(blockIdx.x, gridDim.x, kCuPerXcd) * NC;
+    int col0 = xcd_chunk_order(blockIdx.x, gridDim.x, kCuPerXcd) * NC;
+    if constexpr (EXPERTS) {   // up to 16 R of an expert's rows
+        const GroupedTile t = grouped_tile(p.offsets, p.E, p.R, 16 * R, p.tiles_n, p.N, p.I, xcd_chunk_order(blockIdx.x, gridDim.x, kCuPerXcd));
+        if (t.expert < 0) return;
+        col0 = t.tile_n * NC;
+        p.dy += (size_t)t.row0 * p.N;
+        p.w2 += (size_t)t.expert * p.N * p.I;
+        p.gate_up += (size_t)t.row0 * 2 * p.I;
+        p.dgate_up += (size_t)t.row0 * 2 * p.I;
+        if (p.h) p.h += (size_t)t.row0 * p.I;
+        p.R = t.rows;
+    }
     const int nk = (p.N + kLayoutStep - 1) / kLayoutStep;
     const int s0 = nk * (int)w / S::kWaves, n = nk * ((int)w + 1) / S::kWaves - s0;
 
     // this thread's elements of the result: four columns of a row each, and their kept values
-    constexpr int kItems = (R * S::F * 64 + 255) / 256;
+    constexpr int kItems = (R * S::F * 64 + kThreads - 1) / kThreads;
     v2i kept_g[kItems], kept_u[kItems];
     auto place = [&](int i, int& row, int& col) {
-        const int t = i * 256 + threadIdx.x, l = t & 63;
+        const int t = i * kThreads + threadIdx.x, l = t & 63;
         row = t / (S::F * 64) * 16 + (l & 15);
         col = col0 + (t >> 6) % S::F * 16 + 4 * (l >> 4);
         return t < R * S::F * 64 && row < p.R && col < p.I;
@@ -453,9 +479,9 @@ __global__ __launch_bounds__(256) void gated_dgrad_skinny_kernel(GatedBackward p
     for (int i = 0; i < kItems; ++i) {
         int row, col;
         if (!place(i, row, col)) continue;
-        v4f dh = red[i * 256 + threadIdx.x];
+        v4f dh = red[i * kThreads + threadIdx.x];
 #pragma unroll
-        for (int v = 1; v < S::kWaves; ++v) dh += red[v * R * S::F * 64 + i * 256 + threadIdx.x];
+        for (int v = 1; v < S::kWaves; ++v) dh += red[v * R * S::F * 64 + i * kThreads + threadIdx.x];
         float dg[4], du[4], h[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -515,33 +541,58 @@ static int launch_gated_form(const P& p, hipStream_t s) {
     if (p.clamped) return p.interleaved ? launch_gated<Tile, true, true>(p, s) : launch_gated<Tile, true, false>(p, s);
     return p.interleaved ? launch_gated<Tile, false, true>(p, s) : launch_gated<Tile, false, false>(p, s);
 }
-template <int R, int NW, int D, int NF, bool NT>
-static int launch_gated_skinny_kernel(const GatedForward& p, hipStream_t s) {
-    auto kern = gated_skinny_kernel<R, NW, D, NF, NT>;
+// Workgroups of the kernels for few rows: the column blocks, of every 16 R rows of an expert where there are experts.
+template <int R, typename P>
+static long long skinny_grid(P& p, int cols) {
+    p.tiles_n = (p.I + cols - 1) / cols;
+    return p.offsets ? grouped_tiles_m(p.R, p.E, 16 * R) * p.tiles_n : p.tiles_n;
+}
+// Weights past the caches: where they are too large to stay, and where the rows of memory that the kernels load are whole cache lines; a line that two
+// loads share would come from HBM twice (one row, I = 9408, K = 2360 25.4 us with the hint, 23.4 without; 40 experts of 1432 x 3000, 64 rows 159 / 124;
+// but one row, I = 11008, K = 4096 29.6 / 31.9).
+static bool skinny_nt(const void* w, long long bytes, long long row_bytes) { return bytes >= kSkinnyNtBytes && (((uintptr_t)w | row_bytes) % 128) == 0; }
+template <int R, int NW, int D, int NF, bool EXPERTS = false>
+static int launch_gated_skinny_kernel(GatedForward p, hipStream_t s) {
+    const bool nt = skinny_nt(p.w13, EXPERTS ? kSkinnyNtBytes : 4ll * p.I * p.K, 2ll * p.K);
+    auto kern = nt ? gated_skinny_kernel<R, NW, D, NF, true, EXPERTS> : gated_skinny_kernel<R, NW, D, NF, false, EXPERTS>;
     constexpr int lds_bytes = skinny_lds_bytes(R, NW, D, false, NF);
     static_assert(lds_bytes <= 160 * 1024, "LDS of one CU");
-    static DeviceOnce configured;
-    if (!set_lds_limit_once((const void*)kern, lds_bytes, configured)) return HK_ERR_LAUNCH;
-    hipLaunchKernelGGL(kern, dim3((p.I + 8 * NF - 1) / (8 * NF)), dim3(64 * NW), lds_bytes, s, p);
+    static DeviceOnce configured[2];
+    const long long grid = skinny_grid<R>(p, 8 * NF);
+    if (grid >= kMaxWorkgroups) return HK_ERR_BAD_SHAPE;
+    if (!set_lds_limit_once((const void*)kern, lds_bytes, configured[nt])) return HK_ERR_LAUNCH;
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * NW), lds_bytes, s, p);
     return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
 }
-// R: 16 rows of x each. Rows of the weights a workgroup: 16 (NF = 1) while 32 would leave half of the CUs without one; 64 (NF = 4, three waves of
-// three stages) where their rounds over the CUs, one workgroup each, take in fewer bytes than those of 32 (NF = 2, four waves): x is loaded once
-// a workgroup, and a CU's loads into LDS, not HBM, bound more than 16 rows. (us from HBM, 32 / 64 rows of weights a workgroup / 64-tile kernel:
-// 48 rows, I = 14336, K = 4096 55.7 / 43.6 / 55.0; 32 rows 47.5 / 40.4 / 55.2; 32 rows, I = 9216, K = 8192 65.8 / 68.2 / 74.1; with 16 rows
-// and 32 a workgroup 41.1 / - / 55.1, one row 38.9. 1 row, I = 2048, K = 7168: 11.2 / - / 30.2.)
-template <int R, int D1, int D2>
+// R: 16 rows of x each. Rows of the weights a workgroup: 16 (NF = 1) while 32 would leave half of the CUs without one; 64 (NF = 4) where their rounds
+// over the CUs, one workgroup each, take in fewer bytes than those of 32 (NF = 2): x is loaded once a workgroup, and a CU's loads into LDS, not
+// HBM, bound more than 16 rows. (us from HBM, 32 / 64 rows of weights a workgroup / 64-tile kernel: 48 rows, I = 14336, K = 4096 55.7 / 42.2 /
+// 55.0; 32 rows 47.5 / 39.0 / 55.2; 32 rows, I = 9216, K = 8192 63.7 / 68.2 / 74.1; with 16 rows and 32 a workgroup 37.6 / - / 55.1, one row
+// 36.1. 1 row, I = 2048, K = 7168: 11.2 / - / 30.2.) Rows of weights that are not whole cache lines take two accesses a piece, which bounds a CU, so that one
+// with a workgroup more than the others is waited for: 16 again while x is a few rows (one row, 16 / 32: I = 9408, K = 2360 18.4 / 23.4; 16 rows,
+// I = 7400, K = 3000 28.3 / 25.3).
+// Waves and stages of a workgroup for 16, 32 and 64 rows of weights: as many stages as fit while the CUs hold the workgroups in one round, two workgroups a
+// CU where there are more (I = 14336, K = 4096, one row 38.5 / 35.9; I = 2880, K = 2880 7.4 / 8.0).
+struct SkinnyForm { int waves, stages; };
+template <int R> constexpr SkinnyForm kSkinnyForms[2][3] = {};   // [one round, more]
+template <> constexpr SkinnyForm kSkinnyForms<1>[2][3] = {{{4, 4}, {4, 4}, {}}, {{4, 4}, {4, 3}, {}}};
+template <> constexpr SkinnyForm kSkinnyForms<2>[2][3] = {{{4, 3}, {4, 3}, {3, 3}}, {{}, {3, 3}, {3, 2}}};
+template <> constexpr SkinnyForm kSkinnyForms<3>[2][3] = {{{4, 4}, {4, 4}, {3, 3}}, {{}, {4, 4}, {2, 2}}};
+template <> constexpr SkinnyForm kSkinnyForms<4>[2][3] = {{{4, 3}, {4, 3}, {3, 3}}, {{}, {4, 3}, {2, 2}}};
+template <int R>
 static int launch_gated_skinny_rows(const GatedForward& p, hipStream_t s) {
     const int cus = moe_num_compute_units();
-    const bool nt = 4ll * p.I * p.K >= kSkinnyNtBytes;
-    auto launch = [&]<int W, int D, int NF>() {
-        return nt ? launch_gated_skinny_kernel<R, W, D, NF, true>(p, s) : launch_gated_skinny_kernel<R, W, D, NF, false>(p, s);
-    };
     auto rounds = [&](int cols) { return ((p.I + cols - 1) / cols + cus - 1) / cus; };
-    if (2ll * ((p.I + 15) / 16) <= cus) return launch.template operator()<4, D1, 1>();
+    auto launch = [&]<int I>() {
+        constexpr SkinnyForm one = kSkinnyForms<R>[0][I], more = kSkinnyForms<R>[1][I];
+        if constexpr (more.waves > 0)
+            if (rounds(8 << I) > 1) return launch_gated_skinny_kernel<R, more.waves, more.stages, 1 << I>(p, s);
+        return launch_gated_skinny_kernel<R, one.waves, one.stages, 1 << I>(p, s);
+    };
+    if (2ll * ((p.I + 15) / 16) <= cus || (R == 1 && p.R <= 4 && p.K % 64 != 0)) return launch.template operator()<0>();
     if constexpr (R > 1)
-        if (rounds(32) * (64 + 16 * R) < rounds(16) * (32 + 16 * R)) return launch.template operator()<3, 3, 4>();
-    return launch.template operator()<4, D2, 2>();
+        if (rounds(32) * (64 + 16 * R) < rounds(16) * (32 + 16 * R)) return launch.template operator()<2>();
+    return launch.template operator()<1>();
 }
 // Not for short rows of many columns, where a wave has few K-steps of its own (16 rows, skinny / 64-tile kernel, us: I = 57344, K = 512 35.4 / 27.9;
 // I = 100000, K = 1024 89.4 / 88.9, 64 rows 105 / 95; I = 28672, K = 2048, 64 rows 52.9 / 59.9).
@@ -550,19 +601,21 @@ static bool use_gated_skinny(int R, int I, int K) {
     return (I + 15) / 16 <= moe_num_compute_units() || K >= (R <= 32 ? 1024 : 2048);
 }
 static int launch_gated_skinny(const GatedForward& p, hipStream_t s) {
-    if (p.R <= 16) return launch_gated_skinny_rows<1, 4, 4>(p, s);
-    if (p.R <= 32) return launch_gated_skinny_rows<2, 3, 3>(p, s);
-    if (p.R <= 48) return launch_gated_skinny_rows<3, 4, 4>(p, s);
-    return launch_gated_skinny_rows<4, 3, 3>(p, s);
+    if (p.R <= 16) return launch_gated_skinny_rows<1>(p, s);
+    if (p.R <= 32) return launch_gated_skinny_rows<2>(p, s);
+    if (p.R <= 48) return launch_gated_skinny_rows<3>(p, s);
+    return launch_gated_skinny_rows<4>(p, s);
 }
-template <int R, int NC, int D>
-static int launch_gated_dgrad_skinny_kernel(const GatedBackward& p, hipStream_t s) {
-    const bool nt = 2ll * p.I * p.N >= kSkinnyNtBytes;
-    auto kern = nt ? gated_dgrad_skinny_kernel<R, NC, D, true> : gated_dgrad_skinny_kernel<R, NC, D, false>;
-    constexpr int lds_bytes = SkinnyAcross<R, NC, D>::kLds;
+template <int R, int W, int NC, int D, bool EXPERTS = false>
+static int launch_gated_dgrad_skinny_kernel(GatedBackward p, hipStream_t s) {
+    const bool nt = skinny_nt(p.w2, EXPERTS ? kSkinnyNtBytes : 2ll * p.I * p.N, 2ll * p.I);
+    auto kern = nt ? gated_dgrad_skinny_kernel<R, W, NC, D, true, EXPERTS> : gated_dgrad_skinny_kernel<R, W, NC, D, false, EXPERTS>;
+    constexpr int lds_bytes = SkinnyAcross<R, W, NC, D>::kLds;
     static DeviceOnce configured[2];
+    const long long grid = skinny_grid<R>(p, NC);
+    if (grid >= kMaxWorkgroups) return HK_ERR_BAD_SHAPE;
     if (!set_lds_limit_once((const void*)kern, lds_bytes, configured[nt])) return HK_ERR_LAUNCH;
-    hipLaunchKernelGGL(kern, dim3((p.I + NC - 1) / NC), dim3(256), lds_bytes, s, p);
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * W), lds_bytes, s, p);
     return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
 }
 // 32 columns a workgroup while that gives no CU a second one (rows of W2 in pieces of 64 bytes: what a CU has under way is counted in
@@ -574,9 +627,56 @@ static bool use_gated_dgrad_skinny(int R, int I) {
 }
 static int launch_gated_dgrad_skinny(const GatedBackward& p, hipStream_t s) {
     const bool narrow = (p.I + 31) / 32 <= moe_num_compute_units();
-    if (p.R <= 16) return narrow ? launch_gated_dgrad_skinny_kernel<1, 32, 6>(p, s) : launch_gated_dgrad_skinny_kernel<1, 64, 4>(p, s);
-    if (p.R <= 32) return narrow ? launch_gated_dgrad_skinny_kernel<2, 32, 5>(p, s) : launch_gated_dgrad_skinny_kernel<2, 64, 3>(p, s);
-    return launch_gated_dgrad_skinny_kernel<4, 32, 3>(p, s);
+    if (p.R <= 16) return narrow ? launch_gated_dgrad_skinny_kernel<1, 4, 32, 6>(p, s) : launch_gated_dgrad_skinny_kernel<1, 4, 64, 4>(p, s);
+    if (p.R <= 32) return narrow ? launch_gated_dgrad_skinny_kernel<2, 4, 32, 5>(p, s) : launch_gated_dgrad_skinny_kernel<2, 4, 64, 3>(p, s);
+    return launch_gated_dgrad_skinny_kernel<4, 4, 32, 3>(p, s);
+}
+
+// Experts with few rows, of which the host knows only how many there are on average where they spread evenly. Two workgroups a CU and more, by their LDS: a
+// launch has many rounds of them, and one's start and end are the others' time. Forward: 16 rows of the weights a workgroup while the CUs hold them
+// in one round, 32 for few rounds, else 64; more than 8 rows an expert only where the 128-tile kernel has more than one round of its two
+// workgroups a CU. Backward: 32 columns a workgroup while they are one round, else 64, but for the 128-tile kernel's one round. Beyond one round not
+// for short rows, where a wave has few K-steps. (us, tile kernels / these: forward, 128 experts of 2880 x 2880, 150 rows 531 / 464, 1000 734 / 666, 2000 742 / 678, 3200 756 / 764; 64 of 1536 x 4096,
+// 256 rows 317 / 234; 48 of 2048 x 7168, 1000 rows 467 / 437; 9 of 576 x 2672, one row 16.1 / 8.2, but 40 rows 17.3 / 20.1. Backward, the same 296 /
+// 240, 395 / 347, 402 / 383, 410 / 442; 170 / 140; 282 / 263; 16.6 / 8.9, 17.0 / 12.8; 40 experts of 1432 x 1024, 40 rows, one round of tiles,
+// 22.3 / 29.1. Short rows: 30 of 3000 x 264, 64 rows forward 33.5 / 37.5; 60 of 2048 x 768, 200 rows backward 41.5 / 44.9. Of the forms, forward: 20 experts of 2880 x 2880, 8 rows, 32 a workgroup 42.1, 64 48.1; 128 of 768 x 2048, 256 rows 127 / 118.)
+struct ExpertRows {
+    double used, mean;
+    ExpertRows(int R, int E) : used(-E * std::expm1(R * std::log1p(-1.0 / E))), mean(R / used) {}
+    double blocks(int I, int cols) const { return used * ((I + cols - 1) / cols); }
+};
+constexpr int kExpertRows16 = 8, kExpertRows32 = 20;   // most on average for 16 and for 32 rows a workgroup
+constexpr int kExpertMinWide = 1024;
+constexpr int kExpertMaxI = 1 << 16;   // (their grids grow with I faster than the tiles')
+static bool launch_gated_experts_skinny(const GatedForward& p, hipStream_t s, int& st) {
+    const ExpertRows rows(p.R, p.E);
+    const int cus = moe_num_compute_units();
+    if (rows.mean > kExpertRows32 || p.I > kExpertMaxI || (p.K < kExpertMinWide && rows.blocks(p.I, 16) > cus)) return false;
+    if (rows.mean > kExpertRows16) {
+        if (rows.blocks(p.I, 16) <= cus) st = launch_gated_skinny_kernel<2, 4, 3, 2, true>(p, s);
+        else if (rows.blocks(p.I, 64) > 2 * cus) st = launch_gated_skinny_kernel<2, 2, 3, 4, true>(p, s);
+        else return false;
+    } else if (rows.blocks(p.I, 8) <= cus) {
+        st = launch_gated_skinny_kernel<1, 4, 4, 1, true>(p, s);
+    } else if (rows.blocks(p.I, 16) < (p.K < 2048 ? 2 : 6) * cus) {
+        st = launch_gated_skinny_kernel<1, 4, 3, 2, true>(p, s);
+    } else {
+        st = launch_gated_skinny_kernel<1, 4, 2, 4, true>(p, s);
+    }
+    return true;
+}
+static bool launch_gated_experts_skinny(const GatedBackward& p, hipStream_t s, int& st) {
+    const ExpertRows rows(p.R, p.E);
+    const int cus = moe_num_compute_units();
+    if (rows.mean > kExpertRows32 || p.I > kExpertMaxI) return false;
+    if (rows.blocks(p.I, 32) <= cus) {
+        st = rows.mean <= kExpertRows16 ? launch_gated_dgrad_skinny_kernel<1, 4, 32, 3, true>(p, s) : launch_gated_dgrad_skinny_kernel<2, 4, 32, 5, true>(p, s);
+    } else {
+        const double tiles = rows.blocks(p.I, 128);
+        if (p.N < kExpertMinWide || (tiles > cus && tiles <= 2 * cus)) return false;
+        st = launch_gated_dgrad_skinny_kernel<2, 2, 64, 3, true>(p, s);
+    }
+    return true;
 }
 
 // Whether the forward product takes tiles of 128 rows and 256 columns: by rounds over the CUs times a fixed part and a part per K-step, us (a
@@ -622,6 +722,7 @@ extern "C" int hk_gated_gemm(const void* x_bf16, const void* w13_bf16, const int
                    R, E, I, K, 0, interleaved != 0, activation == 1, {alpha, limit}};
     if (const int st = check_gate(activation, p.gate)) return st;
     if (!p.offsets && use_gated_skinny(R, I, K)) return launch_gated_skinny(p, (hipStream_t)stream);
+    if (int st; p.offsets && launch_gated_experts_skinny(p, (hipStream_t)stream, st)) return st;
     return launch_gated_choice(p, K, 2 * I, (hipStream_t)stream);
 }
 
@@ -637,5 +738,6 @@ extern "C" int hk_gated_gemm_dgrad(const void* dy_bf16, const void* w2_bf16, con
                     (uint16_t*)dgate_up_bf16, (uint16_t*)h_bf16_or_null, R, E, N, I, 0, interleaved != 0, activation == 1, {alpha, limit}};
     if (const int st = check_gate(activation, p.gate)) return st;
     if (!p.offsets && use_gated_dgrad_skinny(R, I)) return launch_gated_dgrad_skinny(p, (hipStream_t)stream);
+    if (int st; p.offsets && launch_gated_experts_skinny(p, (hipStream_t)stream, st)) return st;
     return launch_gated_choice(p, N, I, (hipStream_t)stream);
 }

@@ -46,7 +46,7 @@ struct SkinnyScales {
     const uint8_t* SA; const uint8_t* SB; int sa_pitch, sb_pitch, row_bytes;
 };
 // OUT: what the sums become. SkinnyPlain: C. With kPairs, B is one half of the operand and out.other() the other, each in rows of out.pitch()
-// bytes: a workgroup owns rows n0 .. n0 + 8 NF of both (NF / 2 fragments of the one, then of the other; NF = 1: the two halves of one), and
+// bytes: a workgroup owns rows out.first() .. + 8 NF of both (NF / 2 fragments of the one, then of the other; NF = 1: the two halves of one), and
 // out.store(row, n, first, second) takes both sums of rows n .. n + 4 of them (N % 4 == 0).
 struct SkinnyPlain { static constexpr bool kPairs = false; };
 template <typename MMA, int R, int NW, int D, int NF = 2, bool NT = false, typename OUT = SkinnyPlain>
@@ -63,7 +63,8 @@ __device__ __forceinline__ void gemm_skinny_body(
     static_assert(NW * R * NF * 1024 <= NW * kRegion, "the partial sums reuse the stages");
     const int lane = lane_id(), w = wave_id();
     const uint32_t r = lane & 15, g = lane >> 4;
-    const int n0 = blockIdx.x * kRowsB;
+    int n0 = blockIdx.x * kRowsB;
+    if constexpr (kPairs) n0 = out_pairs.first();
     const int rows_b = N - n0 < kRowsB ? N - n0 : kRowsB;
     uint32_t pitch_b = (uint32_t)K;
     v4i srd_other = {0, 0, 0, 0};

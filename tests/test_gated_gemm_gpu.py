@@ -342,3 +342,13 @@ def test_few_rows_of_wide_blocks(hk, R, act, interleaved):
     """Decode: every number of row fragments, with 16, 32 and 64 rows of weights a workgroup, K that ends inside a K-step, kept values or not."""
     for I, K, keep in ((8, 2056, True), (1032, 136, True), (4104, 1096, False), (9000, 2120, R % 2 == 0)):
         _run(hk, [R], 0, I, K, act, interleaved, R + I, True, keep=keep)
+
+
+@pytest.mark.parametrize("act,interleaved", [("silu", True), ("swiglu_oai", False), ("silu", False), ("swiglu_oai", True)])
+@pytest.mark.parametrize("rows,unused,I,K", [
+    ([0, 1, 3, 0, 1], 0, 136, 2120), ([0, 0, 0, 17, 0, 0, 33], 6, 264, 584), ([5, 2, 0, 1, 0, 0, 20] * 6, 3, 520, 1096), ([1, 0, 7] * 21, 0, 392, 1032),
+    ([16, 17, 7, 12], 1, 264, 1096), ([12, 31, 0, 33, 8, 15, 20] * 9, 40, 520, 1032), ([9, 20, 40, 3] * 14, 0, 1032, 1160), ([1] * 200, 0, 72, 1992)])
+def test_few_rows_of_experts(hk, rows, unused, I, K, act, interleaved):
+    """Decode with experts: one and two row fragments and every number of columns a workgroup in both directions, experts with more rows than a
+    workgroup takes, without any, and with rows behind the last."""
+    _run(hk, rows, unused, I, K, act, interleaved, I + K + len(rows), False, keep=len(rows) % 2 == 0)
