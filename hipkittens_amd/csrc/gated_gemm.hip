@@ -697,8 +697,19 @@ static bool use_wide_tile(const GatedForward& p) {
     return wide < small && wide < rounds(tiles_m(256) * cols / cus) * (kLargeFixed + kLargeStep * steps);
 }
 
+// 64x64 tiles, two workgroups a CU, where the CUs hold them so in one round and one a CU would not; rows of whole cache lines (others take two accesses
+// a piece, which bounds a CU here). (us, the kernel otherwise chosen / this: 128 rows forward, I = 4104, K = 4096, 258 tiles, 39.9 / 29.1; I = 8192,
+// K = 2048, 512 tiles 25.2 / 23.4; I = 14336, K = 4096, 896 tiles 55.7 / 76.3; 190 rows of 2880 x 2880, 270 tiles 25.5 / 26.7; backward, 520 rows of
+// 2880 x 2880, 405 tiles 29.4 / 24.3, of 2440 x 6376, 351 tiles, 56.8 / 72.3. 2 experts of 2048 x 7168, 200 rows forward 69.8 / 39.8; 4 of
+// 2880 x 2880 31.4 / 34.5.)
+static bool use_pair_tile(int R, int E, int in, int out, bool dense) {
+    const int cus = moe_num_compute_units();
+    const double tiles = grouped_tiles(R, E, out, 64, dense);
+    return tiles > cus && tiles <= 2 * cus && in % 64 == 0;
+}
 template <typename P>
 static int launch_gated_choice(const P& p, int in, int out, hipStream_t s) {
+    if (use_pair_tile(p.R, p.E, in, out, !p.offsets)) return launch_gated_form<LayoutTile64Pair>(p, s);
     if constexpr (std::is_same_v<P, GatedForward>)
         if (use_wide_tile(p)) return launch_gated_form<LayoutTileWide>(p, s);
     switch (grouped_choice(p.R, p.E, in, out, !p.offsets)) {

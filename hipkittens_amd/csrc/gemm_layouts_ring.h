@@ -235,20 +235,21 @@ __device__ __forceinline__ void ring_product(uint8_t* smem, const TileOperand& A
 }
 
 // 128x128 and 64x64 tiles in the same manner, for problems with no more tiles than CUs, where one workgroup has a CU to itself: four or
-// eight LDS stages, all but one or two of them ahead, the next fragments read behind the MFMAs of these (a quarter of the tile a wave).
+// eight LDS stages (STAGES), all but one or two of them ahead, the next fragments read behind the MFMAs of these (a quarter of the tile a wave).
 // Weight gradient of 16384 rows, 1024 x 1024, 64 tiles of 256 K-steps: 155 us with two stages of 128x128, 117 with four, 31 bytes a clock
 // into each CU, which bounds it (five stages: 116); 256 tiles of 64x64 with a barrier every K-step 70, every second 66. A K-step of
 // 64x64 takes 0.23 to 0.25 us, of 128x128 0.45, also where few rows leave most of A's loads without memory behind them: the issue of
-// the loads into LDS bounds a CU, not memory.
-template <int TILE>
+// the loads into LDS bounds a CU, not memory. 64x64 with four stages: two workgroups on a CU, for more tiles than CUs.
+template <int TILE, int STAGES>
 struct DeepStages {
-    static constexpr int kStages = TILE == 128 ? 4 : 8, kBytes = 2 * TILE * 128;
-    static constexpr int kGroup = TILE == 128 ? 1 : 2;   // K-steps from barrier to barrier
+    static constexpr int kStages = STAGES, kBytes = 2 * TILE * 128;
+    static constexpr int kGroup = STAGES == 8 ? 2 : 1;   // K-steps from barrier to barrier
 };
-template <int TILE, int A_ORDER, int B_ORDER>
+template <int TILE, int STAGES, int A_ORDER, int B_ORDER>
 __device__ __forceinline__ void deep_product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K,
                                              v4f (&acc)[TILE / 32][TILE / 32]) {
-    constexpr int S = DeepStages<TILE>::kStages, kStage = DeepStages<TILE>::kBytes, U = DeepStages<TILE>::kGroup, F = TILE / 32, kLoads = TILE / 32;
+    typedef DeepStages<TILE, STAGES> Stages;
+    constexpr int S = STAGES, kStage = Stages::kBytes, U = Stages::kGroup, F = TILE / 32, kLoads = TILE / 32;
     const uint32_t lds0 = (uint32_t)(uintptr_t)smem, w = wave_id();
     const uint32_t mine = to_sgpr(lds0 + w * 1024u);
     RingOperand<A_ORDER, TILE> oa;
@@ -545,13 +546,13 @@ struct LayoutTile256 {
     }
 };
 
-template <int TILE>
+template <int TILE, int STAGES>
 struct LayoutTileDeep {
-    static constexpr int kTile = TILE, kPatch = kTile / 2, F = TILE / 32, kLds = DeepStages<TILE>::kStages * DeepStages<TILE>::kBytes;
+    static constexpr int kTile = TILE, kPatch = kTile / 2, F = TILE / 32, kLds = STAGES * DeepStages<TILE, STAGES>::kBytes;
     static constexpr int kTileCols = kTile, kPatchCols = kPatch, FC = F;
     template <int A_ORDER, int B_ORDER>
     static __device__ __forceinline__ void product(uint8_t* smem, const TileOperand& A, const TileOperand& B, int K, v4f (&acc)[F][F]) {
-        deep_product<TILE, A_ORDER, B_ORDER>(smem, A, B, K, acc);
+        deep_product<TILE, STAGES, A_ORDER, B_ORDER>(smem, A, B, K, acc);
     }
     static __device__ __forceinline__ void read_row(const v4f (&acc)[F], v4f (&v)[F]) {
 #pragma unroll
@@ -570,8 +571,9 @@ struct LayoutTileWide {
         for (int n = 0; n < FC; ++n) v[n] = acc[n];
     }
 };
-typedef LayoutTileDeep<128> LayoutTile128Deep;
-typedef LayoutTileDeep<64> LayoutTile64Deep;
+typedef LayoutTileDeep<128, 4> LayoutTile128Deep;
+typedef LayoutTileDeep<64, 8> LayoutTile64Deep;
+typedef LayoutTileDeep<64, 4> LayoutTile64Pair;
 
 // Whether 256x256 tiles take less time than 128x128 ones: rounds of workgroups over the CUs (one of the large kernel or two of
 // the small one on a CU; a round that is not full is a round, later ones run into each other) times a fixed part and a part per

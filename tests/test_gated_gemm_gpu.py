@@ -352,3 +352,12 @@ def test_few_rows_of_experts(hk, rows, unused, I, K, act, interleaved):
     """Decode with experts: one and two row fragments and every number of columns a workgroup in both directions, experts with more rows than a
     workgroup takes, without any, and with rows behind the last."""
     _run(hk, rows, unused, I, K, act, interleaved, I + K + len(rows), False, keep=len(rows) % 2 == 0)
+
+
+@pytest.mark.parametrize("act,interleaved", [("silu", True), ("swiglu_oai", False), ("silu", False), ("swiglu_oai", True)])
+@pytest.mark.parametrize("rows,unused,I,wide,dense", [
+    ([200], 0, 2632, 128, True), ([500], 0, 2312, 64, True), ([449], 0, 2504, 576, True), ([100, 0, 30, 65] * 5, 4, 328, 320, False),
+    ([100, 0, 30, 65] * 5, 0, 712, 256, False)])
+def test_two_small_tiles_a_cu(hk, rows, unused, I, wide, dense, act, interleaved):
+    """64x64 tiles, more of them than CUs and no more than two a CU, forward or backward; fewer K-steps than stages, as many, and more."""
+    _run(hk, rows, unused, I, wide, act, interleaved, I + wide, dense)
