@@ -169,12 +169,13 @@ __device__ __forceinline__ void place_waves(SortLds& lds, int digits, int base) 
     }
     __syncthreads();
 }
-__device__ __forceinline__ void clear_counts(SortLds& lds) {
-    for (int i = threadIdx.x; i < kSortWaves * kMaxDigits; i += kSortThreads) (&lds.count[0][0])[i] = 0;
+__device__ __forceinline__ void clear_counts(SortLds& lds, Digit digit) {
+    for (int i = threadIdx.x; i < kSortWaves << digit.bits; i += kSortThreads) lds.count[i >> digit.bits][i & (digit.count() - 1)] = 0;
     __syncthreads();
 }
 
-// Tokens of one workgroup, ITER a thread: all passes at once, the items in LDS in between. (8192 tokens of 50257 rows: in one workgroup 35 us for the
+// Tokens of one workgroup, ITER a thread: all passes at once, the items in LDS in between. (7 tokens of 1036 rows with one a thread 4.7 us, with four
+// 7.3; 8192 tokens of 50257 rows: in one workgroup 35 us for the
 // whole gradient of 1024 columns, in two by launches 42.)
 template <int ITER>
 __global__ __launch_bounds__(kSortThreads) void embedding_sort_one_kernel(Ids ids, int T, int V, int passes, int bits, int2* __restrict__ sorted,
@@ -190,7 +191,7 @@ __global__ __launch_bounds__(kSortThreads) void embedding_sort_one_kernel(Ids id
     }
     for (int pass = 0; pass < passes; ++pass) {
         const Digit digit{pass * bits, bits};
-        clear_counts(lds);
+        clear_counts(lds, digit);
         rank_items(lds, key, digit, rank);
         __syncthreads();
         int total = 0;
@@ -273,7 +274,7 @@ __global__ __launch_bounds__(kSortThreads) void embedding_scatter_kernel(Ids ids
             token[i] = (int)at;
         }
     }
-    clear_counts(lds);
+    clear_counts(lds, digit);
     rank_items(lds, key, digit, rank);
     __syncthreads();
     place_waves(lds, digits, (int)threadIdx.x < digits ? lds.base[threadIdx.x] + before : 0);
@@ -415,52 +416,76 @@ __global__ __launch_bounds__(256) void embedding_sum_kernel(EmbedSums p, EmbedRe
     }
 }
 
-// Rows whose tokens are spread over several blocks: the workgroup of the block in which they begin adds the partial sums, each wave a
-// run of the blocks behind it, then the waves' in order.
+// Rows whose tokens are spread over several blocks: the wave of the block in which they begin adds the partial sums in order; of more blocks than it
+// looks ahead the workgroup's waves a run each, and then theirs in order. (A workgroup for each block, which searched for the row's end one
+// place at a time: 21880 tokens of 1795 rows, H = 2184, 22.4 us, so 8.8.)
+constexpr int kJoinBlocks = 16;   // blocks behind its own that a wave looks at
 template <typename T>
 __global__ __launch_bounds__(256) void embedding_join_kernel(EmbedSums p, const T* add, T* dtable) {
     __shared__ float part[4][64][9];
+    __shared__ int more[4];   // blocks of the waves' rows that are left to the workgroup
     const int length = *p.length, lane = lane_id(), w = wave_id();
-    const int64_t b = blockIdx.x, end = (b + 1) * p.block;   // the next block's first token
-    if (end >= length) return;
-    const int row = p.sorted[end].x;
-    if (p.sorted[end - 1].x != row) return;
-    if (b > 0 && p.sorted[b * p.block - 1].x == row) return;   // it began earlier
-    // blocks behind this one that begin with the row
-    const int64_t blocks = (length + p.block - 1) / p.block;
-    int64_t lo = b + 1, hi = blocks;   // block lo begins with it; block hi does not, or is none
-    while (hi - lo > 1) {
-        const int64_t mid = (lo + hi) / 2;
-        if (p.sorted[mid * p.block].x == row) lo = mid;
-        else hi = mid;
-    }
+    const int64_t b = (int64_t)blockIdx.x * 4 + w, end = (b + 1) * p.block;   // the next block's first token
+    // lane l: the row of block b + 1 + l's first token; the last two: of the last tokens of block b and the one in front of it
+    const int64_t place = lane < kJoinBlocks ? end + (int64_t)lane * p.block : lane == 62 ? end - 1 : lane == 63 ? b * p.block - 1 : -1;
+    const int key = place >= 0 && place < length ? p.sorted[place].x : -1;
+    const int row = __builtin_amdgcn_readlane(key, 0);
+    const bool begins = row >= 0 && __builtin_amdgcn_readlane(key, 62) == row && __builtin_amdgcn_readlane(key, 63) != row;
+    const int behind = __ffsll((unsigned long long)~__ballot(lane < kJoinBlocks && key == row)) - 1;   // blocks that begin with the row, if few
     const int col = blockIdx.y * 512 + lane * 8;
     const bool mine = col < p.H;
-    const int64_t count = hi - b, from = count * w / 4, to = count * (w + 1) / 4;   // of blocks b, b + 1, .. hi - 1
-    Row8 sum{};
-    if (mine) {
-        for (int64_t i = from; i < to; i += 8) {
+    // partial sums of blocks first + [from, to), eight at a time
+    auto gather = [&](int64_t first, int from, int to, Row8& sum) __attribute__((always_inline)) {
+        for (int i = from; i < to; i += 8) {
             Row8 r[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 r[k] = Row8{};
-                if (i + k < to) r[k] = load8(p.partial + ((size_t)(b + i + k) * 2 + (i + k == 0 ? 1 : 0)) * p.H + col);
+                if (i + k < to) r[k] = load8(p.partial + ((size_t)(first + i + k) * 2 + (i + k == 0 ? 1 : 0)) * p.H + col);
             }
 #pragma unroll
             for (int k = 0; k < 8; ++k)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) sum.v[j] += r[k].v[j];
         }
+    };
+    int left = 0;
+    if (begins && behind < kJoinBlocks) {
+        if (mine) {
+            const Row8 a = add ? load8(add + (size_t)row * p.H + col) : Row8{};
+            Row8 sum{};
+            gather(b, 0, behind + 1, sum);
+            write_row(p, dtable, row, col, add != nullptr, a, sum);
+        }
+    } else if (begins) {
+        const int64_t blocks = ((int64_t)length + p.block - 1) / p.block;
+        int64_t lo = b + kJoinBlocks, hi = blocks;   // block lo begins with the row; block hi does not, or is none
+        while (hi - lo > 1) {
+            const int64_t mid = (lo + hi) / 2;
+            if (p.sorted[mid * p.block].x == row) lo = mid;
+            else hi = mid;
+        }
+        left = (int)(hi - b);
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) part[w][lane][j] = sum.v[j];
+    if (lane == 0) more[w] = left;
     __syncthreads();
-    if (w == 0 && mine) {
+    for (int v = 0; v < 4; ++v) {
+        const int64_t count = more[v], first = (int64_t)blockIdx.x * 4 + v;   // of blocks first, first + 1, ..
+        if (count == 0) continue;
+        Row8 sum{};
+        if (mine) gather(first, (int)(count * w / 4), (int)(count * (w + 1) / 4), sum);
 #pragma unroll
-        for (int v = 1; v < 4; ++v)
+        for (int j = 0; j < 8; ++j) part[w][lane][j] = sum.v[j];
+        __syncthreads();
+        if (w == 0 && mine) {
+            const int here = p.sorted[(first + 1) * p.block].x;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) sum.v[j] += part[v][lane][j];
-        write_row(p, dtable, row, col, add != nullptr, add ? load8(add + (size_t)row * p.H + col) : Row8{}, sum);
+            for (int u = 1; u < 4; ++u)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) sum.v[j] += part[u][lane][j];
+            write_row(p, dtable, here, col, add != nullptr, add ? load8(add + (size_t)here * p.H + col) : Row8{}, sum);
+        }
+        __syncthreads();
     }
 }
 
@@ -552,8 +577,9 @@ static int launch_embedding_backward(Ids ids, const void* dout, const void* add,
     const int2* sorted = a;
     if (tokens <= kSortAlone) {
         const Fill f = part(0);
-        hipLaunchKernelGGL(tokens <= kSortChunk ? embedding_sort_one_kernel<kSortIter> : embedding_sort_one_kernel<2 * kSortIter>, dim3(1 + f.groups),
-                           dim3(kSortThreads), 0, s, ids, tokens, V, L.passes, L.bits, a, length, f);
+        auto kern = tokens <= kSortThreads ? embedding_sort_one_kernel<1>
+                    : tokens <= kSortChunk ? embedding_sort_one_kernel<kSortIter> : embedding_sort_one_kernel<2 * kSortIter>;
+        hipLaunchKernelGGL(kern, dim3(1 + f.groups), dim3(kSortThreads), 0, s, ids, tokens, V, L.passes, L.bits, a, length, f);
     } else {
         const Fill f = part(0);
         hipLaunchKernelGGL(embedding_count_kernel, dim3(L.chunks + f.groups), dim3(kSortThreads), 0, s, ids, tokens, V, L.chunks, Digit{0, L.bits},
@@ -576,7 +602,7 @@ static int launch_embedding_backward(Ids ids, const void* dout, const void* add,
     const unsigned grid = groups * slabs + (unsigned)((rest.to - rest.from + rest.rows - 1) / rest.rows);
     if (add) hipLaunchKernelGGL((embedding_sum_kernel<T, true>), dim3(grid), dim3(256), 0, s, p, rest, (int)groups, (int)slabs, (const T*)add, (T*)dtable);
     else hipLaunchKernelGGL((embedding_sum_kernel<T, false>), dim3(grid), dim3(256), 0, s, p, rest, (int)groups, (int)slabs, (const T*)nullptr, (T*)dtable);
-    if (blocks > 1) hipLaunchKernelGGL(embedding_join_kernel<T>, dim3(blocks - 1, slabs), dim3(256), 0, s, p, (const T*)add, (T*)dtable);
+    if (blocks > 1) hipLaunchKernelGGL(embedding_join_kernel<T>, dim3((blocks + 2) / 4, slabs), dim3(256), 0, s, p, (const T*)add, (T*)dtable);
     return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
 }
 

@@ -201,3 +201,20 @@ def test_a_table_that_passes_32_bits(hk):
     counts[[V - 1, 0, 262_144, 262_143]] = torch.tensor([2.0, 1.0, 1.0, 1.0], device=DEV)
     assert torch.equal(table[:, 0], counts) and torch.equal(table[:, -1], counts)
     assert float(table.sum(dtype=torch.float64)) == 5.0 * H
+
+
+@pytest.mark.parametrize("T", [1023, 1024, 1025])
+def test_gradient_at_one_token_a_thread(hk, T):
+    for kind in ("outside", "frequent"):
+        _backward(hk, T, 5000, 136, kind, torch.float32, torch.int64, "yes", 1.0, T)
+
+
+@pytest.mark.parametrize("first", [0, 3, 8, 27])
+def test_rows_of_about_as_many_blocks_as_a_wave_joins(hk, first):
+    """Rows of 120 to 160 tokens behind `first` single ones (blocks of eight: 15 to 21 of them), two long ones and a run that ends the list."""
+    lengths = [1] * first + list(range(120, 161, 3)) + [700, 1500, 2, 129]
+    ids = torch.repeat_interleave(torch.arange(len(lengths), device=DEV), torch.tensor(lengths, device=DEV))
+    g = torch.Generator(device=DEV).manual_seed(first)
+    ids = ids[torch.randperm(ids.numel(), device=DEV, generator=g)]
+    for dtype, add in ((torch.float32, "yes"), (torch.bfloat16, "no"), (torch.float32, "in place")):
+        _backward(hk, ids.numel(), len(lengths) + 3, 584, "given", dtype, torch.int32, add, 0.5, first, ids=ids)
