@@ -679,22 +679,33 @@ static bool launch_gated_experts_skinny(const GatedBackward& p, hipStream_t s, i
     return true;
 }
 
-// Whether the forward product takes tiles of 128 rows and 256 columns: by rounds over the CUs times a fixed part and a part per K-step, us (a
-// round begun counts whole between one and two), where there are tiles enough that no kernel with many LDS stages is taken. (us, 128x128 or
-// 256x256, whichever would be chosen / 128x256: 32 experts of 2048 x 7168, 128 rows each 492 / 425; 128 of 2880 x 2880, 64 rows 870 / 841,
-// 128 rows 1008 / 990; 64 of 1536 x 4096, 150 rows 435 / 386; 8 of 4096 x 4096, 128 rows 203 / 158, but 64 of 768 x 2048, 128 rows 131 / 141.
-// On 4300 drawn shapes, time over the best kernel's on average: dense blocks 1.020 without it, 1.014 with it, the tenth with the
-// worst choice 1.063 and 1.01; experts 1.030, 1.027. Not in the backward pass, whose epilogue is the longer.)
-static bool use_wide_tile(const GatedForward& p) {
-    const int cus = moe_num_compute_units(), out = 2 * p.I;
-    const LayoutChoice other = grouped_choice(p.R, p.E, p.K, out, !p.offsets);
-    if (other == kLayout64Deep || other == kLayout128Deep) return false;
-    const double used = p.R < p.E ? p.R : p.E, mean = p.R / used, steps = (p.K + kLayoutStep - 1) / kLayoutStep;
-    auto tiles_m = [&](int tile) { return p.offsets ? used * std::max(1.0, mean / tile + 0.6) : (p.R + tile - 1) / tile; };
+// The tile: 64x64 with many LDS stages where there are no more of them than CUs, else the least of rounds over the CUs times a fixed part and a part per
+// K-step, us. A round begun counts whole between one and two, where the last tiles are most of a round by themselves, and less behind that. (us, with
+// choose_layout's rounds / these: forward, 1831 rows, I = 2280, K = 3784 126.5 / 81.5; 11 experts of 1776 x 2688, 1567 rows 90.9 / 66.0; backward,
+// 1636 rows, I = 9472, N = 840 72.0 / 50.1, but 1547 rows, I = 12376, N = 2600 150.3 / 172.4; on 230 drawn shapes of more than 64 rows 1.3 %
+// less on average.) Tiles of 128 rows and 256 columns, 128x128 or 256x256 otherwise / these: 32 experts of 2048 x 7168, 128 rows each 492 / 425; 128 of
+// 2880 x 2880, 64 rows 870 / 841, 128 rows 1008 / 990; 64 of 1536 x 4096, 150 rows 435 / 386; 8 of 4096 x 4096, 128 rows 203 / 158, but 64 of
+// 768 x 2048, 128 rows 131 / 141. Not in the backward pass, whose epilogue is the longer.
+constexpr double kWideFixed = 6.0, kWideStep = 0.97, kDeepFixed = 4.0, kDeepStepBusy = 0.5;
+enum GatedTile { kGatedWide, kGated256, kGated128, kGated128Deep, kGated64Deep };
+static GatedTile gated_tile(int R, int E, int in, int out, bool dense, bool forward) {
+    const int cus = moe_num_compute_units();
+    auto tiles = [&](int rows, int cols) { return grouped_row_tiles(R, E, rows, dense) * ((out + cols - 1) / cols); };
+    if (tiles(64, 64) <= cus) return kGated64Deep;
+    const double steps = (in + kLayoutStep - 1) / kLayoutStep, small = tiles(128, 128);
     auto rounds = [](double t) { return t <= 1 ? 1.0 : std::max(t + 0.2, std::min(2.0, t + 0.65)); };
-    const double cols = (out + 255) / 256, wide = rounds(tiles_m(128) * cols / cus) * (6.0 + 0.97 * steps);
-    const double small = rounds(tiles_m(128) * ((out + 127) / 128) / (2.0 * cus)) * (kSmallFixed + kSmallStepAlong * steps);
-    return wide < small && wide < rounds(tiles_m(256) * cols / cus) * (kLargeFixed + kLargeStep * steps);
+    const bool deep = small <= cus;
+    GatedTile t = deep ? kGated128Deep : kGated128;
+    double best = deep ? kDeepFixed + kDeepStepBusy * steps : rounds(small / (2.0 * cus)) * (kSmallFixed + kSmallStepAlong * steps);
+    auto consider = [&](GatedTile other, double us) {
+        if (us < best) {
+            best = us;
+            t = other;
+        }
+    };
+    consider(kGated256, rounds(tiles(256, 256) / cus) * (kLargeFixed + kLargeStep * steps));
+    if (forward && !deep) consider(kGatedWide, rounds(tiles(128, 256) / cus) * (kWideFixed + kWideStep * steps));
+    return t;
 }
 
 // 64x64 tiles, two workgroups a CU, where the CUs hold them so in one round and one a CU would not; rows of whole cache lines (others take two accesses
@@ -704,18 +715,20 @@ static bool use_wide_tile(const GatedForward& p) {
 // 2880 x 2880 31.4 / 34.5.)
 static bool use_pair_tile(int R, int E, int in, int out, bool dense) {
     const int cus = moe_num_compute_units();
-    const double tiles = grouped_tiles(R, E, out, 64, dense);
+    const double tiles = grouped_row_tiles(R, E, 64, dense) * ((out + 63) / 64);
     return tiles > cus && tiles <= 2 * cus && in % 64 == 0;
 }
 template <typename P>
 static int launch_gated_choice(const P& p, int in, int out, hipStream_t s) {
     if (use_pair_tile(p.R, p.E, in, out, !p.offsets)) return launch_gated_form<LayoutTile64Pair>(p, s);
-    if constexpr (std::is_same_v<P, GatedForward>)
-        if (use_wide_tile(p)) return launch_gated_form<LayoutTileWide>(p, s);
-    switch (grouped_choice(p.R, p.E, in, out, !p.offsets)) {
-        case kLayout256: return launch_gated_form<LayoutTile256>(p, s);
-        case kLayout128: return launch_gated_form<LayoutTile128>(p, s);
-        case kLayout128Deep: return launch_gated_form<LayoutTile128Deep>(p, s);
+    constexpr bool forward = std::is_same_v<P, GatedForward>;
+    const GatedTile t = gated_tile(p.R, p.E, in, out, !p.offsets, forward);
+    if constexpr (forward)
+        if (t == kGatedWide) return launch_gated_form<LayoutTileWide>(p, s);
+    switch (t) {
+        case kGated256: return launch_gated_form<LayoutTile256>(p, s);
+        case kGated128: return launch_gated_form<LayoutTile128>(p, s);
+        case kGated128Deep: return launch_gated_form<LayoutTile128Deep>(p, s);
         default: return launch_gated_form<LayoutTile64Deep>(p, s);
     }
 }

@@ -92,12 +92,12 @@ inline long long grouped_tiles_m(int R, int E, int tile) {
 // unevenly: one at least, else rows / tile + 0.6. (Forward, us, small / large: N = 4096, K = 7168, 32 experts: 1024 rows 320 / 341,
 // 4096 457 / 482, 8192 764 / 539, 65536 4130 / 2873; 128 experts of 5760 x 2880, 16384 rows 1057 / 947; 8 of 1024 x 1024, 4096 rows
 // 20 / 27. The rule's one miss there: 32 experts of 64 rows, small 428, large 359.)
-inline double grouped_tiles(int R, int E, int out, int tile, bool dense) {
+inline double grouped_row_tiles(int R, int E, int tile, bool dense) {
     const double used = R < E ? R : E, m = dense ? (R + tile - 1) / tile : R / used / tile + 0.6;
-    return used * (m > 1 ? m : 1) * ((out + tile - 1) / tile);
+    return used * (m > 1 ? m : 1);
 }
 inline LayoutChoice grouped_choice(int R, int E, int in, int out, bool dense = false) {
-    auto tiles = [&](int tile) { return grouped_tiles(R, E, out, tile, dense); };
+    auto tiles = [&](int tile) { return grouped_row_tiles(R, E, tile, dense) * ((out + tile - 1) / tile); };
     return choose_layout({tiles(256), tiles(128), tiles(64)}, (in + kLayoutStep - 1) / kLayoutStep, moe_num_compute_units());
 }
 
