@@ -361,3 +361,11 @@ def test_few_rows_of_experts(hk, rows, unused, I, K, act, interleaved):
 def test_two_small_tiles_a_cu(hk, rows, unused, I, wide, dense, act, interleaved):
     """64x64 tiles, more of them than CUs and no more than two a CU, forward or backward; fewer K-steps than stages, as many, and more."""
     _run(hk, rows, unused, I, wide, act, interleaved, I + wide, dense)
+
+
+@pytest.mark.parametrize("act,interleaved", [("silu", True), ("swiglu_oai", False), ("silu", False), ("swiglu_oai", True)])
+@pytest.mark.parametrize("rows,unused,I,wide,dense", [
+    ([2100], 0, 2056, 840, True), ([1150], 0, 2056, 1800, True), ([1150], 0, 4616, 520, True), ([700, 0, 1200, 513] * 2, 7, 2056, 520, False)])
+def test_large_tiles(hk, rows, unused, I, wide, dense, act, interleaved):
+    """Each of the kernels of 128 and 256 rows dense and over experts, with every activation and order of the weights' rows."""
+    _run(hk, rows, unused, I, wide, act, interleaved, I + wide + 1, dense)
