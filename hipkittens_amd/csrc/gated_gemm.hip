@@ -137,18 +137,23 @@ struct PatchPairs<F, true> {
     }
 };
 
-// The kept gate and up values of a wave's patch, row block by row block (16 rows) through its share of the LDS that the product is done with: as many
-// blocks as that holds are under way at once. Rows of LDS hold 16-byte chunk c of row r at c ^ swz(r): a read of a column block touches
-// every bank once. (Read straight into registers, a block at a time: 1864 us where this takes 1780, with the activation in one form.)
+// The kept gate and up values of a wave's patch, row block by row block (16 rows) through LDS: the first blocks, as many as what the product leaves of a
+// CU's LDS holds, in front of the product (all of a 64x64 tile's, half of those of a 128x128 tile with a CU to itself; 300 rows of 2880 x 2880 17.3
+// us, so 16.4), the others through the wave's share of the LDS that the product is done with, as many under way at once as that holds. Rows of
+// LDS hold 16-byte chunk c of row r at c ^ swz(r): a read of a column block touches every bank once. (Read straight into registers, a block at a
+// time: 65536 rows of 32 experts, N = 7168, I = 2048 1864 us where this takes 1780, with the activation in one form.)
 template <typename Tile, bool INTERLEAVED>
 struct GateUpLoads {
     static constexpr int F = Tile::FC, kBlocks = Tile::F, kBlockBytes = Tile::kPatchCols * 64, kLoads = kBlockBytes / 1024;
-    static constexpr int kSlots = Tile::kLds / 4 / kBlockBytes < kBlocks ? Tile::kLds / 4 / kBlockBytes : kBlocks;
-    static_assert(kSlots >= 1 && (kSlots - 1) * kLoads < 64);
+    static constexpr int kRoom = 160 * 1024 / (Tile::kLds > 80 * 1024 ? 1 : 2) - Tile::kLds;
+    static constexpr int kAhead = std::min(kRoom / 4 / kBlockBytes, kBlocks), kRest = kBlocks - kAhead;
+    static constexpr int kLds = Tile::kLds + 4 * kAhead * kBlockBytes;
+    static constexpr int kSlots = std::min(Tile::kLds / 4 / kBlockBytes, kRest);
+    static_assert(kRest == 0 || (kSlots >= 1 && (kSlots - 1) * kLoads < 64));
     // 16-byte chunks of a row of LDS: of its gate or of its up values, or of both where they alternate; rows of a load
     static constexpr uint32_t kChunks = INTERLEAVED ? Tile::kPatchCols / 4 : Tile::kPatchCols / 8, kLoadRows = 64 / kChunks;
     v4i srd;
-    uint32_t lds, voff, pitch, half;   // voff: the lane's place in an even load's first row; half: bytes between a row's gate and up values
+    uint32_t lds, lds_ahead, voff, pitch, half;   // voff: the lane's place in an even load's first row; half: bytes between a row's gate and up values
 
     __device__ __forceinline__ static uint32_t swz(uint32_t r) { return kChunks >= 16 ? r & 15u : (r / (16u / kChunks)) & (kChunks - 1); }
     // at: the patch's first row; col: its first column of I; rows: what is left of the rows (none: everything reads as zeros)
@@ -157,10 +162,14 @@ struct GateUpLoads {
         half = 2u * (uint32_t)I;
         srd = make_srd(at, rows > 0 ? (uint32_t)rows * pitch : 0u);   // (at most 256 rows of 4 MB)
         lds = to_sgpr((uint32_t)(uintptr_t)smem + wave_id() * (Tile::kLds / 4));
+        lds_ahead = to_sgpr((uint32_t)(uintptr_t)smem + Tile::kLds + wave_id() * (kAhead * kBlockBytes));
         voff = lane_id() / kChunks * pitch + (uint32_t)col * (INTERLEAVED ? 4u : 2u);
     }
+    __device__ __forceinline__ uint32_t slot(int m) const {
+        return m < kAhead ? lds_ahead + m * kBlockBytes : lds + (m - kAhead) % std::max(kSlots, 1) * kBlockBytes;
+    }
     __device__ __forceinline__ void issue(int m) const {
-        const uint32_t lane = lane_id(), dst = lds + m % kSlots * kBlockBytes;
+        const uint32_t lane = lane_id(), dst = slot(m);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {   // the gate values' loads, then the up values'
             const uint32_t k = INTERLEAVED ? i : i % (kLoads / 2);
@@ -170,7 +179,7 @@ struct GateUpLoads {
         }
     }
     __device__ __forceinline__ void read(int m, v4f (&g)[F], v4f (&u)[F]) const {
-        const uint32_t r = lane_id() & 15, q = lane_id() >> 4, at = lds + m % kSlots * kBlockBytes + r * (kChunks * 16);
+        const uint32_t r = lane_id() & 15, q = lane_id() >> 4, at = slot(m) + r * (kChunks * 16);
 #pragma unroll
         for (int n = 0; n < F; ++n) {
             if constexpr (INTERLEAVED) {
@@ -296,26 +305,31 @@ __global__ __launch_bounds__(256) void gated_dgrad_kernel(GatedBackward p) {
     const GroupedTile t = grouped_tile(p.offsets, p.E, p.R, Tile::kTile, p.tiles_n, p.N, p.I, xcd_chunk_order(blockIdx.x, gridDim.x, kCuPerXcd));
     if (t.expert < 0) return;
     const int col0 = t.tile_n * Tile::kTileCols;
+    const int w = wave_id(), row = (w >> 1) * Tile::kPatch, col = col0 + (w & 1) * Tile::kPatchCols, rows = t.rows - row;
+    const size_t first = (size_t)(t.row0 + row);
+    typedef GateUpLoads<Tile, INTERLEAVED> Loads;
+    const Loads kept(smem, p.gate_up + first * 2 * p.I, col, p.I, rows);
+#pragma unroll
+    for (int m = 0; m < Loads::kAhead; ++m) kept.issue(m);
     v4f acc[Tile::F][Tile::FC];
     Tile::template product<kAlong, kAcross>(smem, operand_along(p.dy, 2ull * p.N, t.row0, t.row0 + t.rows, p.N),
                                             operand_across(p.w2 + (size_t)t.expert * p.N * p.I, 2ull * p.I, col0, p.N), p.N, acc);
-    const int w = wave_id(), row = (w >> 1) * Tile::kPatch, col = col0 + (w & 1) * Tile::kPatchCols, rows = t.rows - row;
-    const size_t first = (size_t)(t.row0 + row);
-    block_barrier();   // everyone is done with the product's LDS
-    typedef GateUpLoads<Tile, INTERLEAVED> Loads;
-    const Loads kept(smem, p.gate_up + first * 2 * p.I, col, p.I, rows);
     const Gate<CLAMPED> gate{p.gate};
     const PatchMatrix<Tile::FC> out(p.h + first * p.I, 2u * p.I, p.h ? rows : 0, col, p.I);
     const PatchPairs<Tile::FC, INTERLEAVED> pairs(p.dgate_up + first * 2 * p.I, rows, col, p.I);
+    wait_vmcnt<0>();   // the first blocks have landed, as the product's loads have
+    if constexpr (Loads::kRest > 0) {
+        block_barrier();   // everyone is done with the product's LDS
 #pragma unroll
-    for (int m = 0; m < Loads::kSlots; ++m) kept.issue(m);
+        for (int m = 0; m < Loads::kSlots; ++m) kept.issue(Loads::kAhead + m);
+    }
     auto block = [&]<int m>() __attribute__((always_inline)) {
         v4f dh[Tile::FC], g[Tile::FC], u[Tile::FC], dg[Tile::FC], du[Tile::FC];
         // the block has landed: no more is under way than the loads issued behind its own (stores in between only make this wait longer)
         constexpr int last = m + Loads::kSlots < Tile::F ? m + Loads::kSlots : Tile::F;
-        wait_vmcnt<(last - 1 - m) * Loads::kLoads>();
+        if constexpr (m >= Loads::kAhead) wait_vmcnt<(last - 1 - m) * Loads::kLoads>();
         kept.read(m, g, u);
-        if constexpr (m + Loads::kSlots < Tile::F) {
+        if constexpr (m >= Loads::kAhead && m + Loads::kSlots < Tile::F) {
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // ... and has been read
             kept.issue(m + Loads::kSlots);
         }
@@ -518,23 +532,23 @@ static int gated_check(int R, int E, int I, int wide, const int32_t* offsets) {
 }
 
 template <typename Tile, typename P>
-static int launch_gated_tile(void (*kern)(P), DeviceOnce& once, P p, int out, hipStream_t s) {
+static int launch_gated_tile(void (*kern)(P), DeviceOnce& once, P p, int out, int lds_bytes, hipStream_t s) {
     p.tiles_n = (out + Tile::kTileCols - 1) / Tile::kTileCols;
     const long long grid = grouped_tiles_m(p.R, p.E, Tile::kTile) * p.tiles_n;
     if (grid >= kMaxWorkgroups) return HK_ERR_BAD_SHAPE;
-    if (!set_lds_limit_once((const void*)kern, Tile::kLds, once)) return HK_ERR_LAUNCH;
-    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), Tile::kLds, s, p);
+    if (!set_lds_limit_once((const void*)kern, lds_bytes, once)) return HK_ERR_LAUNCH;
+    hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(256), lds_bytes, s, p);
     return hipGetLastError() == hipSuccess ? HK_OK : HK_ERR_LAUNCH;
 }
 template <typename Tile, bool CLAMPED, bool INTERLEAVED>
 static int launch_gated(const GatedForward& p, hipStream_t s) {
     static DeviceOnce once;
-    return launch_gated_tile<Tile>(gated_gemm_kernel<Tile, CLAMPED, INTERLEAVED>, once, p, 2 * p.I, s);
+    return launch_gated_tile<Tile>(gated_gemm_kernel<Tile, CLAMPED, INTERLEAVED>, once, p, 2 * p.I, Tile::kLds, s);
 }
 template <typename Tile, bool CLAMPED, bool INTERLEAVED>
 static int launch_gated(const GatedBackward& p, hipStream_t s) {
     static DeviceOnce once;
-    return launch_gated_tile<Tile>(gated_dgrad_kernel<Tile, CLAMPED, INTERLEAVED>, once, p, p.I, s);
+    return launch_gated_tile<Tile>(gated_dgrad_kernel<Tile, CLAMPED, INTERLEAVED>, once, p, p.I, GateUpLoads<Tile, INTERLEAVED>::kLds, s);
 }
 template <typename Tile, typename P>
 static int launch_gated_form(const P& p, hipStream_t s) {
