@@ -59,7 +59,11 @@ constexpr int kSortChunk = kSortThreads * kSortIter;   // tokens of a workgroup
 constexpr int kSortAlone = 2 * kSortChunk;             // most that one workgroup sorts by itself
 constexpr int kMaxDigitBits = 9, kMaxDigits = 1 << kMaxDigitBits;
 
-constexpr size_t kSortFillBytes = (size_t)128 << 20;   // that a sorting launch writes besides (half of it where it is read first)
+// Bytes that a launch that sorts writes besides, about what takes as long as it does: zeros (which the memory-side cache takes for a table that
+// fits it), or copies of `add`, more of them beside the longest lists that one workgroup sorts. (us: 1111 tokens of 50257 rows of 1024 in bf16, 24 MB of
+// zeros 31.8, 48 28.0, 128 26.3, written over and over 72 28.9, 128 26.0; 700 tokens of 20000 rows in fp32 with `add`, copies of 24 MB 42.1,
+// 64 48.8; 20000 tokens of 50000 rows 121, 137; 8000 of 30000 rows in bf16, 48 MB 46.5, 64 42.9.)
+constexpr size_t kSortZeros = (size_t)128 << 20, kSortCopies = (size_t)24 << 20, kSortCopiesLong = (size_t)64 << 20;
 // What the sorting launches write besides: `out`'s 16-byte pieces [from, to), from `add` or zeros.
 struct Fill {
     v4i* out;
@@ -566,9 +570,13 @@ static int launch_embedding_backward(Ids ids, const void* dout, const void* add,
     // writes the others, where there are no tokens.
     const int launches = tokens <= kSortAlone ? 1 : 1 + L.passes;
     const size_t row_bytes = (size_t)H * sizeof(T), all_bytes = V * row_bytes;
-    const int blind = add == dtable ? 0 : (int)std::min<size_t>(V, launches * (add ? kSortFillBytes / 2 : kSortFillBytes) / row_bytes);
+    const size_t beside = !add ? kSortZeros : tokens > kSortChunk && launches == 1 ? kSortCopiesLong : kSortCopies;   // a launch
+    const int blind = add == dtable ? 0 : (int)std::min<size_t>(V, launches * beside / row_bytes);
     const size_t pieces = blind * row_bytes / 16;
-    EmbedRest rest{blind, add == dtable ? blind : V, (int)std::min<size_t>(kRestRows, std::max<size_t>(4, (128u << 10) / row_bytes)), all_bytes > (256u << 20)};
+    // rows of a workgroup: 128 KB, and less where that would be few workgroups (8000 tokens of 30000 rows of 1024 with `add` 52.2 us, so 46.5)
+    const int to = add == dtable ? blind : V;
+    const size_t rest_rows = std::max<size_t>(4, std::min<size_t>((128u << 10) / row_bytes, (size_t)(to - blind) / 512));
+    const EmbedRest rest{blind, to, (int)std::min<size_t>(kRestRows, rest_rows), all_bytes > (256u << 20)};
     auto part = [&](int launch) {
         Fill f{(v4i*)dtable, (const v4i*)add, pieces * launch / launches, pieces * (launch + 1) / launches, 0, rest.stream};
         f.groups = (int)std::min<size_t>(512, (f.to - f.from + 4 * kSortThreads - 1) / (4 * kSortThreads));
