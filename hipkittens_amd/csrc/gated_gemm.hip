@@ -648,12 +648,15 @@ static int launch_gated_dgrad_skinny(const GatedBackward& p, hipStream_t s) {
 
 // Experts with few rows, of which the host knows only how many there are on average where they spread evenly. Two workgroups a CU and more, by their LDS: a
 // launch has many rounds of them, and one's start and end are the others' time. Forward: 16 rows of the weights a workgroup while the CUs hold them
-// in one round, 32 for few rounds, else 64; more than 8 rows an expert only where the 128-tile kernel has more than one round of its two
-// workgroups a CU. Backward: 32 columns a workgroup while they are one round, else 64, but for the 128-tile kernel's one round. Beyond one round not
-// for short rows, where a wave has few K-steps. (us, tile kernels / these: forward, 128 experts of 2880 x 2880, 150 rows 531 / 464, 1000 734 / 666, 2000 742 / 678, 3200 756 / 764; 64 of 1536 x 4096,
-// 256 rows 317 / 234; 48 of 2048 x 7168, 1000 rows 467 / 437; 9 of 576 x 2672, one row 16.1 / 8.2, but 40 rows 17.3 / 20.1. Backward, the same 296 /
-// 240, 395 / 347, 402 / 383, 410 / 442; 170 / 140; 282 / 263; 16.6 / 8.9, 17.0 / 12.8; 40 experts of 1432 x 1024, 40 rows, one round of tiles,
-// 22.3 / 29.1. Short rows: 30 of 3000 x 264, 64 rows forward 33.5 / 37.5; 60 of 2048 x 768, 200 rows backward 41.5 / 44.9. Of the forms, forward: 20 experts of 2880 x 2880, 8 rows, 32 a workgroup 42.1, 64 48.1; 128 of 768 x 2048, 256 rows 127 / 118.)
+// in one round, 32 for few rounds, else 64 of up to 32 rows of x (16 rows of x take 0 to 8 % less where the experts' rows are even, up to 10 % more where
+// they are not); more than 8 rows an expert only where the 128-tile kernel has more than one round of its two workgroups a CU. Backward: 32
+// columns a workgroup while they are one round, else 64, but for the 128-tile kernel's one round. Beyond one round not for short rows, where a wave has few
+// K-steps. (us, tile kernels / these: forward, 128 experts of 2880 x 2880, 300 rows 662 / 573, 1000 732 / 650, 2000 742 / 678, 3200 756 / 764; 200 of
+// 1024 x 4096, 500 rows 549 / 468; 40 of 2048 x 7168, 300 rows 425 / 349; 9 of 576 x 2672, one row 16.1 / 7.6, but 40 rows 17.3 / 19.7. Shares of the
+// experts as 1 / rank: 128 of 2880 x 2880, 1000 rows 669 / 653, 200 of 1024 x 4096, 1500 rows 561 / 497, but 32 of 2880 x 2880, 600 rows, 141 of
+// them one expert's, 190 / 216. Backward, the first four 372 / 299, 394 / 347, 402 / 383, 410 / 442; 275 / 246; 265 / 207; 16.6 / 8.9, 17.0 / 12.8; uneven
+// 377 / 341, 272 / 268, 121 / 117; 40 experts of 1432 x 1024, 40 rows, one round of tiles, 22.3 / 29.1. Short rows: 30 of 3000 x 264, 64 rows
+// forward 33.5 / 37.5; 60 of 2048 x 768, 200 rows backward 41.5 / 44.9.)
 struct ExpertRows {
     double used, mean;
     ExpertRows(int R, int E) : used(-E * std::expm1(R * std::log1p(-1.0 / E))), mean(R / used) {}
@@ -666,16 +669,13 @@ static bool launch_gated_experts_skinny(const GatedForward& p, hipStream_t s, in
     const ExpertRows rows(p.R, p.E);
     const int cus = moe_num_compute_units();
     if (rows.mean > kExpertRows32 || p.I > kExpertMaxI || (p.K < kExpertMinWide && rows.blocks(p.I, 16) > cus)) return false;
-    if (rows.mean > kExpertRows16) {
-        if (rows.blocks(p.I, 16) <= cus) st = launch_gated_skinny_kernel<2, 4, 3, 2, true>(p, s);
-        else if (rows.blocks(p.I, 64) > 2 * cus) st = launch_gated_skinny_kernel<2, 2, 3, 4, true>(p, s);
-        else return false;
-    } else if (rows.blocks(p.I, 8) <= cus) {
+    if (rows.blocks(p.I, 8) <= cus && rows.mean <= kExpertRows16) {
         st = launch_gated_skinny_kernel<1, 4, 4, 1, true>(p, s);
-    } else if (rows.blocks(p.I, 16) < (p.K < 2048 ? 2 : 6) * cus) {
-        st = launch_gated_skinny_kernel<1, 4, 3, 2, true>(p, s);
+    } else if (rows.blocks(p.I, 16) <= cus || (rows.mean <= kExpertRows16 && rows.blocks(p.I, 16) < (p.K < 2048 ? 2 : 6) * cus)) {
+        st = rows.mean <= kExpertRows16 ? launch_gated_skinny_kernel<1, 4, 3, 2, true>(p, s) : launch_gated_skinny_kernel<2, 4, 3, 2, true>(p, s);
     } else {
-        st = launch_gated_skinny_kernel<1, 4, 2, 4, true>(p, s);
+        if (rows.mean > kExpertRows16 && rows.blocks(p.I, 64) <= 2 * cus) return false;
+        st = launch_gated_skinny_kernel<2, 2, 3, 4, true>(p, s);
     }
     return true;
 }
