@@ -583,8 +583,8 @@ static int launch_gated_skinny_kernel(GatedForward p, hipStream_t s) {
 // HBM, bound more than 16 rows. (us from HBM, 32 / 64 rows of weights a workgroup / 64-tile kernel: 48 rows, I = 14336, K = 4096 55.7 / 42.2 /
 // 55.0; 32 rows 47.5 / 39.0 / 55.2; 32 rows, I = 9216, K = 8192 63.7 / 68.2 / 74.1; with 16 rows and 32 a workgroup 37.6 / - / 55.1, one row
 // 36.1. 1 row, I = 2048, K = 7168: 11.2 / - / 30.2.) Rows of weights that are not whole cache lines take two accesses a piece, which bounds a CU, so that one
-// with a workgroup more than the others is waited for: 16 again while x is a few rows (one row, 16 / 32: I = 9408, K = 2360 18.4 / 23.4; 16 rows,
-// I = 7400, K = 3000 28.3 / 25.3).
+// with a workgroup more than the others is waited for: 16 again while x is a few rows (16 / 32: one row, I = 9408, K = 2360 18.4 / 23.4; 8 rows, I =
+// 4176, K = 6512 31.7 / 37.2; 12 rows, I = 13000, K = 4072 55.6 / 53.2).
 // Waves and stages of a workgroup for 16, 32 and 64 rows of weights: as many stages as fit while the CUs hold the workgroups in one round, two workgroups a
 // CU where there are more (I = 14336, K = 4096, one row 38.5 / 35.9; I = 2880, K = 2880 7.4 / 8.0).
 struct SkinnyForm { int waves, stages; };
@@ -603,7 +603,7 @@ static int launch_gated_skinny_rows(const GatedForward& p, hipStream_t s) {
             if (rounds(8 << I) > 1) return launch_gated_skinny_kernel<R, more.waves, more.stages, 1 << I>(p, s);
         return launch_gated_skinny_kernel<R, one.waves, one.stages, 1 << I>(p, s);
     };
-    if (2ll * ((p.I + 15) / 16) <= cus || (R == 1 && p.R <= 4 && p.K % 64 != 0)) return launch.template operator()<0>();
+    if (2ll * ((p.I + 15) / 16) <= cus || (R == 1 && p.R <= 8 && p.K % 64 != 0 && rounds(16) > 1)) return launch.template operator()<0>();
     if constexpr (R > 1)
         if (rounds(32) * (64 + 16 * R) < rounds(16) * (32 + 16 * R)) return launch.template operator()<2>();
     return launch.template operator()<1>();
