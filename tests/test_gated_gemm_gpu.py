@@ -369,3 +369,34 @@ def test_two_small_tiles_a_cu(hk, rows, unused, I, wide, dense, act, interleaved
 def test_large_tiles(hk, rows, unused, I, wide, dense, act, interleaved):
     """Each of the kernels of 128 and 256 rows dense and over experts, with every activation and order of the weights' rows."""
     _run(hk, rows, unused, I, wide, act, interleaved, I + wide + 1, dense)
+
+
+@pytest.mark.parametrize("act,interleaved", [("silu", True), ("swiglu_oai", False)])
+@pytest.mark.parametrize("rows,I,wide,dense", [
+    ([1], 4160, 1088, True), ([8], 2048, 2112, True), ([17], 4160, 1088, True), ([40], 8256, 2176, True), ([64], 2112, 2112, True),
+    ([0, 1, 3, 0, 1], 192, 2112, False), ([0, 0, 0, 17, 0, 0, 33], 256, 640, False), ([5, 2, 0, 1, 0, 0, 20] * 6, 576, 1088, False),
+    ([1, 0, 7] * 21, 384, 1024, False), ([12, 31, 0, 33, 8, 15, 20] * 9, 576, 1024, False), ([1, 0, 2] * 8, 576, 2112, False),
+    ([16, 17, 7, 12], 256, 1088, False)])
+def test_few_rows_with_weights_past_the_caches(hk, rows, I, wide, dense, act, interleaved):
+    """Rows of weights that are whole cache lines, as most checkpoints', of every kernel for few rows in both directions."""
+    _run(hk, rows, 0, I, wide, act, interleaved, I + wide + len(rows), dense)
+
+
+def test_few_rows_with_weights_inside_a_cache_line(hk):
+    """The same weights at an address that is no multiple of a cache line's: the same values."""
+    print("gated weights inside a line", flush=True)
+    tk, R, I, K = hk.tk_kernel, 3, 2112, 2112
+    g = torch.Generator(device=DEV).manual_seed(31)
+    x, dy, gu = _rand(g, R, K), _rand(g, R, K), _rand(g, R, 2 * I)
+    pools = [torch.empty(2 * I * K + 64, dtype=torch.bfloat16, device=DEV) for _ in range(2)]
+    w = _rand(g, 2 * I * K, std=K**-0.5)
+    got = []
+    for pool, skip in zip(pools, (0, 8)):
+        at = pool[skip:skip + 2 * I * K]
+        at.copy_(w)
+        h, d = torch.empty(R, I, dtype=torch.bfloat16, device=DEV), torch.empty(R, 2 * I, dtype=torch.bfloat16, device=DEV)
+        tk.dispatch_gated_gemm(x, at.view(2 * I, K), h)
+        tk.dispatch_gated_gemm_dgrad(dy, at[:I * K].view(K, I), gu, d)
+        got.append((h, d))
+    for a, b in zip(*got):
+        assert torch.equal(a.view(torch.int16), b.view(torch.int16))
