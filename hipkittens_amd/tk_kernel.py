@@ -1065,7 +1065,9 @@ def dispatch_embedding_backward(ids, dout, dtable, workspace, scale: float = 1.0
 class GradTensors:
     """Gradients that are clipped together: bf16 and fp32 tensors of any shape on one device, contiguous, none overlapping another. `outs`: where
     the scaled ones go, tensor by tensor, of the same numbers of elements in bf16 or fp32 (None: in place). The tensors are kept, and a
-    table of them on the device, made once (a host copy, outside a captured graph): make another where gradients move to new memory."""
+    table of them on the device, made once (a host copy, outside a captured graph): make another where gradients move to new memory. The list
+    may be dropped once its calls are queued, on whatever streams (the tensors follow torch's rules for theirs); a graph that its calls were
+    captured in needs it as long as the graph is replayed."""
 
     def __init__(self, grads, outs=None):
         self.grads = list(grads)
@@ -1102,6 +1104,13 @@ class GradTensors:
                                          types(self.grads), types(self.outs), n, host.data_ptr(), host.numel(), ctypes.byref(chunks)),
                    "GradTensors")
         self.n, self.chunks, self.list = n, chunks.value, host.to(self.device)
+        self.stream = _stream(self.list)   # the one whose work torch's allocator keeps the table's memory for
+
+    def _before_launch(self):
+        """Has the allocator keep the table's memory for the current stream's work too: a list may be dropped before that has run, and
+        the clip takes the addresses that it writes to from the table."""
+        if _stream(self.list) != self.stream:
+            self.list.record_stream(torch.cuda.current_stream(self.device))
 
 
 def grad_norm_workspace_bytes() -> int:
@@ -1116,12 +1125,14 @@ def _check_norm(grads, norm):
     if norm.shape[0] != 1:
         raise RuntimeError("norm must be [1]")
     _same_device(grads.list, norm)
+    grads._before_launch()
 
 
 def dispatch_grad_norm(grads, norm, workspace) -> None:
     """norm [1] fp32 = the square root of the sum of the squares of all of `grads` (a GradTensors), added in 64 bits. workspace:
     grad_norm_workspace_bytes() bytes."""
     if type(grads) is GradTensors:
+        grads._before_launch()
         st = (_native or _load_native()).grad_norm(grads.list, grads.n, grads.chunks, norm, workspace)
         if st is not None:
             return _lib.check(st, "dispatch_grad_norm")
@@ -1138,6 +1149,7 @@ def dispatch_grad_clip(grads, norm, max_norm: float) -> None:
     """Every gradient of `grads` times min(1, max_norm / (norm + 1e-6)), in place or into its outs; norm [1] of dispatch_grad_norm, or of
     all ranks together."""
     if type(grads) is GradTensors:
+        grads._before_launch()
         st = (_native or _load_native()).grad_clip(grads.list, grads.n, grads.chunks, norm, max_norm)
         if st is not None:
             return _lib.check(st, "dispatch_grad_clip")
