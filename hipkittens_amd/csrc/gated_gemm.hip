@@ -252,8 +252,8 @@ struct GatedMma {
 struct GatedSkinnyOut {
     static constexpr bool kPairs = true;
     GatedForward p;
-    int col0;
-    __device__ __forceinline__ int first() const { return col0; }
+    int column_block;
+    __device__ __forceinline__ int block() const { return column_block; }
     __device__ __forceinline__ uint32_t pitch() const { return (uint32_t)p.K * (p.interleaved ? 4u : 2u); }
     __device__ __forceinline__ const uint8_t* other() const { return (const uint8_t*)(p.w13 + (p.interleaved ? (size_t)p.K : (size_t)p.I * p.K)); }
     // columns c .. c + 4 of h
@@ -275,11 +275,11 @@ struct GatedSkinnyOut {
 template <int R, int NW, int D, int NF, bool NT, bool EXPERTS>
 __global__ __launch_bounds__(64 * NW) void gated_skinny_kernel(GatedForward p) {
     extern __shared__ __attribute__((aligned(2048))) uint8_t smem[];
-    int col0 = blockIdx.x * (8 * NF);
+    int column_block = blockIdx.x;
     if constexpr (EXPERTS) {   // up to 16 R of an expert's rows
         const GroupedTile t = grouped_tile(p.offsets, p.E, p.R, 16 * R, p.tiles_n, p.K, 2 * p.I, xcd_chunk_order(blockIdx.x, gridDim.x, kCuPerXcd));
         if (t.expert < 0) return;
-        col0 = t.tile_n * (8 * NF);
+        column_block = t.tile_n;
         p.x += (size_t)t.row0 * p.K;
         p.w13 += (size_t)t.expert * 2 * p.I * p.K;
         p.h += (size_t)t.row0 * p.I;
@@ -287,7 +287,7 @@ __global__ __launch_bounds__(64 * NW) void gated_skinny_kernel(GatedForward p) {
         p.R = t.rows;
     }
     gemm_skinny_body<GatedMma, R, NW, D, NF, NT>(smem, (const uint8_t*)p.x, (const uint8_t*)p.w13, nullptr, p.R, p.I, 2 * p.K, 1.0f,
-                                                 SkinnyScales{nullptr, nullptr, 0, 0, 0}, GatedSkinnyOut{p, col0});
+                                                 SkinnyScales{nullptr, nullptr, 0, 0, 0}, GatedSkinnyOut{p, column_block});
 }
 
 struct GatedBackward {

@@ -46,7 +46,7 @@ struct SkinnyScales {
     const uint8_t* SA; const uint8_t* SB; int sa_pitch, sb_pitch, row_bytes;
 };
 // OUT: what the sums become. SkinnyPlain: C. With kPairs, B is one half of the operand and out.other() the other, each in rows of out.pitch()
-// bytes: a workgroup owns rows out.first() .. + 8 NF of both (NF / 2 fragments of the one, then of the other; NF = 1: the two halves of one), and
+// bytes: a workgroup owns rows 8 NF out.block() .. + 8 NF of both (NF / 2 fragments of the one, then of the other; NF = 1: the two halves of one), and
 // out.store(row, n, first, second) takes both sums of rows n .. n + 4 of them (N % 4 == 0).
 struct SkinnyPlain { static constexpr bool kPairs = false; };
 template <typename MMA, int R, int NW, int D, int NF = 2, bool NT = false, typename OUT = SkinnyPlain>
@@ -63,8 +63,9 @@ __device__ __forceinline__ void gemm_skinny_body(
     static_assert(NW * R * NF * 1024 <= NW * kRegion, "the partial sums reuse the stages");
     const int lane = lane_id(), w = wave_id();
     const uint32_t r = lane & 15, g = lane >> 4;
-    int n0 = blockIdx.x * kRowsB;
-    if constexpr (kPairs) n0 = out_pairs.first();
+    int block = blockIdx.x;   // of columns of C
+    if constexpr (kPairs) block = out_pairs.block();
+    const int n0 = block * kRowsB;
     const int rows_b = N - n0 < kRowsB ? N - n0 : kRowsB;
     uint32_t pitch_b = (uint32_t)K;
     v4i srd_other = {0, 0, 0, 0};
@@ -95,9 +96,10 @@ __device__ __forceinline__ void gemm_skinny_body(
     // wraps around): rows whose length is a multiple of the memory channels' interleave (16 KiB: K = 8192 in bf16)
     // would otherwise have every workgroup at the same offset into its rows at the same time, i.e. in the same few
     // channels (M = 16, N = 8192, 16 KiB rows: 4.2 TB/s against 5.7 with rows of 18 KiB). The order is fixed by
-    // the workgroup's index, so the result still does not depend on timing. (With scales the K-steps stay in
-    // order: the scale tiles are fetched one ahead of a monotonic walk.)
-    const int rot = kScaled || n == 0 ? 0 : (int)((blockIdx.x * 5u) % (uint32_t)n);
+    // the block of columns, so the result still does not depend on timing, nor, where the workgroups are those of several
+    // experts, on how many rows the others have. (With scales the K-steps stay in order: the scale tiles are fetched one
+    // ahead of a monotonic walk.)
+    const int rot = kScaled || n == 0 ? 0 : (int)(((uint32_t)block * 5u) % (uint32_t)n);
     auto step_of = [&](int kt_local) {
         const int x = kt_local + rot;
         return s0 + (x >= n ? x - n : x);

@@ -400,3 +400,34 @@ def test_few_rows_with_weights_inside_a_cache_line(hk):
         got.append((h, d))
     for a, b in zip(*got):
         assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("rows,other,kept,I,wide", [
+    ([1, 1, 1, 5, 1, 1], [3, 0, 0, 5, 1, 1], 3, 392, 2056), ([1, 1, 1, 5, 1, 1], [0, 0, 4, 5, 0, 1], 3, 1096, 2056),
+    ([12, 14, 10, 12], [20, 0, 10, 18], 2, 776, 2056),
+    ([1, 2, 0, 3] * 10, [3, 0] * 12 + [0, 0, 0, 3, 6, 0, 3, 0] + [3, 0] * 4, 27, 1096, 1032),
+    ([12, 9] * 16, [21, 0] * 3 + [12, 9] + [21, 0] * 12, 7, 1160, 1096), ([12, 9] * 16, [21, 0] * 3 + [12, 9] + [21, 0] * 12, 7, 1152, 1088)])
+def test_an_expert_of_few_rows_among_others(hk, rows, other, kept, I, wide, interleaved):
+    """As many rows in all, spread over the other experts in another way, and `kept`'s elsewhere: the bits of its rows stay. (Each of the forward
+    kernels for few rows of experts and the backward ones, one row fragment and two, weights through the caches and past them.)"""
+    print(f"gated expert of few rows {rows[:6]} {other[:6]} I={I} wide={wide} interleaved={interleaved}", flush=True)
+    tk, E = hk.tk_kernel, len(rows)
+    g = torch.Generator(device=DEV).manual_seed(I + E)
+    assert sum(rows) == sum(other)
+    n = min(rows[kept], other[kept])
+    w13, w2 = _rand(g, E, 2 * I, wide, std=1.5 * wide**-0.5), _rand(g, E, wide, I, std=I**-0.5)
+    mine, mine_dy, mine_gu = _rand(g, n, wide), _rand(g, n, wide), _rand(g, n, 2 * I)
+    got = []
+    for each in (rows, other):
+        R, at = sum(each), sum(each[:kept])
+        x, dy, kept_gu = _rand(g, R, wide), _rand(g, R, wide), _rand(g, R, 2 * I)
+        x[at:at + n], dy[at:at + n], kept_gu[at:at + n] = mine, mine_dy, mine_gu
+        offsets = torch.tensor([sum(each[:e]) for e in range(E + 1)], dtype=torch.int32, device=DEV)
+        mk = lambda c: torch.zeros(R, c, dtype=torch.bfloat16, device=DEV)
+        h, gu, dgu, h2 = mk(I), mk(2 * I), mk(2 * I), mk(I)
+        tk.dispatch_gated_gemm(x, w13, h, gu, expert_offsets=offsets, interleaved=interleaved)
+        tk.dispatch_gated_gemm_dgrad(dy, w2, kept_gu, dgu, h2, expert_offsets=offsets, interleaved=interleaved)
+        got.append([t[at:at + n].clone() for t in (h, gu, dgu, h2)])
+    for name, a, b in zip(("h", "gate_up", "dgate_up", "h again"), *got):
+        assert torch.equal(a.view(torch.int16), b.view(torch.int16)), (name, int((a != b).sum()))
