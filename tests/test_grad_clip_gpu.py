@@ -188,3 +188,46 @@ def test_captured_and_the_same_on_every_call(hk):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(norm, norm2) and all(torch.equal(a, b) for a, b in zip(outs, outs2)), i
+
+
+# (elements of gradient and result, types): lists whose chunks are more than 8192, which the kernels read and write past the caches
+LONG = {"one tensor beyond 2^32 bytes": [(2**31 + 12_345, BF, BF), (100_003, F32, F32), (1, BF, BF), (0, F32, F32), (16_385, BF, BF)],
+        "fp32 beyond 2^32 bytes": [(77, BF, BF), (2**30 + 4_097, F32, F32), (16_384, BF, BF), (3, F32, F32)],
+        "many": [(n, (BF, F32)[i % 3 % 2], (BF, F32)[i % 3 % 2]) for i, n in enumerate([999_999, 1, 2_000_001, 16_384, 0] * 46)],
+        "into others": [(90_000_001, BF, F32), (50_000_007, F32, BF), (20_000_003, BF, BF), (33, F32, F32), (8_000_000, F32, F32)]}
+
+
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("name,elsewhere", [(n, e) for n in LONG for e in (False, True) if e or n != "into others"])
+def test_lists_beyond_the_caches(hk, name, elsewhere, shift):
+    """Every gradient `shift` elements behind an aligned address and every result there or one element further, with elements of 777 around
+    them; compared some million elements at a time."""
+    print(f"clip of a long list: {name}, elsewhere={elsewhere}, shift={shift}", flush=True)
+    tk, parts = hk.tk_kernel, LONG[name]
+    assert sum((n + 16383) // 16384 for n, _, _ in parts) > 8192
+    g = torch.Generator(device=DEV).manual_seed(shift + len(parts))
+    room = lambda n, t: torch.full((n + 24,), 777.0, dtype=t, device=DEV)
+    bufs = [room(n, t) for n, t, _ in parts]
+    grads = [b[8 + shift:8 + shift + n] for b, (n, _, _) in zip(bufs, parts)]
+    for i, t in enumerate(grads):
+        t.normal_(0.0, 1.0 + i % 3, generator=g)
+    before = [t.clone() for t in grads]
+    out_bufs = [room(n, t) for n, _, t in parts] if elsewhere else bufs
+    skip = [8 + shift + (i % 2 if elsewhere else 0) for i in range(len(parts))]
+    outs = [b[s:s + n] for b, s, (n, _, _) in zip(out_bufs, skip, parts)]
+    plan = tk.GradTensors(grads, outs if elsewhere else None)
+    norm = _norm(tk, plan)
+    pieces = lambda t: t.split(1 << 26) if t.numel() else ()
+    want = sum((p.double() ** 2).sum().item() for t in before for p in pieces(t)) ** 0.5
+    assert abs(norm.item() - want) <= want * 2**-23
+    assert want > 2000.0
+    tk.dispatch_grad_clip(plan, norm, 1000.0)
+    factor = 1000.0 / (want + 1e-6)
+    for i, (a, b) in enumerate(zip(before, outs)):
+        for p, q in zip(pieces(a), pieces(b)):
+            exact = p.double() * factor
+            assert ((q.double() - exact).abs() <= exact.abs() * (6 * 2**-24 + HALF[b.dtype]) + 1e-37).all(), i
+        assert torch.all(out_bufs[i][:skip[i]] == 777.0) and torch.all(out_bufs[i][skip[i] + b.numel():] == 777.0), i
+    if elsewhere:
+        assert all(torch.equal(a.view(torch.int16 if a.dtype is BF else torch.int32), b.view(torch.int16 if a.dtype is BF else torch.int32))
+                   for a, b in zip(before, grads))
