@@ -42,7 +42,9 @@ struct Gate {
     // h of (g, u), and from dh the gradients of both
     __device__ __forceinline__ float gradients(float g, float u, float dh, float& dg, float& du) const {
         const float t = top(g), v = lin(u), z = CLAMPED ? a.alpha * t : t, s = sig(z), ts = t * s;
-        dg = dh * v * __builtin_fmaf(z * s, 1.0f - s, s);   // s (1 + z (1 - s))
+        // s (1 + z (1 - s)); alpha comes last, behind products that are 0 where s is 0 or 1: z may have left fp32 (a gate value
+        // that is the type's lowest, as a mask), and infinity times 0 is no number
+        dg = dh * v * (CLAMPED ? __builtin_fmaf(a.alpha, ts * (1.0f - s), s) : __builtin_fmaf(ts, 1.0f - s, s));
         du = dh * ts;
         if (CLAMPED) {
             dg = g > a.limit ? 0.f : dg;

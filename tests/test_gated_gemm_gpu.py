@@ -431,3 +431,33 @@ def test_an_expert_of_few_rows_among_others(hk, rows, other, kept, I, wide, inte
         got.append([t[at:at + n].clone() for t in (h, gu, dgu, h2)])
     for name, a, b in zip(("h", "gate_up", "dgate_up", "h again"), *got):
         assert torch.equal(a.view(torch.int16), b.view(torch.int16)), (name, int((a != b).sum()))
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("experts,R,I,N", [(0, 3, 136, 264), (0, 40, 136, 264), (0, 300, 264, 136), (0, 2100, 2056, 200), (3, 9, 136, 1032), (3, 700, 264, 136)])
+def test_gradients_of_the_lowest_gate_values(hk, experts, R, I, N, interleaved):
+    """Gate values whose product with alpha leaves fp32, the type's lowest as a mask among them: the logistic function is 0 there, and so are h and
+    both gradients, exactly; without a limit, far above, it is 1, and the slope too."""
+    print(f"gated lowest values experts={experts} R={R} I={I} N={N} interleaved={interleaved}", flush=True)
+    tk = hk.tk_kernel
+    g = torch.Generator(device=DEV).manual_seed(R + I)
+    dy, w2 = _rand(g, R, N), _rand(g, max(experts, 1), N, I, std=N**-0.5)
+    gu = _rand(g, R, 2 * I)
+    gate, up = _split(gu, interleaved)
+    low, far = -torch.finfo(torch.bfloat16).max, torch.finfo(torch.bfloat16).max
+    gate[0, 1], gate[1, :], gate[R - 1, I - 1], gate[2, 5] = low, low, -2.5e38, far
+    up[2, 5] = 0.5
+    offsets = torch.tensor([0] + [R * (e + 1) // experts for e in range(experts)], dtype=torch.int32, device=DEV) if experts else None
+    mk = lambda n: torch.full((R, n), 777.0, dtype=torch.bfloat16, device=DEV)
+    for limit in (LIMIT, math.inf):
+        dgu, h = mk(2 * I), mk(I)
+        tk.dispatch_gated_gemm_dgrad(dy, w2 if experts else w2[0], gu, dgu, h, expert_offsets=offsets, interleaved=interleaved,
+                                     activation="swiglu_oai", alpha=ALPHA, limit=limit)
+        dg, du = _split(dgu, interleaved)
+        assert torch.isfinite(dgu).all() or limit == math.inf
+        for at in ((0, 1), (1, slice(None)), (R - 1, I - 1)):
+            assert torch.all(dg[at] == 0) and torch.all(du[at] == 0) and torch.all(h[at] == 0), (limit, at)
+        if limit == math.inf:   # dg = dh (u + 1)
+            dh = float(dy[2].double() @ w2[0][:, 5].double())
+            size = float(dy[2].double().abs() @ w2[0][:, 5].double().abs())
+            assert abs(float(dg[2, 5]) - 1.5 * dh) <= abs(1.5 * dh) * (HALF + 2**-20) + 1.5 * size * 2 * (N + 8) * 2**-24
