@@ -320,8 +320,8 @@ __device__ __forceinline__ void write_row(const EmbedSums& p, T* dtable, int row
     store8(dtable + (size_t)row * p.H + col, r);
 }
 
-// Rows [from, to) without tokens: zeros, or a copy of `add`; a workgroup takes kRestRows of them, a thread finds out whether its row has tokens, a
-// wave writes a row.
+// Rows [from, to) without tokens: zeros, or a copy of `add`; a workgroup takes `rows` of them (4 to kRestRows), a thread finds out whether its row has
+// tokens, a wave writes a row.
 struct EmbedRest {
     int from, to, rows;   // rows of a workgroup
     int stream;           // more than the memory-side cache holds: past it

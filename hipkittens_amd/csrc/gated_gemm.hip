@@ -563,9 +563,9 @@ static long long skinny_grid(P& p, int cols) {
     p.tiles_n = (p.I + cols - 1) / cols;
     return p.offsets ? grouped_tiles_m(p.R, p.E, 16 * R) * p.tiles_n : p.tiles_n;
 }
-// Weights past the caches: where they are too large to stay, and where the rows of memory that the kernels load are whole cache lines; a line that two
-// loads share would come from HBM twice (one row, I = 9408, K = 2360 25.4 us with the hint, 23.4 without; 40 experts of 1432 x 3000, 64 rows 159 / 124;
-// but one row, I = 11008, K = 4096 29.6 / 31.9).
+// Weights past the caches: where they are too large to stay (a dense block's; experts' of any size, whose workgroups read them once), and where the rows
+// of memory that the kernels load are whole cache lines; a line that two loads share would come from HBM twice (one row, I = 9408, K = 2360
+// 25.4 us with the hint, 23.4 without; 40 experts of 1432 x 3000, 64 rows 159 / 124; but one row, I = 11008, K = 4096 29.6 / 31.9).
 static bool skinny_nt(const void* w, long long bytes, long long row_bytes) { return bytes >= kSkinnyNtBytes && (((uintptr_t)w | row_bytes) % 128) == 0; }
 template <int R, int NW, int D, int NF, bool EXPERTS = false>
 static int launch_gated_skinny_kernel(GatedForward p, hipStream_t s) {
@@ -587,14 +587,16 @@ static int launch_gated_skinny_kernel(GatedForward p, hipStream_t s) {
 // 36.1. 1 row, I = 2048, K = 7168: 11.2 / - / 30.2.) Rows of weights that are not whole cache lines take two accesses a piece, which bounds a CU, so that one
 // with a workgroup more than the others is waited for: 16 again while x is a few rows (16 / 32: one row, I = 9408, K = 2360 18.4 / 23.4; 8 rows, I =
 // 4176, K = 6512 31.7 / 37.2; 12 rows, I = 13000, K = 4072 55.6 / 53.2).
-// Waves and stages of a workgroup for 16, 32 and 64 rows of weights: as many stages as fit while the CUs hold the workgroups in one round, two workgroups a
-// CU where there are more (I = 14336, K = 4096, one row 38.5 / 35.9; I = 2880, K = 2880 7.4 / 8.0).
+// Waves and stages of a workgroup for 16, 32 and 64 rows of weights. Where there are more workgroups than CUs, two of them fit a CU (one row of 14336 x
+// 4096 with one a CU 38.5 us, so 35.9; 32 rows, with more stages: 9216 x 8192 65.1, so 63.0, 14336 x 4096 40.7, so 38.8). In one round 12 to 30 KB under
+// way a wave are enough, and more stages, as many as the LDS holds, only start later (one row of 912 x 3728 6.4, so 5.5; of 2048 x 7168 11.3 / 11.1; 32
+// rows of it 16.1 / 16.1). Of 48 and 64 rows, more than one round is always one of 64 rows of weights.
 struct SkinnyForm { int waves, stages; };
 template <int R> constexpr SkinnyForm kSkinnyForms[2][3] = {};   // [one round, more]
 template <> constexpr SkinnyForm kSkinnyForms<1>[2][3] = {{{4, 4}, {4, 4}, {}}, {{4, 4}, {4, 3}, {}}};
 template <> constexpr SkinnyForm kSkinnyForms<2>[2][3] = {{{4, 3}, {4, 3}, {3, 3}}, {{}, {3, 3}, {3, 2}}};
-template <> constexpr SkinnyForm kSkinnyForms<3>[2][3] = {{{4, 4}, {4, 4}, {3, 3}}, {{}, {4, 4}, {2, 2}}};
-template <> constexpr SkinnyForm kSkinnyForms<4>[2][3] = {{{4, 3}, {4, 3}, {3, 3}}, {{}, {4, 3}, {2, 2}}};
+template <> constexpr SkinnyForm kSkinnyForms<3>[2][3] = {{{4, 4}, {4, 4}, {3, 3}}, {{}, {}, {2, 2}}};
+template <> constexpr SkinnyForm kSkinnyForms<4>[2][3] = {{{4, 3}, {4, 3}, {3, 3}}, {{}, {}, {2, 2}}};
 template <int R>
 static int launch_gated_skinny_rows(const GatedForward& p, hipStream_t s) {
     const int cus = moe_num_compute_units();
@@ -653,10 +655,10 @@ static int launch_gated_dgrad_skinny(const GatedBackward& p, hipStream_t s) {
 // in one round, 32 for few rounds, else 64 of up to 32 rows of x (16 rows of x take 0 to 8 % less where the experts' rows are even, up to 10 % more where
 // they are not); more than 8 rows an expert only where the 128-tile kernel has more than one round of its two workgroups a CU. Backward: 32
 // columns a workgroup while they are one round, else 64, but for the 128-tile kernel's one round. Beyond one round not for short rows, where a wave has few
-// K-steps. (us, tile kernels / these: forward, 128 experts of 2880 x 2880, 300 rows 662 / 573, 1000 732 / 650, 2000 742 / 678, 3200 756 / 764; 200 of
-// 1024 x 4096, 500 rows 549 / 468; 40 of 2048 x 7168, 300 rows 425 / 349; 9 of 576 x 2672, one row 16.1 / 7.6, but 40 rows 17.3 / 19.7. Shares of the
-// experts as 1 / rank: 128 of 2880 x 2880, 1000 rows 669 / 653, 200 of 1024 x 4096, 1500 rows 561 / 497, but 32 of 2880 x 2880, 600 rows, 141 of
-// them one expert's, 190 / 216. Backward, the first four 372 / 299, 394 / 347, 402 / 383, 410 / 442; 275 / 246; 265 / 207; 16.6 / 8.9, 17.0 / 12.8; uneven
+// K-steps. (us, tile kernels / these: forward, 128 experts of 2880 x 2880, 300 rows 662 / 578, 1000 732 / 650, 2000 742 / 675, 3200 756 / 764; 200 of
+// 1024 x 4096, 500 rows 549 / 451; 40 of 2048 x 7168, 300 rows 425 / 348; 9 of 576 x 2672, one row 16.1 / 7.4, but 40 rows 17.3 / 18.9. Shares of the
+// experts as 1 / rank: 128 of 2880 x 2880, 1000 rows 669 / 646, 200 of 1024 x 4096, 1500 rows 561 / 477, but 32 of 2880 x 2880, 600 rows, 141 of
+// them one expert's, 190 / 212. Backward, the first four 372 / 299, 394 / 347, 402 / 383, 410 / 442; 275 / 246; 265 / 207; 16.6 / 8.9, 17.0 / 12.8; uneven
 // 377 / 341, 272 / 268, 121 / 117; 40 experts of 1432 x 1024, 40 rows, one round of tiles, 22.3 / 29.1. Short rows: 30 of 3000 x 264, 64 rows
 // forward 33.5 / 37.5; 60 of 2048 x 768, 200 rows backward 41.5 / 44.9.)
 struct ExpertRows {
@@ -700,8 +702,10 @@ static bool launch_gated_experts_skinny(const GatedBackward& p, hipStream_t s, i
 // choose_layout's rounds / these: forward, 1831 rows, I = 2280, K = 3784 126.5 / 81.5; 11 experts of 1776 x 2688, 1567 rows 90.9 / 66.0; backward,
 // 1636 rows, I = 9472, N = 840 72.0 / 50.1, but 1547 rows, I = 12376, N = 2600 150.3 / 172.4; on 230 drawn shapes of more than 64 rows 1.3 %
 // less on average.) Tiles of 128 rows and 256 columns, 128x128 or 256x256 otherwise / these: 32 experts of 2048 x 7168, 128 rows each 492 / 425; 128 of
-// 2880 x 2880, 64 rows 870 / 841, 128 rows 1008 / 990; 64 of 1536 x 4096, 150 rows 435 / 386; 8 of 4096 x 4096, 128 rows 203 / 158, but 64 of
-// 768 x 2048, 128 rows 131 / 141. Not in the backward pass, whose epilogue is the longer.
+// 2880 x 2880, 64 rows 870 / 841; 64 of 1536 x 4096, 150 rows 435 / 386; 8 of 4096 x 4096, 128 rows 203 / 158, but 64 of 768 x 2048, 128 rows
+// 131 / 141; and 128 of 2880 x 2880 with 128 rows, where the rule stays with 256x256, 1008 / 990. Not in the backward pass, where the same rule
+// would gain at 128 rows an expert (32 of 2048 x 7168 280 / 270, 8 of 4096 x 4096 92 / 82) and lose beyond and beside it (256 rows 355 / 389; 64 of
+// 1536 x 4096, 150 rows 240 / 267; 128 of 2880 x 2880, 64 rows 472 / 490).
 constexpr double kWideFixed = 6.0, kWideStep = 0.97, kDeepFixed = 4.0, kDeepStepBusy = 0.5;
 enum GatedTile { kGatedWide, kGated256, kGated128, kGated128Deep, kGated64Deep };
 static GatedTile gated_tile(int R, int E, int in, int out, bool dense, bool forward) {

@@ -46,9 +46,12 @@ __device__ __forceinline__ void for_chunks(const GradEntry* __restrict__ list, i
     }
 }
 
-// Lists that do not fit the memory-side cache together (256 MB) go past it: with the non-temporal hint the norm of 2.4 GB takes 342 us instead of
-// 385, the clip 879 instead of 913; smaller ones are still there for the clip when the norm has read them. The clip goes from the last chunk to
-// the first, whose read the caches remember best (both together 1222 us, so 1179).
+// Lists of more chunks than the memory-side cache (256 MB) holds in bf16 go past it, but for tensors that the clip converts or meets at two alignments:
+// with the non-temporal hint the norm of 2.4 GB takes 342 us instead of 385, the clip 879 instead of 913; smaller ones are still there for the clip
+// when the norm has read them. The rule counts chunks, so that fp32, of which 256 MB are half as many, goes past the cache from 512 MB on. (Norm and clip
+// in place, us without the hint / with it: lists that the caches held before, bf16 200 MB 99 / 108, 300 MB 153 / 160, 400 MB 210 / 207, fp32 300 MB 155 / 167,
+// 500 MB 284 / 272; behind a write of 300 MB, which the figure holds, bf16 200 MB 177 / 155, 300 MB 237 / 206, fp32 300 MB 238 / 211, 500 MB 364 / 320.)
+// The clip goes from the last chunk to the first, whose read the caches remember best (both together 1222 us, so 1179).
 constexpr int64_t kClipStreamChunks = (256ll << 20) / (2 * kClipChunk);
 template <bool NT>
 __device__ __forceinline__ v4i load_piece(const v4i* p) {
