@@ -530,7 +530,7 @@ int hk_linear_cross_entropy_backward(const void* x_bf16, const void* w_bf16, con
  * x [R, K], w13 [E, 2I, K] (gate rows 0 .. I-1, then up rows; interleaved != 0: gate and up rows of column c are rows 2c and 2c + 1),
  * h [R, I], gate_up [R, 2I] or NULL: both projections in the order of w13's rows, rounded to bf16, for the backward pass (h comes from the
  * unrounded ones). activation 0: silu(g) u (alpha and limit are not used); 1: (clamp(u, -limit, limit) + 1) g' / (1 + exp(-alpha g')) with
- * g' = min(g, limit), limit > 0, alpha finite. A NaN stays one. Rows, offsets and rows behind the last as for hk_moe_grouped_gemm.
+ * g' = min(g, limit), limit > 0, alpha finite. No bias. A NaN stays one. Rows, offsets and rows behind the last as for hk_moe_grouped_gemm.
  * Requirements: I % 8 == 0, I <= 2^20, K % 8 == 0, K <= 2^21, E <= 512, R < 2^30, fewer than 2^24 tiles of 128 x 128 of [R, 2I]; everything
  * 16-byte aligned; no workspace. */
 int hk_gated_gemm(const void* x_bf16, const void* w13_bf16, const int32_t* expert_offsets_or_null, void* h_bf16,
@@ -567,7 +567,8 @@ int hk_embedding_backward(const void* ids, int id_type, const void* dout_bf16, c
                           int T, int V, int H, float scale, void* workspace, size_t workspace_bytes, void* stream);
 
 /* A list of gradients for hk_grad_norm and hk_grad_clip: hk_grad_list_fill writes a table of hk_grad_list_bytes(n) bytes to host memory (8-byte
- * aligned) and how many chunks of work it holds; the caller copies it to the device once and keeps it while the tensors stay where they are.
+ * aligned) and how many chunks of work it holds; the caller copies it to the device once and keeps it while the tensors stay where they are and
+ * until the last call that was given it has run, a captured graph's replays among them.
  * grads[i] (device) holds counts[i] elements (0 or more, below 2^40) of type types[i] (0 bf16, 1 fp32), aligned to its element; outs[i] takes
  * the scaled ones, in out_types[i]; outs NULL: in place. 1 <= n <= 2^20. No tensor may overlap another, but outs[i] may be grads[i]
  * (of the same type). */
